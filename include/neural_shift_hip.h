@@ -473,6 +473,102 @@ NSH_API int64_t nsh_metropolis_backward_workspace_bytes(int64_t B, int64_t S, in
 NSH_API int nsh_stream_probe(int kind, const void* src, void* dst, int64_t bytes, int workgroups,
                              void* stream);
 
+/* -------------------------------------------------------------------------
+ * Token operators: attention over sequences of tokens (patch tokens, packed
+ * crops, answers made token by token), with the norm and rotation of its
+ * queries and keys and a learned relative position bias.  Extensions with no
+ * counterpart in the reference.  fp16/bf16/fp32; sums, norms and softmax
+ * statistics are float.  Tensors are (B, heads, tokens, width) with a unit
+ * last stride and the given strides, in elements, of the other three.
+ * ------------------------------------------------------------------------- */
+
+/* Norm and rotation of queries and keys, per head and token:
+ *   y = x * (mean(x^2) + eps)^(-1/2) * weight
+ *   (a, b) -> (a cos - b sin, a sin + b cos) for the pairs of the first 2 * half
+ *   elements: (i, i + half), or (2i, 2i + 1) if `interleaved`
+ * cos, sin: float (rows, half); positions: int32, the row of each token.  A position outside [0, rows) gives NaN and reads nothing.  A NULL
+ * weight is 1.  D <= 512, 2 * half <= D.  Outputs are contiguous
+ * (B, heads, L, D) in `dtype`; q or k may have no heads.
+ * Any alignment and strides. */
+typedef struct nsh_norm_rotary_args {
+    const void *q, *k, *q_weight, *k_weight;
+    const float *cos, *sin;
+    const int32_t* positions; /* NULL: token t stands at t */
+    int64_t position_stride;  /* from a batch to the next: L, or 0 for one row */
+    int64_t B, Hq, Hk, L, D, half, rows;
+    int64_t q_stride[3], k_stride[3]; /* batch, head, token */
+    double eps;
+    int32_t dtype, interleaved;
+    void *q_out, *k_out; /* forward */
+    /* backward: upstream gradients, with strides; gradients of q and k
+     * (contiguous) and of the weights (D; NULL = not wanted) */
+    const void *grad_q_out, *grad_k_out;
+    int64_t gq_stride[3], gk_stride[3];
+    void *grad_q, *grad_k, *grad_q_weight, *grad_k_weight;
+    void* workspace; /* nsh_norm_rotary_workspace_bytes, 16-byte aligned */
+    int64_t workspace_bytes;
+} nsh_norm_rotary_args;
+NSH_API int nsh_norm_rotary_forward(const nsh_norm_rotary_args* args, void* stream);
+NSH_API int nsh_norm_rotary_backward(const nsh_norm_rotary_args* args, void* stream);
+NSH_API int64_t nsh_norm_rotary_workspace_bytes(const nsh_norm_rotary_args* args);
+
+/* Relative position bias by buckets: query i of Lq stands at key position
+ * i + Lk - Lq;  rel = clamp(j - (i + Lk - Lq), -reach, reach),
+ *   out[h, i, j] = table[buckets[rel + reach], h]
+ * table (num_buckets, H) in `dtype`, buckets int32 (2 * reach + 1), out
+ * (H, Lq, Lk).  A bucket outside [0, num_buckets) gives NaN (and has no
+ * gradient).  Backward: grad_table (num_buckets, H) from grad_out, sums in
+ * float in a fixed order.  reach <= 2048, num_buckets <= 4097. */
+NSH_API int nsh_position_bias_forward(const void* table, const int32_t* buckets, int64_t H,
+                                      int64_t Lq, int64_t Lk, int64_t num_buckets, int64_t reach,
+                                      int dtype, void* out, void* stream);
+NSH_API int nsh_position_bias_backward(const void* grad_out, const int32_t* buckets, int64_t H,
+                                       int64_t Lq, int64_t Lk, int64_t num_buckets, int64_t reach,
+                                       int dtype, void* grad_table, void* workspace,
+                                       int64_t workspace_bytes, void* stream);
+NSH_API int64_t nsh_position_bias_workspace_bytes(int64_t H, int64_t Lq, int64_t Lk,
+                                                  int64_t reach);
+
+/* Attention with capped scores, distance biases and masks.  n = lengths[b]
+ * (Lk without lengths; clamped to [0, Lk]) keys are filled, and query i stands
+ * at position p = i + n - Lq:
+ *   x = scale * q_i . k_j;  y = cap * tanh(x / cap) (cap 0: y = x)
+ *   s = y - slopes[h] * |j - p| + table[buckets[clamp(j - p)], h]
+ * over the keys j < n with (j <= p or j < prefix[b], if `causal`) and (if
+ * `documents`, int32 (B, Lk)) documents[b, j] == documents[b, p] >= 0, where a
+ * query with p outside [0, n) sees nothing.
+ *   out = softmax(s) v,  log_degree = log sum exp s  (float, (B, Hq, Lq));
+ * a row that sees nothing gives 0 and -inf.  Query head h reads key head
+ * h / (Hq / Hk).  D <= 128, D a multiple of 8; the rows of q, k, v, out and of
+ * the gradients start on 16 bytes.  Keys that a query does not see add
+ * nothing to it, whatever they hold. */
+typedef struct nsh_attention_args {
+    const void *q, *k, *v;
+    int64_t B, Hq, Hk, Lq, Lk, D;
+    int64_t q_stride[3], k_stride[3], v_stride[3], out_stride[3]; /* batch, head, token */
+    const int32_t *lengths, *prefix; /* (B) or NULL */
+    const int32_t* documents;        /* (B, Lk) or NULL */
+    const float* slopes;             /* (Hq) or NULL */
+    const void* bias_table;          /* (num_buckets, Hq) in `dtype` or NULL */
+    const int32_t* buckets;          /* (2 * reach + 1) */
+    int64_t num_buckets, reach;
+    double scale, cap;
+    int32_t dtype, causal;
+    void* out;
+    float* log_degree; /* forward: NULL = not wanted */
+    /* backward: `out` and `log_degree` of the forward; grad_log_degree and
+     * grad_bias_table may be NULL.  grad_q has q's shape and gq_stride, ... */
+    const void* grad_out;
+    const float* grad_log_degree;
+    int64_t go_stride[3], gq_stride[3], gk_stride[3], gv_stride[3];
+    void *grad_q, *grad_k, *grad_v, *grad_bias_table;
+    void* workspace; /* nsh_attention_workspace_bytes, 16-byte aligned */
+    int64_t workspace_bytes;
+} nsh_attention_args;
+NSH_API int nsh_attention_forward(const nsh_attention_args* args, void* stream);
+NSH_API int nsh_attention_backward(const nsh_attention_args* args, void* stream);
+NSH_API int64_t nsh_attention_workspace_bytes(const nsh_attention_args* args, int backward);
+
 #ifdef __cplusplus
 }
 #endif

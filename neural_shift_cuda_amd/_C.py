@@ -886,3 +886,205 @@ def stream_probe(kind: str, src, dst: torch.Tensor, workgroups: int = 0, *, unro
                 | (PROBE_RING if ring else 0))
         _call("nsh_stream_probe", code, _ptr(src), dst.data_ptr(), nbytes, int(workgroups),
               _stream(dst))
+
+
+# ---------------------------------------------------------------------------
+# Token operators (extensions: no counterpart in the reference's module)
+# ---------------------------------------------------------------------------
+
+_F64 = ctypes.c_double
+_I32 = ctypes.c_int32
+_S3 = _I64 * 3
+
+
+class _NormRotaryArgs(ctypes.Structure):
+    _fields_ = [
+        ("q", _P), ("k", _P), ("q_weight", _P), ("k_weight", _P), ("cos", _P), ("sin", _P),
+        ("positions", _P), ("position_stride", _I64),
+        ("B", _I64), ("Hq", _I64), ("Hk", _I64), ("L", _I64), ("D", _I64), ("half", _I64),
+        ("rows", _I64), ("q_stride", _S3), ("k_stride", _S3), ("eps", _F64), ("dtype", _I32),
+        ("interleaved", _I32), ("q_out", _P), ("k_out", _P), ("grad_q_out", _P),
+        ("grad_k_out", _P), ("gq_stride", _S3), ("gk_stride", _S3), ("grad_q", _P),
+        ("grad_k", _P), ("grad_q_weight", _P), ("grad_k_weight", _P), ("workspace", _P),
+        ("workspace_bytes", _I64)]
+
+
+class _AttentionArgs(ctypes.Structure):
+    _fields_ = [
+        ("q", _P), ("k", _P), ("v", _P), ("B", _I64), ("Hq", _I64), ("Hk", _I64), ("Lq", _I64),
+        ("Lk", _I64), ("D", _I64), ("q_stride", _S3), ("k_stride", _S3), ("v_stride", _S3),
+        ("out_stride", _S3), ("lengths", _P), ("prefix", _P), ("documents", _P), ("slopes", _P),
+        ("bias_table", _P), ("buckets", _P), ("num_buckets", _I64), ("reach", _I64),
+        ("scale", _F64), ("cap", _F64), ("dtype", _I32), ("causal", _I32), ("out", _P),
+        ("log_degree", _P), ("grad_out", _P), ("grad_log_degree", _P), ("go_stride", _S3),
+        ("gq_stride", _S3), ("gk_stride", _S3), ("gv_stride", _S3), ("grad_q", _P),
+        ("grad_k", _P), ("grad_v", _P), ("grad_bias_table", _P), ("workspace", _P),
+        ("workspace_bytes", _I64)]
+
+
+for _name, _args, _res in (
+        ("nsh_norm_rotary_forward", [_P, _P], _I),
+        ("nsh_norm_rotary_backward", [_P, _P], _I),
+        ("nsh_norm_rotary_workspace_bytes", [_P], _I64),
+        ("nsh_position_bias_forward", [_P, _P, _I64, _I64, _I64, _I64, _I64, _I, _P, _P], _I),
+        ("nsh_position_bias_backward", [_P, _P, _I64, _I64, _I64, _I64, _I64, _I, _P, _P, _I64,
+                                        _P], _I),
+        ("nsh_position_bias_workspace_bytes", [_I64, _I64, _I64, _I64], _I64),
+        ("nsh_attention_forward", [_P, _P], _I),
+        ("nsh_attention_backward", [_P, _P], _I),
+        ("nsh_attention_workspace_bytes", [_P, _I], _I64)):
+    _fn = getattr(_lib, _name)
+    _fn.argtypes = _args
+    _fn.restype = _res
+
+
+def _heads_code(t: torch.Tensor, op: str) -> int:
+    code = _code(t, op)
+    if code == 4:
+        raise RuntimeError(f"\"{op}\" not implemented for '{t.dtype}'")
+    return code
+
+
+def _strides(t: torch.Tensor):
+    return t.stride()[:3]
+
+
+def _like(t: torch.Tensor, heads: int, tokens: int, width: int) -> torch.Tensor:
+    """A new (B, heads, tokens, width) tensor that keeps t's order of heads and
+    tokens in memory."""
+    B = t.shape[0]
+    if t.stride(1) < t.stride(2):
+        return t.new_empty((B, tokens, heads, width)).transpose(1, 2)
+    return t.new_empty((B, heads, tokens, width))
+
+
+def _workspace(t: torch.Tensor, n: int) -> Optional[torch.Tensor]:
+    return torch.empty(n, dtype=torch.uint8, device=t.device) if n > 0 else None
+
+
+def _norm_rotary_args(op, q, k, q_weight, k_weight, cos, sin, positions, eps, interleaved):
+    B, Hq, L, D = q.shape
+    return _NormRotaryArgs(
+        q=q.data_ptr(), k=k.data_ptr(), q_weight=_ptr(q_weight), k_weight=_ptr(k_weight),
+        cos=cos.data_ptr(), sin=sin.data_ptr(), positions=_ptr(positions),
+        position_stride=L if positions is not None and positions.dim() == 2 else 0,
+        B=B, Hq=Hq, Hk=k.shape[1], L=L, D=D, half=cos.shape[1], rows=cos.shape[0],
+        q_stride=_strides(q), k_stride=_strides(k), eps=eps, dtype=_heads_code(q, op),
+        interleaved=interleaved)
+
+
+def norm_rotary_forward(q, k, q_weight, k_weight, cos, sin, positions, eps, interleaved):
+    """[q', k'] (nsh_norm_rotary_forward): (B, heads, L, D) tensors of any
+    strides with a unit last one; weights (D) or None; cos, sin contiguous
+    float (rows, half); positions contiguous int32 (L) or (B, L), or None."""
+    a = _norm_rotary_args("norm_rotary", q, k, q_weight, k_weight, cos, sin, positions, eps,
+                          interleaved)
+    outs = [torch.empty(t.shape, dtype=t.dtype, device=t.device) for t in (q, k)]
+    if a.B and a.L and a.D and (a.Hq or a.Hk):
+        a.q_out, a.k_out = outs[0].data_ptr(), outs[1].data_ptr()
+        _call_on(q, "nsh_norm_rotary_forward", ctypes.byref(a))
+    return outs
+
+
+def norm_rotary_backward(q, k, q_weight, k_weight, cos, sin, positions, eps, interleaved, gq, gk,
+                         need_weights):
+    """[grad_q, grad_k, grad_q_weight, grad_k_weight] (nsh_norm_rotary_backward);
+    the weights' gradients None where there is no weight, or not wanted."""
+    a = _norm_rotary_args("norm_rotary", q, k, q_weight, k_weight, cos, sin, positions, eps,
+                          interleaved)
+    grads = [torch.empty(t.shape, dtype=t.dtype, device=t.device) for t in (q, k)]
+    wgrads = [torch.empty_like(w) if w is not None and need else None
+              for w, need in zip((q_weight, k_weight), need_weights)]
+    if not (a.B and a.L and a.D and (a.Hq or a.Hk)):
+        return grads + [None if w is None else w.zero_() for w in wgrads]
+    a.grad_q_out, a.grad_k_out = gq.data_ptr(), gk.data_ptr()
+    a.gq_stride, a.gk_stride = _strides(gq), _strides(gk)
+    a.grad_q, a.grad_k = grads[0].data_ptr(), grads[1].data_ptr()
+    a.grad_q_weight, a.grad_k_weight = _ptr(wgrads[0]), _ptr(wgrads[1])
+    if wgrads[0] is not None or wgrads[1] is not None:
+        ws = _workspace(q, int(_lib.nsh_norm_rotary_workspace_bytes(ctypes.byref(a))))
+        a.workspace, a.workspace_bytes = _ptr(ws), ws.numel() if ws is not None else 0
+    _call_on(q, "nsh_norm_rotary_backward", ctypes.byref(a))
+    return grads + wgrads
+
+
+def position_bias_forward(table, buckets, q_len, k_len):
+    """(H, q_len, k_len) (nsh_position_bias_forward): table contiguous
+    (num_buckets, H), buckets contiguous int32 (2 * reach + 1)."""
+    code = _heads_code(table, "position_bias")
+    nb, H = table.shape
+    out = torch.empty((H, q_len, k_len), dtype=table.dtype, device=table.device)
+    if out.numel():
+        _call_on(table, "nsh_position_bias_forward", table.data_ptr(), buckets.data_ptr(), H,
+                 q_len, k_len, nb, (buckets.numel() - 1) // 2, code, out.data_ptr())
+    return out
+
+
+def position_bias_backward(grad_out, buckets, num_buckets):
+    """(num_buckets, H) from a contiguous (H, q_len, k_len) gradient."""
+    code = _heads_code(grad_out, "position_bias")
+    H, q_len, k_len = grad_out.shape
+    reach = (buckets.numel() - 1) // 2
+    grad = torch.empty((num_buckets, H), dtype=grad_out.dtype, device=grad_out.device)
+    if not grad_out.numel():
+        return grad.zero_()
+    n = int(_lib.nsh_position_bias_workspace_bytes(H, q_len, k_len, reach))
+    ws = _workspace(grad_out, n)
+    _call_on(grad_out, "nsh_position_bias_backward", grad_out.data_ptr(), buckets.data_ptr(), H,
+             q_len, k_len, num_buckets, reach, code, grad.data_ptr(), _ptr(ws), n)
+    return grad
+
+
+def _attention_args(q, k, v, out, log_degree, rules):
+    B, Hq, Lq, D = q.shape
+    table, buckets = rules["bias_table"], rules["buckets"]
+    return _AttentionArgs(
+        q=q.data_ptr(), k=k.data_ptr(), v=v.data_ptr(), B=B, Hq=Hq, Hk=k.shape[1], Lq=Lq,
+        Lk=k.shape[2], D=D, q_stride=_strides(q), k_stride=_strides(k), v_stride=_strides(v),
+        out_stride=_strides(out), lengths=_ptr(rules["lengths"]), prefix=_ptr(rules["prefix"]),
+        documents=_ptr(rules["documents"]), slopes=_ptr(rules["slopes"]), bias_table=_ptr(table),
+        buckets=_ptr(buckets), num_buckets=table.shape[0] if table is not None else 0,
+        reach=(buckets.numel() - 1) // 2 if table is not None else 0, scale=rules["scale"],
+        cap=rules["cap"], dtype=_heads_code(q, "attention"), causal=rules["causal"],
+        out=out.data_ptr(), log_degree=_ptr(log_degree))
+
+
+def attention_forward(q, k, v, rules, want_degree):
+    """[out, log_degree or None] (nsh_attention_forward): (B, heads, tokens, D)
+    tensors with 16-byte rows; `rules` holds scale, cap, causal and the mask and
+    bias tensors (or None) as the C ABI takes them."""
+    B, Hq, Lq, D = q.shape
+    out = _like(q, Hq, Lq, D)
+    degree = (torch.empty((B, Hq, Lq), dtype=torch.float32, device=q.device)
+              if want_degree else None)
+    if not out.numel():
+        return out, degree
+    if not k.numel():
+        return out.zero_(), degree.fill_(float("-inf")) if want_degree else None
+    a = _attention_args(q, k, v, out, degree, rules)
+    n = int(_lib.nsh_attention_workspace_bytes(ctypes.byref(a), 0))
+    ws = _workspace(q, n)
+    a.workspace, a.workspace_bytes = _ptr(ws), n
+    _call_on(q, "nsh_attention_forward", ctypes.byref(a))
+    return out, degree
+
+
+def attention_backward(q, k, v, out, log_degree, rules, grad_out, grad_log_degree, need_table):
+    """[grad_q, grad_k, grad_v, grad_bias_table or None] (nsh_attention_backward)."""
+    B, Hq, Lq, D = q.shape
+    grads = [_like(q, Hq, Lq, D), _like(k, *k.shape[1:]), _like(v, *v.shape[1:])]
+    table = rules["bias_table"]
+    gt = torch.empty_like(table) if need_table else None
+    if not q.numel() or not k.numel():
+        return [g.zero_() for g in grads] + [None if gt is None else gt.zero_()]
+    a = _attention_args(q, k, v, out, log_degree, rules)
+    a.grad_out, a.go_stride = grad_out.data_ptr(), _strides(grad_out)
+    a.grad_log_degree = _ptr(grad_log_degree)
+    a.grad_q, a.grad_k, a.grad_v = (g.data_ptr() for g in grads)
+    a.gq_stride, a.gk_stride, a.gv_stride = (_strides(g) for g in grads)
+    a.grad_bias_table = _ptr(gt)
+    n = int(_lib.nsh_attention_workspace_bytes(ctypes.byref(a), 1))
+    ws = _workspace(q, n)
+    a.workspace, a.workspace_bytes = _ptr(ws), n
+    _call_on(q, "nsh_attention_backward", ctypes.byref(a))
+    return grads + [gt]

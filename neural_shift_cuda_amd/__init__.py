@@ -18,6 +18,16 @@ from .ops import (
     shift_gather_reference,
 )
 from .metropolis import metropolis_aggregate
+from .attention import (
+    biased_attention,
+    biased_attention_reference,
+    qk_norm_rotary,
+    qk_norm_rotary_reference,
+    relative_buckets,
+    relative_position_bias,
+    relative_position_bias_reference,
+    rotary_table,
+)
 
 __version__ = "0.12.0"
 __all__ = [
@@ -32,4 +42,12 @@ __all__ = [
     "normalized_accumulate_uz_reference",
     "accumulate_uz_scalar_reference",
     "metropolis_aggregate",
+    "biased_attention",
+    "qk_norm_rotary",
+    "relative_position_bias",
+    "relative_buckets",
+    "rotary_table",
+    "biased_attention_reference",
+    "qk_norm_rotary_reference",
+    "relative_position_bias_reference",
 ]

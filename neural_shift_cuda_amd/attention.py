@@ -1,0 +1,540 @@
+"""Token operators: attention over sequences of tokens, next to the shift
+windows of ``ops.py`` (extensions, no counterpart in the reference).
+
+    qk_norm_rotary(q, k, q_weight, k_weight, cos, sin, positions=None, *,
+        eps=1e-6, interleaved=False)                 -> (q', k')
+    relative_position_bias(table, buckets, q_len, k_len)  -> (H, q_len, k_len)
+    biased_attention(q, k, v, *, scale, cap, causal, prefix, documents,
+        lengths, slopes, bias_table, buckets,
+        return_log_degree=False)                     -> D or (D, log_C)
+
+and the tables a program makes once: ``rotary_table``, ``relative_buckets``.
+
+Tensors are (B, heads, tokens, width).  The conventions are those of the
+normalized accumulation: D = sum_j a_j v_j / sum_j a_j with a = exp(score),
+log_C the logarithm of the sum, and a row that sees nothing gives D = 0 and
+log_C = -inf.  GPU tensors go through the autograd Functions below into the HIP
+library (fp16, bf16, fp32; sums, norms and softmax statistics in fp32); CPU
+tensors use the ``*_reference`` implementations (any floating type), which are
+also exported.  A GPU tensor never falls back to them.
+
+Where tokens stand: the Lq queries are the last of the n filled keys (n = Lk,
+or ``lengths[b]``), so query i has position i + n - Lq.  A training step has
+Lq = Lk, a single new token Lq = 1.
+"""
+from __future__ import annotations
+
+import math
+from typing import Optional, Tuple
+
+import torch
+from torch.autograd.function import once_differentiable
+
+from . import ops
+
+_C = ops._C
+_NEG_INF = float("-inf")
+MAX_REACH = 2048  # relative positions a bucket map may tell apart, each way
+
+
+# ---------------------------------------------------------------------------
+# Tables a program makes once
+# ---------------------------------------------------------------------------
+
+def rotary_table(positions, dim: int, *, base: float = 10000.0, device=None
+                 ) -> Tuple[torch.Tensor, torch.Tensor]:
+    """(cos, sin), float32 (P, dim / 2), of the angles position * base^(-2 i / dim).
+
+    `positions` is a count P (positions 0 .. P-1) or a tensor of P positions,
+    or of (P, A) coordinates: the dim / 2 pairs are then shared out to the A axes
+    in equal parts (image tokens: row and column).  The angles are formed in
+    64 bits: in 32, position 10^5 is already 4e-3 rad off."""
+    if isinstance(positions, int):
+        positions = torch.arange(positions, device=device)
+    if positions.dim() not in (1, 2):
+        raise ValueError(f"positions must be a count, (P,) or (P, A); got {tuple(positions.shape)}")
+    at = positions.to(device=device, dtype=torch.float64)
+    at = at[:, None] if at.dim() == 1 else at
+    axes = at.shape[1]
+    if dim < 0 or dim % 2 or axes < 1 or (dim // 2) % axes:
+        raise ValueError(f"dim must be even and its pairs divide among {axes} axes; got {dim}")
+    part = dim // axes
+    freq = base ** (-torch.arange(0, part, 2, dtype=torch.float64, device=at.device) / max(part, 1))
+    angle = (at[:, :, None] * freq).flatten(1)
+    return angle.cos().float(), angle.sin().float()
+
+
+def relative_buckets(num_buckets: int, reach: int, *, bidirectional: bool = True, device=None
+                     ) -> torch.Tensor:
+    """int32 (2 * reach + 1): the bucket of each relative position (key minus
+    query) from -reach to reach; those beyond share the ends' buckets.
+
+    Half of the buckets are single distances, the others grow with the
+    logarithm of the distance up to `reach`.  `bidirectional`: keys after the
+    query have the second half of the buckets to themselves; otherwise they
+    share bucket 0 with the query's own position."""
+    n = num_buckets // 2 if bidirectional else num_buckets
+    near = n // 2
+    if near < 1 or not near < reach <= MAX_REACH:
+        raise ValueError(f"relative_buckets needs num_buckets >= {4 if bidirectional else 2} and "
+                         f"{near} < reach <= {MAX_REACH}; got {num_buckets}, {reach}")
+    rel = torch.arange(-reach, reach + 1)
+    d = rel.abs() if bidirectional else (-rel).clamp_min(0)
+    far = near + (torch.log(d.clamp_min(near).double() / near) / math.log(reach / near)
+                  * (n - near)).long()
+    out = torch.where(d < near, d, far.clamp_max(n - 1))
+    if bidirectional:
+        out = out + n * (rel > 0)
+    return out.to(device=device, dtype=torch.int32)
+
+
+# ---------------------------------------------------------------------------
+# Argument handling
+# ---------------------------------------------------------------------------
+
+def _heads(t: torch.Tensor, name: str) -> None:
+    if t.dim() != 4:
+        raise ValueError(f"{name} must be (B, heads, tokens, width); got {tuple(t.shape)}")
+    if not t.is_floating_point():
+        raise TypeError(f"{name} must be floating point; got {t.dtype}")
+
+
+def _same(name: str, t: torch.Tensor, like: torch.Tensor, dtype: bool = True) -> None:
+    if t.device != like.device:
+        raise ValueError(f"{name} must be on {like.device}; got {t.device}")
+    if dtype and t.dtype != like.dtype:
+        raise ValueError(f"{name} must have dtype {like.dtype}; got {t.dtype}")
+
+
+def _whole(name: str, t: Optional[torch.Tensor], shape, like: torch.Tensor
+           ) -> Optional[torch.Tensor]:
+    """An integer tensor of a given shape as contiguous int32 (values beyond
+    it at its ends: no row, bucket or length that the operators serve)."""
+    if t is None:
+        return None
+    if t.is_floating_point() or t.is_complex() or t.dtype == torch.bool:
+        raise TypeError(f"{name} must hold integers; got {t.dtype}")
+    if tuple(t.shape) != tuple(shape):
+        raise ValueError(f"{name} must be {tuple(shape)}; got {tuple(t.shape)}")
+    _same(name, t, like, dtype=False)
+    if t.dtype == torch.int64:
+        t = t.clamp(-(1 << 31), (1 << 31) - 1)
+    return t.to(torch.int32).contiguous()
+
+
+def _acc(t: torch.Tensor) -> torch.dtype:
+    return torch.float64 if t.dtype == torch.float64 else torch.float32
+
+
+def _check_norm(q, k, q_weight, k_weight, cos, sin, positions):
+    _heads(q, "q")
+    _heads(k, "k")
+    _same("k", k, q)
+    B, _, L, D = q.shape
+    if k.shape[0] != B or k.shape[2] != L or k.shape[3] != D:
+        raise ValueError(f"q and k must agree but for their heads; got {tuple(q.shape)} and "
+                         f"{tuple(k.shape)}")
+    for name, w in (("q_weight", q_weight), ("k_weight", k_weight)):
+        if w is not None:
+            _same(name, w, q)
+            if tuple(w.shape) != (D,):
+                raise ValueError(f"{name} must be ({D},); got {tuple(w.shape)}")
+    for name, t in (("cos", cos), ("sin", sin)):
+        _same(name, t, q, dtype=False)
+        if t.dim() != 2 or t.shape != cos.shape or 2 * t.shape[1] > D:
+            raise ValueError(f"cos and sin must both be (rows, half) with 2 * half <= {D}; got "
+                             f"{tuple(cos.shape)} and {tuple(sin.shape)}")
+        if t.dtype not in (torch.float32, torch.float64):
+            raise TypeError(f"{name} must be float32 (or float64); got {t.dtype}")
+        if t.requires_grad:
+            raise ValueError(f"{name} takes no gradient")
+    if positions is None:
+        if L > cos.shape[0]:
+            raise ValueError(f"cos and sin have {cos.shape[0]} rows for {L} tokens")
+        return None
+    shape = (L,) if positions.dim() == 1 else (B, L)
+    return _whole("positions", positions, shape, q)
+
+
+def _check_buckets(table: torch.Tensor, buckets: Optional[torch.Tensor], name: str
+                   ) -> torch.Tensor:
+    if table.dim() != 2 or table.shape[0] < 1:
+        raise ValueError(f"{name} must be (num_buckets, heads); got {tuple(table.shape)}")
+    if not table.is_floating_point():
+        raise TypeError(f"{name} must be floating point; got {table.dtype}")
+    if buckets is None or buckets.dim() != 1 or buckets.shape[0] % 2 == 0 \
+            or buckets.shape[0] > 2 * MAX_REACH + 1:
+        raise ValueError(f"buckets must be (2 * reach + 1,) with reach <= {MAX_REACH}")
+    if table.shape[0] > 2 * MAX_REACH + 1:
+        raise ValueError(f"{name} has more than {2 * MAX_REACH + 1} buckets")
+    return _whole("buckets", buckets, buckets.shape, table)
+
+
+def _check_attention(q, k, v, scale, cap, causal, prefix, documents, lengths, slopes, bias_table,
+                     buckets) -> dict:
+    """The checked call, as the native functions take it."""
+    for name, t in (("q", q), ("k", k), ("v", v)):
+        _heads(t, name)
+        _same(name, t, q)
+    B, Hq, Lq, D = q.shape
+    Hk, Lk = k.shape[1:3]
+    if k.shape != v.shape or k.shape[0] != B or k.shape[3] != D:
+        raise ValueError(f"k and v must both be ({B}, heads, tokens, {D}); got {tuple(k.shape)} "
+                         f"and {tuple(v.shape)}")
+    if (Hk == 0 and Hq) or (Hk and Hq % Hk):
+        raise ValueError(f"the {Hq} heads of q must be a multiple of the {Hk} of k")
+    if D < 1:
+        raise ValueError("the head width must be at least 1")
+    scale = D ** -0.5 if scale is None else float(scale)
+    cap = 0.0 if cap is None else float(cap)
+    if not math.isfinite(scale) or not math.isfinite(cap) or cap < 0:
+        raise ValueError(f"scale and cap must be finite and cap not negative; got {scale}, {cap}")
+    if prefix is not None and not causal:
+        raise ValueError("prefix needs causal=True: without it every key is seen already")
+    if slopes is not None:
+        if tuple(slopes.shape) != (Hq,):
+            raise ValueError(f"slopes must be ({Hq},); got {tuple(slopes.shape)}")
+        if not slopes.is_floating_point():
+            raise TypeError(f"slopes must be floating point; got {slopes.dtype}")
+        _same("slopes", slopes, q, dtype=False)
+        if slopes.requires_grad:
+            raise ValueError("slopes take no gradient; a learned bias is bias_table's")
+        slopes = slopes.to(_acc(q)).contiguous()
+    if bias_table is not None:
+        _same("bias_table", bias_table, q)
+        buckets = _check_buckets(bias_table, buckets, "bias_table")
+        if bias_table.shape[1] != Hq:
+            raise ValueError(f"bias_table must have {Hq} heads; got {tuple(bias_table.shape)}")
+    elif buckets is not None:
+        raise ValueError("buckets come with a bias_table")
+    return {"scale": scale, "cap": cap, "causal": bool(causal),
+            "prefix": _whole("prefix", prefix, (B,), q),
+            "documents": _whole("documents", documents, (B, Lk), q),
+            "lengths": _whole("lengths", lengths, (B,), q), "slopes": slopes,
+            "bias_table": bias_table, "buckets": buckets}
+
+
+# ---------------------------------------------------------------------------
+# CPU reference implementations (pure PyTorch, differentiable)
+# ---------------------------------------------------------------------------
+
+def qk_norm_rotary_reference(q, k, q_weight, k_weight, cos, sin, positions=None, *,
+                             eps: float = 1e-6, interleaved: bool = False
+                             ) -> Tuple[torch.Tensor, torch.Tensor]:
+    """CPU reference for ``qk_norm_rotary``."""
+    positions = _check_norm(q, k, q_weight, k_weight, cos, sin, positions)
+    L = q.shape[2]
+    at = torch.arange(L, device=q.device) if positions is None else positions.long()
+    rows, half = cos.shape
+    ok = ((at >= 0) & (at < rows))[..., None]
+    acc = _acc(q)
+
+    def picked(t):
+        if rows == 0:
+            return at.new_full((*at.shape, half), float("nan"), dtype=acc)
+        return torch.where(ok, t.to(acc)[at.clamp(0, rows - 1)], float("nan"))
+
+    c, s = picked(cos), picked(sin)
+    if c.dim() == 3:
+        c, s = c[:, None], s[:, None]
+    out = []
+    for x, w in ((q, q_weight), (k, k_weight)):
+        y = x.to(acc)
+        y = y * torch.rsqrt(y.square().mean(-1, keepdim=True) + eps)
+        if w is not None:
+            y = y * w.to(acc)
+        turn, rest = y[..., :2 * half], y[..., 2 * half:]
+        if interleaved:
+            a, b = turn[..., 0::2], turn[..., 1::2]
+            turn = torch.stack((a * c - b * s, a * s + b * c), -1).flatten(-2)
+        else:
+            a, b = turn[..., :half], turn[..., half:]
+            turn = torch.cat((a * c - b * s, a * s + b * c), -1)
+        out.append(torch.cat((turn, rest), -1).to(x.dtype))
+    return out[0], out[1]
+
+
+def _table_rows(table: torch.Tensor, buckets: torch.Tensor) -> torch.Tensor:
+    """The table's row of each relative position, NaN for a bucket it lacks."""
+    b = buckets.long()
+    ok = (b >= 0) & (b < table.shape[0])
+    return torch.where(ok[:, None], table[b.clamp(0, table.shape[0] - 1)], float("nan"))
+
+
+def relative_position_bias_reference(table: torch.Tensor, buckets: torch.Tensor, q_len: int,
+                                     k_len: int) -> torch.Tensor:
+    """CPU reference for ``relative_position_bias``."""
+    buckets = _check_buckets(table, buckets, "table")
+    reach = (buckets.numel() - 1) // 2
+    at = torch.arange(q_len, device=table.device)[:, None] + (k_len - q_len)
+    rel = (torch.arange(k_len, device=table.device)[None] - at).clamp(-reach, reach) + reach
+    return _table_rows(table.to(_acc(table)), buckets)[rel].permute(2, 0, 1).to(table.dtype)
+
+
+def _seen(rules: dict, B: int, Lq: int, Lk: int, device):
+    """(relative positions, visibility), both (B, Lq, Lk)."""
+    n = torch.full((B,), Lk, device=device) if rules["lengths"] is None \
+        else rules["lengths"].long().clamp(0, Lk)
+    j = torch.arange(Lk, device=device)
+    p = torch.arange(Lq, device=device) + (n - Lq)[:, None]           # (B, Lq)
+    rel = j - p[:, :, None]
+    see = (j < n[:, None])[:, None, :].expand(rel.shape)
+    if rules["causal"]:
+        near = rel <= 0
+        if rules["prefix"] is not None:
+            near = near | (j < rules["prefix"].long()[:, None])[:, None, :]
+        see = see & near
+    if rules["documents"] is not None:
+        d = rules["documents"].long()
+        own = torch.gather(d, 1, p.clamp(0, max(Lk - 1, 0))) if Lk else p
+        own = torch.where(p >= 0, own, -1)[:, :, None]
+        see = see & (own == d[:, None, :]) & (own >= 0)
+    return rel, see
+
+
+def biased_attention_reference(q, k, v, *, scale: Optional[float] = None,
+                               cap: Optional[float] = None, causal: bool = False, prefix=None,
+                               documents=None, lengths=None, slopes=None, bias_table=None,
+                               buckets=None, return_log_degree: bool = False):
+    """CPU reference for ``biased_attention``."""
+    r = _check_attention(q, k, v, scale, cap, causal, prefix, documents, lengths, slopes,
+                         bias_table, buckets)
+    acc = _acc(q)
+    B, Hq, Lq, D = q.shape
+    Hk, Lk = k.shape[1:3]
+    per = Hq // Hk if Hk else 1
+    rel, see = _seen(r, B, Lq, Lk, q.device)
+    see = see[:, None]
+    # what no query sees, whatever it holds, is out of every product
+    dead = ~see.any(2)[:, :, :, None]
+    kd, vd = (torch.where(dead, 0.0, t.to(acc)).repeat_interleave(per, 1) for t in (k, v))
+    s = torch.matmul(q.to(acc), kd.transpose(2, 3).contiguous()) * r["scale"]
+    if r["cap"]:
+        s = r["cap"] * torch.tanh(s / r["cap"])
+    if r["slopes"] is not None:
+        s = s - r["slopes"][:, None, None] * rel.abs()[:, None]
+    if bias_table is not None:
+        reach = (r["buckets"].numel() - 1) // 2
+        rows = _table_rows(bias_table.to(acc), r["buckets"])
+        s = s + rows[rel.clamp(-reach, reach) + reach].permute(0, 3, 1, 2)
+    s = torch.where(see, s, _NEG_INF)
+    m = s.detach().amax(-1, keepdim=True) if Lk else s.new_full((B, Hq, Lq, 1), _NEG_INF)
+    m = torch.where(m == _NEG_INF, 0.0, m)
+    e = torch.where(see, torch.exp(s - m), 0.0)
+    z = e.sum(-1, keepdim=True)
+    empty = z == 0
+    out = torch.where(empty, 0.0, torch.matmul(e, vd) / torch.where(empty, 1.0, z)).to(q.dtype)
+    if not return_log_degree:
+        return out
+    log_C = torch.where(empty, _NEG_INF, m + torch.log(torch.where(empty, 1.0, z)))
+    return out, log_C.squeeze(-1)
+
+
+# ---------------------------------------------------------------------------
+# autograd Functions over the HIP library
+# ---------------------------------------------------------------------------
+
+def _unit(t: torch.Tensor) -> torch.Tensor:
+    """t with a unit last stride (a broadcast or transposed row is copied)."""
+    return t if t.stride(3) == 1 or t.shape[3] == 1 else t.contiguous()
+
+
+class _QkNormRotaryFn(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, q, k, q_weight, k_weight, cos, sin, positions, eps, interleaved):
+        q, k = _unit(q), _unit(k)
+        out = _C.norm_rotary_forward(q, k, q_weight, k_weight, cos, sin, positions, eps,
+                                     interleaved)
+        ctx.save_for_backward(q, k, q_weight, k_weight, cos, sin, positions)
+        ctx.rules = (eps, interleaved)
+        return out[0], out[1]
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx, gq, gk):
+        q, k, q_weight, k_weight, cos, sin, positions = ctx.saved_tensors
+        grads = _C.norm_rotary_backward(q, k, q_weight, k_weight, cos, sin, positions, *ctx.rules,
+                                        _unit(gq), _unit(gk), ctx.needs_input_grad[2:4])
+        return (*grads, None, None, None, None, None)
+
+
+class _PositionBiasFn(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, table, buckets, q_len, k_len):
+        ctx.save_for_backward(buckets)
+        ctx.num_buckets = table.shape[0]
+        return _C.position_bias_forward(table.contiguous(), buckets, q_len, k_len)
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx, grad_out):
+        (buckets,) = ctx.saved_tensors
+        return (_C.position_bias_backward(grad_out.contiguous(), buckets, ctx.num_buckets),
+                None, None, None)
+
+
+def _rows16(t: torch.Tensor) -> torch.Tensor:
+    """t with rows that start on 16 bytes and a unit last stride, copied where
+    they do not (their width is a multiple of 8 by then)."""
+    bytes_ = t.element_size()
+    if (t.stride(3) == 1 and t.data_ptr() % 16 == 0
+            and all(s * bytes_ % 16 == 0 for s in t.stride()[:3])):
+        return t
+    return t.clone(memory_format=torch.contiguous_format)
+
+
+_TENSOR_RULES = ("prefix", "documents", "lengths", "slopes", "buckets")
+
+
+class _BiasedAttentionFn(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, q, k, v, bias_table, rules, want_degree):
+        table = bias_table.contiguous() if bias_table is not None else None
+        rules = {**rules, "bias_table": table}
+        # the gradients need the degree of every row
+        keep = any(ctx.needs_input_grad[:4])
+        out, degree = _C.attention_forward(q, k, v, rules, want_degree or keep)
+        if keep:
+            ctx.save_for_backward(q, k, v, table, out, degree, *(rules[n] for n in _TENSOR_RULES))
+            ctx.plain = {n: rules[n] for n in ("scale", "cap", "causal")}
+        ctx.set_materialize_grads(False)
+        return out, degree if want_degree else None
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx, grad_out, grad_degree):
+        q, k, v, table, out, degree, *rest = ctx.saved_tensors
+        rules = {**ctx.plain, "bias_table": table, **dict(zip(_TENSOR_RULES, rest))}
+        grad_out = torch.zeros_like(out) if grad_out is None else _rows16(grad_out)
+        grads = _C.attention_backward(q, k, v, out, degree, rules, grad_out,
+                                      None if grad_degree is None else grad_degree.contiguous(),
+                                      ctx.needs_input_grad[3])
+        return (*grads, None, None)
+
+
+# ---------------------------------------------------------------------------
+# Public API
+# ---------------------------------------------------------------------------
+
+def qk_norm_rotary(q: torch.Tensor, k: torch.Tensor, q_weight: Optional[torch.Tensor],
+                   k_weight: Optional[torch.Tensor], cos: torch.Tensor, sin: torch.Tensor,
+                   positions: Optional[torch.Tensor] = None, *, eps: float = 1e-6,
+                   interleaved: bool = False) -> Tuple[torch.Tensor, torch.Tensor]:
+    """Norm of queries and keys for each head, then the rotation by position.
+
+        y = x / sqrt(mean(x^2) + eps) * weight
+        (a, b) -> (a cos - b sin, a sin + b cos)
+
+    q (B, Hq, L, D) and k (B, Hk, L, D) of any strides (a projection's
+    (B, L, H, D) transposed is read where it lies); weights (D,) in their type
+    or None.  cos, sin (rows, half), float32, from ``rotary_table``: the first
+    2 * half of the D elements turn in pairs (i, i + half), or (2i, 2i + 1) with
+    `interleaved`, the others are left as normed.  `positions`: the row of each
+    token, integers (L,) or (B, L); None takes 0 .. L-1.  A position outside
+    the table makes its tokens NaN.  D <= 512 on the GPU.
+
+    Returns contiguous (q', k') in the inputs' type.  Differentiable in q, k and
+    the weights; the weights' gradients are summed in a fixed order."""
+    if not q.is_cuda:
+        return qk_norm_rotary_reference(q, k, q_weight, k_weight, cos, sin, positions, eps=eps,
+                                        interleaved=interleaved)
+    positions = _check_norm(q, k, q_weight, k_weight, cos, sin, positions)
+    if q.shape[3] > 512:
+        raise ValueError(f"heads wider than 512 are not served on the GPU; got {q.shape[3]}")
+    ops._require_cuda_ext("qk_norm_rotary")
+    w = [None if t is None else t.contiguous() for t in (q_weight, k_weight)]
+    return _QkNormRotaryFn.apply(q, k, w[0], w[1], cos.float().contiguous(),
+                                 sin.float().contiguous(), positions, float(eps),
+                                 bool(interleaved))
+
+
+def relative_position_bias(table: torch.Tensor, buckets: torch.Tensor, q_len: int, k_len: int
+                           ) -> torch.Tensor:
+    """The learned bias of every query and key, (H, q_len, k_len):
+
+        out[h, i, j] = table[buckets[clamp(j - (i + k_len - q_len))], h]
+
+    table (num_buckets, H); buckets (2 * reach + 1,) integers from
+    ``relative_buckets`` or of the caller's own (a bucket that the table lacks
+    gives NaN).  The relative position is clamped to +-reach.  Differentiable in
+    the table; its gradient is summed in fp32 in a fixed order.
+    ``biased_attention`` takes table and buckets themselves, without this tensor."""
+    if q_len < 0 or k_len < 0:
+        raise ValueError(f"q_len and k_len must not be negative; got {q_len}, {k_len}")
+    if not table.is_cuda:
+        return relative_position_bias_reference(table, buckets, q_len, k_len)
+    buckets = _check_buckets(table, buckets, "table")
+    ops._require_cuda_ext("relative_position_bias")
+    return _PositionBiasFn.apply(table, buckets, int(q_len), int(k_len))
+
+
+def biased_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, *,
+                     scale: Optional[float] = None, cap: Optional[float] = None,
+                     causal: bool = False, prefix: Optional[torch.Tensor] = None,
+                     documents: Optional[torch.Tensor] = None,
+                     lengths: Optional[torch.Tensor] = None,
+                     slopes: Optional[torch.Tensor] = None,
+                     bias_table: Optional[torch.Tensor] = None,
+                     buckets: Optional[torch.Tensor] = None, return_log_degree: bool = False):
+    """Attention with capped scores, distance biases and masks:
+
+        x = scale * q_i . k_j        s = cap * tanh(x / cap)       (no cap: s = x)
+        s = s - slopes[h] * |j - p| + bias_table[buckets[clamp(j - p)], h]
+        D_i = sum_j exp(s) v_j / sum_j exp(s)        log_C_i = log sum_j exp(s)
+
+    over the keys that query i, at position p, sees.  q (B, Hq, Lq, D), k and v
+    (B, Hk, Lk, D), Hq a multiple of Hk (query head h reads key head
+    h // (Hq // Hk)); scale defaults to D ** -0.5.
+
+    * lengths (B,): only the first lengths[b] keys are filled (a cache); the
+      queries are the last Lq of them, p = i + lengths[b] - Lq.
+    * causal: keys after p are not seen, except the first prefix[b] ones, which
+      every query sees.
+    * documents (B, Lk): several sequences in one row; a query sees the keys of
+      its own position's document only, and a negative one (padding) sees nothing
+      and is not seen.
+    * slopes (Hq,): linear distance bias, no gradient.
+    * bias_table (num_buckets, Hq) with buckets (2 * reach + 1,): a learned bias
+      by buckets of the relative position, as ``relative_position_bias`` writes
+      out; it has q's type and its gradient is summed in fp32.  -inf in it
+      excludes the distance.
+
+    A row that sees nothing gives 0 (and log_C = -inf).  What a query does not
+    see adds nothing to it, whatever it holds.
+
+    Returns D in q's type (and with q's order of heads and tokens in memory), or
+    (D, log_C) with return_log_degree, log_C fp32 (B, Hq, Lq).  Differentiable in
+    q, k, v and bias_table; the gradients are summed in a fixed order.  The GPU
+    serves fp16, bf16 and fp32 with D <= 128 (a width that is no multiple of 8,
+    or rows that do not start on 16 bytes, are copied first)."""
+    if not q.is_cuda:
+        return biased_attention_reference(
+            q, k, v, scale=scale, cap=cap, causal=causal, prefix=prefix, documents=documents,
+            lengths=lengths, slopes=slopes, bias_table=bias_table, buckets=buckets,
+            return_log_degree=return_log_degree)
+    rules = _check_attention(q, k, v, scale, cap, causal, prefix, documents, lengths, slopes,
+                             bias_table, buckets)
+    D = q.shape[3]
+    if D > 128:
+        raise ValueError(f"heads wider than 128 are not served on the GPU; got {D}")
+    ops._require_cuda_ext("biased_attention")
+    if D % 8:
+        q, k, v = (torch.nn.functional.pad(t, (0, -D % 8)) for t in (q, k, v))
+    q, k, v = _rows16(q), _rows16(k), _rows16(v)
+    del rules["bias_table"]
+    out, log_C = _BiasedAttentionFn.apply(q, k, v, bias_table, rules, bool(return_log_degree))
+    if D % 8:
+        out = out[..., :D]
+    return (out, log_C) if return_log_degree else out
+
+
+__all__ = [
+    "qk_norm_rotary",
+    "relative_position_bias",
+    "biased_attention",
+    "rotary_table",
+    "relative_buckets",
+    "qk_norm_rotary_reference",
+    "relative_position_bias_reference",
+    "biased_attention_reference",
+]
