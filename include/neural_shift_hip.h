@@ -556,14 +556,18 @@ typedef struct nsh_attention_args {
     int32_t dtype, causal;
     void* out;
     float* log_degree; /* forward: NULL = not wanted */
-    /* backward: `out` and `log_degree` of the forward; grad_log_degree and
-     * grad_bias_table may be NULL.  grad_q has q's shape and gq_stride, ... */
+    /* backward: `out`, and `row_stats` or `log_degree`, of the forward;
+     * grad_log_degree and grad_bias_table may be NULL.  grad_q has q's shape and gq_stride, ... */
     const void* grad_out;
     const float* grad_log_degree;
     int64_t go_stride[3], gq_stride[3], gk_stride[3], gv_stride[3];
     void *grad_q, *grad_k, *grad_v, *grad_bias_table;
     void* workspace; /* nsh_attention_workspace_bytes, 16-byte aligned */
     int64_t workspace_bytes;
+    /* (B, Hq, Lq, 2) or NULL.  Forward: written, every row's largest score (in
+     * units of log 2) and 1 / its sum.  Backward: used in log_degree's place,
+     * which loses the sum of a row whose scores are beyond 2^20 or so. */
+    float* row_stats;
 } nsh_attention_args;
 NSH_API int nsh_attention_forward(const nsh_attention_args* args, void* stream);
 NSH_API int nsh_attention_backward(const nsh_attention_args* args, void* stream);

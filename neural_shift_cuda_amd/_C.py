@@ -919,7 +919,7 @@ class _AttentionArgs(ctypes.Structure):
         ("log_degree", _P), ("grad_out", _P), ("grad_log_degree", _P), ("go_stride", _S3),
         ("gq_stride", _S3), ("gk_stride", _S3), ("gv_stride", _S3), ("grad_q", _P),
         ("grad_k", _P), ("grad_v", _P), ("grad_bias_table", _P), ("workspace", _P),
-        ("workspace_bytes", _I64)]
+        ("workspace_bytes", _I64), ("row_stats", _P)]
 
 
 for _name, _args, _res in (
@@ -1035,7 +1035,7 @@ def position_bias_backward(grad_out, buckets, num_buckets):
     return grad
 
 
-def _attention_args(q, k, v, out, log_degree, rules):
+def _attention_args(q, k, v, out, log_degree, row_stats, rules):
     B, Hq, Lq, D = q.shape
     table, buckets = rules["bias_table"], rules["buckets"]
     return _AttentionArgs(
@@ -1046,30 +1046,33 @@ def _attention_args(q, k, v, out, log_degree, rules):
         buckets=_ptr(buckets), num_buckets=table.shape[0] if table is not None else 0,
         reach=(buckets.numel() - 1) // 2 if table is not None else 0, scale=rules["scale"],
         cap=rules["cap"], dtype=_heads_code(q, "attention"), causal=rules["causal"],
-        out=out.data_ptr(), log_degree=_ptr(log_degree))
+        out=out.data_ptr(), log_degree=_ptr(log_degree), row_stats=_ptr(row_stats))
 
 
-def attention_forward(q, k, v, rules, want_degree):
-    """[out, log_degree or None] (nsh_attention_forward): (B, heads, tokens, D)
-    tensors with 16-byte rows; `rules` holds scale, cap, causal and the mask and
-    bias tensors (or None) as the C ABI takes them."""
+def attention_forward(q, k, v, rules, want_degree, want_stats):
+    """[out, log_degree or None, row_stats or None] (nsh_attention_forward):
+    (B, heads, tokens, D) tensors with 16-byte rows; `rules` holds scale, cap,
+    causal and the mask and bias tensors (or None) as the C ABI takes them."""
     B, Hq, Lq, D = q.shape
     out = _like(q, Hq, Lq, D)
     degree = (torch.empty((B, Hq, Lq), dtype=torch.float32, device=q.device)
               if want_degree else None)
+    stats = (torch.empty((B, Hq, Lq, 2), dtype=torch.float32, device=q.device)
+             if want_stats else None)
     if not out.numel():
-        return out, degree
+        return out, degree, stats
     if not k.numel():
-        return out.zero_(), degree.fill_(float("-inf")) if want_degree else None
-    a = _attention_args(q, k, v, out, degree, rules)
+        return (out.zero_(), degree.fill_(float("-inf")) if want_degree else None,
+                stats.zero_() if want_stats else None)
+    a = _attention_args(q, k, v, out, degree, stats, rules)
     n = int(_lib.nsh_attention_workspace_bytes(ctypes.byref(a), 0))
     ws = _workspace(q, n)
     a.workspace, a.workspace_bytes = _ptr(ws), n
     _call_on(q, "nsh_attention_forward", ctypes.byref(a))
-    return out, degree
+    return out, degree, stats
 
 
-def attention_backward(q, k, v, out, log_degree, rules, grad_out, grad_log_degree, need_table):
+def attention_backward(q, k, v, out, row_stats, rules, grad_out, grad_log_degree, need_table):
     """[grad_q, grad_k, grad_v, grad_bias_table or None] (nsh_attention_backward)."""
     B, Hq, Lq, D = q.shape
     grads = [_like(q, Hq, Lq, D), _like(k, *k.shape[1:]), _like(v, *v.shape[1:])]
@@ -1077,7 +1080,7 @@ def attention_backward(q, k, v, out, log_degree, rules, grad_out, grad_log_degre
     gt = torch.empty_like(table) if need_table else None
     if not q.numel() or not k.numel():
         return [g.zero_() for g in grads] + [None if gt is None else gt.zero_()]
-    a = _attention_args(q, k, v, out, log_degree, rules)
+    a = _attention_args(q, k, v, out, None, row_stats, rules)
     a.grad_out, a.go_stride = grad_out.data_ptr(), _strides(grad_out)
     a.grad_log_degree = _ptr(grad_log_degree)
     a.grad_q, a.grad_k, a.grad_v = (g.data_ptr() for g in grads)

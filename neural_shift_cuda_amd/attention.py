@@ -378,7 +378,8 @@ def _rows16(t: torch.Tensor) -> torch.Tensor:
     they do not (their width is a multiple of 8 by then)."""
     bytes_ = t.element_size()
     if (t.stride(3) == 1 and t.data_ptr() % 16 == 0
-            and all(s * bytes_ % 16 == 0 for s in t.stride()[:3])):
+            and all(s * bytes_ % 16 == 0 for s in t.stride()[:3])
+            and t.stride(2) * bytes_ <= 1 << 24):
         return t
     return t.clone(memory_format=torch.contiguous_format)
 
@@ -391,22 +392,22 @@ class _BiasedAttentionFn(torch.autograd.Function):
     def forward(ctx, q, k, v, bias_table, rules, want_degree):
         table = bias_table.contiguous() if bias_table is not None else None
         rules = {**rules, "bias_table": table}
-        # the gradients need the degree of every row
+        # the gradients need every row's largest score and sum
         keep = any(ctx.needs_input_grad[:4])
-        out, degree = _C.attention_forward(q, k, v, rules, want_degree or keep)
+        out, degree, stats = _C.attention_forward(q, k, v, rules, want_degree, keep)
         if keep:
-            ctx.save_for_backward(q, k, v, table, out, degree, *(rules[n] for n in _TENSOR_RULES))
+            ctx.save_for_backward(q, k, v, table, out, stats, *(rules[n] for n in _TENSOR_RULES))
             ctx.plain = {n: rules[n] for n in ("scale", "cap", "causal")}
         ctx.set_materialize_grads(False)
-        return out, degree if want_degree else None
+        return out, degree
 
     @staticmethod
     @once_differentiable
     def backward(ctx, grad_out, grad_degree):
-        q, k, v, table, out, degree, *rest = ctx.saved_tensors
+        q, k, v, table, out, stats, *rest = ctx.saved_tensors
         rules = {**ctx.plain, "bias_table": table, **dict(zip(_TENSOR_RULES, rest))}
         grad_out = torch.zeros_like(out) if grad_out is None else _rows16(grad_out)
-        grads = _C.attention_backward(q, k, v, out, degree, rules, grad_out,
+        grads = _C.attention_backward(q, k, v, out, stats, rules, grad_out,
                                       None if grad_degree is None else grad_degree.contiguous(),
                                       ctx.needs_input_grad[3])
         return (*grads, None, None)

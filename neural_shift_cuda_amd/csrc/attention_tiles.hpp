@@ -1,0 +1,369 @@
+// attention_tiles.hpp -- tiles of rows in LDS and the 32 x 32 matrix products
+// over them, for fp16, bf16 and fp32 alike.
+//
+// A wave's products have the rows of an LDS tile on their first side and 32
+// rows held in registers, one to a lane (lane l: row l % 32), on their second;
+// lane halves (g = l / 32) share a row's contraction.  The result leaves every
+// lane with 16 of the tile's 32 rows for its own row,
+//     element r <-> tile row 8 (r / 4) + 4 g + r % 4,
+// which is also the order in which the second product (weights times the
+// tile's rows, contracted over those) wants its second side: it needs no
+// exchange of lanes, only the tile read by columns in the same order.
+#pragma once
+
+#include "attention.hpp"
+
+namespace nsh {
+
+typedef float f32x16 __attribute__((ext_vector_type(16)));
+typedef float f32x8 __attribute__((ext_vector_type(8)));
+typedef float f32x4 __attribute__((ext_vector_type(4)));
+typedef _Float16 f16x8 __attribute__((ext_vector_type(8)));
+typedef _Float16 f16x4 __attribute__((ext_vector_type(4)));
+typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
+typedef __bf16 bf16x4 __attribute__((ext_vector_type(4)));
+typedef short s16x4 __attribute__((ext_vector_type(4)));
+typedef short s16x8 __attribute__((ext_vector_type(8)));
+typedef int i32x4 __attribute__((ext_vector_type(4)));
+
+#define NSH_LDS __attribute__((address_space(3)))
+
+// Eight contraction steps of a lane half: what one row contributes to 16.
+template <typename T> struct Eight;
+template <> struct Eight<f16> {
+    using V = f16x8;
+    static __device__ __forceinline__ f32x16 mma(V a, V b, f32x16 c) {
+        return __builtin_amdgcn_mfma_f32_32x32x16_f16(a, b, c, 0, 0, 0);
+    }
+    static __device__ __forceinline__ V pack(f32x8 v) { return __builtin_convertvector(v, f16x8); }
+    static __device__ __forceinline__ V negate(V v) { return -v; }
+};
+template <> struct Eight<bf16> {
+    using V = bf16x8;
+    static __device__ __forceinline__ f32x16 mma(V a, V b, f32x16 c) {
+        return __builtin_amdgcn_mfma_f32_32x32x16_bf16(a, b, c, 0, 0, 0);
+    }
+    static __device__ __forceinline__ V pack(f32x8 v) { return __builtin_convertvector(v, bf16x8); }
+    static __device__ __forceinline__ V negate(V v) {
+        return __builtin_bit_cast(V, __builtin_bit_cast(s16x8, v) ^ static_cast<short>(0x8000));
+    }
+};
+template <> struct Eight<float> {
+    using V = f32x8;
+    static __device__ __forceinline__ f32x16 mma(V a, V b, f32x16 c) {
+#pragma unroll
+        for (int e = 0; e < 8; ++e) c = __builtin_amdgcn_mfma_f32_32x32x2f32(a[e], b[e], c, 0, 0, 0);
+        return c;
+    }
+    static __device__ __forceinline__ V pack(f32x8 v) { return v; }
+    static __device__ __forceinline__ V negate(V v) { return -v; }
+};
+
+// Four results rounded to T, stored together.
+template <typename T>
+__device__ __forceinline__ void store4(T* p, f32x4 v) {
+    if constexpr (sizeof(T) == 4)
+        *reinterpret_cast<f32x4*>(p) = v;
+    else if constexpr (__is_same(T, f16))
+        *reinterpret_cast<f16x4*>(p) = __builtin_convertvector(v, f16x4);
+    else
+        *reinterpret_cast<bf16x4*>(p) = __builtin_convertvector(v, bf16x4);
+}
+
+// Tile row of result element r, less the lane half's 4 g.
+__device__ __forceinline__ constexpr int el(int r) { return 8 * (r / 4) + r % 4; }
+
+// The other lane half's value joined to one's own.
+__device__ __forceinline__ float halves_max(float v) {
+    const auto r = __builtin_amdgcn_permlane32_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+    return fmaxf(__uint_as_float(r[0]), __uint_as_float(r[1]));
+}
+__device__ __forceinline__ float halves_sum(float v) {
+    const auto r = __builtin_amdgcn_permlane32_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+    return __uint_as_float(r[0]) + __uint_as_float(r[1]);
+}
+
+// Rows of DP elements in LDS, 16-byte chunks.  A row's chunks are permuted by
+// turn(row) so that eight rows read at one chunk, and four rows read at 32
+// bytes by columns, meet no bank twice.
+template <typename T, int DP>
+struct Tile {
+    static constexpr int CE = 16 / sizeof(T), NC = DP / CE, ROW = DP * sizeof(T);
+    static constexpr int NS = DP / 16, ND = DP / 32;
+    using V = typename Eight<T>::V;
+
+    static __device__ __forceinline__ int turn(int r) {
+        if constexpr (NC % 8 == 0)
+            return (r & 3) << 1 | (r >> 2 & 1);
+        else
+            return (r >> 1 & 1) << 1 | (r >> 2 & 1);
+    }
+    static __device__ __forceinline__ int at(int r, int c) { return r * ROW + ((c ^ turn(r)) * 16); }
+
+    // Steps s of row r0 + l % 32.
+    static __device__ __forceinline__ V row(const char* lds, int r0, int s, int l) {
+        const int r = l & 31, g = l >> 5;
+        lds += r0 * ROW;
+        if constexpr (sizeof(T) == 2) {
+            return *reinterpret_cast<const V*>(lds + at(r, 2 * s + g));
+        } else {
+            const f32x4 a = *reinterpret_cast<const f32x4*>(lds + at(r, 4 * s + 2 * g));
+            const f32x4 b = *reinterpret_cast<const f32x4*>(lds + at(r, 4 * s + 2 * g + 1));
+            return __builtin_shufflevector(a, b, 0, 1, 2, 3, 4, 5, 6, 7);
+        }
+    }
+    // Column 32 db + l % 32 of the 16 rows from r0 (a multiple of 16), in the
+    // order of result elements.
+    static __device__ __forceinline__ V col(const char* lds, int r0, int db, int l) {
+        const int g = l >> 5;
+        lds += r0 * ROW;
+        if constexpr (sizeof(T) == 2) {
+            // a transposing read takes four rows by 16 columns from 16 lanes
+            const int i = l & 15, d = db * 32 + (l & 16) + 4 * (i & 3);
+            const char* p = lds + at(4 * g + (i >> 2), d / 8) + (d & 7) * 2;
+            const s16x4 a = __builtin_amdgcn_ds_read_tr16_b64_v4i16((NSH_LDS s16x4*)(p));
+            const s16x4 b = __builtin_amdgcn_ds_read_tr16_b64_v4i16((NSH_LDS s16x4*)(p + 8 * ROW));
+            return __builtin_bit_cast(V, __builtin_shufflevector(a, b, 0, 1, 2, 3, 4, 5, 6, 7));
+        } else {
+            const int d = db * 32 + (l & 31);
+            V v;
+#pragma unroll
+            for (int e = 0; e < 8; ++e)
+                v[e] = *reinterpret_cast<const float*>(lds + at(el(e) + 4 * g, d / 4) + (d & 3) * 4);
+            return v;
+        }
+    }
+};
+
+// BYTES a lane from its offset in the buffer to LDS, the lanes side by side
+// from `lds` on; nothing passes through registers.
+template <int BYTES>
+__device__ __forceinline__ void to_lds(__amdgpu_buffer_rsrc_t rs, void* lds, uint32_t off) {
+#ifdef __HIP_DEVICE_COMPILE__  // the host's parse of this header knows no 16-byte form
+    if constexpr (BYTES == 16)
+        __builtin_amdgcn_raw_ptr_buffer_load_lds(rs, (NSH_LDS void*)(lds), 16, off, 0, 0, 0);
+    else
+        __builtin_amdgcn_raw_ptr_buffer_load_lds(rs, (NSH_LDS void*)(lds), 4, off, 0, 0, 0);
+#endif
+}
+
+// Tile rows [0, ROWS) of a tensor from global memory straight into LDS by NW
+// waves.  Rows past the tensor's end, and columns past D, arrive as zeros (the
+// buffer's range check): nothing behind a cache's filled part is read.
+template <typename T, int DP, int ROWS, int NW>
+struct Loader {
+    using L = Tile<T, DP>;
+    static constexpr int NI = ROWS * L::NC / (NW * 64);
+    static_assert(NI * NW * 64 == ROWS * L::NC, "whole instructions");
+    uint32_t off[NI];
+
+    __device__ __forceinline__ void init(int id, int64_t stride, int D) {
+#pragma unroll
+        for (int i = 0; i < NI; ++i) {
+            const int x = i * NW * 64 + id, r = x / L::NC, c = (x % L::NC) ^ L::turn(r);
+            off[i] = c * L::CE < D ? static_cast<uint32_t>(r * stride * sizeof(T)) + c * 16 : 0x80000000u;
+        }
+    }
+    // base: the tensor's row 0; first: the tile's first row; rows: its end.
+    __device__ __forceinline__ void load(char* lds, const T* base, int64_t stride, int first, int rows,
+                                         int D, int wave) const {
+        const int64_t left = (rows - 1 - static_cast<int64_t>(first)) * stride * sizeof(T) + D * sizeof(T);
+        const uint32_t bytes = rows <= first ? 0u : static_cast<uint32_t>(left < 0x7fffffff ? left : 0x7fffffff);
+        const __amdgpu_buffer_rsrc_t rs = __builtin_amdgcn_make_buffer_rsrc(
+            const_cast<T*>(base + first * stride), static_cast<short>(0), static_cast<int>(bytes), 0x00020000);
+#pragma unroll
+        for (int i = 0; i < NI; ++i)
+            to_lds<16>(rs, lds + (i * NW + wave) * 1024, off[i]);
+    }
+};
+
+// The lane's row, as the second side of the products (zeros past D).
+template <typename T, int DP>
+__device__ __forceinline__ void load_row(typename Eight<T>::V (&v)[DP / 16], const T* row, int D, int l) {
+    using V = typename Eight<T>::V;
+#pragma unroll
+    for (int s = 0; s < DP / 16; ++s) {
+        const int d = s * 16 + (l >> 5) * 8;
+        if constexpr (sizeof(T) == 2) {
+            i32x4 x = {};
+            if (d < D) x = *reinterpret_cast<const i32x4*>(row + d);
+            v[s] = __builtin_bit_cast(V, x);
+        } else {
+            f32x4 x = {}, y = {};
+            if (d < D) {
+                x = *reinterpret_cast<const f32x4*>(row + d);
+                y = *reinterpret_cast<const f32x4*>(row + d + 4);
+            }
+            v[s] = __builtin_shufflevector(x, y, 0, 1, 2, 3, 4, 5, 6, 7);
+        }
+    }
+}
+
+// Products of 32 tile rows from r0 with the lane's row.
+template <typename T, int DP>
+__device__ __forceinline__ f32x16 products(const char* lds, int r0, const typename Eight<T>::V (&v)[DP / 16],
+                                           int l) {
+    f32x16 c = {};
+#pragma unroll
+    for (int s = 0; s < DP / 16; ++s) c = Eight<T>::mma(Tile<T, DP>::row(lds, r0, s, l), v[s], c);
+    return c;
+}
+
+// acc[db] += (32 tile rows from r0, by columns) x weights w.
+template <typename T, int DP>
+__device__ __forceinline__ void weigh(f32x16 (&acc)[DP / 32], const char* lds, int r0, const f32x16& w, int l) {
+    const typename Eight<T>::V lo = Eight<T>::pack(__builtin_shufflevector(w, w, 0, 1, 2, 3, 4, 5, 6, 7));
+    const typename Eight<T>::V hi = Eight<T>::pack(__builtin_shufflevector(w, w, 8, 9, 10, 11, 12, 13, 14, 15));
+#pragma unroll
+    for (int db = 0; db < DP / 32; ++db) {
+        acc[db] = Eight<T>::mma(Tile<T, DP>::col(lds, r0, db, l), lo, acc[db]);
+        acc[db] = Eight<T>::mma(Tile<T, DP>::col(lds, r0 + 16, db, l), hi, acc[db]);
+    }
+}
+
+// ---------------------------------------------------------------------------
+// Scores, in units of log 2.
+// ---------------------------------------------------------------------------
+
+// cap * tanh(x |scale| / cap) is 1 - 2 / (1 + exp) in three cheap steps, off by
+// some 2^-22 of the cap; with fp32 results, or a cap above 256 (2^-14, where a
+// 16-bit weight's half step is 2^-12), small arguments take the series.
+constexpr float kQuickCap = 256.f;
+
+struct Cap {
+    int mode;      // 0: none, 1: quick, 2: accurate
+    float c;       // |scale| log2 e
+    float k;       // 2 log2 e |scale| / cap
+    float top;     // cap log2 e
+    float inv;     // |scale| / cap
+};
+
+template <typename T>
+__device__ __forceinline__ Cap cap_of(const Att& a) {
+    Cap c;
+    const float s = fabsf(a.scale);
+    c.mode = a.cap <= 0.f ? 0 : (sizeof(T) == 4 || a.cap > kQuickCap) ? 2 : 1;
+    c.c = s * kLog2e;
+    c.inv = a.cap > 0.f ? s / a.cap : 0.f;
+    c.k = 2.f * kLog2e * c.inv;
+    c.top = a.cap * kLog2e;
+    return c;
+}
+
+__device__ __forceinline__ float quick_r(float x, float k) {
+    return __builtin_amdgcn_rcpf(1.f + __builtin_amdgcn_exp2f(x * k));
+}
+
+// tanh with a small relative error everywhere: its series up to x^11 below
+// 0.3 (the next term is 2e-9 of it).
+__device__ __forceinline__ float tanh_rel(float x) {
+    const float y = x * x;
+    float p = fma_acc(y, -1382.f / 155925.f, 62.f / 2835.f);
+    p = fma_acc(y, p, -17.f / 315.f);
+    p = fma_acc(y, p, 2.f / 15.f);
+    p = fma_acc(y, p, -1.f / 3.f);
+    p = fma_acc(y * x, p, x);
+    const float q = 1.f - 2.f * __builtin_amdgcn_rcpf(1.f + __builtin_amdgcn_exp2f(2.f * kLog2e * fabsf(x)));
+    return fabsf(x) < 0.3f ? p : copysignf(q, x);
+}
+
+// Raw products to scores; SLOPE: also the cap's derivative.
+template <bool SLOPE>
+__device__ __forceinline__ void cap_scores(const Cap& c, f32x16& s, f32x16& w) {
+    if (c.mode == 0) {
+#pragma unroll
+        for (int r = 0; r < 16; ++r) s[r] *= c.c;
+    } else if (c.mode == 1) {
+#pragma unroll
+        for (int r = 0; r < 16; ++r) {
+            const float q = quick_r(s[r], c.k);
+            s[r] = fma_acc(q, -2.f * c.top, c.top);
+            if (SLOPE) w[r] = 4.f * fma_acc(-q, q, q);
+        }
+    } else {
+#pragma unroll
+        for (int r = 0; r < 16; ++r) {
+            const float t = tanh_rel(s[r] * c.inv);
+            s[r] = c.top * t;
+            if (SLOPE) w[r] = fma_acc(-t, t, 1.f);
+        }
+    }
+}
+
+// The bias of a lane's 16 pairs with relative positions rel0 + sign * el(r).
+struct Bias {
+    float slope;        // the lane's, in units of log 2
+    const float* line;  // the table by relative position + reach, in LDS
+};
+
+template <int SIGN>
+__device__ __forceinline__ void add_bias(const Att& a, const Bias& bs, int rel0, int least, int most,
+                                         f32x16& s) {
+    if (a.slopes) {
+        const float f = static_cast<float>(rel0);
+#pragma unroll
+        for (int r = 0; r < 16; ++r) s[r] = fma_acc(-bs.slope, fabsf(f + SIGN * el(r)), s[r]);
+    }
+    if (!a.table) return;
+    if (most <= -a.reach || least >= a.reach) {  // the tile's extremes: one value
+        const float far = bs.line[least >= a.reach ? 2 * a.reach : 0];
+#pragma unroll
+        for (int r = 0; r < 16; ++r) s[r] += far;
+    } else {
+#pragma unroll
+        for (int r = 0; r < 16; ++r) {
+            int rel = rel0 + SIGN * el(r);
+            rel = min(max(rel, -a.reach), a.reach);
+            s[r] += bs.line[rel + a.reach];
+        }
+    }
+}
+
+// The head's table by relative position, in units of log 2, by all threads.
+template <typename T>
+__device__ __forceinline__ void stage_line(const Att& a, int h, float* line) {
+    for (int r = threadIdx.x; r <= 2 * a.reach; r += kAttThreads)
+        line[r] = table_value<T>(a, h, r - a.reach);
+}
+
+// ---------------------------------------------------------------------------
+// Which workgroup does what.  Workgroups are dealt to the eight XCDs in turn;
+// where the head groups divide among them, an XCD keeps its groups, whose keys
+// then stay in its L2.  Late rows of a causal call see the most: they go first.
+// ---------------------------------------------------------------------------
+
+__device__ __forceinline__ void place(int n, int groups, int& group, int& rest) {
+    const int x = n % groups;
+    rest = n / groups;
+    group = groups % 8 == 0 ? (x % 8) * (groups / 8) + x / 8 : x;
+}
+
+// Which of a run of tiles are needed, 64 at a time.
+template <typename F>
+struct Needed {
+    F f;
+    unsigned long long bits = 0;
+    int w = -1;
+    __device__ __forceinline__ bool operator()(int t) {
+        if (t >> 6 != w) {
+            w = t >> 6;
+            bits = __ballot(f((w << 6) + (threadIdx.x & 63)));
+        }
+        return bits >> (t & 63) & 1;
+    }
+    // The first needed tile from t on, or end.
+    __device__ __forceinline__ int next(int t, int end) {
+        while (t < end) {
+            (*this)(t);
+            const unsigned long long left = bits >> (t & 63);
+            if (left) {
+                t += __builtin_ctzll(left);
+                return t < end ? t : end;
+            }
+            t = ((t >> 6) + 1) << 6;
+        }
+        return end;
+    }
+};
+
+}  // namespace nsh
