@@ -91,14 +91,12 @@ __device__ __forceinline__ void row_gradient(const Att& a, const Cap& cap, const
                                              const typename Eight<T>::V (&go)[DP / 16], float2 stat, float delta,
                                              const char* K, const char* V, int r0, const int* kd, int j0, int l,
                                              TableSums* ts, f32x16 (&dq)[DP / 32]) {
-    f32x16 s = products<T, DP>(K, r0, q, l);
+    const Scores y = cap_scores<true>(cap, products<T, DP>(K, r0, q, l));
     f32x16 dp = products<T, DP>(V, r0, go, l);
-    f32x16 w;
-    cap_scores<true>(cap, s, w);
     const int rel0 = j0 + 4 * (l >> 5) - x.p, least = j0 - wr.last, most = j0 + 31 - wr.first;
-    add_bias<1>(a, bs, rel0, least, most, s);
+    f32x16 s = add_bias<1>(a, bs, rel0, least, most, y.s);
     const bool whole = j0 + 32 <= wr.least && !a.documents;
-    if (!whole) mask_keys(a, x, j0, kd, l, s);
+    if (!whole) s = mask_keys(a, x, j0, kd, l, s);
 #pragma unroll
     for (int r = 0; r < 16; ++r) dp[r] = __builtin_amdgcn_exp2f(s[r] - stat.x) * fma_acc(dp[r], stat.y, -delta);
     if (!whole) {  // 0 times what an unseen pair holds is not always 0
@@ -106,10 +104,7 @@ __device__ __forceinline__ void row_gradient(const Att& a, const Cap& cap, const
         for (int r = 0; r < 16; ++r) dp[r] = s[r] == -INFINITY ? 0.f : dp[r];
     }
     if (ts) add_table(a, *ts, j0 - wr.first, least, most, l, dp);
-    if (cap.mode != 0) {
-#pragma unroll
-        for (int r = 0; r < 16; ++r) dp[r] *= w[r];
-    }
+    if (cap.mode != 0) dp *= y.w;
     weigh<T, DP>(dq, K, r0, dp, l);
 }
 
@@ -400,11 +395,9 @@ __global__ __launch_bounds__(kAttThreads, DP * sizeof(T) >= 256 ? 1 : 2) void at
             const int most = a.causal ? min(n, max(pf + ends, prefix)) : n;
             if (j0 >= most) continue;
             const bool whole = j0 + 32 <= least && !a.documents;
-            f32x16 s = products<T, DP>(tile, qb * 32, k, l);
+            const Scores y = cap_scores<true>(cap, products<T, DP>(tile, qb * 32, k, l));
             f32x16 dp = products<T, DP>(tile + HALF, qb * 32, v, l);
-            f32x16 w;
-            cap_scores<true>(cap, s, w);
-            add_bias<-1>(a, bs, j - pf - 4 * g, j0 - pf - 31, j0 + 31 - pf, s);
+            f32x16 s = add_bias<-1>(a, bs, j - pf - 4 * g, j0 - pf - 31, j0 + 31 - pf, y.s);
             if (!whole) {
 #pragma unroll
                 for (int c = 0; c < 4; ++c) {
@@ -431,7 +424,7 @@ __global__ __launch_bounds__(kAttThreads, DP * sizeof(T) >= 256 ? 1 : 2) void at
                     const int r = 4 * c + e;
                     const float p = __builtin_amdgcn_exp2f(s[r] - top[e]);
                     float x = p * fma_acc(dp[r], inv[e], -del[e]);
-                    if (cap.mode != 0) x *= w[r];
+                    if (cap.mode != 0) x *= y.w[r];
                     dp[r] = !whole && s[r] == -INFINITY ? 0.f : x;
                     s[r] = p * inv[e];
                 }

@@ -42,10 +42,10 @@ __device__ __forceinline__ void attend(const Att& a, const Cap& cap, const Bias&
     } else {
 #pragma unroll
         for (int kb = 0; kb < NB; ++kb) {
-            cap_scores<false>(cap, s[kb], s[kb]);
+            s[kb] = cap_scores<false>(cap, s[kb]).s;
             const int rel0 = j0 + kb * 32 + 4 * (l >> 5) - x.p;
-            add_bias<1>(a, bs, rel0, j0 + kb * 32 - wr.last, j0 + kb * 32 + 31 - wr.first, s[kb]);
-            if (!whole) mask_keys(a, x, j0 + kb * 32, kd + kb * 32, l, s[kb]);
+            s[kb] = add_bias<1>(a, bs, rel0, j0 + kb * 32 - wr.last, j0 + kb * 32 + 31 - wr.first, s[kb]);
+            if (!whole) s[kb] = mask_keys(a, x, j0 + kb * 32, kd + kb * 32, l, s[kb]);
         }
     }
     float top = s[0][0];

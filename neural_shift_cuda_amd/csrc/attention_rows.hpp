@@ -62,8 +62,8 @@ __device__ __forceinline__ Bias lane_bias(const Att& a, int h, const float* line
 }
 
 // Not seen -> -inf, for 32 keys from j0 (kd: their documents, in LDS).
-__device__ __forceinline__ void mask_keys(const Att& a, const Row& x, int j0, const int* kd, int l,
-                                          f32x16& s) {
+__device__ __forceinline__ f32x16 mask_keys(const Att& a, const Row& x, int j0, const int* kd, int l,
+                                            f32x16 s) {
     const int j = j0 + 4 * (l >> 5);
 #pragma unroll
     for (int r = 0; r < 16; ++r) s[r] = j + el(r) < x.lim ? s[r] : -INFINITY;
@@ -75,6 +75,7 @@ __device__ __forceinline__ void mask_keys(const Att& a, const Row& x, int j0, co
             for (int e = 0; e < 4; ++e) s[4 * c + e] = d[e] == x.doc ? s[4 * c + e] : -INFINITY;
         }
     }
+    return s;
 }
 
 }  // namespace nsh

@@ -267,12 +267,17 @@ __device__ __forceinline__ float tanh_rel(float x) {
     return fabsf(x) < 0.3f ? p : copysignf(q, x);
 }
 
-// Raw products to scores; SLOPE: also the cap's derivative.
+// Raw products to scores, and the cap's derivative.  (Vectors go by value here
+// and below: through references they have ended in scratch memory.)
+struct Scores {
+    f32x16 s, w;
+};
+
 template <bool SLOPE>
-__device__ __forceinline__ void cap_scores(const Cap& c, f32x16& s, f32x16& w) {
+__device__ __forceinline__ Scores cap_scores(const Cap& c, f32x16 s) {
+    f32x16 w = {};
     if (c.mode == 0) {
-#pragma unroll
-        for (int r = 0; r < 16; ++r) s[r] *= c.c;
+        s *= c.c;
     } else if (c.mode == 1) {
 #pragma unroll
         for (int r = 0; r < 16; ++r) {
@@ -288,6 +293,7 @@ __device__ __forceinline__ void cap_scores(const Cap& c, f32x16& s, f32x16& w) {
             if (SLOPE) w[r] = fma_acc(-t, t, 1.f);
         }
     }
+    return Scores{s, w};
 }
 
 // The bias of a lane's 16 pairs with relative positions rel0 + sign * el(r).
@@ -297,18 +303,17 @@ struct Bias {
 };
 
 template <int SIGN>
-__device__ __forceinline__ void add_bias(const Att& a, const Bias& bs, int rel0, int least, int most,
-                                         f32x16& s) {
+__device__ __forceinline__ f32x16 add_bias(const Att& a, const Bias& bs, int rel0, int least, int most,
+                                           f32x16 s) {
     if (a.slopes) {
         const float f = static_cast<float>(rel0);
 #pragma unroll
         for (int r = 0; r < 16; ++r) s[r] = fma_acc(-bs.slope, fabsf(f + SIGN * el(r)), s[r]);
     }
-    if (!a.table) return;
+    if (!a.table) return s;
     if (most <= -a.reach || least >= a.reach) {  // the tile's extremes: one value
         const float far = bs.line[least >= a.reach ? 2 * a.reach : 0];
-#pragma unroll
-        for (int r = 0; r < 16; ++r) s[r] += far;
+        s += far;
     } else {
 #pragma unroll
         for (int r = 0; r < 16; ++r) {
@@ -317,6 +322,7 @@ __device__ __forceinline__ void add_bias(const Att& a, const Bias& bs, int rel0,
             s[r] += bs.line[rel + a.reach];
         }
     }
+    return s;
 }
 
 // The head's table by relative position, in units of log 2, by all threads.
