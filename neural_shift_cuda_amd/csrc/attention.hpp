@@ -278,6 +278,11 @@ __device__ __forceinline__ void exact_key_gradient(const Att& a, int b, int hk, 
         if (l + c * 64 < a.D) ok[l + c * 64] = from_acc<T>(gk[c]), ov[l + c * 64] = from_acc<T>(gv[c]);
 }
 
+// cap * tanh(x |scale| / cap) is 1 - 2 / (1 + exp) in three cheap steps, off by
+// some 2^-22 of the cap; with fp32 results, or a cap above 256 (2^-14, where a
+// 16-bit weight's half step is 2^-12), small arguments take the series.
+constexpr float kQuickCap = 256.f;
+
 // Launches of one type's kernels (attention_fwd_*.hip, attention_bwd_*.hip).
 template <typename T> int attention_forward_launch(const Att& a, hipStream_t st);
 template <typename T> int attention_backward_launch(const Att& a, hipStream_t st);

@@ -84,32 +84,64 @@ struct BwdShape {
     static constexpr int NBUF = L::ROW > 256 ? 1 : 2;
 };
 
-// dS of 32 keys for the wave's rows, and dx in its place (delta: over the row's sum).
-template <typename T, int DP>
+// 32 keys' part of the wave's dq, and of the table's sums.
+template <typename T, int DP, Kind KIND>
 __device__ __forceinline__ void row_gradient(const Att& a, const Cap& cap, const Bias& bs, const Row& x,
                                              const WaveRows& wr, const typename Eight<T>::V (&q)[DP / 16],
                                              const typename Eight<T>::V (&go)[DP / 16], float2 stat, float delta,
                                              const char* K, const char* V, int r0, const int* kd, int j0, int l,
                                              TableSums* ts, f32x16 (&dq)[DP / 32]) {
-    const Scores y = cap_scores<true>(cap, products<T, DP>(K, r0, q, l));
-    f32x16 dp = products<T, DP>(V, r0, go, l);
-    const int rel0 = j0 + 4 * (l >> 5) - x.p, least = j0 - wr.last, most = j0 + 31 - wr.first;
-    f32x16 s = add_bias<1>(a, bs, rel0, least, most, y.s);
-    const bool whole = j0 + 32 <= wr.least && !a.documents;
-    if (!whole) s = mask_keys(a, x, j0, kd, l, s);
-#pragma unroll
-    for (int r = 0; r < 16; ++r) dp[r] = __builtin_amdgcn_exp2f(s[r] - stat.x) * fma_acc(dp[r], stat.y, -delta);
-    if (!whole) {  // 0 times what an unseen pair holds is not always 0
-#pragma unroll
-        for (int r = 0; r < 16; ++r) dp[r] = s[r] == -INFINITY ? 0.f : dp[r];
+    f32x16 s, dp;
+    {
+        RowFragments<T, DP> fk, fv;
+        fk.read(K, r0, l), fv.read(V, r0, l);
+        order();
+        s = fk.products(q), dp = fv.products(go);
     }
-    if (ts) add_table(a, *ts, j0 - wr.first, least, most, l, dp);
-    if (cap.mode != 0) dp *= y.w;
-    weigh<T, DP>(dq, K, r0, dp, l);
+    ColumnFragments<T, DP> f;
+    f.read(K, r0, l);
+    if (KIND != kGeneral) {
+        order();
+        // p's two constants in one: 1 / sum joins the exponent
+        const float up = __builtin_amdgcn_logf(stat.y) - stat.x + (KIND == kCapped ? cap.top : 0.f);
+#pragma unroll
+        for (int r = 0; r < 16; ++r) {
+            if (KIND == kPlain) {
+                dp[r] = __builtin_amdgcn_exp2f(fma_acc(s[r], cap.c, up)) * (dp[r] - delta);
+            } else {
+                const float c = quick_r(s[r], cap.k);
+                dp[r] = __builtin_amdgcn_exp2f(fma_acc(c, -2.f * cap.top, up)) * (dp[r] - delta) *
+                        (4.f * fma_acc(-c, c, c));
+            }
+        }
+        if (j0 + 32 > wr.least) {  // 0 times what an unseen pair holds is not always 0
+#pragma unroll
+            for (int r = 0; r < 16; ++r) dp[r] = j0 + 4 * (l >> 5) + el(r) < x.lim ? dp[r] : 0.f;
+        }
+    } else {
+        settle<T>();
+        const Scores y = cap_scores<true>(cap, s);
+        const int rel0 = j0 + 4 * (l >> 5) - x.p, least = j0 - wr.last, most = j0 + 31 - wr.first;
+        s = add_bias<1>(a, bs, rel0, least, most, y.s);
+        const bool whole = j0 + 32 <= wr.least && !a.documents;
+        if (!whole) s = mask_keys(a, x, j0, kd, l, s);
+        const float d = delta * stat.y;
+#pragma unroll
+        for (int r = 0; r < 16; ++r) dp[r] = __builtin_amdgcn_exp2f(s[r] - stat.x) * fma_acc(dp[r], stat.y, -d);
+        if (!whole) {
+#pragma unroll
+            for (int r = 0; r < 16; ++r) dp[r] = s[r] == -INFINITY ? 0.f : dp[r];
+        }
+        if (ts) add_table(a, *ts, j0 - wr.first, least, most, l, dp);
+        if (cap.mode != 0) dp *= y.w;
+    }
+    order();
+    f.weigh(dq, dp);
+    settle<T>();
 }
 
-template <typename T, int DP, bool SPLIT>
-__global__ __launch_bounds__(kAttThreads, SPLIT || DP * sizeof(T) > 256 ? 1 : 2) void att_bwd_row_kernel(Att a) {
+template <typename T, int DP, bool SPLIT, Kind KIND>
+__global__ __launch_bounds__(kAttThreads, SPLIT || DP * sizeof(T) > (KIND == kGeneral ? 192 : 256) ? 1 : 2) void att_bwd_row_kernel(Att a) {
     using L = Tile<T, DP>;
     using S = BwdShape<T, DP>;
     constexpr int KT = SPLIT ? 32 : S::KT, NB = KT / 32, HALF = KT * L::ROW;
@@ -121,18 +153,18 @@ __global__ __launch_bounds__(kAttThreads, SPLIT || DP * sizeof(T) > 256 ? 1 : 2)
     __shared__ __attribute__((aligned(1024))) char tiles1[NBUF == 2 ? OWN : 1][2][NBUF == 2 ? HALF : 16];
     __shared__ __attribute__((aligned(256))) int docs0[OWN][64], docs1[OWN][64];
     extern __shared__ __attribute__((aligned(16))) float room[];  // line, then the table's sums
-    const int l = threadIdx.x & 63, wave = threadIdx.x >> 6;
+    const int l = threadIdx.x & 63, wave = wave_id();
     int bh, rest;
     place(blockIdx.x, a.B * a.Hq, bh, rest);
     const int b = bh / a.Hq, h = bh - b * a.Hq, rb = a.rblocks - 1 - rest;
     const int n = filled_keys(a, b), hk = h / a.per;
     const LaneRow x = lane_row(a, b, h, rb * ROWS + (SPLIT ? 0 : wave * 32) + (l & 31), n);
     const WaveRows wr = wave_rows(x);
-    const Cap cap = cap_of<T>(a);
-    if (a.table) stage_line<T>(a, h, room);
+    const Cap cap = cap_of<T, KIND>(a);
+    if (KIND == kGeneral && a.table) stage_line<T>(a, h, room);
     const Bias bs = lane_bias(a, h, room);
     TableSums sums{};
-    if (a.gtable) {
+    if (KIND == kGeneral && a.gtable) {
         const int n2 = 2 * a.reach + 1;
         sums.lines = room + ((n2 + 3) & ~3) + wave * kDiagonals;
         sums.out = a.bins + (((static_cast<int64_t>(h) * a.B + b) * a.rblocks + rb) * kAttWaves + wave) * n2;
@@ -140,7 +172,7 @@ __global__ __launch_bounds__(kAttThreads, SPLIT || DP * sizeof(T) > 256 ? 1 : 2)
         for (int i = l; i < n2; i += 64) sums.out[i] = 0.f;
         sums.next = -0x40000000;
     }
-    if (a.table) __syncthreads();
+    if (KIND == kGeneral && a.table) __syncthreads();
 
     const int64_t at = (static_cast<int64_t>(b) * a.Hq + h) * a.Lq + x.i;
     typename Eight<T>::V q[L::NS], go[L::NS];
@@ -165,7 +197,7 @@ __global__ __launch_bounds__(kAttThreads, SPLIT || DP * sizeof(T) > 256 ? 1 : 2)
     lv.init(SPLIT ? l : threadIdx.x, a.vs[2], a.D);
     const T* kbase = row_at<T>(a.k, a.ks, b, hk, 0);
     const T* vbase = row_at<T>(a.v, a.vs, b, hk, 0);
-    const int32_t* dbase = a.documents ? a.documents + static_cast<int64_t>(b) * a.Lk : nullptr;
+    const int32_t* dbase = KIND == kGeneral && a.documents ? a.documents + static_cast<int64_t>(b) * a.Lk : nullptr;
     auto load = [&](int t, char* tile, int* docs) {
         lk.load(tile, kbase, a.ks[2], t * KT, n, a.D, SPLIT ? 0 : wave);
         lv.load(tile + HALF, vbase, a.vs[2], t * KT, n, a.D, SPLIT ? 0 : wave);
@@ -179,9 +211,9 @@ __global__ __launch_bounds__(kAttThreads, SPLIT || DP * sizeof(T) > 256 ? 1 : 2)
     const int64_t tiles_all = (keys_end(a, b, rb * ROWS + ROWS - 1, n) + KT - 1) / KT;
     const int begin = SPLIT ? static_cast<int>(tiles_all * wave / kAttWaves) : 0;
     const int end = SPLIT ? static_cast<int>(tiles_all * (wave + 1) / kAttWaves) : static_cast<int>(tiles_all);
-    const int2 own = a.documents ? row_documents(a, b, rb * ROWS, ROWS, n) : make_int2(0, 0);
+    const int2 own = KIND == kGeneral && a.documents ? row_documents(a, b, rb * ROWS, ROWS, n) : make_int2(0, 0);
     auto wanted = [&](int t) {
-        if (!a.documents) return true;
+        if (KIND != kGeneral || !a.documents) return true;
         const int e = t * KT / kRangeKeys;
         if (e >= a.nranges) return false;
         const int2 r = a.ranges[b * a.nranges + e];
@@ -190,14 +222,16 @@ __global__ __launch_bounds__(kAttThreads, SPLIT || DP * sizeof(T) > 256 ? 1 : 2)
     Needed<decltype(wanted)> need{wanted};
     f32x16 dq[L::ND] = {};
     int t = need.next(begin, end);
-    TableSums* const ts = a.gtable ? &sums : nullptr;
+    TableSums* const ts = KIND == kGeneral && a.gtable ? &sums : nullptr;
     auto compute = [&](const char* tile, const int* docs) {
-        if (t * KT >= wr.most) return;
-#pragma unroll
+#pragma unroll 1
         for (int kb = 0; kb < NB; ++kb)
-            if (t * KT + kb * 32 < wr.most)
-                row_gradient<T, DP>(a, cap, bs, x.r, wr, q, go, stat, delta * stat.y, tile, tile + HALF, kb * 32,
-                                    docs + kb * 32, t * KT + kb * 32, l, ts, dq);
+        {
+            const int j0 = t * KT + kb * 32;
+            if (j0 >= wr.most) break;
+            row_gradient<T, DP, KIND>(a, cap, bs, x.r, wr, q, go, stat, delta, tile, tile + HALF, kb * 32,
+                                      docs + kb * 32, j0, l, ts, dq);
+        }
     };
     auto step = [&](char* tile, int* docs, char* ahead, int* docs_ahead) {
         const int tn = need.next(t + 1, end);
@@ -281,7 +315,7 @@ __global__ __launch_bounds__(kAttThreads, SPLIT || DP * sizeof(T) > 256 ? 1 : 2)
             exact_row_gradient<T>(a, b, h, __shfl(x.i, u), __shfl(delta, u));
         }
     }
-    if (!a.gtable) return;
+    if (KIND != kGeneral || !a.gtable) return;
     if (sums.next != -0x40000000) table_flush(a, sums, l);
     sums.low = wave_sum(sums.low), sums.high = wave_sum(sums.high);
     if (l == 0) {
@@ -290,21 +324,21 @@ __global__ __launch_bounds__(kAttThreads, SPLIT || DP * sizeof(T) > 256 ? 1 : 2)
     }
 }
 
-template <typename T, int DP>
+template <typename T, int DP, Kind KIND>
 __global__ __launch_bounds__(kAttThreads, DP * sizeof(T) >= 256 ? 1 : 2) void att_bwd_key_kernel(Att a) {
     using L = Tile<T, DP>;
     constexpr int QT = BwdShape<T, DP>::KT, NB = QT / 32, HALF = QT * L::ROW;
     __shared__ __attribute__((aligned(1024))) char tiles0[2][HALF];
     __shared__ __attribute__((aligned(1024))) char tiles1[2][HALF];
-    __shared__ __attribute__((aligned(256))) float info[2][5][QT];  // statistics, delta over the sum, key end, document
+    __shared__ __attribute__((aligned(256))) float info[2][6][QT];  // log 2 of weight over score, maximum, 1 / sum, delta, key end, document
     extern __shared__ float line[];
-    const int l = threadIdx.x & 63, wave = threadIdx.x >> 6, g = l >> 5;
+    const int l = threadIdx.x & 63, wave = wave_id(), g = l >> 5;
     int bg, rest;
     place(blockIdx.x, a.B * a.Hk, bg, rest);
     const int b = bg / a.Hk, hk = bg - b * a.Hk, part = rest % a.parts, kb = rest / a.parts;
     const int n = filled_keys(a, b), off = n - a.Lq;
     const int j0 = kb * 128 + wave * 32, j = j0 + (l & 31);
-    const Cap cap = cap_of<T>(a);
+    const Cap cap = cap_of<T, KIND>(a);
     const int prefix = a.prefix ? a.prefix[b] : 0;
     const int doc = a.documents && j < n ? a.documents[static_cast<int64_t>(b) * a.Lk + j] : 0;
 
@@ -328,7 +362,7 @@ __global__ __launch_bounds__(kAttThreads, DP * sizeof(T) >= 256 ? 1 : 2) void at
     const int64_t units = static_cast<int64_t>(t1 - t0) * a.per;
     const int u0 = static_cast<int>(units * part / a.parts), u1 = static_cast<int>(units * (part + 1) / a.parts);
     int2 own = make_int2(0, 0);
-    if (a.documents && jb < n) {
+    if (KIND == kGeneral && a.documents && jb < n) {
         const int e = jb / kRangeKeys;
         own = a.ranges[b * a.nranges + e];
         if (e + 1 < a.nranges) {
@@ -338,7 +372,7 @@ __global__ __launch_bounds__(kAttThreads, DP * sizeof(T) >= 256 ? 1 : 2) void at
     }
     // `t` counts the key block's units: a head's query tiles, then the next's
     auto wanted = [&](int u) {
-        if (!a.documents) return true;
+        if (KIND != kGeneral || !a.documents) return true;
         if (u >= u1) return false;
         const int i0 = (t0 + u % (t1 - t0)) * QT;
         const int p0 = max(0, i0 + off), p1 = min(n, min(a.Lq, i0 + QT) + off) - 1;
@@ -372,72 +406,138 @@ __global__ __launch_bounds__(kAttThreads, DP * sizeof(T) >= 256 ? 1 : 2) void at
         if (i < a.Lq) {
             const int64_t at = (static_cast<int64_t>(b) * a.Hq + head(u)) * a.Lq + i;
             const Row r = row_of(a, b, i, n);
-            r_stat = get_stats(a, at), r_delta = a.delta[at] * r_stat.y, r_lim = r.lim, r_doc = r.doc;
+            r_stat = get_stats(a, at), r_delta = a.delta[at], r_lim = r.lim, r_doc = r.doc;
         }
     };
     auto put = [&](int buf) {
         const int x = threadIdx.x;
         if (x >= QT) return;
-        info[buf][0][x] = r_stat.x, info[buf][1][x] = r_stat.y, info[buf][2][x] = r_delta;
-        info[buf][3][x] = __int_as_float(r_lim), info[buf][4][x] = __int_as_float(r_doc);
+        info[buf][0][x] = __builtin_amdgcn_logf(r_stat.y) - r_stat.x + (cap.mode == 1 ? cap.top : 0.f);
+        info[buf][1][x] = r_stat.x, info[buf][2][x] = r_stat.y, info[buf][3][x] = r_delta;
+        info[buf][4][x] = __int_as_float(r_lim), info[buf][5][x] = __int_as_float(r_doc);
     };
     f32x16 dk[L::ND] = {}, dv[L::ND] = {};
     int u = need.next(u0, u1), staged = -1;
     Bias bs{0.f, line};
-    auto compute = [&](const char* tile, int buf) {
-        const int i0 = first(u), p0 = i0 + off;
-#pragma unroll 1
-        for (int qb = 0; qb < NB; ++qb) {
-            const int pf = p0 + qb * 32, ends = min(a.Lq - i0 - qb * 32, 32);
-            if (ends <= 0) break;
-            // the rows' key ends rise with their position
-            const int least = a.causal ? min(n, max(pf + 1, prefix)) : n;
-            const int most = a.causal ? min(n, max(pf + ends, prefix)) : n;
-            if (j0 >= most) continue;
-            const bool whole = j0 + 32 <= least && !a.documents;
-            const Scores y = cap_scores<true>(cap, products<T, DP>(tile, qb * 32, k, l));
-            f32x16 dp = products<T, DP>(tile + HALF, qb * 32, v, l);
-            f32x16 s = add_bias<-1>(a, bs, j - pf - 4 * g, j0 - pf - 31, j0 + 31 - pf, y.s);
-            if (!whole) {
-#pragma unroll
-                for (int c = 0; c < 4; ++c) {
-                    const i32x4 m = *reinterpret_cast<const i32x4*>(&info[buf][3][qb * 32 + 8 * c + 4 * g]);
-#pragma unroll
-                    for (int e = 0; e < 4; ++e) s[4 * c + e] = j < m[e] ? s[4 * c + e] : -INFINITY;
-                }
-                if (a.documents) {
-#pragma unroll
-                    for (int c = 0; c < 4; ++c) {
-                        const i32x4 d = *reinterpret_cast<const i32x4*>(&info[buf][4][qb * 32 + 8 * c + 4 * g]);
-#pragma unroll
-                        for (int e = 0; e < 4; ++e) s[4 * c + e] = d[e] == doc ? s[4 * c + e] : -INFINITY;
-                    }
-                }
-            }
+    // one 32-row part of a tile, whatever it holds
+    auto general = [&](const char* tile, int buf, int qb, int pf, bool whole) {
+        const float* rows = &info[buf][0][qb * 32 + 4 * g];
+        RowFragments<T, DP> fq, fg;
+        fq.read(tile, qb * 32, l), fg.read(tile + HALF, qb * 32, l);
+        order();
+        const f32x16 xs = fq.products(k);
+        f32x16 dp = fg.products(v);
+        settle<T>();
+        const Scores y = cap_scores<true>(cap, xs);
+        f32x16 s = add_bias<-1>(a, bs, j - pf - 4 * g, j0 - pf - 31, j0 + 31 - pf, y.s);
+        if (!whole) {
 #pragma unroll
             for (int c = 0; c < 4; ++c) {
-                const f32x4 top = *reinterpret_cast<const f32x4*>(&info[buf][0][qb * 32 + 8 * c + 4 * g]);
-                const f32x4 inv = *reinterpret_cast<const f32x4*>(&info[buf][1][qb * 32 + 8 * c + 4 * g]);
-                const f32x4 del = *reinterpret_cast<const f32x4*>(&info[buf][2][qb * 32 + 8 * c + 4 * g]);
+                const i32x4 m = *reinterpret_cast<const i32x4*>(rows + 4 * QT + 8 * c);
+#pragma unroll
+                for (int e = 0; e < 4; ++e) s[4 * c + e] = j < m[e] ? s[4 * c + e] : -INFINITY;
+            }
+            if (a.documents) {
+#pragma unroll
+                for (int c = 0; c < 4; ++c) {
+                    const i32x4 d = *reinterpret_cast<const i32x4*>(rows + 5 * QT + 8 * c);
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) s[4 * c + e] = d[e] == doc ? s[4 * c + e] : -INFINITY;
+                }
+            }
+        }
+#pragma unroll
+        for (int c = 0; c < 4; ++c) {
+            const f32x4 top = *reinterpret_cast<const f32x4*>(rows + QT + 8 * c);
+            const f32x4 inv = *reinterpret_cast<const f32x4*>(rows + 2 * QT + 8 * c);
+            const f32x4 del = *reinterpret_cast<const f32x4*>(rows + 3 * QT + 8 * c);
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+                const int r = 4 * c + e;
+                const float w = __builtin_amdgcn_exp2f(s[r] - top[e]) * inv[e];
+                float x = w * (dp[r] - del[e]);
+                if (cap.mode != 0) x *= y.w[r];
+                dp[r] = !whole && s[r] == -INFINITY ? 0.f : x;
+                s[r] = w;
+            }
+        }
+        order();
+        ColumnFragments<T, DP> f;
+        f.read(tile + HALF, qb * 32, l);
+        f.weigh(dv, s);
+        f.read(tile, qb * 32, l);
+        f.weigh(dk, dp);
+        settle<T>();
+    };
+    // the weights p (in place of the products s) and dx, of a part that the
+    // wave's keys see whole, without a bias
+    auto weights = [&](int buf, int qb, bool whole, f32x16& s, f32x16& dp) {
+        const float* rows = &info[buf][0][qb * 32 + 4 * g];
+        f32x16 w = s, x = dp;
+#pragma unroll
+        for (int c = 0; c < 4; ++c) {
+            const f32x4 up = *reinterpret_cast<const f32x4*>(rows + 8 * c);
+            const f32x4 del = *reinterpret_cast<const f32x4*>(rows + 3 * QT + 8 * c);
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+                const int r = 4 * c + e;
+                if constexpr (KIND == kPlain) {
+                    w[r] = __builtin_amdgcn_exp2f(fma_acc(w[r], cap.c, up[e]));
+                    x[r] = w[r] * (x[r] - del[e]);
+                } else {
+                    const float q = quick_r(w[r], cap.k);
+                    w[r] = __builtin_amdgcn_exp2f(fma_acc(q, -2.f * cap.top, up[e]));
+                    x[r] = w[r] * (x[r] - del[e]) * (4.f * fma_acc(-q, q, q));
+                }
+            }
+        }
+        if (!whole) {
+#pragma unroll
+            for (int c = 0; c < 4; ++c) {
+                const i32x4 lim = *reinterpret_cast<const i32x4*>(rows + 4 * QT + 8 * c);
 #pragma unroll
                 for (int e = 0; e < 4; ++e) {
                     const int r = 4 * c + e;
-                    const float p = __builtin_amdgcn_exp2f(s[r] - top[e]);
-                    float x = p * fma_acc(dp[r], inv[e], -del[e]);
-                    if (cap.mode != 0) x *= y.w[r];
-                    dp[r] = !whole && s[r] == -INFINITY ? 0.f : x;
-                    s[r] = p * inv[e];
+                    w[r] = j < lim[e] ? w[r] : 0.f, x[r] = j < lim[e] ? x[r] : 0.f;
                 }
             }
-            weigh<T, DP>(dv, tile + HALF, qb * 32, s, l);
-            weigh<T, DP>(dk, tile, qb * 32, dp, l);
+        }
+        s = w, dp = x;
+    };
+    auto simple = [&](const char* tile, int buf, int qb, bool whole) {
+        RowFragments<T, DP> fq, fg;
+        fq.read(tile, qb * 32, l), fg.read(tile + HALF, qb * 32, l);
+        order();
+        f32x16 s = fq.products(k), dp = fg.products(v);
+        ColumnFragments<T, DP> cg, cq;
+        cg.read(tile + HALF, qb * 32, l);
+        order();
+        weights(buf, qb, whole, s, dp);
+        cq.read(tile, qb * 32, l);
+        order();
+        cg.weigh(dv, s);
+        cq.weigh(dk, dp);
+        settle<T>();
+    };
+    auto compute = [&](const char* tile, int buf) {
+        const int i0 = first(u), p0 = i0 + off;
+        // the rows' key ends rise with their position
+        auto ends = [&](int p) { return a.causal ? min(n, max(p + 1, prefix)) : n; };
+#pragma unroll 1
+        for (int qb = 0; qb < NB; ++qb) {
+            const int pf = p0 + qb * 32, count = min(a.Lq - i0 - qb * 32, 32);
+            if (count <= 0) break;
+            if (j0 >= ends(pf + count - 1)) continue;
+            const bool whole = j0 + 32 <= ends(pf) && !a.documents;
+            if constexpr (KIND == kGeneral) general(tile, buf, qb, pf, whole);
+            else simple(tile, buf, qb, whole);
         }
     };
     auto step = [&](char* tile, char* ahead, int buf) {
         const int un = need.next(u + 1, u1);
-        if ((a.table || a.slopes) && head(u) != staged) {
+        if (KIND == kGeneral && (a.table || a.slopes) && head(u) != staged) {
             staged = head(u);
-            if (a.table) {
+            if (KIND == kGeneral && a.table) {
                 __syncthreads();
                 stage_line<T>(a, staged, line);
             }
@@ -531,16 +631,25 @@ __global__ __launch_bounds__(kAttThreads) void att_bwd_join_kernel(Att a) {
     if (__any(bad != 0.f)) exact_key_gradient<T>(a, b, hk, j);
 }
 
-template <typename T, int DP>
-static void backward_width(const Att& a, hipStream_t st) {
+template <typename T, int DP, Kind KIND>
+static void backward_kind(const Att& a, hipStream_t st) {
     const unsigned line = a.table ? ((2 * a.reach + 4) & ~3) * 4 : 0;
     const int64_t rows = static_cast<int64_t>(a.B) * a.Hq * a.rblocks;
     if (a.splits)
-        att_bwd_row_kernel<T, DP, true><<<static_cast<unsigned>(rows), kAttThreads, attention_row_lds(a), st>>>(a);
+        att_bwd_row_kernel<T, DP, true, KIND><<<static_cast<unsigned>(rows), kAttThreads, attention_row_lds(a), st>>>(a);
     else
-        att_bwd_row_kernel<T, DP, false><<<static_cast<unsigned>(rows), kAttThreads, attention_row_lds(a), st>>>(a);
+        att_bwd_row_kernel<T, DP, false, KIND><<<static_cast<unsigned>(rows), kAttThreads, attention_row_lds(a), st>>>(a);
     const int64_t keys = static_cast<int64_t>(a.B) * a.Hk * a.kblocks * a.parts;
-    att_bwd_key_kernel<T, DP><<<static_cast<unsigned>(keys), kAttThreads, line, st>>>(a);
+    att_bwd_key_kernel<T, DP, KIND><<<static_cast<unsigned>(keys), kAttThreads, line, st>>>(a);
+}
+
+template <typename T, int DP>
+static void backward_width(const Att& a, hipStream_t st) {
+    const Kind kind = kind_of<T>(a);
+    if constexpr (sizeof(T) == 2)  // fp32 has no quick cap
+        if (kind == kCapped) return backward_kind<T, DP, kCapped>(a, st);
+    if (kind == kPlain) backward_kind<T, DP, kPlain>(a, st);
+    else backward_kind<T, DP, kGeneral>(a, st);
 }
 
 template <typename T>

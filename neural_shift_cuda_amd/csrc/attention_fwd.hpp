@@ -26,20 +26,34 @@ struct Running {
 // weights then reach 2^8 and the sums' rescaling is skipped.
 constexpr float kLazy = 8.f;
 
-template <typename T, int DP, int NB>
+template <typename T, int DP, int NB, Kind KIND>
 __device__ __forceinline__ void attend(const Att& a, const Cap& cap, const Bias& bs, const Row& x,
                                        const WaveRows& wr, const typename Eight<T>::V (&q)[DP / 16],
                                        const char* K, const char* V, const int* kd, int j0, int l,
                                        Running<DP / 32>& st) {
     f32x16 s[NB];
+    {
+        RowFragments<T, DP> f[NB];
 #pragma unroll
-    for (int kb = 0; kb < NB; ++kb) s[kb] = products<T, DP>(K, kb * 32, q, l);
-    const bool whole = j0 + NB * 32 <= wr.least && !a.documents;
-    const bool plain = whole && !a.slopes && !a.table && cap.mode != 2;
-    float c = 1.f;  // s * c are the scores
-    if (plain) {
-        c = cap.mode == 0 ? cap.c : 1.f;  // with a cap: formed below, from the raw maximum
+        for (int kb = 0; kb < NB; ++kb) f[kb].read(K, kb * 32, l);
+        order();
+#pragma unroll
+        for (int kb = 0; kb < NB; ++kb) s[kb] = f[kb].products(q);
+    }
+    ColumnFragments<T, DP> f;
+    const bool whole = j0 + NB * 32 <= wr.least && !(KIND == kGeneral && a.documents);
+    if (KIND != kGeneral) {
+        f.read(V, 0, l);
+        settle<T>();
+        if (!whole) {
+#pragma unroll
+            for (int kb = 0; kb < NB; ++kb)
+#pragma unroll
+                for (int r = 0; r < 16; ++r)
+                    s[kb][r] = j0 + kb * 32 + 4 * (l >> 5) + el(r) < x.lim ? s[kb][r] : -INFINITY;
+        }
     } else {
+        settle<T>();
 #pragma unroll
         for (int kb = 0; kb < NB; ++kb) {
             s[kb] = cap_scores<false>(cap, s[kb]).s;
@@ -54,8 +68,10 @@ __device__ __forceinline__ void attend(const Att& a, const Cap& cap, const Bias&
 #pragma unroll
         for (int r = 0; r < 16; ++r) top = fmaxf(top, s[kb][r]);
     top = halves_max(top);
-    const bool quick = plain && cap.mode == 1;
-    top = quick ? fma_acc(quick_r(top, cap.k), -2.f * cap.top, cap.top) : top * c;
+    // the maximum so far is of raw products
+    if (KIND == kPlain) top *= cap.c;
+    if (KIND == kCapped)
+        top = top == -INFINITY ? top : fma_acc(quick_r(top, cap.k), -2.f * cap.top, cap.top);
     const bool grow = top > st.m + kLazy;
     if (__any(grow)) {
         const float keep = grow ? __builtin_amdgcn_exp2f(st.m - top) : 1.f;
@@ -65,18 +81,22 @@ __device__ __forceinline__ void attend(const Att& a, const Cap& cap, const Bias&
         for (int d = 0; d < DP / 32; ++d) st.o[d] *= keep;
     }
     const float m = st.m == -INFINITY ? 0.f : st.m;
-    if (quick) {
-        const float up = cap.top - m;
+    const float up = cap.top - m;
+#pragma unroll
+    for (int kb = 0; kb < NB; ++kb)
+#pragma unroll
+        for (int r = 0; r < 16; ++r) {
+            const float y = KIND == kPlain    ? fma_acc(s[kb][r], cap.c, -m)
+                            : KIND == kCapped ? fma_acc(quick_r(s[kb][r], cap.k), -2.f * cap.top, up)
+                                              : s[kb][r] - m;
+            s[kb][r] = __builtin_amdgcn_exp2f(y);
+        }
+    if (KIND == kCapped && !whole) {  // the cap of -inf is finite
 #pragma unroll
         for (int kb = 0; kb < NB; ++kb)
 #pragma unroll
             for (int r = 0; r < 16; ++r)
-                s[kb][r] = __builtin_amdgcn_exp2f(fma_acc(quick_r(s[kb][r], cap.k), -2.f * cap.top, up));
-    } else {
-#pragma unroll
-        for (int kb = 0; kb < NB; ++kb)
-#pragma unroll
-            for (int r = 0; r < 16; ++r) s[kb][r] = __builtin_amdgcn_exp2f(fma_acc(s[kb][r], c, -m));
+                s[kb][r] = j0 + kb * 32 + 4 * (l >> 5) + el(r) < x.lim ? s[kb][r] : 0.f;
     }
     float z0 = 0.f, z1 = 0.f;
 #pragma unroll
@@ -84,8 +104,17 @@ __device__ __forceinline__ void attend(const Att& a, const Cap& cap, const Bias&
 #pragma unroll
         for (int r = 0; r < 16; r += 2) z0 += s[kb][r], z1 += s[kb][r + 1];
     st.z += z0 + z1;
+    order();
+    if (KIND == kGeneral) f.read(V, 0, l);
 #pragma unroll
-    for (int kb = 0; kb < NB; ++kb) weigh<T, DP>(st.o, V, kb * 32, s[kb], l);
+    for (int kb = 0; kb < NB; ++kb) {
+        ColumnFragments<T, DP> ahead;
+        if (kb + 1 < NB) ahead.read(V, kb * 32 + 32, l);
+        f.weigh(st.o, s[kb]);
+        order();
+        if (kb + 1 < NB) f = ahead;
+    }
+    settle<T>();
 }
 
 // Rows whose result is no number are computed again pair by pair.
@@ -114,7 +143,7 @@ struct FwdShape {
     static constexpr int kOwn = kAttWaves * NBUF * 2 * 32 * L::ROW;
 };
 
-template <typename T, int DP>
+template <typename T, int DP, Kind KIND>
 __global__ __launch_bounds__(kAttThreads, DP * sizeof(T) > 384 ? 1 : 2) void att_fwd_kernel(Att a) {
     using S = FwdShape<T, DP>;
     using L = Tile<T, DP>;
@@ -125,7 +154,7 @@ __global__ __launch_bounds__(kAttThreads, DP * sizeof(T) > 384 ? 1 : 2) void att
     __shared__ __attribute__((aligned(1024))) char tiles1[2][HALF];
     __shared__ __attribute__((aligned(256))) int docs0[64], docs1[64];
     extern __shared__ float line[];
-    const int l = threadIdx.x & 63, wave = threadIdx.x >> 6;
+    const int l = threadIdx.x & 63, wave = wave_id();
     const int G = a.Hq / a.pack;
     int bg, rest;
     place(blockIdx.x, a.B * G, bg, rest);
@@ -133,8 +162,8 @@ __global__ __launch_bounds__(kAttThreads, DP * sizeof(T) > 384 ? 1 : 2) void att
     const int n = filled_keys(a, b), hk = group * a.pack / a.per;
     const LaneRow x = lane_row(a, b, group, rb * 128 + wave * 32 + (l & 31), n);
     const WaveRows wr = wave_rows(x);
-    const Cap cap = cap_of<T>(a);
-    if (a.table) stage_line<T>(a, group, line);  // read after the first barrier
+    const Cap cap = cap_of<T, KIND>(a);
+    if (KIND == kGeneral && a.table) stage_line<T>(a, group, line);  // read after the first barrier
     const Bias bs = lane_bias(a, x.h, line);
     typename Eight<T>::V q[L::NS];
     load_row<T, DP>(q, row_at<T>(a.q, a.qs, b, x.h, x.i), a.D, l);
@@ -146,7 +175,7 @@ __global__ __launch_bounds__(kAttThreads, DP * sizeof(T) > 384 ? 1 : 2) void att
     lv.init(threadIdx.x, a.vs[2], a.D);
     const T* kbase = row_at<T>(a.k, a.ks, b, hk, 0);
     const T* vbase = row_at<T>(a.v, a.vs, b, hk, 0);
-    const int32_t* dbase = a.documents ? a.documents + static_cast<int64_t>(b) * a.Lk : nullptr;
+    const int32_t* dbase = KIND == kGeneral && a.documents ? a.documents + static_cast<int64_t>(b) * a.Lk : nullptr;
     auto load = [&](int t, char (&tiles)[2][HALF], int (&docs)[64]) {
         lk.load(tiles[0], kbase, a.ks[2], t * KT, n, a.D, wave);
         lv.load(tiles[1], vbase, a.vs[2], t * KT, n, a.D, wave);
@@ -158,9 +187,9 @@ __global__ __launch_bounds__(kAttThreads, DP * sizeof(T) > 384 ? 1 : 2) void att
         }
     };
     const int end = (keys_end(a, b, rb * 128 + 127, n) + KT - 1) / KT;
-    const int2 own = a.documents ? row_documents(a, b, rb * 128, 128, n) : make_int2(0, 0);
+    const int2 own = KIND == kGeneral && a.documents ? row_documents(a, b, rb * 128, 128, n) : make_int2(0, 0);
     auto wanted = [&](int t) {
-        if (!a.documents) return true;
+        if (KIND != kGeneral || !a.documents) return true;
         const int e = t * KT / kRangeKeys;
         if (e >= a.nranges) return false;
         const int2 r = a.ranges[b * a.nranges + e];
@@ -176,7 +205,7 @@ __global__ __launch_bounds__(kAttThreads, DP * sizeof(T) > 384 ? 1 : 2) void att
         __syncthreads();
         if (tn < end) load(tn, ahead, docs_ahead);
         if (t * KT < wr.most)
-            attend<T, DP, NB>(a, cap, bs, x.r, wr, q, tiles[0], tiles[1], docs, t * KT, l, st);
+            attend<T, DP, NB, KIND>(a, cap, bs, x.r, wr, q, tiles[0], tiles[1], docs, t * KT, l, st);
         t = tn;
     };
     if (t < end) load(t, tiles0, docs0);
@@ -204,7 +233,7 @@ __global__ __launch_bounds__(kAttThreads, DP * sizeof(T) > 384 ? 1 : 2) void att
 }
 
 // The waves split the keys.
-template <typename T, int DP>
+template <typename T, int DP, Kind KIND>
 __global__ __launch_bounds__(kAttThreads, 1) void att_fwd_split_kernel(Att a) {
     using S = FwdShape<T, DP>;
     using L = Tile<T, DP>;
@@ -215,7 +244,7 @@ __global__ __launch_bounds__(kAttThreads, 1) void att_fwd_split_kernel(Att a) {
     __shared__ float stat[kAttWaves][2][32];
     extern __shared__ float line[];
     static_assert(sizeof(tiles0) >= kAttWaves * 32 * DP * 4, "the waves' sums take the tiles' place");
-    const int l = threadIdx.x & 63, wave = threadIdx.x >> 6;
+    const int l = threadIdx.x & 63, wave = wave_id();
     const int G = a.Hq / a.pack;
     int bg, rest;
     place(blockIdx.x, a.B * G, bg, rest);
@@ -223,8 +252,8 @@ __global__ __launch_bounds__(kAttThreads, 1) void att_fwd_split_kernel(Att a) {
     const int n = filled_keys(a, b), hk = group * a.pack / a.per;
     const LaneRow x = lane_row(a, b, group, rb * 32 + (l & 31), n);
     const WaveRows wr = wave_rows(x);
-    const Cap cap = cap_of<T>(a);
-    if (a.table) {
+    const Cap cap = cap_of<T, KIND>(a);
+    if (KIND == kGeneral && a.table) {
         stage_line<T>(a, group, line);
         __syncthreads();
     }
@@ -235,7 +264,7 @@ __global__ __launch_bounds__(kAttThreads, 1) void att_fwd_split_kernel(Att a) {
     lv.init(l, a.vs[2], a.D);
     const T* kbase = row_at<T>(a.k, a.ks, b, hk, 0);
     const T* vbase = row_at<T>(a.v, a.vs, b, hk, 0);
-    const int32_t* dbase = a.documents ? a.documents + static_cast<int64_t>(b) * a.Lk : nullptr;
+    const int32_t* dbase = KIND == kGeneral && a.documents ? a.documents + static_cast<int64_t>(b) * a.Lk : nullptr;
     auto load = [&](int t, char* tile, int* docs) {
         lk.load(tile, kbase, a.ks[2], t * 32, n, a.D, 0);
         lv.load(tile + HALF, vbase, a.vs[2], t * 32, n, a.D, 0);
@@ -249,9 +278,9 @@ __global__ __launch_bounds__(kAttThreads, 1) void att_fwd_split_kernel(Att a) {
     const int64_t tiles_all = (keys_end(a, b, rb * 32 + 31, n) + 31) / 32;
     const int unit = split * kAttWaves + wave, units = a.splits * kAttWaves;
     const int begin = static_cast<int>(tiles_all * unit / units), end = static_cast<int>(tiles_all * (unit + 1) / units);
-    const int2 own = a.documents ? row_documents(a, b, rb * 32, 32, n) : make_int2(0, 0);
+    const int2 own = KIND == kGeneral && a.documents ? row_documents(a, b, rb * 32, 32, n) : make_int2(0, 0);
     auto wanted = [&](int t) {
-        if (!a.documents) return true;
+        if (KIND != kGeneral || !a.documents) return true;
         const int e = t * 32 / kRangeKeys;
         if (e >= a.nranges) return false;
         const int2 r = a.ranges[b * a.nranges + e];
@@ -270,7 +299,7 @@ __global__ __launch_bounds__(kAttThreads, 1) void att_fwd_split_kernel(Att a) {
         const int tn = need.next(t + 1, end);
         __builtin_amdgcn_s_waitcnt(0x0f70);  // vmcnt(0): the tile has landed
         if (S::NBUF == 2 && tn < end) load(tn, ahead, docs_ahead);
-        attend<T, DP, 1>(a, cap, bs, x.r, wr, q, tile, tile + HALF, docs, t * 32, l, st);
+        attend<T, DP, 1, KIND>(a, cap, bs, x.r, wr, q, tile, tile + HALF, docs, t * 32, l, st);
         if (S::NBUF == 1 && tn < end) {
             __builtin_amdgcn_s_waitcnt(0xc07f);  // lgkmcnt(0): the tile has been read
             load(tn, tile, docs);
@@ -376,14 +405,23 @@ __global__ __launch_bounds__(kAttThreads) void att_join_kernel(Att a) {
     if (__any(bad != 0.f)) exact_row<T>(a, b, h, i);
 }
 
-template <typename T, int DP>
-static void forward_width(const Att& a, hipStream_t st) {
+template <typename T, int DP, Kind KIND>
+static void forward_kind(const Att& a, hipStream_t st) {
     const unsigned lds = a.table ? (2 * a.reach + 1) * 4 : 0;
     const int64_t blocks = static_cast<int64_t>(a.B) * (a.Hq / a.pack) * a.rblocks;
     if (a.splits == 0)
-        att_fwd_kernel<T, DP><<<static_cast<unsigned>(blocks), kAttThreads, lds, st>>>(a);
+        att_fwd_kernel<T, DP, KIND><<<static_cast<unsigned>(blocks), kAttThreads, lds, st>>>(a);
     else
-        att_fwd_split_kernel<T, DP><<<static_cast<unsigned>(blocks * a.splits), kAttThreads, lds, st>>>(a);
+        att_fwd_split_kernel<T, DP, KIND><<<static_cast<unsigned>(blocks * a.splits), kAttThreads, lds, st>>>(a);
+}
+
+template <typename T, int DP>
+static void forward_width(const Att& a, hipStream_t st) {
+    const Kind kind = kind_of<T>(a);
+    if constexpr (sizeof(T) == 2)  // fp32 has no quick cap
+        if (kind == kCapped) return forward_kind<T, DP, kCapped>(a, st);
+    if (kind == kPlain) forward_kind<T, DP, kPlain>(a, st);
+    else forward_kind<T, DP, kGeneral>(a, st);
 }
 
 template <typename T>

@@ -199,36 +199,70 @@ __device__ __forceinline__ void load_row(typename Eight<T>::V (&v)[DP / 16], con
     }
 }
 
-// Products of 32 tile rows from r0 with the lane's row.
-template <typename T, int DP>
-__device__ __forceinline__ f32x16 products(const char* lds, int r0, const typename Eight<T>::V (&v)[DP / 16],
-                                           int l) {
-    f32x16 c = {};
-#pragma unroll
-    for (int s = 0; s < DP / 16; ++s) c = Eight<T>::mma(Tile<T, DP>::row(lds, r0, s, l), v[s], c);
-    return c;
+// Reads from LDS take some hundred cycles.  They go out together, ahead of the
+// products that use them; order() keeps the compiler from moving them back to
+// their uses, one read and one wait at a time.
+__device__ __forceinline__ void order() { __builtin_amdgcn_sched_barrier(0); }
+
+// Ends a run of products ahead of a branch.  Their results may be read 12 wait
+// states (18 for the fp32 products) after the last one at the earliest, and the
+// hardware does not wait by itself; the compiler counts the states, but has
+// been seen to miss a read in another block (a copy of the sums behind a loop's
+// exit took their last two rows too early).
+template <typename T>
+__device__ __forceinline__ void settle() {
+    order();
+    if constexpr (sizeof(T) == 4)
+        asm volatile("s_nop 15\n\ts_nop 1");
+    else
+        asm volatile("s_nop 11");
+    order();
 }
 
-// acc[db] += (32 tile rows from r0, by columns) x weights w.
+__device__ __forceinline__ int wave_id() { return __builtin_amdgcn_readfirstlane(threadIdx.x >> 6); }
+
+// Kinds of call, each with kernels of its own: no bias and no documents, without
+// a cap (kPlain) or with the quick one (kCapped), whose tiles take no branch; or
+// whatever a call may hold (kGeneral), at a cost in registers.
+enum Kind { kPlain, kCapped, kGeneral };
+
 template <typename T, int DP>
-__device__ __forceinline__ void weigh(f32x16 (&acc)[DP / 32], const char* lds, int r0, const f32x16& w, int l) {
-    const typename Eight<T>::V lo = Eight<T>::pack(__builtin_shufflevector(w, w, 0, 1, 2, 3, 4, 5, 6, 7));
-    const typename Eight<T>::V hi = Eight<T>::pack(__builtin_shufflevector(w, w, 8, 9, 10, 11, 12, 13, 14, 15));
+struct RowFragments {  // 32 tile rows from r0
+    typename Eight<T>::V f[DP / 16];
+    __device__ __forceinline__ void read(const char* lds, int r0, int l) {
 #pragma unroll
-    for (int db = 0; db < DP / 32; ++db) {
-        acc[db] = Eight<T>::mma(Tile<T, DP>::col(lds, r0, db, l), lo, acc[db]);
-        acc[db] = Eight<T>::mma(Tile<T, DP>::col(lds, r0 + 16, db, l), hi, acc[db]);
+        for (int s = 0; s < DP / 16; ++s) f[s] = Tile<T, DP>::row(lds, r0, s, l);
     }
-}
+    // their products with the lane's row
+    __device__ __forceinline__ f32x16 products(const typename Eight<T>::V (&v)[DP / 16]) const {
+        f32x16 c = {};
+#pragma unroll
+        for (int s = 0; s < DP / 16; ++s) c = Eight<T>::mma(f[s], v[s], c);
+        return c;
+    }
+};
+
+template <typename T, int DP>
+struct ColumnFragments {  // 32 tile rows from r0, by columns
+    typename Eight<T>::V f[DP / 32][2];
+    __device__ __forceinline__ void read(const char* lds, int r0, int l) {
+#pragma unroll
+        for (int d = 0; d < DP / 32; ++d) f[d][0] = Tile<T, DP>::col(lds, r0, d, l), f[d][1] = Tile<T, DP>::col(lds, r0 + 16, d, l);
+    }
+    // acc += their columns times the weights w
+    __device__ __forceinline__ void weigh(f32x16 (&acc)[DP / 32], const f32x16& w) const {
+        const typename Eight<T>::V lo = Eight<T>::pack(__builtin_shufflevector(w, w, 0, 1, 2, 3, 4, 5, 6, 7));
+        const typename Eight<T>::V hi = Eight<T>::pack(__builtin_shufflevector(w, w, 8, 9, 10, 11, 12, 13, 14, 15));
+#pragma unroll
+        for (int d = 0; d < DP / 32; ++d) acc[d] = Eight<T>::mma(f[d][0], lo, acc[d]);
+#pragma unroll
+        for (int d = 0; d < DP / 32; ++d) acc[d] = Eight<T>::mma(f[d][1], hi, acc[d]);
+    }
+};
 
 // ---------------------------------------------------------------------------
 // Scores, in units of log 2.
 // ---------------------------------------------------------------------------
-
-// cap * tanh(x |scale| / cap) is 1 - 2 / (1 + exp) in three cheap steps, off by
-// some 2^-22 of the cap; with fp32 results, or a cap above 256 (2^-14, where a
-// 16-bit weight's half step is 2^-12), small arguments take the series.
-constexpr float kQuickCap = 256.f;
 
 struct Cap {
     int mode;      // 0: none, 1: quick, 2: accurate
@@ -239,10 +273,16 @@ struct Cap {
 };
 
 template <typename T>
+inline Kind kind_of(const Att& a) {
+    if (a.slopes || a.table || a.documents) return kGeneral;
+    return a.cap <= 0.f ? kPlain : sizeof(T) == 2 && a.cap <= kQuickCap ? kCapped : kGeneral;
+}
+
+template <typename T, Kind KIND>
 __device__ __forceinline__ Cap cap_of(const Att& a) {
     Cap c;
     const float s = fabsf(a.scale);
-    c.mode = a.cap <= 0.f ? 0 : (sizeof(T) == 4 || a.cap > kQuickCap) ? 2 : 1;
+    c.mode = KIND == kPlain ? 0 : KIND == kCapped ? 1 : a.cap <= 0.f ? 0 : sizeof(T) == 2 && a.cap <= kQuickCap ? 1 : 2;
     c.c = s * kLog2e;
     c.inv = a.cap > 0.f ? s / a.cap : 0.f;
     c.k = 2.f * kLog2e * c.inv;
