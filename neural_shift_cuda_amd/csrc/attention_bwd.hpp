@@ -469,40 +469,44 @@ __global__ __launch_bounds__(kAttThreads, DP * sizeof(T) >= 256 ? 1 : 2) void at
         f.weigh(dk, dp);
         settle<T>();
     };
-    // the weights p (in place of the products s) and dx, of a part that the
-    // wave's keys see whole, without a bias
-    auto weights = [&](int buf, int qb, bool whole, f32x16& s, f32x16& dp) {
+    // The weights p (in place of the products s) and dx, without a bias.
+    struct RowInfo {
+        f32x4 up[4], del[4];
+    };
+    auto row_info = [&](int buf, int qb) {
         const float* rows = &info[buf][0][qb * 32 + 4 * g];
-        f32x16 w = s, x = dp;
+        RowInfo x;
 #pragma unroll
         for (int c = 0; c < 4; ++c) {
-            const f32x4 up = *reinterpret_cast<const f32x4*>(rows + 8 * c);
-            const f32x4 del = *reinterpret_cast<const f32x4*>(rows + 3 * QT + 8 * c);
+            x.up[c] = *reinterpret_cast<const f32x4*>(rows + 8 * c);
+            x.del[c] = *reinterpret_cast<const f32x4*>(rows + 3 * QT + 8 * c);
+        }
+        return x;
+    };
+    auto weights = [&](const RowInfo& x, f32x16& s, f32x16& dp) {
+#pragma unroll
+        for (int r = 0; r < 16; ++r) {
+            if constexpr (KIND == kPlain) {
+                s[r] = __builtin_amdgcn_exp2f(fma_acc(s[r], cap.c, x.up[r / 4][r % 4]));
+                dp[r] = s[r] * (dp[r] - x.del[r / 4][r % 4]);
+            } else {
+                const float q = quick_r(s[r], cap.k);
+                s[r] = __builtin_amdgcn_exp2f(fma_acc(q, -2.f * cap.top, x.up[r / 4][r % 4]));
+                dp[r] = s[r] * (dp[r] - x.del[r / 4][r % 4]) * (4.f * fma_acc(-q, q, q));
+            }
+        }
+    };
+    auto unsee = [&](int buf, int qb, f32x16& s, f32x16& dp) {
+        const float* rows = &info[buf][4][qb * 32 + 4 * g];
+#pragma unroll
+        for (int c = 0; c < 4; ++c) {
+            const i32x4 lim = *reinterpret_cast<const i32x4*>(rows + 8 * c);
 #pragma unroll
             for (int e = 0; e < 4; ++e) {
                 const int r = 4 * c + e;
-                if constexpr (KIND == kPlain) {
-                    w[r] = __builtin_amdgcn_exp2f(fma_acc(w[r], cap.c, up[e]));
-                    x[r] = w[r] * (x[r] - del[e]);
-                } else {
-                    const float q = quick_r(w[r], cap.k);
-                    w[r] = __builtin_amdgcn_exp2f(fma_acc(q, -2.f * cap.top, up[e]));
-                    x[r] = w[r] * (x[r] - del[e]) * (4.f * fma_acc(-q, q, q));
-                }
+                s[r] = j < lim[e] ? s[r] : 0.f, dp[r] = j < lim[e] ? dp[r] : 0.f;
             }
         }
-        if (!whole) {
-#pragma unroll
-            for (int c = 0; c < 4; ++c) {
-                const i32x4 lim = *reinterpret_cast<const i32x4*>(rows + 4 * QT + 8 * c);
-#pragma unroll
-                for (int e = 0; e < 4; ++e) {
-                    const int r = 4 * c + e;
-                    w[r] = j < lim[e] ? w[r] : 0.f, x[r] = j < lim[e] ? x[r] : 0.f;
-                }
-            }
-        }
-        s = w, dp = x;
     };
     auto simple = [&](const char* tile, int buf, int qb, bool whole) {
         RowFragments<T, DP> fq, fg;
@@ -511,26 +515,65 @@ __global__ __launch_bounds__(kAttThreads, DP * sizeof(T) >= 256 ? 1 : 2) void at
         f32x16 s = fq.products(k), dp = fg.products(v);
         ColumnFragments<T, DP> cg, cq;
         cg.read(tile + HALF, qb * 32, l);
-        order();
-        weights(buf, qb, whole, s, dp);
+        const RowInfo x = row_info(buf, qb);
+        settle<T>();
+        weights(x, s, dp);
+        if (!whole) unsee(buf, qb, s, dp);
         cq.read(tile, qb * 32, l);
         order();
         cg.weigh(dv, s);
         cq.weigh(dk, dp);
         settle<T>();
     };
+    // Both parts of a 64-row tile: one part's products run under the other's
+    // weights.  (One path for all tiles, with the masks in branches of their
+    // own: where the sums were updated on several, they were copied each time.)
+    auto both = [&](const char* tile, int buf, bool whole0, bool whole1) {
+        constexpr int V = KIND == kPlain ? 6 : 11;
+        RowFragments<T, DP> fq, fg;
+        fq.read(tile, 0, l), fg.read(tile + HALF, 0, l);
+        order();
+        f32x16 s0 = fq.products(k), dp0 = fg.products(v);
+        const RowInfo x0 = row_info(buf, 0);
+        order();
+        fq.read(tile, 32, l), fg.read(tile + HALF, 32, l);
+        order();
+        f32x16 s1 = fq.products(k), dp1 = fg.products(v);
+        weights(x0, s0, dp0);
+        mix<2 * DP / 16, V>();
+        settle<T>();
+        if (!whole0) unsee(buf, 0, s0, dp0);
+        ColumnFragments<T, DP> cg, cq;
+        cg.read(tile + HALF, 0, l), cq.read(tile, 0, l);
+        const RowInfo x1 = row_info(buf, 1);
+        order();
+        cg.weigh(dv, s0), cq.weigh(dk, dp0);
+        weights(x1, s1, dp1);
+        mix<4 * DP / 32, V>();
+        settle<T>();
+        if (!whole1) unsee(buf, 1, s1, dp1);
+        cg.read(tile + HALF, 32, l), cq.read(tile, 32, l);
+        order();
+        cg.weigh(dv, s1), cq.weigh(dk, dp1);
+        settle<T>();
+    };
     auto compute = [&](const char* tile, int buf) {
         const int i0 = first(u), p0 = i0 + off;
         // the rows' key ends rise with their position
         auto ends = [&](int p) { return a.causal ? min(n, max(p + 1, prefix)) : n; };
+        if constexpr (KIND != kGeneral && NB == 2) {
+            if (j0 < ends(p0 + min(a.Lq - i0, 64) - 1))
+                both(tile, buf, j0 + 32 <= ends(p0), j0 + 32 <= ends(p0 + 32));
+        } else {
 #pragma unroll 1
-        for (int qb = 0; qb < NB; ++qb) {
-            const int pf = p0 + qb * 32, count = min(a.Lq - i0 - qb * 32, 32);
-            if (count <= 0) break;
-            if (j0 >= ends(pf + count - 1)) continue;
-            const bool whole = j0 + 32 <= ends(pf) && !a.documents;
-            if constexpr (KIND == kGeneral) general(tile, buf, qb, pf, whole);
-            else simple(tile, buf, qb, whole);
+            for (int qb = 0; qb < NB; ++qb) {
+                const int pf = p0 + qb * 32, count = min(a.Lq - i0 - qb * 32, 32);
+                if (count <= 0) break;
+                if (j0 >= ends(pf + count - 1)) continue;
+                const bool whole = j0 + 32 <= ends(pf) && !(KIND == kGeneral && a.documents);
+                if constexpr (KIND == kGeneral) general(tile, buf, qb, pf, whole);
+                else simple(tile, buf, qb, whole);
+            }
         }
     };
     auto step = [&](char* tile, char* ahead, int buf) {

@@ -84,8 +84,9 @@ __device__ __forceinline__ float halves_sum(float v) {
 }
 
 // Rows of DP elements in LDS, 16-byte chunks.  A row's chunks are permuted by
-// turn(row) so that eight rows read at one chunk, and four rows read at 32
-// bytes by columns, meet no bank twice.
+// turn(row): LDS serves 256 bytes a cycle from 64 banks, and 16 rows read at
+// one chunk, as well as four rows read at 64 bytes by columns, then fall on
+// every bank once.
 template <typename T, int DP>
 struct Tile {
     static constexpr int CE = 16 / sizeof(T), NC = DP / CE, ROW = DP * sizeof(T);
@@ -93,10 +94,14 @@ struct Tile {
     using V = typename Eight<T>::V;
 
     static __device__ __forceinline__ int turn(int r) {
-        if constexpr (NC % 8 == 0)
-            return (r & 3) << 1 | (r >> 2 & 1);
+        if constexpr (NC % 16 == 0 && sizeof(T) == 2)
+            return (r & 3) << 2 | (r >> 2 & 3);
+        else if constexpr (NC % 16 == 0)  // by columns, rows r and r + 4 are read at 128 bytes
+            return (r >> 2 & 1) << 3 | (r & 3) << 1 | (r >> 3 & 1);
+        else if constexpr (NC % 8 == 0)
+            return (r >> 1 & 1) << 2 | (r >> 2 & 3);
         else
-            return (r >> 1 & 1) << 1 | (r >> 2 & 1);
+            return r >> 2 & 3;
     }
     static __device__ __forceinline__ int at(int r, int c) { return r * ROW + ((c ^ turn(r)) * 16); }
 
@@ -121,8 +126,9 @@ struct Tile {
             // a transposing read takes four rows by 16 columns from 16 lanes
             const int i = l & 15, d = db * 32 + (l & 16) + 4 * (i & 3);
             const char* p = lds + at(4 * g + (i >> 2), d / 8) + (d & 7) * 2;
+            const char* q = lds + at(4 * g + (i >> 2) + 8, d / 8) + (d & 7) * 2;
             const s16x4 a = __builtin_amdgcn_ds_read_tr16_b64_v4i16((NSH_LDS s16x4*)(p));
-            const s16x4 b = __builtin_amdgcn_ds_read_tr16_b64_v4i16((NSH_LDS s16x4*)(p + 8 * ROW));
+            const s16x4 b = __builtin_amdgcn_ds_read_tr16_b64_v4i16((NSH_LDS s16x4*)(q));
             return __builtin_bit_cast(V, __builtin_shufflevector(a, b, 0, 1, 2, 3, 4, 5, 6, 7));
         } else {
             const int d = db * 32 + (l & 31);
@@ -203,6 +209,18 @@ __device__ __forceinline__ void load_row(typename Eight<T>::V (&v)[DP / 16], con
 // products that use them; order() keeps the compiler from moving them back to
 // their uses, one read and one wait at a time.
 __device__ __forceinline__ void order() { __builtin_amdgcn_sched_barrier(0); }
+
+// Mixes a region's products into its other arithmetic: one product, V others,
+// N times.  A product keeps the matrix cores busy for 32 cycles after the wave
+// has gone on; in a row they would make it wait.
+template <int N, int V>
+__device__ __forceinline__ void mix() {
+#pragma unroll
+    for (int i = 0; i < N; ++i) {
+        __builtin_amdgcn_sched_group_barrier(0x008, 1, 0);
+        __builtin_amdgcn_sched_group_barrier(0x402, V, 0);
+    }
+}
 
 // Ends a run of products ahead of a branch.  Their results may be read 12 wait
 // states (18 for the fp32 products) after the last one at the earliest, and the
