@@ -35,9 +35,16 @@ static int ranges_launch(const Att& a, hipStream_t st) {
 // Rows go 128 to a workgroup where that gives every CU one; otherwise 32, and
 // the workgroup's waves split the keys.  A forward short of workgroups even so
 // (single tokens over a cache) shares a row block's keys among `splits` more,
-// as long as a wave keeps four tiles of 32 keys.  Fewer rows than a wave holds
-// (32) take the rows of all the heads of a key head side by side, which then
-// reads its keys once; a bias table is staged for one head, and keeps to one.
+// up to what the CUs hold at once (one of these workgroups where its tiles take
+// most of the LDS, or two), as long as a wave keeps four tiles of 32 keys, or
+// two in fp32, whose products take 16 times as long.  16 x 32 heads, 8 of keys,
+// one token over 8192, bf16: 82 us in all with two workgroups for every CU,
+// 77 with one; 2 x 5 heads, 333 over 517 tokens, fp32: 34 us with four tiles
+// kept, 30 with two; 8 heads, one token over 500, fp16: 10.8 with four, 11.4
+// with two.
+// Fewer rows than a wave holds (32) take the rows of all the heads of a key head
+// side by side, which then reads its keys once; a bias table is staged for one
+// head, and keeps to one.
 static void cut_rows(Att& a, bool backward) {
     const int64_t cus = nsh_host::compute_units();
     a.pack = !backward && a.Lq < 32 && !a.table ? a.per : 1;
@@ -49,19 +56,27 @@ static void cut_rows(Att& a, bool backward) {
     a.rblocks = static_cast<int>(nsh_host::ceil_div(rows, int64_t(32)));
     a.splits = 1;
     if (backward) return;
-    const int64_t blocks = groups * a.rblocks, most = nsh_host::ceil_div(a.Lk, 32) / (4 * kAttWaves);
-    a.splits = static_cast<int>(std::max<int64_t>(1, std::min<int64_t>({2 * cus / blocks, most, 64})));
+    const int64_t blocks = groups * a.rblocks, keep = (a.wide ? 2 : 4) * kAttWaves;
+    const int64_t room = cus * (a.D * (a.wide ? 4 : 2) > 128 ? 1 : 2);
+    a.splits = static_cast<int>(std::max<int64_t>(
+        1, std::min<int64_t>({room / blocks, nsh_host::ceil_div(a.Lk, 32) / keep, 64})));
 }
 
 // Keys go 128 to a workgroup.  `parts` workgroups share a key block's queries
-// where there are fewer than two workgroups to a CU, as long as each keeps four
-// query tiles.
+// where there are too few of them to go round, as long as each keeps two query
+// tiles; the third launch that adds up their sums costs more than it brings from
+// five workgroups to four CUs on.  4 x 12 heads, 1024 tokens, width 64, bf16 (384
+// workgroups): 86 us alone, 92 + 16 with two parts; 2 x 16 heads, 4 of keys, 4096
+// tokens, width 128, causal (256): 791 alone, 500 + 18; 2 x 5 heads, 333 over 517
+// tokens, fp32: 60 + 5 with four tiles kept, 38 + 5 with two, 48 + 8 with one.
 static void cut_keys(Att& a) {
     const int64_t cus = nsh_host::compute_units(), tile = a.wide ? 32 : 64;
     a.kblocks = static_cast<int>(nsh_host::ceil_div(a.Lk, 128));
     const int64_t blocks = static_cast<int64_t>(a.B) * a.Hk * a.kblocks;
     const int64_t units = nsh_host::ceil_div(a.Lq, tile) * a.per;
-    a.parts = static_cast<int>(std::max<int64_t>(1, std::min<int64_t>({nsh_host::ceil_div(2 * cus, blocks), units / 4, 64})));
+    a.parts = 1;
+    if (4 * blocks < 5 * cus)
+        a.parts = static_cast<int>(std::max<int64_t>(1, std::min<int64_t>({nsh_host::ceil_div(2 * cus, blocks), units / 2, 64})));
 }
 
 }  // namespace nsh

@@ -89,17 +89,17 @@ template <typename T, int DP, Kind KIND>
 __device__ __forceinline__ void row_gradient(const Att& a, const Cap& cap, const Bias& bs, const Row& x,
                                              const WaveRows& wr, const typename Eight<T>::V (&q)[DP / 16],
                                              const typename Eight<T>::V (&go)[DP / 16], float2 stat, float delta,
-                                             const char* K, const char* V, int r0, const int* kd, int j0, int l,
+                                             const char* K, const char* V, int by_row, int by_col, const int* kd, int j0, int l,
                                              TableSums* ts, f32x16 (&dq)[DP / 32]) {
     f32x16 s, dp;
     {
         RowFragments<T, DP> fk, fv;
-        fk.read(K, r0, l), fv.read(V, r0, l);
+        fk.read(K, by_row), fv.read(V, by_row);
         order();
         s = fk.products(q), dp = fv.products(go);
     }
     ColumnFragments<T, DP> f;
-    f.read(K, r0, l);
+    f.read(K, by_col);
     if (KIND != kGeneral) {
         order();
         // p's two constants in one: 1 / sum joins the exponent
@@ -160,7 +160,7 @@ __global__ __launch_bounds__(kAttThreads, SPLIT || DP * sizeof(T) > (KIND == kGe
     const int n = filled_keys(a, b), hk = h / a.per;
     const LaneRow x = lane_row(a, b, h, rb * ROWS + (SPLIT ? 0 : wave * 32) + (l & 31), n);
     const WaveRows wr = wave_rows(x);
-    const Cap cap = cap_of<T, KIND>(a);
+    const Cap cap = cap_of<T, KIND>(a, true);
     if (KIND == kGeneral && a.table) stage_line<T>(a, h, room);
     const Bias bs = lane_bias(a, h, room);
     TableSums sums{};
@@ -186,8 +186,6 @@ __global__ __launch_bounds__(kAttThreads, SPLIT || DP * sizeof(T) > (KIND == kGe
     delta = halves_sum(delta) - (a.gdegree ? a.gdegree[at] : 0.f);
     if (x.live && l < 32 && (!SPLIT || wave == 0)) a.delta[at] = delta;
     load_row<T, DP>(q, row_at<T>(a.q, a.qs, b, h, x.i), a.D, l);
-    if (a.scale < 0.f)
-        for (int s = 0; s < L::NS; ++s) q[s] = Eight<T>::negate(q[s]);
     // rows that see nothing, and lanes that stand in for no row, weigh nothing
     float2 stat = get_stats(a, at);
     if (!x.live) stat.y = 0.f;
@@ -223,14 +221,15 @@ __global__ __launch_bounds__(kAttThreads, SPLIT || DP * sizeof(T) > (KIND == kGe
     f32x16 dq[L::ND] = {};
     int t = need.next(begin, end);
     TableSums* const ts = KIND == kGeneral && a.gtable ? &sums : nullptr;
+    const int by_row = L::row_base(0, l), by_col = L::col_base(0, l);
     auto compute = [&](const char* tile, const int* docs) {
 #pragma unroll 1
         for (int kb = 0; kb < NB; ++kb)
         {
             const int j0 = t * KT + kb * 32;
             if (j0 >= wr.most) break;
-            row_gradient<T, DP, KIND>(a, cap, bs, x.r, wr, q, go, stat, delta, tile, tile + HALF, kb * 32,
-                                      docs + kb * 32, j0, l, ts, dq);
+            row_gradient<T, DP, KIND>(a, cap, bs, x.r, wr, q, go, stat, delta, tile + kb * 32 * L::ROW,
+                                      tile + HALF + kb * 32 * L::ROW, by_row, by_col, docs + kb * 32, j0, l, ts, dq);
         }
     };
     auto step = [&](char* tile, int* docs, char* ahead, int* docs_ahead) {
@@ -324,21 +323,28 @@ __global__ __launch_bounds__(kAttThreads, SPLIT || DP * sizeof(T) > (KIND == kGe
     }
 }
 
-template <typename T, int DP, Kind KIND>
-__global__ __launch_bounds__(kAttThreads, DP * sizeof(T) >= 256 ? 1 : 2) void att_bwd_key_kernel(Att a) {
+// PAIRED: eight waves, two to 32 keys, one for each half of a 64-row tile.  K and
+// V then stay in LDS rather than in registers: of those, the sums of wide heads
+// leave too few for two waves to a SIMD otherwise, and one wave waits for its
+// own products.
+template <typename T, int DP, Kind KIND, bool PAIRED>
+__global__ __launch_bounds__(PAIRED ? 512 : kAttThreads, PAIRED ? 1 : DP * sizeof(T) >= 256 ? 1 : 2)
+void att_bwd_key_kernel(Att a) {
     using L = Tile<T, DP>;
     constexpr int QT = BwdShape<T, DP>::KT, NB = QT / 32, HALF = QT * L::ROW;
+    constexpr int KV = PAIRED ? 128 * L::ROW : 16;
+    __shared__ __attribute__((aligned(1024))) char kv[2][KV];
     __shared__ __attribute__((aligned(1024))) char tiles0[2][HALF];
     __shared__ __attribute__((aligned(1024))) char tiles1[2][HALF];
     __shared__ __attribute__((aligned(256))) float info[2][6][QT];  // log 2 of weight over score, maximum, 1 / sum, delta, key end, document
     extern __shared__ float line[];
-    const int l = threadIdx.x & 63, wave = wave_id(), g = l >> 5;
+    const int l = threadIdx.x & 63, wave = wave_id(), g = l >> 5, kw = wave & 3;
     int bg, rest;
     place(blockIdx.x, a.B * a.Hk, bg, rest);
     const int b = bg / a.Hk, hk = bg - b * a.Hk, part = rest % a.parts, kb = rest / a.parts;
     const int n = filled_keys(a, b), off = n - a.Lq;
-    const int j0 = kb * 128 + wave * 32, j = j0 + (l & 31);
-    const Cap cap = cap_of<T, KIND>(a);
+    const int j0 = kb * 128 + kw * 32, j = j0 + (l & 31);
+    const Cap cap = cap_of<T, KIND>(a, true);
     const int prefix = a.prefix ? a.prefix[b] : 0;
     const int doc = a.documents && j < n ? a.documents[static_cast<int64_t>(b) * a.Lk + j] : 0;
 
@@ -346,12 +352,17 @@ __global__ __launch_bounds__(kAttThreads, DP * sizeof(T) >= 256 ? 1 : 2) void at
     V k[L::NS], v[L::NS];
 #pragma unroll
     for (int s = 0; s < L::NS; ++s) k[s] = V{}, v[s] = V{};
-    if (j < n) {
+    const bool second = PAIRED && wave >= 4;  // these waves load the tiles' second tensor
+    if (PAIRED) {
+        const int64_t stride = second ? a.vs[2] : a.ks[2];
+        const T* base = second ? row_at<T>(a.v, a.vs, b, hk, 0) : row_at<T>(a.k, a.ks, b, hk, 0);
+        Loader<T, DP, PAIRED ? 128 : QT, 4> lk;
+        lk.init(threadIdx.x & 255, stride, a.D);
+        lk.load(second ? kv[1] : kv[0], base, stride, kb * 128, n, a.D, kw);
+    } else if (j < n) {
         load_row<T, DP>(k, row_at<T>(a.k, a.ks, b, hk, j), a.D, l);
         load_row<T, DP>(v, row_at<T>(a.v, a.vs, b, hk, j), a.D, l);
     }
-    if (a.scale < 0.f)
-        for (int s = 0; s < L::NS; ++s) k[s] = Eight<T>::negate(k[s]);
 
     // the queries that see any of the block's keys: all of them, or those from
     // the first key's position on
@@ -384,15 +395,20 @@ __global__ __launch_bounds__(kAttThreads, DP * sizeof(T) >= 256 ? 1 : 2) void at
     };
     Needed<decltype(wanted)> need{wanted};
 
-    Loader<T, DP, QT, kAttWaves> lq, lg;
-    lq.init(threadIdx.x, a.qs[2], a.D);
-    lg.init(threadIdx.x, a.gos[2], a.D);
+    Loader<T, DP, QT, 4> lq, lg;
+    lq.init(threadIdx.x & 255, second ? a.gos[2] : a.qs[2], a.D);
+    if (!PAIRED) lg.init(threadIdx.x, a.gos[2], a.D);
     auto head = [&](int u) { return hk * a.per + u / (t1 - t0); };
     auto first = [&](int u) { return (t0 + u % (t1 - t0)) * QT; };
     auto load = [&](int u, char* tile) {
         const int h = head(u), i0 = first(u);
-        lq.load(tile, row_at<T>(a.q, a.qs, b, h, 0), a.qs[2], i0, a.Lq, a.D, wave);
-        lg.load(tile + HALF, row_at<T>(a.go, a.gos, b, h, 0), a.gos[2], i0, a.Lq, a.D, wave);
+        if (PAIRED) {
+            const T* base = second ? row_at<T>(a.go, a.gos, b, h, 0) : row_at<T>(a.q, a.qs, b, h, 0);
+            lq.load(tile + (second ? HALF : 0), base, second ? a.gos[2] : a.qs[2], i0, a.Lq, a.D, kw);
+        } else {
+            lq.load(tile, row_at<T>(a.q, a.qs, b, h, 0), a.qs[2], i0, a.Lq, a.D, wave);
+            lg.load(tile + HALF, row_at<T>(a.go, a.gos, b, h, 0), a.gos[2], i0, a.Lq, a.D, wave);
+        }
     };
     // row values of a unit, in registers until its tile is the next
     float2 r_stat{};
@@ -419,11 +435,15 @@ __global__ __launch_bounds__(kAttThreads, DP * sizeof(T) >= 256 ? 1 : 2) void at
     f32x16 dk[L::ND] = {}, dv[L::ND] = {};
     int u = need.next(u0, u1), staged = -1;
     Bias bs{0.f, line};
+    // a wave's places in a tile (its half of one, if paired) and among the keys
+    const int half = PAIRED ? (wave >> 2) * 32 : 0;
+    const int by_row = L::row_base(half, l), by_col = L::col_base(half, l), by_key = L::row_base(kw * 32, l);
     // one 32-row part of a tile, whatever it holds
     auto general = [&](const char* tile, int buf, int qb, int pf, bool whole) {
+        const char* part = tile + qb * 32 * L::ROW;
         const float* rows = &info[buf][0][qb * 32 + 4 * g];
         RowFragments<T, DP> fq, fg;
-        fq.read(tile, qb * 32, l), fg.read(tile + HALF, qb * 32, l);
+        fq.read(part, by_row), fg.read(part + HALF, by_row);
         order();
         const f32x16 xs = fq.products(k);
         f32x16 dp = fg.products(v);
@@ -463,9 +483,9 @@ __global__ __launch_bounds__(kAttThreads, DP * sizeof(T) >= 256 ? 1 : 2) void at
         }
         order();
         ColumnFragments<T, DP> f;
-        f.read(tile + HALF, qb * 32, l);
+        f.read(part + HALF, by_col);
         f.weigh(dv, s);
-        f.read(tile, qb * 32, l);
+        f.read(part, by_col);
         f.weigh(dk, dp);
         settle<T>();
     };
@@ -509,17 +529,18 @@ __global__ __launch_bounds__(kAttThreads, DP * sizeof(T) >= 256 ? 1 : 2) void at
         }
     };
     auto simple = [&](const char* tile, int buf, int qb, bool whole) {
+        const char* part = tile + qb * 32 * L::ROW;
         RowFragments<T, DP> fq, fg;
-        fq.read(tile, qb * 32, l), fg.read(tile + HALF, qb * 32, l);
+        fq.read(part, by_row), fg.read(part + HALF, by_row);
         order();
         f32x16 s = fq.products(k), dp = fg.products(v);
         ColumnFragments<T, DP> cg, cq;
-        cg.read(tile + HALF, qb * 32, l);
+        cg.read(part + HALF, by_col);
         const RowInfo x = row_info(buf, qb);
         settle<T>();
         weights(x, s, dp);
         if (!whole) unsee(buf, qb, s, dp);
-        cq.read(tile, qb * 32, l);
+        cq.read(part, by_col);
         order();
         cg.weigh(dv, s);
         cq.weigh(dk, dp);
@@ -531,12 +552,12 @@ __global__ __launch_bounds__(kAttThreads, DP * sizeof(T) >= 256 ? 1 : 2) void at
     auto both = [&](const char* tile, int buf, bool whole0, bool whole1) {
         constexpr int V = KIND == kPlain ? 6 : 11;
         RowFragments<T, DP> fq, fg;
-        fq.read(tile, 0, l), fg.read(tile + HALF, 0, l);
+        fq.read(tile, by_row), fg.read(tile + HALF, by_row);
         order();
         f32x16 s0 = fq.products(k), dp0 = fg.products(v);
         const RowInfo x0 = row_info(buf, 0);
         order();
-        fq.read(tile, 32, l), fg.read(tile + HALF, 32, l);
+        fq.read(tile, by_row, 32), fg.read(tile + HALF, by_row, 32);
         order();
         f32x16 s1 = fq.products(k), dp1 = fg.products(v);
         weights(x0, s0, dp0);
@@ -544,7 +565,7 @@ __global__ __launch_bounds__(kAttThreads, DP * sizeof(T) >= 256 ? 1 : 2) void at
         settle<T>();
         if (!whole0) unsee(buf, 0, s0, dp0);
         ColumnFragments<T, DP> cg, cq;
-        cg.read(tile + HALF, 0, l), cq.read(tile, 0, l);
+        cg.read(tile + HALF, by_col), cq.read(tile, by_col);
         const RowInfo x1 = row_info(buf, 1);
         order();
         cg.weigh(dv, s0), cq.weigh(dk, dp0);
@@ -552,16 +573,47 @@ __global__ __launch_bounds__(kAttThreads, DP * sizeof(T) >= 256 ? 1 : 2) void at
         mix<4 * DP / 32, V>();
         settle<T>();
         if (!whole1) unsee(buf, 1, s1, dp1);
-        cg.read(tile + HALF, 32, l), cq.read(tile, 32, l);
+        cg.read(tile + HALF, by_col, 32), cq.read(tile, by_col, 32);
         order();
         cg.weigh(dv, s1), cq.weigh(dk, dp1);
+        settle<T>();
+    };
+    auto paired = [&](const char* tile, int buf, int qb, bool whole) {
+        // formed anew for each tile: kept, the reads' addresses would be spilled
+        int rows = by_row, cols = by_col, keys = by_key;
+        asm volatile("" : "+v"(rows), "+v"(cols), "+v"(keys));
+        f32x16 s, dp;
+        {
+            RowFragments<T, DP> f, key;
+            f.read(tile, rows), key.read(kv[0], keys);
+            order();
+            s = f.products(key.f);
+        }
+        {
+            RowFragments<T, DP> f, key;
+            f.read(tile + HALF, rows), key.read(kv[1], keys);
+            order();
+            dp = f.products(key.f);
+        }
+        settle<T>();
+        weights(row_info(buf, qb), s, dp);
+        ColumnFragments<T, DP> cg, cq;
+        cg.read(tile + HALF, cols);
+        if (!whole) unsee(buf, qb, s, dp);
+        cq.read(tile, cols);
+        order();
+        cg.weigh(dv, s);
+        cq.weigh(dk, dp);
         settle<T>();
     };
     auto compute = [&](const char* tile, int buf) {
         const int i0 = first(u), p0 = i0 + off;
         // the rows' key ends rise with their position
         auto ends = [&](int p) { return a.causal ? min(n, max(p + 1, prefix)) : n; };
-        if constexpr (KIND != kGeneral && NB == 2) {
+        if constexpr (PAIRED) {
+            const int qb = wave >> 2, pf = p0 + qb * 32, count = min(a.Lq - i0 - qb * 32, 32);
+            if (count > 0 && j0 < ends(pf + count - 1)) paired(tile, buf, qb, j0 + 32 <= ends(pf));
+        } else if constexpr (KIND != kGeneral && NB == 2) {
             if (j0 < ends(p0 + min(a.Lq - i0, 64) - 1))
                 both(tile, buf, j0 + 32 <= ends(p0), j0 + 32 <= ends(p0 + 32));
         } else {
@@ -604,6 +656,29 @@ __global__ __launch_bounds__(kAttThreads, DP * sizeof(T) >= 256 ? 1 : 2) void at
     while (u < u1) {
         step(tiles0[0], tiles1[0], 0);
         if (u < u1) step(tiles1[0], tiles0[0], 1);
+    }
+    if constexpr (PAIRED) {  // the second waves' sums join the first's
+        float* sums = reinterpret_cast<float*>(&kv[0][0]) + (kw * DP + 4 * g) * 32 + (l & 31);  // [keys][column][key]
+        static_assert(sizeof(kv) >= 4 * DP * 32 * 4, "four waves' sums of dk take the keys' place");
+        auto join = [&](f32x16 (&acc)[L::ND]) {
+            __syncthreads();
+            if (wave >= 4) {
+#pragma unroll
+                for (int d = 0; d < L::ND; ++d)
+#pragma unroll
+                    for (int r = 0; r < 16; ++r) sums[(d * 32 + el(r)) * 32] = acc[d][r];
+            }
+            __syncthreads();
+            if (wave < 4) {
+#pragma unroll
+                for (int d = 0; d < L::ND; ++d)
+#pragma unroll
+                    for (int r = 0; r < 16; ++r) acc[d][r] += sums[(d * 32 + el(r)) * 32];
+            }
+        };
+        join(dk);
+        join(dv);
+        if (wave >= 4) return;
     }
     float bad = 0.f;
 #pragma unroll
@@ -683,7 +758,9 @@ static void backward_kind(const Att& a, hipStream_t st) {
     else
         att_bwd_row_kernel<T, DP, false, KIND><<<static_cast<unsigned>(rows), kAttThreads, attention_row_lds(a), st>>>(a);
     const int64_t keys = static_cast<int64_t>(a.B) * a.Hk * a.kblocks * a.parts;
-    att_bwd_key_kernel<T, DP, KIND><<<static_cast<unsigned>(keys), kAttThreads, line, st>>>(a);
+    constexpr bool kPaired = KIND != kGeneral && sizeof(T) == 2 && DP >= 96;
+    att_bwd_key_kernel<T, DP, KIND, kPaired>
+        <<<static_cast<unsigned>(keys), kPaired ? 512 : kAttThreads, line, st>>>(a);
 }
 
 template <typename T, int DP>

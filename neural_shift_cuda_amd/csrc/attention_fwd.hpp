@@ -29,13 +29,13 @@ constexpr float kLazy = 8.f;
 template <typename T, int DP, int NB, Kind KIND>
 __device__ __forceinline__ void attend(const Att& a, const Cap& cap, const Bias& bs, const Row& x,
                                        const WaveRows& wr, const typename Eight<T>::V (&q)[DP / 16],
-                                       const char* K, const char* V, const int* kd, int j0, int l,
-                                       Running<DP / 32>& st) {
+                                       const char* K, const char* V, int by_row, int by_col, const int* kd, int j0,
+                                       int l, Running<DP / 32>& st) {
     f32x16 s[NB];
     {
         RowFragments<T, DP> f[NB];
 #pragma unroll
-        for (int kb = 0; kb < NB; ++kb) f[kb].read(K, kb * 32, l);
+        for (int kb = 0; kb < NB; ++kb) f[kb].read(K, by_row, kb * 32);
         order();
 #pragma unroll
         for (int kb = 0; kb < NB; ++kb) s[kb] = f[kb].products(q);
@@ -43,7 +43,7 @@ __device__ __forceinline__ void attend(const Att& a, const Cap& cap, const Bias&
     ColumnFragments<T, DP> f;
     const bool whole = j0 + NB * 32 <= wr.least && !(KIND == kGeneral && a.documents);
     if (KIND != kGeneral) {
-        f.read(V, 0, l);
+        f.read(V, by_col);
         settle<T>();
         if (!whole) {
 #pragma unroll
@@ -105,11 +105,11 @@ __device__ __forceinline__ void attend(const Att& a, const Cap& cap, const Bias&
         for (int r = 0; r < 16; r += 2) z0 += s[kb][r], z1 += s[kb][r + 1];
     st.z += z0 + z1;
     order();
-    if (KIND == kGeneral) f.read(V, 0, l);
+    if (KIND == kGeneral) f.read(V, by_col);
 #pragma unroll
     for (int kb = 0; kb < NB; ++kb) {
         ColumnFragments<T, DP> ahead;
-        if (kb + 1 < NB) ahead.read(V, kb * 32 + 32, l);
+        if (kb + 1 < NB) ahead.read(V, by_col, kb * 32 + 32);
         f.weigh(st.o, s[kb]);
         order();
         if (kb + 1 < NB) f = ahead;
@@ -162,7 +162,7 @@ __global__ __launch_bounds__(kAttThreads, DP * sizeof(T) > 384 ? 1 : 2) void att
     const int n = filled_keys(a, b), hk = group * a.pack / a.per;
     const LaneRow x = lane_row(a, b, group, rb * 128 + wave * 32 + (l & 31), n);
     const WaveRows wr = wave_rows(x);
-    const Cap cap = cap_of<T, KIND>(a);
+    const Cap cap = cap_of<T, KIND>(a, false);
     if (KIND == kGeneral && a.table) stage_line<T>(a, group, line);  // read after the first barrier
     const Bias bs = lane_bias(a, x.h, line);
     typename Eight<T>::V q[L::NS];
@@ -199,13 +199,14 @@ __global__ __launch_bounds__(kAttThreads, DP * sizeof(T) > 384 ? 1 : 2) void att
     Running<L::ND> st{};
     st.m = -INFINITY;
     int t = need.next(0, end);
+    const int by_row = L::row_base(0, l), by_col = L::col_base(0, l);
     auto step = [&](char (&tiles)[2][HALF], int (&docs)[64], char (&ahead)[2][HALF], int (&docs_ahead)[64]) {
         const int tn = need.next(t + 1, end);
         __builtin_amdgcn_s_waitcnt(0x0f70);  // vmcnt(0): the tile has landed
         __syncthreads();
         if (tn < end) load(tn, ahead, docs_ahead);
         if (t * KT < wr.most)
-            attend<T, DP, NB, KIND>(a, cap, bs, x.r, wr, q, tiles[0], tiles[1], docs, t * KT, l, st);
+            attend<T, DP, NB, KIND>(a, cap, bs, x.r, wr, q, tiles[0], tiles[1], by_row, by_col, docs, t * KT, l, st);
         t = tn;
     };
     if (t < end) load(t, tiles0, docs0);
@@ -252,7 +253,7 @@ __global__ __launch_bounds__(kAttThreads, 1) void att_fwd_split_kernel(Att a) {
     const int n = filled_keys(a, b), hk = group * a.pack / a.per;
     const LaneRow x = lane_row(a, b, group, rb * 32 + (l & 31), n);
     const WaveRows wr = wave_rows(x);
-    const Cap cap = cap_of<T, KIND>(a);
+    const Cap cap = cap_of<T, KIND>(a, false);
     if (KIND == kGeneral && a.table) {
         stage_line<T>(a, group, line);
         __syncthreads();
@@ -295,11 +296,12 @@ __global__ __launch_bounds__(kAttThreads, 1) void att_fwd_split_kernel(Att a) {
     load_row<T, DP>(q, row_at<T>(a.q, a.qs, b, x.h, x.i), a.D, l);
     if (a.scale < 0.f)
         for (int s = 0; s < L::NS; ++s) q[s] = Eight<T>::negate(q[s]);
+    const int by_row = L::row_base(0, l), by_col = L::col_base(0, l);
     auto step = [&](char* tile, int* docs, char* ahead, int* docs_ahead) {
         const int tn = need.next(t + 1, end);
         __builtin_amdgcn_s_waitcnt(0x0f70);  // vmcnt(0): the tile has landed
         if (S::NBUF == 2 && tn < end) load(tn, ahead, docs_ahead);
-        attend<T, DP, 1, KIND>(a, cap, bs, x.r, wr, q, tile, tile + HALF, docs, t * 32, l, st);
+        attend<T, DP, 1, KIND>(a, cap, bs, x.r, wr, q, tile, tile + HALF, by_row, by_col, docs, t * 32, l, st);
         if (S::NBUF == 1 && tn < end) {
             __builtin_amdgcn_s_waitcnt(0xc07f);  // lgkmcnt(0): the tile has been read
             load(tn, tile, docs);

@@ -93,7 +93,11 @@ struct Tile {
     static constexpr int NS = DP / 16, ND = DP / 32;
     using V = typename Eight<T>::V;
 
-    static __device__ __forceinline__ int turn(int r) {
+    // turn() only moves bits of the row about, so that a place's address is one
+    // of the lane's with constants joined by exclusive or, within FIELD bytes,
+    // and by addition beyond.
+    static constexpr int FIELD = NC % 16 == 0 ? 256 : NC % 8 == 0 ? 128 : 64;
+    static __host__ __device__ __forceinline__ constexpr int turn(int r) {
         if constexpr (NC % 16 == 0 && sizeof(T) == 2)
             return (r & 3) << 2 | (r >> 2 & 3);
         else if constexpr (NC % 16 == 0)  // by columns, rows r and r + 4 are read at 128 bytes
@@ -104,38 +108,47 @@ struct Tile {
             return r >> 2 & 3;
     }
     static __device__ __forceinline__ int at(int r, int c) { return r * ROW + ((c ^ turn(r)) * 16); }
+    static __device__ __forceinline__ int moved(int base, int bytes, int row) {
+        return (base ^ (bytes % FIELD) ^ turn(row) * 16) + bytes / FIELD * FIELD + row * ROW;
+    }
 
-    // Steps s of row r0 + l % 32.
-    static __device__ __forceinline__ V row(const char* lds, int r0, int s, int l) {
-        const int r = l & 31, g = l >> 5;
-        lds += r0 * ROW;
+    // The lane's place in row r0 + l % 32 (r0 a multiple of 32), and by columns.
+    static __device__ __forceinline__ int row_base(int r0, int l) {
+        return at(r0 + (l & 31), (l >> 5) * (sizeof(T) / 2));
+    }
+    static __device__ __forceinline__ int col_base(int r0, int l) {
         if constexpr (sizeof(T) == 2) {
-            return *reinterpret_cast<const V*>(lds + at(r, 2 * s + g));
+            // a transposing read takes four rows by 16 columns from 16 lanes
+            const int i = l & 15, d = (l & 16) + 4 * (i & 3);
+            return at(r0 + 4 * (l >> 5) + (i >> 2), d / 8) + (d & 7) * 2;
         } else {
-            const f32x4 a = *reinterpret_cast<const f32x4*>(lds + at(r, 4 * s + 2 * g));
-            const f32x4 b = *reinterpret_cast<const f32x4*>(lds + at(r, 4 * s + 2 * g + 1));
+            const int d = l & 31;
+            return at(r0 + 4 * (l >> 5), d / 4) + (d & 3) * 4;
+        }
+    }
+
+    // Steps s of the lane's row, `row` rows on (a multiple of 32).
+    static __device__ __forceinline__ V row(const char* lds, int base, int row, int s) {
+        if constexpr (sizeof(T) == 2) {
+            return *reinterpret_cast<const V*>(lds + moved(base, 32 * s, row));
+        } else {
+            const f32x4 a = *reinterpret_cast<const f32x4*>(lds + moved(base, 64 * s, row));
+            const f32x4 b = *reinterpret_cast<const f32x4*>(lds + moved(base, 64 * s + 16, row));
             return __builtin_shufflevector(a, b, 0, 1, 2, 3, 4, 5, 6, 7);
         }
     }
-    // Column 32 db + l % 32 of the 16 rows from r0 (a multiple of 16), in the
+    // Column 32 db + l % 32 of 16 rows, `row` rows on (a multiple of 16), in the
     // order of result elements.
-    static __device__ __forceinline__ V col(const char* lds, int r0, int db, int l) {
-        const int g = l >> 5;
-        lds += r0 * ROW;
+    static __device__ __forceinline__ V col(const char* lds, int base, int row, int db) {
         if constexpr (sizeof(T) == 2) {
-            // a transposing read takes four rows by 16 columns from 16 lanes
-            const int i = l & 15, d = db * 32 + (l & 16) + 4 * (i & 3);
-            const char* p = lds + at(4 * g + (i >> 2), d / 8) + (d & 7) * 2;
-            const char* q = lds + at(4 * g + (i >> 2) + 8, d / 8) + (d & 7) * 2;
-            const s16x4 a = __builtin_amdgcn_ds_read_tr16_b64_v4i16((NSH_LDS s16x4*)(p));
-            const s16x4 b = __builtin_amdgcn_ds_read_tr16_b64_v4i16((NSH_LDS s16x4*)(q));
+            const s16x4 a = __builtin_amdgcn_ds_read_tr16_b64_v4i16((NSH_LDS s16x4*)(lds + moved(base, 64 * db, row)));
+            const s16x4 b = __builtin_amdgcn_ds_read_tr16_b64_v4i16((NSH_LDS s16x4*)(lds + moved(base, 64 * db, row + 8)));
             return __builtin_bit_cast(V, __builtin_shufflevector(a, b, 0, 1, 2, 3, 4, 5, 6, 7));
         } else {
-            const int d = db * 32 + (l & 31);
             V v;
 #pragma unroll
             for (int e = 0; e < 8; ++e)
-                v[e] = *reinterpret_cast<const float*>(lds + at(el(e) + 4 * g, d / 4) + (d & 3) * 4);
+                v[e] = *reinterpret_cast<const float*>(lds + moved(base, 128 * db, row + el(e)));
             return v;
         }
     }
@@ -245,11 +258,11 @@ __device__ __forceinline__ int wave_id() { return __builtin_amdgcn_readfirstlane
 enum Kind { kPlain, kCapped, kGeneral };
 
 template <typename T, int DP>
-struct RowFragments {  // 32 tile rows from r0
+struct RowFragments {  // 32 tile rows, `row` rows on from the base's
     typename Eight<T>::V f[DP / 16];
-    __device__ __forceinline__ void read(const char* lds, int r0, int l) {
+    __device__ __forceinline__ void read(const char* lds, int base, int row = 0) {
 #pragma unroll
-        for (int s = 0; s < DP / 16; ++s) f[s] = Tile<T, DP>::row(lds, r0, s, l);
+        for (int s = 0; s < DP / 16; ++s) f[s] = Tile<T, DP>::row(lds, base, row, s);
     }
     // their products with the lane's row
     __device__ __forceinline__ f32x16 products(const typename Eight<T>::V (&v)[DP / 16]) const {
@@ -261,11 +274,12 @@ struct RowFragments {  // 32 tile rows from r0
 };
 
 template <typename T, int DP>
-struct ColumnFragments {  // 32 tile rows from r0, by columns
+struct ColumnFragments {  // 32 tile rows, `row` rows on from the base's, by columns
     typename Eight<T>::V f[DP / 32][2];
-    __device__ __forceinline__ void read(const char* lds, int r0, int l) {
+    __device__ __forceinline__ void read(const char* lds, int base, int row = 0) {
 #pragma unroll
-        for (int d = 0; d < DP / 32; ++d) f[d][0] = Tile<T, DP>::col(lds, r0, d, l), f[d][1] = Tile<T, DP>::col(lds, r0 + 16, d, l);
+        for (int d = 0; d < DP / 32; ++d)
+            f[d][0] = Tile<T, DP>::col(lds, base, row, d), f[d][1] = Tile<T, DP>::col(lds, base, row + 16, d);
     }
     // acc += their columns times the weights w
     __device__ __forceinline__ void weigh(f32x16 (&acc)[DP / 32], const f32x16& w) const {
@@ -284,10 +298,10 @@ struct ColumnFragments {  // 32 tile rows from r0, by columns
 
 struct Cap {
     int mode;      // 0: none, 1: quick, 2: accurate
-    float c;       // |scale| log2 e
-    float k;       // 2 log2 e |scale| / cap
+    float c;       // scale log2 e
+    float k;       // 2 log2 e scale / cap
     float top;     // cap log2 e
-    float inv;     // |scale| / cap
+    float inv;     // scale / cap
 };
 
 template <typename T>
@@ -296,10 +310,12 @@ inline Kind kind_of(const Att& a) {
     return a.cap <= 0.f ? kPlain : sizeof(T) == 2 && a.cap <= kQuickCap ? kCapped : kGeneral;
 }
 
+// (The forward has its rows' signs turned where the scale is negative, for the
+// largest product to be the largest score; the gradients take it as it is.)
 template <typename T, Kind KIND>
-__device__ __forceinline__ Cap cap_of(const Att& a) {
+__device__ __forceinline__ Cap cap_of(const Att& a, bool backward) {
     Cap c;
-    const float s = fabsf(a.scale);
+    const float s = backward ? a.scale : fabsf(a.scale);
     c.mode = KIND == kPlain ? 0 : KIND == kCapped ? 1 : a.cap <= 0.f ? 0 : sizeof(T) == 2 && a.cap <= kQuickCap ? 1 : 2;
     c.c = s * kLog2e;
     c.inv = a.cap > 0.f ? s / a.cap : 0.f;
