@@ -136,7 +136,7 @@ __device__ __forceinline__ void row_gradient(const Att& a, const Cap& cap, const
         if (cap.mode != 0) dp *= y.w;
     }
     order();
-    f.weigh(dq, dp);
+    f.weigh_fine(dq, dp);
     settle<T>();
 }
 
@@ -486,7 +486,7 @@ void att_bwd_key_kernel(Att a) {
         f.read(part + HALF, by_col);
         f.weigh(dv, s);
         f.read(part, by_col);
-        f.weigh(dk, dp);
+        f.weigh_fine(dk, dp);
         settle<T>();
     };
     // The weights p (in place of the products s) and dx, without a bias.
@@ -543,7 +543,7 @@ void att_bwd_key_kernel(Att a) {
         cq.read(part, by_col);
         order();
         cg.weigh(dv, s);
-        cq.weigh(dk, dp);
+        cq.weigh_fine(dk, dp);
         settle<T>();
     };
     // Both parts of a 64-row tile: one part's products run under the other's
@@ -568,14 +568,14 @@ void att_bwd_key_kernel(Att a) {
         cg.read(tile + HALF, by_col), cq.read(tile, by_col);
         const RowInfo x1 = row_info(buf, 1);
         order();
-        cg.weigh(dv, s0), cq.weigh(dk, dp0);
+        cg.weigh(dv, s0), cq.weigh_fine(dk, dp0);
         weights(x1, s1, dp1);
-        mix<4 * DP / 32, V>();
+        mix<(__is_same(T, f16) ? 6 : 4) * DP / 32, V>();
         settle<T>();
         if (!whole1) unsee(buf, 1, s1, dp1);
         cg.read(tile + HALF, by_col, 32), cq.read(tile, by_col, 32);
         order();
-        cg.weigh(dv, s1), cq.weigh(dk, dp1);
+        cg.weigh(dv, s1), cq.weigh_fine(dk, dp1);
         settle<T>();
     };
     auto paired = [&](const char* tile, int buf, int qb, bool whole) {
@@ -603,7 +603,7 @@ void att_bwd_key_kernel(Att a) {
         cq.read(tile, cols);
         order();
         cg.weigh(dv, s);
-        cq.weigh(dk, dp);
+        cq.weigh_fine(dk, dp);
         settle<T>();
     };
     auto compute = [&](const char* tile, int buf) {

@@ -290,6 +290,29 @@ struct ColumnFragments {  // 32 tile rows, `row` rows on from the base's, by col
 #pragma unroll
         for (int d = 0; d < DP / 32; ++d) acc[d] = Eight<T>::mma(f[d][1], hi, acc[d]);
     }
+    // The same for the gradients of q and k, whose weights dx take both signs and
+    // cancel: in fp16, which is chosen for its 11 bits, w goes in two parts, what
+    // the type takes of it and of the rest (errors of those gradients 3.4e-4 to
+    // 2.9e-4 at 2500 tokens of width 64, where the result's own rounding makes
+    // 2.1e-4; 5% of the gradients' time).  In bf16 one part's rounding, at most
+    // 2^-9 of every dx, is of the size of the results' own; two would cost 15%.
+    __device__ __forceinline__ void weigh_fine(f32x16 (&acc)[DP / 32], const f32x16& w) const {
+        if constexpr (!__is_same(T, f16)) return weigh(acc, w);
+        using V = typename Eight<T>::V;
+        const f32x8 a = __builtin_shufflevector(w, w, 0, 1, 2, 3, 4, 5, 6, 7);
+        const f32x8 b = __builtin_shufflevector(w, w, 8, 9, 10, 11, 12, 13, 14, 15);
+        const V lo = Eight<T>::pack(a), hi = Eight<T>::pack(b);
+        const V lo2 = Eight<T>::pack(a - __builtin_convertvector(lo, f32x8));
+        const V hi2 = Eight<T>::pack(b - __builtin_convertvector(hi, f32x8));
+#pragma unroll
+        for (int d = 0; d < DP / 32; ++d) acc[d] = Eight<T>::mma(f[d][0], lo, acc[d]);
+#pragma unroll
+        for (int d = 0; d < DP / 32; ++d) acc[d] = Eight<T>::mma(f[d][1], hi, acc[d]);
+#pragma unroll
+        for (int d = 0; d < DP / 32; ++d) acc[d] = Eight<T>::mma(f[d][0], lo2, acc[d]);
+#pragma unroll
+        for (int d = 0; d < DP / 32; ++d) acc[d] = Eight<T>::mma(f[d][1], hi2, acc[d]);
+    }
 };
 
 // ---------------------------------------------------------------------------
