@@ -339,6 +339,11 @@ def _unit(t: torch.Tensor) -> torch.Tensor:
     return t if t.stride(3) == 1 or t.shape[3] == 1 else t.contiguous()
 
 
+def _graph(*tensors: Optional[torch.Tensor]) -> bool:
+    """A gradient of one of them may be asked for."""
+    return torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in tensors)
+
+
 class _QkNormRotaryFn(torch.autograd.Function):
     @staticmethod
     def forward(ctx, q, k, q_weight, k_weight, cos, sin, positions, eps, interleaved):
@@ -444,9 +449,12 @@ def qk_norm_rotary(q: torch.Tensor, k: torch.Tensor, q_weight: Optional[torch.Te
         raise ValueError(f"heads wider than 512 are not served on the GPU; got {q.shape[3]}")
     ops._require_cuda_ext("qk_norm_rotary")
     w = [None if t is None else t.contiguous() for t in (q_weight, k_weight)]
-    return _QkNormRotaryFn.apply(q, k, w[0], w[1], cos.float().contiguous(),
-                                 sin.float().contiguous(), positions, float(eps),
-                                 bool(interleaved))
+    rest = (w[0], w[1], cos.float().contiguous(), sin.float().contiguous(), positions, float(eps),
+            bool(interleaved))
+    if not _graph(q, k, *w):
+        out = _C.norm_rotary_forward(_unit(q), _unit(k), *rest)
+        return out[0], out[1]
+    return _QkNormRotaryFn.apply(q, k, *rest)
 
 
 def relative_position_bias(table: torch.Tensor, buckets: torch.Tensor, q_len: int, k_len: int
@@ -466,6 +474,8 @@ def relative_position_bias(table: torch.Tensor, buckets: torch.Tensor, q_len: in
         return relative_position_bias_reference(table, buckets, q_len, k_len)
     buckets = _check_buckets(table, buckets, "table")
     ops._require_cuda_ext("relative_position_bias")
+    if not _graph(table):
+        return _C.position_bias_forward(table.contiguous(), buckets, int(q_len), int(k_len))
     return _PositionBiasFn.apply(table, buckets, int(q_len), int(k_len))
 
 
@@ -522,8 +532,13 @@ def biased_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, *,
     if D % 8:
         q, k, v = (torch.nn.functional.pad(t, (0, -D % 8)) for t in (q, k, v))
     q, k, v = _rows16(q), _rows16(k), _rows16(v)
-    del rules["bias_table"]
-    out, log_C = _BiasedAttentionFn.apply(q, k, v, bias_table, rules, bool(return_log_degree))
+    if _graph(q, k, v, bias_table):
+        del rules["bias_table"]
+        out, log_C = _BiasedAttentionFn.apply(q, k, v, bias_table, rules, bool(return_log_degree))
+    else:
+        if bias_table is not None:
+            rules["bias_table"] = bias_table.contiguous()
+        out, log_C, _ = _C.attention_forward(q, k, v, rules, bool(return_log_degree), False)
     if D % 8:
         out = out[..., :D]
     return (out, log_C) if return_log_degree else out

@@ -16,7 +16,7 @@
 #include <algorithm>
 #include <cmath>
 
-#include "nsh_common.hpp"
+#include "divisor.hpp"
 
 namespace nsh {
 
@@ -29,6 +29,7 @@ struct NormSide {
     int64_t xs[3], gs[3];
     void *out, *gw;
     int H, blocks;
+    Divisor by_h;
 };
 
 struct NormArgs {
@@ -37,7 +38,10 @@ struct NormArgs {
     const int32_t* positions;
     int64_t pos_stride;
     int L, D, half, interleaved;
+    int full;         // the row's two halves are its lanes' two halves
+    float inv_d;      // 1 / D
     uint32_t tokens;  // B * L
+    Divisor by_l;
     int64_t rows;
     float eps;
     float* partial;  // (blocks of both, D)
@@ -54,6 +58,60 @@ __device__ __forceinline__ void load_cols(const T* p, int d0, int D, float (&o)[
 #pragma unroll
             for (int k = 0; k < VEC; ++k) o[k] = 0.f;
         }
+    }
+}
+
+typedef float fx8 __attribute__((ext_vector_type(8)));
+typedef float fx4 __attribute__((ext_vector_type(4)));
+
+// Rounded to nearest even by the conversion instructions.
+template <typename T, int VEC>
+__device__ __forceinline__ void store_cols(T* p, const float (&v)[VEC]) {
+    if constexpr (VEC == 8 && __is_same(T, bf16)) {
+        typedef __bf16 V __attribute__((ext_vector_type(8)));
+        *reinterpret_cast<V*>(p) = __builtin_convertvector((fx8{v[0], v[1], v[2], v[3], v[4], v[5], v[6], v[7]}), V);
+    } else if constexpr (VEC == 8 && __is_same(T, f16)) {
+        typedef _Float16 V __attribute__((ext_vector_type(8)));
+        *reinterpret_cast<V*>(p) = __builtin_convertvector((fx8{v[0], v[1], v[2], v[3], v[4], v[5], v[6], v[7]}), V);
+    } else if constexpr (VEC == 4 && __is_same(T, float)) {
+        *reinterpret_cast<fx4*>(p) = fx4{v[0], v[1], v[2], v[3]};
+    } else {
+        store_acc<T, VEC>(p, v, false);
+    }
+}
+
+// Lane exchanges within a group without LDS: DPP in rows of 16 lanes, swaps of
+// rows beyond.
+template <int CTRL>
+__device__ __forceinline__ float dpp(float v) {
+    return __int_as_float(__builtin_amdgcn_mov_dpp(__float_as_int(v), CTRL, 0xf, 0xf, true));
+}
+__device__ __forceinline__ float sum_rows(float v) {  // with the row of 16 lanes next to it
+    const auto r = __builtin_amdgcn_permlane16_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+    return __uint_as_float(r[0]) + __uint_as_float(r[1]);
+}
+__device__ __forceinline__ float sum_halves(float v) {
+    const auto r = __builtin_amdgcn_permlane32_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+    return __uint_as_float(r[0]) + __uint_as_float(r[1]);
+}
+
+// The value of lane ^ (G / 2).
+template <int G>
+__device__ __forceinline__ float across(float v) {
+    const uint32_t x = __float_as_uint(v);
+    if constexpr (G == 8) {
+        // lanes 4 b .. 4 b + 3 of a row of 16: even b from four lanes on, odd from four before
+        int t = __builtin_amdgcn_update_dpp(0, static_cast<int>(x), 0x104, 0xf, 0x5, true);
+        t = __builtin_amdgcn_update_dpp(t, static_cast<int>(x), 0x114, 0xf, 0xa, false);
+        return __int_as_float(t);
+    } else if constexpr (G == 16) {
+        return dpp<0x128>(v);  // rotation by 8
+    } else if constexpr (G == 32) {
+        const auto r = __builtin_amdgcn_permlane16_swap(x, x, false, false);
+        return __uint_as_float(threadIdx.x & 16 ? r[0] : r[1]);
+    } else {
+        const auto r = __builtin_amdgcn_permlane32_swap(x, x, false, false);
+        return __uint_as_float(threadIdx.x & 32 ? r[0] : r[1]);
     }
 }
 
@@ -85,8 +143,13 @@ __device__ __forceinline__ void rotate(float (&y)[N][VEC], const NormArgs& a, in
             const int other = first ? lane + a.half / VEC : lane - a.half / VEC;
             const int base = (threadIdx.x & 63 & ~(G - 1)) + (other & (G - 1));
             float z[VEC];
+            if (a.full) {
 #pragma unroll
-            for (int k = 0; k < VEC; ++k) z[k] = __shfl(y[0][k], base);
+                for (int k = 0; k < VEC; ++k) z[k] = across<G>(y[0][k]);
+            } else {
+#pragma unroll
+                for (int k = 0; k < VEC; ++k) z[k] = __shfl(y[0][k], base);
+            }
             if (d0 < rot) {
                 const int e = first ? d0 : d0 - a.half;
                 float c[VEC], s[VEC];
@@ -125,18 +188,24 @@ __device__ __forceinline__ void rotate(float (&y)[N][VEC], const NormArgs& a, in
 
 template <int G>
 __device__ __forceinline__ float group_sum(float v) {
-#pragma unroll
-    for (int k = G / 2; k; k >>= 1) v += __shfl_xor(v, k);
+    v += dpp<0xB1>(v);   // lane ^ 1
+    v += dpp<0x4E>(v);   // lane ^ 2
+    v += dpp<0x141>(v);  // mirrored in eight lanes, whose fours agree
+    if constexpr (G >= 16) v += dpp<0x140>(v);  // mirrored in 16
+    if constexpr (G >= 32) v = sum_rows(v);
+    if constexpr (G >= 64) v = sum_halves(v);
     return v;
 }
 
-template <typename T, int VEC, int N, int G, int THREADS, bool BWD>
+// ROWS rows of a group go at once, all their loads first: a row's loads hang on
+// its position's, and one row a group leaves too few bytes under way.
+template <typename T, int VEC, int N, int G, int THREADS, bool BWD, int ROWS>
 __global__ __launch_bounds__(THREADS) void norm_rotary_kernel(NormArgs a) {
     __shared__ float lds[VEC == 1 || BWD ? (VEC == 1 ? kNormMaxD : THREADS * VEC) : 1];
     const bool key = static_cast<int>(blockIdx.x) >= a.side[0].blocks;
     const NormSide& sd = a.side[key];
     const int block = key ? blockIdx.x - a.side[0].blocks : blockIdx.x;
-    constexpr int kRows = THREADS / G;
+    constexpr int kRows = THREADS / G * ROWS;
     const int lane = threadIdx.x % G, group = threadIdx.x / G;
     const int64_t total = static_cast<int64_t>(a.tokens) * sd.H;
     float w[N][VEC], gw[N][VEC];
@@ -149,60 +218,68 @@ __global__ __launch_bounds__(THREADS) void norm_rotary_kernel(NormArgs a) {
     // every lane of the workgroup takes every turn: the groups meet in shuffles
     for (int64_t r0 = static_cast<int64_t>(block) * kRows; r0 < total;
          r0 += static_cast<int64_t>(sd.blocks) * kRows) {
-        const int64_t r = r0 + group;
-        const bool live = r < total;
-        const uint32_t rr = live ? static_cast<uint32_t>(r) : 0u;
-        const uint32_t token = rr / static_cast<uint32_t>(sd.H), h = rr - token * sd.H;
-        const uint32_t b = token / static_cast<uint32_t>(a.L), t = token - b * a.L;
-        const int64_t pos = a.positions ? a.positions[b * a.pos_stride + t] : t;
-        const bool ok = pos >= 0 && pos < a.rows;
-        const float* cs = a.cos + (ok ? pos : 0) * a.half;
-        const float* sn = a.sin + (ok ? pos : 0) * a.half;
-        const T* x = static_cast<const T*>(sd.x) + b * sd.xs[0] + h * sd.xs[1] + t * sd.xs[2];
-        float v[N][VEC], sq = 0.f;
+        float v[ROWS][N][VEC], g[BWD ? ROWS : 1][N][VEC];
+        bool live[ROWS], ok[ROWS];
+        int64_t pos[ROWS];
+        T* out[ROWS];
 #pragma unroll
-        for (int n = 0; n < N; ++n) {
-            load_cols<T, VEC>(x, (n * G + lane) * VEC, a.D, v[n]);
+        for (int u = 0; u < ROWS; ++u) {
+            const int64_t r = r0 + group * ROWS + u;
+            live[u] = r < total;
+            const uint32_t rr = live[u] ? static_cast<uint32_t>(r) : 0u;
+            const uint32_t token = sd.by_h(rr), h = rr - token * sd.H;
+            const uint32_t b = a.by_l(token), t = token - b * a.L;
+            pos[u] = a.positions ? a.positions[b * a.pos_stride + t] : t;
+            const T* x = static_cast<const T*>(sd.x) + b * sd.xs[0] + h * sd.xs[1] + t * sd.xs[2];
+            out[u] = static_cast<T*>(sd.out) + ((static_cast<int64_t>(b) * sd.H + h) * a.L + t) * a.D;
 #pragma unroll
-            for (int k = 0; k < VEC; ++k) sq = fma_acc(v[n][k], v[n][k], sq);
+            for (int n = 0; n < N; ++n) load_cols<T, VEC>(x, (n * G + lane) * VEC, a.D, v[u][n]);
+            if constexpr (BWD) {
+                const T* gp = static_cast<const T*>(sd.g) + b * sd.gs[0] + h * sd.gs[1] + t * sd.gs[2];
+#pragma unroll
+                for (int n = 0; n < N; ++n) load_cols<T, VEC>(gp, (n * G + lane) * VEC, a.D, g[u][n]);
+            }
         }
-        float g[N][VEC];
-        if constexpr (BWD) {
-            const T* gp = static_cast<const T*>(sd.g) + b * sd.gs[0] + h * sd.gs[1] + t * sd.gs[2];
 #pragma unroll
-            for (int n = 0; n < N; ++n) load_cols<T, VEC>(gp, (n * G + lane) * VEC, a.D, g[n]);
-        }
-        const float rs = 1.f / sqrtf(group_sum<G>(sq) / a.D + a.eps);
-        if constexpr (!BWD) {
+        for (int u = 0; u < ROWS; ++u) {
+            ok[u] = pos[u] >= 0 && pos[u] < a.rows;
+            const float* cs = a.cos + (ok[u] ? pos[u] : 0) * a.half;
+            const float* sn = a.sin + (ok[u] ? pos[u] : 0) * a.half;
+            float sq = 0.f;
 #pragma unroll
             for (int n = 0; n < N; ++n)
 #pragma unroll
-                for (int k = 0; k < VEC; ++k) v[n][k] = v[n][k] * rs * w[n][k];
-            rotate<VEC, N, G>(v, a, lane, cs, sn, ok, 1.f, lds);
-        } else {
-            rotate<VEC, N, G>(g, a, lane, cs, sn, ok, -1.f, lds);
-            float dot = 0.f;
+                for (int k = 0; k < VEC; ++k) sq = fma_acc(v[u][n][k], v[u][n][k], sq);
+            const float rs = __builtin_amdgcn_rsqf(fma_acc(group_sum<G>(sq), a.inv_d, a.eps));
+            if constexpr (!BWD) {
 #pragma unroll
-            for (int n = 0; n < N; ++n)
+                for (int n = 0; n < N; ++n)
 #pragma unroll
-                for (int k = 0; k < VEC; ++k) {
-                    if (live) gw[n][k] = fma_acc(g[n][k] * rs, v[n][k], gw[n][k]);
-                    g[n][k] *= w[n][k];
-                    dot = fma_acc(g[n][k], v[n][k], dot);
+                    for (int k = 0; k < VEC; ++k) v[u][n][k] = v[u][n][k] * rs * w[n][k];
+                rotate<VEC, N, G>(v[u], a, lane, cs, sn, ok[u], 1.f, lds);
+            } else {
+                rotate<VEC, N, G>(g[u], a, lane, cs, sn, ok[u], -1.f, lds);
+                float dot = 0.f;
+#pragma unroll
+                for (int n = 0; n < N; ++n)
+#pragma unroll
+                    for (int k = 0; k < VEC; ++k) {
+                        if (live[u]) gw[n][k] = fma_acc(g[u][n][k] * rs, v[u][n][k], gw[n][k]);
+                        g[u][n][k] *= w[n][k];
+                        dot = fma_acc(g[u][n][k], v[u][n][k], dot);
+                    }
+                dot = group_sum<G>(dot) * a.inv_d * rs * rs;
+#pragma unroll
+                for (int n = 0; n < N; ++n)
+#pragma unroll
+                    for (int k = 0; k < VEC; ++k) v[u][n][k] = rs * (g[u][n][k] - v[u][n][k] * dot);
+            }
+            if (live[u]) {
+#pragma unroll
+                for (int n = 0; n < N; ++n) {
+                    const int d0 = (n * G + lane) * VEC;
+                    if (d0 < a.D) store_cols<T, VEC>(out[u] + d0, v[u][n]);
                 }
-            dot = group_sum<G>(dot) / a.D * rs * rs;
-#pragma unroll
-            for (int n = 0; n < N; ++n)
-#pragma unroll
-                for (int k = 0; k < VEC; ++k) v[n][k] = rs * (g[n][k] - v[n][k] * dot);
-        }
-        if (live) {
-            T* out = static_cast<T*>(sd.out) +
-                     ((static_cast<int64_t>(b) * sd.H + h) * a.L + t) * a.D;
-#pragma unroll
-            for (int n = 0; n < N; ++n) {
-                const int d0 = (n * G + lane) * VEC;
-                if (d0 < a.D) store_acc<T, VEC>(out + d0, v[n], false);
             }
         }
     }
@@ -219,31 +296,31 @@ __global__ __launch_bounds__(THREADS) void norm_rotary_kernel(NormArgs a) {
             __syncthreads();
             for (int d = threadIdx.x; d < a.D; d += THREADS) {
                 float s = 0.f;
-                for (int i = 0; i < kRows; ++i) s += lds[i * G * VEC + d];
+                for (int i = 0; i < THREADS / G; ++i) s += lds[i * G * VEC + d];
                 part[d] = s;
             }
         }
     }
 }
 
-// 32 columns of one side per workgroup, eight runs of blocks each.
+// 32 columns of one side per workgroup, 32 runs of blocks each.
 template <typename T>
-__global__ __launch_bounds__(256) void norm_weight_kernel(NormArgs a) {
-    __shared__ float part[8][32];
+__global__ __launch_bounds__(1024) void norm_weight_kernel(NormArgs a) {
+    __shared__ float part[32][32];
     const NormSide& sd = a.side[blockIdx.y];
     if (!sd.gw) return;
     const int c = threadIdx.x % 32, run = threadIdx.x / 32, d = blockIdx.x * 32 + c;
     const float* at = a.partial + (blockIdx.y ? static_cast<int64_t>(a.side[0].blocks) * a.D : 0);
-    const int len = (sd.blocks + 7) / 8, end = min(sd.blocks, (run + 1) * len);
+    const int len = (sd.blocks + 31) / 32, end = min(sd.blocks, (run + 1) * len);
     float s = 0.f;
     if (d < a.D) {
-#pragma unroll 8
+#pragma unroll 16
         for (int i = run * len; i < end; ++i) s += at[static_cast<int64_t>(i) * a.D + d];
     }
     part[run][c] = s;
     __syncthreads();
     if (run == 0 && d < a.D) {
-        for (int i = 1; i < 8; ++i) s += part[i][c];
+        for (int i = 1; i < 32; ++i) s += part[i][c];
         static_cast<T*>(sd.gw)[d] = from_acc<T>(s);
     }
 }
@@ -265,35 +342,48 @@ static bool norm_vectors(const nsh_norm_rotary_args* g, bool bwd) {
 // Workgroups of a side: enough to fill the card, few enough that their sums of
 // the weight gradient stay small.
 static int norm_blocks(int64_t rows, int per, bool bwd) {
-    const int64_t most = static_cast<int64_t>(nsh_host::compute_units()) * (bwd ? 8 : 64);
+    const int64_t most = static_cast<int64_t>(nsh_host::compute_units()) * (bwd ? 8 : 16);
     return static_cast<int>(std::min(nsh_host::ceil_div(rows, per), most));
 }
 
-template <typename T, int VEC, int N, int G, int THREADS>
+template <typename T, int VEC, int N, int G, int THREADS, int ROWS>
 static int norm_launch(NormArgs a, bool bwd, hipStream_t st) {
     for (auto& sd : a.side)
-        sd.blocks = norm_blocks(static_cast<int64_t>(a.tokens) * sd.H, THREADS / G, bwd);
+        sd.blocks = norm_blocks(static_cast<int64_t>(a.tokens) * sd.H, THREADS / G * ROWS, bwd);
+    a.full = VEC > 1 && !a.interleaved && 2 * a.half == G * VEC;
     const unsigned grid = a.side[0].blocks + a.side[1].blocks;
     if (bwd) {
-        norm_rotary_kernel<T, VEC, N, G, THREADS, true><<<grid, THREADS, 0, st>>>(a);
+        norm_rotary_kernel<T, VEC, N, G, THREADS, true, ROWS><<<grid, THREADS, 0, st>>>(a);
         if (a.partial)
-            norm_weight_kernel<T><<<dim3((a.D + 31) / 32, 2), 256, 0, st>>>(a);
+            norm_weight_kernel<T><<<dim3((a.D + 31) / 32, 2), 1024, 0, st>>>(a);
     } else {
-        norm_rotary_kernel<T, VEC, N, G, THREADS, false><<<grid, THREADS, 0, st>>>(a);
+        norm_rotary_kernel<T, VEC, N, G, THREADS, false, ROWS><<<grid, THREADS, 0, st>>>(a);
     }
     return nsh_host::check_launch(bwd ? "norm_rotary_backward" : "norm_rotary_forward");
+}
+
+// Two rows at once, forward, where that leaves no CU without work (4 x 20 heads
+// of 4096 tokens, bf16: 38.7 us with one, 35.1 with two, 40.1 with four).  The
+// backward has two tensors' loads under way with one (60.5 us, 67.9 with two).
+template <typename T, int G>
+static int norm_rows(const NormArgs& a, bool bwd, hipStream_t st) {
+    constexpr int V = 16 / sizeof(T);
+    const int64_t rows = static_cast<int64_t>(a.tokens) * (a.side[0].H + a.side[1].H);
+    const bool many = rows * G >= static_cast<int64_t>(nsh_host::compute_units()) * kNormThreads * 8;
+    return many && !bwd ? norm_launch<T, V, 1, G, kNormThreads, 2>(a, bwd, st)
+                        : norm_launch<T, V, 1, G, kNormThreads, 1>(a, bwd, st);
 }
 
 template <typename T>
 static int norm_dispatch(const NormArgs& a, bool vectors, bool bwd, hipStream_t st) {
     constexpr int V = 16 / sizeof(T);
-    if (!vectors) return norm_launch<T, 1, kNormMaxD / 64, 64, 64>(a, bwd, st);
+    if (!vectors) return norm_launch<T, 1, kNormMaxD / 64, 64, 64, 1>(a, bwd, st);
     const int lanes = a.D / V;
-    if (lanes <= 8) return norm_launch<T, V, 1, 8, kNormThreads>(a, bwd, st);
-    if (lanes <= 16) return norm_launch<T, V, 1, 16, kNormThreads>(a, bwd, st);
-    if (lanes <= 32) return norm_launch<T, V, 1, 32, kNormThreads>(a, bwd, st);
-    if (lanes <= 64) return norm_launch<T, V, 1, 64, kNormThreads>(a, bwd, st);
-    return norm_launch<T, 1, kNormMaxD / 64, 64, 64>(a, bwd, st);
+    if (lanes <= 8) return norm_rows<T, 8>(a, bwd, st);
+    if (lanes <= 16) return norm_rows<T, 16>(a, bwd, st);
+    if (lanes <= 32) return norm_rows<T, 32>(a, bwd, st);
+    if (lanes <= 64) return norm_rows<T, 64>(a, bwd, st);
+    return norm_launch<T, 1, kNormMaxD / 64, 64, 64, 1>(a, bwd, st);
 }
 
 }  // namespace nsh
@@ -331,10 +421,12 @@ static int norm_rotary(const char* op, const nsh_norm_rotary_args* g, bool bwd, 
     a.L = static_cast<int>(g->L), a.D = static_cast<int>(g->D), a.half = static_cast<int>(g->half);
     a.interleaved = g->interleaved != 0;
     a.tokens = static_cast<uint32_t>(g->B * g->L);
+    a.inv_d = 1.f / static_cast<float>(a.D), a.by_l = nsh::Divisor::of(static_cast<uint32_t>(g->L));
     a.rows = g->rows, a.eps = static_cast<float>(g->eps);
     nsh::NormSide &q = a.side[0], &k = a.side[1];
     q.x = g->q, q.w = g->q_weight, q.H = static_cast<int>(g->Hq);
     k.x = g->k, k.w = g->k_weight, k.H = static_cast<int>(g->Hk);
+    for (auto& sd : a.side) sd.by_h = nsh::Divisor::of(static_cast<uint32_t>(std::max(sd.H, 1)));
     for (int i = 0; i < 3; ++i) q.xs[i] = g->q_stride[i], k.xs[i] = g->k_stride[i];
     if (bwd) {
         q.g = g->grad_q_out, k.g = g->grad_k_out, q.out = g->grad_q, k.out = g->grad_k;

@@ -8,14 +8,16 @@
 // each of the 2R + 1 relative positions in LDS and writes a run of the head's
 // places; a vector whose places are all beyond R takes one value.
 // Backward: a read of every element once.  A workgroup takes kBiasRows rows of
-// a head.  Within the reach, a thread owns relative positions and walks the
-// rows along its diagonals (neighbouring lanes read neighbouring elements); the
-// two far ends of a row, one relative position each, go 16 bytes a lane.  The
+// a head, which are one run of memory: 16 bytes a lane, for the two far ends of
+// every row, one relative position each.  Within the reach, a thread then owns
+// relative positions and walks the rows along its diagonals (neighbouring lanes
+// read neighbouring elements), which are in the caches by then.  The
 // sums per relative position go to a workspace, and one workgroup per head adds
 // them, first over the workgroups, then over each bucket's relative positions:
 // all in a fixed order.
 #include <algorithm>
 
+#include "divisor.hpp"
 #include "positionbias.hpp"
 
 namespace nsh {
@@ -86,39 +88,80 @@ __global__ __launch_bounds__(kBiasThreads) void bias_fwd_kernel(
     }
 }
 
-// The sum of p[0..n) over the workgroup's lanes (each lane's own share).
+// The far sums of `rows` whole rows from row i on, which lie in one run of
+// memory: 16 bytes a lane at a time, eight loads under way.  A vector across a
+// border of the reach, or of a row, is taken apart.
 template <typename T, int VEC>
-__device__ __forceinline__ float span_sum(const T* p, int n, int lane, int lanes) {
-    float s = 0.f;
-    const int lead = static_cast<int>(
-        (VEC - reinterpret_cast<uintptr_t>(p) / sizeof(T) % VEC) % VEC);
-    if (n <= lead) return lane < n ? to_acc(p[lane]) : 0.f;
-    if (lane < lead) s = to_acc(p[lane]);
-    p += lead, n -= lead;
-    const int whole = n / VEC;
-#pragma unroll 4
-    for (int k = lane; k < whole; k += lanes) {
-        float v[VEC];
-        load_acc<T, VEC>(p + static_cast<int64_t>(k) * VEC, v);
+__device__ __forceinline__ void far_sums(const T* g, int i, int rows, int Lk, Divisor by_lk, int off, int R,
+                                         float& low, float& high) {
+    const uint32_t n = static_cast<uint32_t>(rows) * Lk;  // below 2^31
+    const uint32_t cut = static_cast<uint32_t>((VEC - reinterpret_cast<uintptr_t>(g) / sizeof(T) % VEC) % VEC);
+    const uint32_t lead = cut < n ? cut : n, whole = (n - lead) / VEC;
+    auto one = [&](uint32_t e) {
+        const uint32_t row = by_lk(e);
+        const int rel = static_cast<int>(e - row * Lk) - (i + static_cast<int>(row) + off);
+        const float v = to_acc(g[e]);
+        if (rel <= -R) low += v;
+        else if (rel >= R) high += v;
+    };
+    if (threadIdx.x < lead) one(threadIdx.x);
+    auto take = [&](uint32_t k, const float (&v)[VEC]) {
+        const uint32_t e = lead + k * VEC;
+        const uint32_t row = by_lk(e);
+        int j = static_cast<int>(e - row * Lk), rel = j - (i + static_cast<int>(row) + off);
+        const bool split = j + VEC > Lk;
         float u = v[0];
 #pragma unroll
         for (int c = 1; c < VEC; ++c) u += v[c];
-        s += u;
+        if (!split && (rel + VEC - 1 <= -R || rel >= R)) {
+            (rel >= R ? high : low) += u;
+        } else if (split || rel <= -R || rel + VEC - 1 >= R) {
+#pragma unroll
+            for (int c = 0; c < VEC; ++c) {
+                if (rel <= -R) low += v[c];
+                else if (rel >= R) high += v[c];
+                ++rel;
+                if (++j == Lk) j = 0, rel -= Lk + 1;
+            }
+        }
+    };
+    constexpr int kWay = 8;
+    uint32_t k = threadIdx.x;
+    for (; k + (kWay - 1) * kBiasThreads < whole; k += kWay * kBiasThreads) {
+        Pack<T, VEC> p[kWay];
+#pragma unroll
+        for (int w = 0; w < kWay; ++w) p[w] = load_pack<T, VEC>(g + lead + (k + w * kBiasThreads) * VEC);
+#pragma unroll
+        for (int w = 0; w < kWay; ++w) {
+            float v[VEC];
+#pragma unroll
+            for (int c = 0; c < VEC; ++c) v[c] = to_acc(p[w].e[c]);
+            take(k + w * kBiasThreads, v);
+        }
     }
-    if (lane < n - whole * VEC) s += to_acc(p[static_cast<int64_t>(whole) * VEC + lane]);
-    return s;
+    for (; k < whole; k += kBiasThreads) {
+        float v[VEC];
+        load_acc<T, VEC>(g + lead + k * VEC, v);
+        take(k, v);
+    }
+    const uint32_t tail = lead + whole * VEC + threadIdx.x;
+    if (tail < n) one(tail);
 }
 
 template <typename T, int VEC>
 __global__ __launch_bounds__(kBiasThreads) void bias_bwd_kernel(const T* __restrict__ go, int Lq,
-                                                                int Lk, int R,
+                                                                int Lk, Divisor by_lk, int R,
                                                                 float* __restrict__ partial) {
     __shared__ float ends[2][kBiasThreads / 64];
     const int h = blockIdx.y, i0 = blockIdx.x * kBiasRows, i1 = min(Lq, i0 + kBiasRows);
     const int off = Lk - Lq, t = threadIdx.x;
     const T* g = go + static_cast<int64_t>(h) * Lq * Lk;
     float* part = partial + (static_cast<int64_t>(h) * gridDim.x + blockIdx.x) * (2 * R + 1);
-    for (int r = t - R + 1; r < R; r += kBiasThreads) {
+    float low = 0.f, high = 0.f;
+    const int step = Lk <= (1 << 25) ? kBiasRows : 1;
+    for (int i = i0; i < i1; i += step)
+        far_sums<T, VEC>(g + static_cast<int64_t>(i) * Lk, i, min(step, i1 - i), Lk, by_lk, off, R, low, high);
+    for (int r = t - R + 1; r < R; r += kBiasThreads) {  // of what the far sums have just brought in
         float s = 0.f;
 #pragma unroll 8
         for (int i = i0; i < i1; ++i) {
@@ -127,14 +170,7 @@ __global__ __launch_bounds__(kBiasThreads) void bias_bwd_kernel(const T* __restr
         }
         part[r + R] = s;
     }
-    float low = 0.f, high = 0.f;
     const int wave = t / 64, lane = t % 64;
-    for (int i = i0 + wave; i < i1; i += kBiasThreads / 64) {
-        const T* row = g + static_cast<int64_t>(i) * Lk;
-        const int left = min(Lk, max(0, i + off - R + 1)), right = min(Lk, max(left, i + off + R));
-        low += span_sum<T, VEC>(row, left, lane, 64);
-        high += span_sum<T, VEC>(row + right, Lk - right, lane, 64);
-    }
 #pragma unroll
     for (int k = 32; k; k >>= 1) low += __shfl_xor(low, k), high += __shfl_xor(high, k);
     if (lane == 0) ends[0][wave] = low, ends[1][wave] = high;
@@ -221,7 +257,7 @@ static int bias_backward(const void* go, const int32_t* buckets, int64_t H, int6
     bias_bwd_kernel<T, 16 / sizeof(T)>
         <<<dim3(static_cast<unsigned>(chunks), static_cast<unsigned>(H)), kBiasThreads, 0, st>>>(
             static_cast<const T*>(go), static_cast<int>(Lq), static_cast<int>(Lk),
-            static_cast<int>(R), partial);
+            Divisor::of(static_cast<uint32_t>(Lk)), static_cast<int>(R), partial);
     if (int rc = nsh_host::check_launch("position_bias_backward")) return rc;
     return table_gradient(partial, buckets, H, chunks, nb, R, dtype, gt, st);
 }
