@@ -61,10 +61,9 @@ struct Row {
     int p, lim, doc;
 };
 
-__device__ __forceinline__ Row row_of(const Att& a, int b, int i, int n) {
+__device__ __forceinline__ Row row_of(const Att& a, int b, int i, int n, int prefix) {
     Row r;
     r.p = i + n - a.Lq;
-    const int prefix = a.prefix ? a.prefix[b] : 0;
     r.lim = a.causal ? min(n, max(r.p + 1, prefix)) : n;
     r.doc = 0;
     if (a.documents) {
@@ -72,6 +71,9 @@ __device__ __forceinline__ Row row_of(const Att& a, int b, int i, int n) {
         if (r.doc < 0) r.lim = 0;
     }
     return r;
+}
+__device__ __forceinline__ Row row_of(const Att& a, int b, int i, int n) {
+    return row_of(a, b, i, n, a.prefix ? a.prefix[b] : 0);
 }
 
 __device__ __forceinline__ bool sees(const Att& a, const Row& r, int b, int j) {

@@ -233,7 +233,7 @@ __global__ __launch_bounds__(kAttThreads, SPLIT || DP * sizeof(T) > (KIND == kGe
         }
     };
     auto step = [&](char* tile, int* docs, char* ahead, int* docs_ahead) {
-        const int tn = need.next(t + 1, end);
+        const int tn = KIND == kGeneral && a.documents ? need.next(t + 1, end) : t + 1;
         __builtin_amdgcn_s_waitcnt(0x0f70);  // vmcnt(0): the tile has landed
         if (!SPLIT) __syncthreads();
         if (NBUF == 2 && tn < end) load(tn, ahead, docs_ahead);
@@ -398,10 +398,20 @@ void att_bwd_key_kernel(Att a) {
     Loader<T, DP, QT, 4> lq, lg;
     lq.init(threadIdx.x & 255, second ? a.gos[2] : a.qs[2], a.D);
     if (!PAIRED) lg.init(threadIdx.x, a.gos[2], a.D);
-    auto head = [&](int u) { return hk * a.per + u / (t1 - t0); };
-    auto first = [&](int u) { return (t0 + u % (t1 - t0)) * QT; };
-    auto load = [&](int u, char* tile) {
-        const int h = head(u), i0 = first(u);
+    // a unit's head and first row, kept up by addition
+    struct Unit {
+        int u, h, i0;
+    };
+    auto onward = [&](Unit x) {
+        const int u = KIND == kGeneral && a.documents ? need.next(x.u + 1, u1) : x.u + 1;
+        int64_t i0 = x.i0 + static_cast<int64_t>(u - x.u) * QT;
+        if (u < u1)
+            while (i0 >= static_cast<int64_t>(t1) * QT) i0 -= static_cast<int64_t>(t1 - t0) * QT, ++x.h;
+        x.u = u, x.i0 = static_cast<int>(i0);
+        return x;
+    };
+    auto load = [&](const Unit& x, char* tile) {
+        const int h = x.h, i0 = x.i0;
         if (PAIRED) {
             const T* base = second ? row_at<T>(a.go, a.gos, b, h, 0) : row_at<T>(a.q, a.qs, b, h, 0);
             lq.load(tile + (second ? HALF : 0), base, second ? a.gos[2] : a.qs[2], i0, a.Lq, a.D, kw);
@@ -414,14 +424,14 @@ void att_bwd_key_kernel(Att a) {
     float2 r_stat{};
     float r_delta = 0.f;
     int r_lim = 0, r_doc = -1;
-    auto fetch = [&](int u) {
+    auto fetch = [&](const Unit& y) {
         const int x = threadIdx.x;
         if (x >= QT) return;
-        const int i = first(u) + x;
+        const int i = y.i0 + x;
         r_stat = make_float2(0.f, 0.f), r_delta = 0.f, r_lim = 0, r_doc = -1;
         if (i < a.Lq) {
-            const int64_t at = (static_cast<int64_t>(b) * a.Hq + head(u)) * a.Lq + i;
-            const Row r = row_of(a, b, i, n);
+            const int64_t at = (static_cast<int64_t>(b) * a.Hq + y.h) * a.Lq + i;
+            const Row r = row_of(a, b, i, n, prefix);
             r_stat = get_stats(a, at), r_delta = a.delta[at], r_lim = r.lim, r_doc = r.doc;
         }
     };
@@ -433,7 +443,9 @@ void att_bwd_key_kernel(Att a) {
         info[buf][4][x] = __int_as_float(r_lim), info[buf][5][x] = __int_as_float(r_doc);
     };
     f32x16 dk[L::ND] = {}, dv[L::ND] = {};
-    int u = need.next(u0, u1), staged = -1;
+    Unit now{need.next(u0, u1), 0, 0};
+    if (now.u < u1) now.h = hk * a.per + now.u / (t1 - t0), now.i0 = (t0 + now.u % (t1 - t0)) * QT;
+    int staged = -1;
     Bias bs{0.f, line};
     // a wave's places in a tile (its half of one, if paired) and among the keys
     const int half = PAIRED ? (wave >> 2) * 32 : 0;
@@ -447,6 +459,8 @@ void att_bwd_key_kernel(Att a) {
         order();
         const f32x16 xs = fq.products(k);
         f32x16 dp = fg.products(v);
+        ColumnFragments<T, DP> cg, cq;
+        if (DP <= 64) cg.read(part + HALF, by_col);
         settle<T>();
         const Scores y = cap_scores<true>(cap, xs);
         f32x16 s = add_bias<-1>(a, bs, j - pf - 4 * g, j0 - pf - 31, j0 + 31 - pf, y.s);
@@ -482,11 +496,11 @@ void att_bwd_key_kernel(Att a) {
             }
         }
         order();
-        ColumnFragments<T, DP> f;
-        f.read(part + HALF, by_col);
-        f.weigh(dv, s);
-        f.read(part, by_col);
-        f.weigh_fine(dk, dp);
+        if (DP > 64) cg.read(part + HALF, by_col);
+        if (DP <= 64) cq.read(part, by_col);
+        cg.weigh(dv, s);
+        if (DP > 64) cq.read(part, by_col);
+        cq.weigh_fine(dk, dp);
         settle<T>();
     };
     // The weights p (in place of the products s) and dx, without a bias.
@@ -607,7 +621,7 @@ void att_bwd_key_kernel(Att a) {
         settle<T>();
     };
     auto compute = [&](const char* tile, int buf) {
-        const int i0 = first(u), p0 = i0 + off;
+        const int i0 = now.i0, p0 = i0 + off;
         // the rows' key ends rise with their position
         auto ends = [&](int p) { return a.causal ? min(n, max(p + 1, prefix)) : n; };
         if constexpr (PAIRED) {
@@ -629,10 +643,10 @@ void att_bwd_key_kernel(Att a) {
         }
     };
     auto step = [&](char* tile, char* ahead, int buf) {
-        const int un = need.next(u + 1, u1);
-        if (KIND == kGeneral && (a.table || a.slopes) && head(u) != staged) {
-            staged = head(u);
-            if (KIND == kGeneral && a.table) {
+        const Unit then = onward(now);
+        if (KIND == kGeneral && (a.table || a.slopes) && now.h != staged) {
+            staged = now.h;
+            if (a.table) {
                 __syncthreads();
                 stage_line<T>(a, staged, line);
             }
@@ -640,22 +654,22 @@ void att_bwd_key_kernel(Att a) {
         }
         __builtin_amdgcn_s_waitcnt(0x0f70);  // vmcnt(0): the tile has landed
         __syncthreads();
-        if (un < u1) {
-            fetch(un);
-            load(un, ahead);
+        if (then.u < u1) {
+            fetch(then);
+            load(then, ahead);
         }
         compute(tile, buf);
-        if (un < u1) put(buf ^ 1);
-        u = un;
+        if (then.u < u1) put(buf ^ 1);
+        now = then;
     };
-    if (u < u1) {
-        fetch(u);
-        load(u, tiles0[0]);
+    if (now.u < u1) {
+        fetch(now);
+        load(now, tiles0[0]);
         put(0);
     }
-    while (u < u1) {
+    while (now.u < u1) {
         step(tiles0[0], tiles1[0], 0);
-        if (u < u1) step(tiles1[0], tiles0[0], 1);
+        if (now.u < u1) step(tiles1[0], tiles0[0], 1);
     }
     if constexpr (PAIRED) {  // the second waves' sums join the first's
         float* sums = reinterpret_cast<float*>(&kv[0][0]) + (kw * DP + 4 * g) * 32 + (l & 31);  // [keys][column][key]

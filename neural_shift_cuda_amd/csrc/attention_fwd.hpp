@@ -201,7 +201,7 @@ __global__ __launch_bounds__(kAttThreads, DP * sizeof(T) > 384 ? 1 : 2) void att
     int t = need.next(0, end);
     const int by_row = L::row_base(0, l), by_col = L::col_base(0, l);
     auto step = [&](char (&tiles)[2][HALF], int (&docs)[64], char (&ahead)[2][HALF], int (&docs_ahead)[64]) {
-        const int tn = need.next(t + 1, end);
+        const int tn = KIND == kGeneral && a.documents ? need.next(t + 1, end) : t + 1;
         __builtin_amdgcn_s_waitcnt(0x0f70);  // vmcnt(0): the tile has landed
         __syncthreads();
         if (tn < end) load(tn, ahead, docs_ahead);
@@ -298,7 +298,7 @@ __global__ __launch_bounds__(kAttThreads, 1) void att_fwd_split_kernel(Att a) {
         for (int s = 0; s < L::NS; ++s) q[s] = Eight<T>::negate(q[s]);
     const int by_row = L::row_base(0, l), by_col = L::col_base(0, l);
     auto step = [&](char* tile, int* docs, char* ahead, int* docs_ahead) {
-        const int tn = need.next(t + 1, end);
+        const int tn = KIND == kGeneral && a.documents ? need.next(t + 1, end) : t + 1;
         __builtin_amdgcn_s_waitcnt(0x0f70);  // vmcnt(0): the tile has landed
         if (S::NBUF == 2 && tn < end) load(tn, ahead, docs_ahead);
         attend<T, DP, 1, KIND>(a, cap, bs, x.r, wr, q, tile, tile + HALF, by_row, by_col, docs, t * 32, l, st);

@@ -180,16 +180,19 @@ struct Loader {
 #pragma unroll
         for (int i = 0; i < NI; ++i) {
             const int x = i * NW * 64 + id, r = x / L::NC, c = (x % L::NC) ^ L::turn(r);
-            off[i] = c * L::CE < D ? static_cast<uint32_t>(r * stride * sizeof(T)) + c * 16 : 0x80000000u;
+            off[i] = c * L::CE < D ? static_cast<uint32_t>(r) * static_cast<uint32_t>(stride * sizeof(T)) + c * 16 : 0x80000000u;
         }
     }
-    // base: the tensor's row 0; first: the tile's first row; rows: its end.
+    // base: the tensor's row 0; bytes: from row to row (2^24 at most); first: the
+    // tile's first row; rows: the tensor's end.
     __device__ __forceinline__ void load(char* lds, const T* base, int64_t stride, int first, int rows,
                                          int D, int wave) const {
-        const int64_t left = (rows - 1 - static_cast<int64_t>(first)) * stride * sizeof(T) + D * sizeof(T);
-        const uint32_t bytes = rows <= first ? 0u : static_cast<uint32_t>(left < 0x7fffffff ? left : 0x7fffffff);
+        const uint32_t bytes = static_cast<uint32_t>(stride) * sizeof(T);
+        const uint32_t left = static_cast<uint32_t>(max(min(rows - first, ROWS), 0));  // rows past the tile are not asked for
+        const uint32_t size = left ? (left - 1) * bytes + D * static_cast<uint32_t>(sizeof(T)) : 0u;
         const __amdgpu_buffer_rsrc_t rs = __builtin_amdgcn_make_buffer_rsrc(
-            const_cast<T*>(base + first * stride), static_cast<short>(0), static_cast<int>(bytes), 0x00020000);
+            const_cast<char*>(reinterpret_cast<const char*>(base) + static_cast<uint64_t>(static_cast<uint32_t>(first)) * bytes),
+            static_cast<short>(0), static_cast<int>(size), 0x00020000);
 #pragma unroll
         for (int i = 0; i < NI; ++i)
             to_lds<16>(rs, lds + (i * NW + wave) * 1024, off[i]);
