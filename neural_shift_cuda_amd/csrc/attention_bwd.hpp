@@ -489,11 +489,14 @@ void att_bwd_key_kernel(Att a) {
             for (int e = 0; e < 4; ++e) {
                 const int r = 4 * c + e;
                 const float w = __builtin_amdgcn_exp2f(s[r] - top[e]) * inv[e];
-                float x = w * (dp[r] - del[e]);
-                if (cap.mode != 0) x *= y.w[r];
-                dp[r] = !whole && s[r] == -INFINITY ? 0.f : x;
+                dp[r] = w * (dp[r] - del[e]);
                 s[r] = w;
             }
+        }
+        if (cap.mode != 0) dp *= y.w;
+        if (!whole) {  // 0 times what an unseen pair holds is not always 0
+#pragma unroll
+            for (int r = 0; r < 16; ++r) dp[r] = s[r] == 0.f ? 0.f : dp[r];
         }
         order();
         if (DP > 64) cg.read(part + HALF, by_col);

@@ -373,27 +373,28 @@ struct Scores {
     f32x16 s, w;
 };
 
+// (w is left open without a cap: nothing reads it.)
 template <bool SLOPE>
 __device__ __forceinline__ Scores cap_scores(const Cap& c, f32x16 s) {
-    f32x16 w = {};
+    Scores x;
     if (c.mode == 0) {
-        s *= c.c;
+        x.s = s * c.c;
     } else if (c.mode == 1) {
 #pragma unroll
         for (int r = 0; r < 16; ++r) {
             const float q = quick_r(s[r], c.k);
-            s[r] = fma_acc(q, -2.f * c.top, c.top);
-            if (SLOPE) w[r] = 4.f * fma_acc(-q, q, q);
+            x.s[r] = fma_acc(q, -2.f * c.top, c.top);
+            if (SLOPE) x.w[r] = 4.f * fma_acc(-q, q, q);
         }
     } else {
 #pragma unroll
         for (int r = 0; r < 16; ++r) {
             const float t = tanh_rel(s[r] * c.inv);
-            s[r] = c.top * t;
-            if (SLOPE) w[r] = fma_acc(-t, t, 1.f);
+            x.s[r] = c.top * t;
+            if (SLOPE) x.w[r] = fma_acc(-t, t, 1.f);
         }
     }
-    return Scores{s, w};
+    return x;
 }
 
 // The bias of a lane's 16 pairs with relative positions rel0 + sign * el(r).
