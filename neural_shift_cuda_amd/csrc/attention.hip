@@ -62,7 +62,7 @@ static void cut_rows(Att& a, bool backward) {
         1, std::min<int64_t>({room / blocks, nsh_host::ceil_div(a.Lk, 32) / keep, 64})));
 }
 
-// Keys go 128 to a workgroup.  `parts` workgroups share a key block's queries
+// Keys go key_block() to a workgroup.  `parts` workgroups share a key block's queries
 // where there are too few of them to go round, as long as each keeps two query
 // tiles; the third launch that adds up their sums costs more than it brings from
 // five workgroups to four CUs on.  4 x 12 heads, 1024 tokens, width 64, bf16 (384
@@ -71,7 +71,7 @@ static void cut_rows(Att& a, bool backward) {
 // tokens, fp32: 60 + 5 with four tiles kept, 38 + 5 with two, 48 + 8 with one.
 static void cut_keys(Att& a) {
     const int64_t cus = nsh_host::compute_units(), tile = a.wide ? 32 : 64;
-    a.kblocks = static_cast<int>(nsh_host::ceil_div(a.Lk, 128));
+    a.kblocks = static_cast<int>(nsh_host::ceil_div(a.Lk, key_block(a.wide ? 4 : 2, a.D)));
     const int64_t blocks = static_cast<int64_t>(a.B) * a.Hk * a.kblocks;
     const int64_t units = nsh_host::ceil_div(a.Lq, tile) * a.per;
     a.parts = 1;

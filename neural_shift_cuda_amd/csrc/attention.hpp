@@ -285,6 +285,9 @@ __device__ __forceinline__ void exact_key_gradient(const Att& a, int b, int hk, 
 // 16-bit weight's half step is 2^-12), small arguments take the series.
 constexpr float kQuickCap = 256.f;
 
+// Keys of a workgroup of the gradients by keys.
+constexpr int key_block(int bytes, int D) { return bytes == 2 && D <= 64 ? 64 : 128; }
+
 // Launches of one type's kernels (attention_fwd_*.hip, attention_bwd_*.hip).
 template <typename T> int attention_forward_launch(const Att& a, hipStream_t st);
 template <typename T> int attention_backward_launch(const Att& a, hipStream_t st);

@@ -323,13 +323,22 @@ __global__ __launch_bounds__(kAttThreads, SPLIT || DP * sizeof(T) > (KIND == kGe
     }
 }
 
-// PAIRED: eight waves, two to 32 keys, one for each half of a 64-row tile.  K and
-// V then stay in LDS rather than in registers: of those, the sums of wide heads
-// leave too few for two waves to a SIMD otherwise, and one wave waits for its
-// own products.
-template <typename T, int DP, Kind KIND, bool PAIRED>
-__global__ __launch_bounds__(PAIRED ? 512 : kAttThreads, PAIRED ? 1 : DP * sizeof(T) >= 256 ? 1 : 2)
+// How the waves share a workgroup's work: KG groups of 32 keys, and QP waves to
+// a group, one for each half of a 64-row tile; the second waves' sums join the
+// first's at the end.
+//   kAlone   4 x 1
+//   kTwin    2 x 2: for heads up to 64 wide, twice the workgroups of half the
+//            length each
+//   kPaired  4 x 2, with K and V in LDS rather than in registers: of those, the
+//            sums of wider heads leave too few for two waves to a SIMD otherwise,
+//            and one wave waits for its own products
+enum Share { kAlone, kTwin, kPaired };
+
+template <typename T, int DP, Kind KIND, Share SHARE>
+__global__ __launch_bounds__(SHARE == kPaired ? 512 : kAttThreads, SHARE != kPaired && DP * sizeof(T) < 256 ? 2 : 1)
 void att_bwd_key_kernel(Att a) {
+    constexpr int KG = SHARE == kTwin ? 2 : 4, QP = SHARE == kAlone ? 1 : 2;
+    constexpr bool PAIRED = SHARE == kPaired;
     using L = Tile<T, DP>;
     constexpr int QT = BwdShape<T, DP>::KT, NB = QT / 32, HALF = QT * L::ROW;
     constexpr int KV = PAIRED ? 128 * L::ROW : 16;
@@ -338,12 +347,12 @@ void att_bwd_key_kernel(Att a) {
     __shared__ __attribute__((aligned(1024))) char tiles1[2][HALF];
     __shared__ __attribute__((aligned(256))) float info[2][6][QT];  // log 2 of weight over score, maximum, 1 / sum, delta, key end, document
     extern __shared__ float line[];
-    const int l = threadIdx.x & 63, wave = wave_id(), g = l >> 5, kw = wave & 3;
+    const int l = threadIdx.x & 63, wave = wave_id(), g = l >> 5, kw = wave % KG;
     int bg, rest;
     place(blockIdx.x, a.B * a.Hk, bg, rest);
     const int b = bg / a.Hk, hk = bg - b * a.Hk, part = rest % a.parts, kb = rest / a.parts;
     const int n = filled_keys(a, b), off = n - a.Lq;
-    const int j0 = kb * 128 + kw * 32, j = j0 + (l & 31);
+    const int j0 = kb * KG * 32 + kw * 32, j = j0 + (l & 31);
     const Cap cap = cap_of<T, KIND>(a, true);
     const int prefix = a.prefix ? a.prefix[b] : 0;
     const int doc = a.documents && j < n ? a.documents[static_cast<int64_t>(b) * a.Lk + j] : 0;
@@ -366,7 +375,7 @@ void att_bwd_key_kernel(Att a) {
 
     // the queries that see any of the block's keys: all of them, or those from
     // the first key's position on
-    const int jb = kb * 128;
+    const int jb = kb * KG * 32;
     int t0 = 0, t1 = jb < n ? (a.Lq + QT - 1) / QT : 0;
     if (a.causal && jb >= prefix) t0 = max(0, jb - off) / QT;
     t0 = min(t0, t1);
@@ -376,7 +385,7 @@ void att_bwd_key_kernel(Att a) {
     if (KIND == kGeneral && a.documents && jb < n) {
         const int e = jb / kRangeKeys;
         own = a.ranges[b * a.nranges + e];
-        if (e + 1 < a.nranges) {
+        if (KG == 4 && e + 1 < a.nranges) {
             const int2 r = a.ranges[b * a.nranges + e + 1];
             own.x = min(own.x, r.x), own.y = max(own.y, r.y);
         }
@@ -448,11 +457,11 @@ void att_bwd_key_kernel(Att a) {
     int staged = -1;
     Bias bs{0.f, line};
     // a wave's places in a tile (its half of one, if paired) and among the keys
-    const int half = PAIRED ? (wave >> 2) * 32 : 0;
+    const int half = QP == 2 ? wave / KG * 32 : 0;
     const int by_row = L::row_base(half, l), by_col = L::col_base(half, l), by_key = L::row_base(kw * 32, l);
     // one 32-row part of a tile, whatever it holds
     auto general = [&](const char* tile, int buf, int qb, int pf, bool whole) {
-        const char* part = tile + qb * 32 * L::ROW;
+        const char* part = QP == 2 ? tile : tile + qb * 32 * L::ROW;
         const float* rows = &info[buf][0][qb * 32 + 4 * g];
         RowFragments<T, DP> fq, fg;
         fq.read(part, by_row), fg.read(part + HALF, by_row);
@@ -546,7 +555,7 @@ void att_bwd_key_kernel(Att a) {
         }
     };
     auto simple = [&](const char* tile, int buf, int qb, bool whole) {
-        const char* part = tile + qb * 32 * L::ROW;
+        const char* part = QP == 2 ? tile : tile + qb * 32 * L::ROW;
         RowFragments<T, DP> fq, fg;
         fq.read(part, by_row), fg.read(part + HALF, by_row);
         order();
@@ -627,9 +636,13 @@ void att_bwd_key_kernel(Att a) {
         const int i0 = now.i0, p0 = i0 + off;
         // the rows' key ends rise with their position
         auto ends = [&](int p) { return a.causal ? min(n, max(p + 1, prefix)) : n; };
-        if constexpr (PAIRED) {
-            const int qb = wave >> 2, pf = p0 + qb * 32, count = min(a.Lq - i0 - qb * 32, 32);
-            if (count > 0 && j0 < ends(pf + count - 1)) paired(tile, buf, qb, j0 + 32 <= ends(pf));
+        if constexpr (QP == 2) {
+            const int qb = wave / KG, pf = p0 + qb * 32, count = min(a.Lq - i0 - qb * 32, 32);
+            if (count <= 0 || j0 >= ends(pf + count - 1)) return;
+            const bool whole = j0 + 32 <= ends(pf) && !(KIND == kGeneral && a.documents);
+            if constexpr (KIND == kGeneral) general(tile, buf, qb, pf, whole);
+            else if constexpr (PAIRED) paired(tile, buf, qb, whole);
+            else simple(tile, buf, qb, whole);
         } else if constexpr (KIND != kGeneral && NB == 2) {
             if (j0 < ends(p0 + min(a.Lq - i0, 64) - 1))
                 both(tile, buf, j0 + 32 <= ends(p0), j0 + 32 <= ends(p0 + 32));
@@ -674,19 +687,20 @@ void att_bwd_key_kernel(Att a) {
         step(tiles0[0], tiles1[0], 0);
         if (now.u < u1) step(tiles1[0], tiles0[0], 1);
     }
-    if constexpr (PAIRED) {  // the second waves' sums join the first's
-        float* sums = reinterpret_cast<float*>(&kv[0][0]) + (kw * DP + 4 * g) * 32 + (l & 31);  // [keys][column][key]
-        static_assert(sizeof(kv) >= 4 * DP * 32 * 4, "four waves' sums of dk take the keys' place");
+    if constexpr (QP == 2) {  // the second waves' sums join the first's
+        float* const room = reinterpret_cast<float*>(PAIRED ? &kv[0][0] : &tiles0[0][0]);
+        float* sums = room + (kw * DP + 4 * g) * 32 + (l & 31);  // [keys][column][key]
+        static_assert((PAIRED ? sizeof(kv) : sizeof(tiles0)) >= KG * DP * 32 * 4, "the sums of dk take the tiles' place");
         auto join = [&](f32x16 (&acc)[L::ND]) {
             __syncthreads();
-            if (wave >= 4) {
+            if (wave >= KG) {
 #pragma unroll
                 for (int d = 0; d < L::ND; ++d)
 #pragma unroll
                     for (int r = 0; r < 16; ++r) sums[(d * 32 + el(r)) * 32] = acc[d][r];
             }
             __syncthreads();
-            if (wave < 4) {
+            if (wave < KG) {
 #pragma unroll
                 for (int d = 0; d < L::ND; ++d)
 #pragma unroll
@@ -695,7 +709,7 @@ void att_bwd_key_kernel(Att a) {
         };
         join(dk);
         join(dv);
-        if (wave >= 4) return;
+        if (wave >= KG) return;
     }
     float bad = 0.f;
 #pragma unroll
@@ -775,9 +789,10 @@ static void backward_kind(const Att& a, hipStream_t st) {
     else
         att_bwd_row_kernel<T, DP, false, KIND><<<static_cast<unsigned>(rows), kAttThreads, attention_row_lds(a), st>>>(a);
     const int64_t keys = static_cast<int64_t>(a.B) * a.Hk * a.kblocks * a.parts;
-    constexpr bool kPaired = KIND != kGeneral && sizeof(T) == 2 && DP >= 96;
-    att_bwd_key_kernel<T, DP, KIND, kPaired>
-        <<<static_cast<unsigned>(keys), kPaired ? 512 : kAttThreads, line, st>>>(a);
+    constexpr Share share = sizeof(T) == 4 ? kAlone : DP <= 64 ? kTwin : KIND != kGeneral ? kPaired : kAlone;
+    static_assert((share == kTwin) == (key_block(sizeof(T), DP) == 64), "the cut agrees");
+    att_bwd_key_kernel<T, DP, KIND, share>
+        <<<static_cast<unsigned>(keys), share == kPaired ? 512 : kAttThreads, line, st>>>(a);
 }
 
 template <typename T, int DP>
