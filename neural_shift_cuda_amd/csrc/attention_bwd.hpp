@@ -115,8 +115,9 @@ __device__ __forceinline__ void row_gradient(const Att& a, const Cap& cap, const
             }
         }
         if (j0 + 32 > wr.least) {  // 0 times what an unseen pair holds is not always 0
+            const int left = here(x.lim - j0 - 4 * (l >> 5));
 #pragma unroll
-            for (int r = 0; r < 16; ++r) dp[r] = j0 + 4 * (l >> 5) + el(r) < x.lim ? dp[r] : 0.f;
+            for (int r = 0; r < 16; ++r) dp[r] = el(r) < left ? dp[r] : 0.f;
         }
     } else {
         settle<T>();
@@ -441,7 +442,8 @@ void att_bwd_key_kernel(Att a) {
         if (i < a.Lq) {
             const int64_t at = (static_cast<int64_t>(b) * a.Hq + y.h) * a.Lq + i;
             const Row r = row_of(a, b, i, n, prefix);
-            r_stat = get_stats(a, at), r_delta = a.delta[at], r_lim = r.lim, r_doc = r.doc;
+            r_stat = get_stats(a, at), r_delta = a.delta[at], r_lim = r.lim;
+            if (KIND == kGeneral) r_doc = r.doc;
         }
     };
     auto put = [&](int buf) {
@@ -449,7 +451,8 @@ void att_bwd_key_kernel(Att a) {
         if (x >= QT) return;
         info[buf][0][x] = __builtin_amdgcn_logf(r_stat.y) - r_stat.x + (cap.mode == 1 ? cap.top : 0.f);
         info[buf][1][x] = r_stat.x, info[buf][2][x] = r_stat.y, info[buf][3][x] = r_delta;
-        info[buf][4][x] = __int_as_float(r_lim), info[buf][5][x] = __int_as_float(r_doc);
+        info[buf][4][x] = __int_as_float(r_lim);
+        if (KIND == kGeneral) info[buf][5][x] = __int_as_float(r_doc);
     };
     f32x16 dk[L::ND] = {}, dv[L::ND] = {};
     Unit now{need.next(u0, u1), 0, 0};
@@ -458,7 +461,8 @@ void att_bwd_key_kernel(Att a) {
     Bias bs{0.f, line};
     // a wave's places in a tile (its half of one, if paired) and among the keys
     const int half = QP == 2 ? wave / KG * 32 : 0;
-    const int by_row = L::row_base(half, l), by_col = L::col_base(half, l), by_key = L::row_base(kw * 32, l);
+    const int by_row = L::row_base(half, l), by_col = L::col_base(half, l);
+    const int key_off = (kw * 32 - half) * L::ROW;  // from a row's place to the keys'
     // one 32-row part of a tile, whatever it holds
     auto general = [&](const char* tile, int buf, int qb, int pf, bool whole) {
         const char* part = QP == 2 ? tile : tile + qb * 32 * L::ROW;
@@ -606,8 +610,7 @@ void att_bwd_key_kernel(Att a) {
     };
     auto paired = [&](const char* tile, int buf, int qb, bool whole) {
         // formed anew for each tile: kept, the reads' addresses would be spilled
-        int rows = by_row, cols = by_col, keys = by_key;
-        asm volatile("" : "+v"(rows), "+v"(cols), "+v"(keys));
+        const int rows = here(by_row), cols = here(by_col), keys = rows + key_off;
         f32x16 s, dp;
         {
             RowFragments<T, DP> f, key;

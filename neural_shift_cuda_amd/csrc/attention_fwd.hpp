@@ -46,11 +46,11 @@ __device__ __forceinline__ void attend(const Att& a, const Cap& cap, const Bias&
         f.read(V, by_col);
         settle<T>();
         if (!whole) {
+            const int left = here(x.lim - j0 - 4 * (l >> 5));
 #pragma unroll
             for (int kb = 0; kb < NB; ++kb)
 #pragma unroll
-                for (int r = 0; r < 16; ++r)
-                    s[kb][r] = j0 + kb * 32 + 4 * (l >> 5) + el(r) < x.lim ? s[kb][r] : -INFINITY;
+                for (int r = 0; r < 16; ++r) s[kb][r] = kb * 32 + el(r) < left ? s[kb][r] : -INFINITY;
         }
     } else {
         settle<T>();
@@ -92,11 +92,11 @@ __device__ __forceinline__ void attend(const Att& a, const Cap& cap, const Bias&
             s[kb][r] = __builtin_amdgcn_exp2f(y);
         }
     if (KIND == kCapped && !whole) {  // the cap of -inf is finite
+        const int left = here(x.lim - j0 - 4 * (l >> 5));
 #pragma unroll
         for (int kb = 0; kb < NB; ++kb)
 #pragma unroll
-            for (int r = 0; r < 16; ++r)
-                s[kb][r] = j0 + kb * 32 + 4 * (l >> 5) + el(r) < x.lim ? s[kb][r] : 0.f;
+            for (int r = 0; r < 16; ++r) s[kb][r] = kb * 32 + el(r) < left ? s[kb][r] : 0.f;
     }
     float z0 = 0.f, z1 = 0.f;
 #pragma unroll

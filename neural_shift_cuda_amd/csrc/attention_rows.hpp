@@ -64,9 +64,9 @@ __device__ __forceinline__ Bias lane_bias(const Att& a, int h, const float* line
 // Not seen -> -inf, for 32 keys from j0 (kd: their documents, in LDS).
 __device__ __forceinline__ f32x16 mask_keys(const Att& a, const Row& x, int j0, const int* kd, int l,
                                             f32x16 s) {
-    const int j = j0 + 4 * (l >> 5);
+    const int left = here(x.lim - j0 - 4 * (l >> 5));
 #pragma unroll
-    for (int r = 0; r < 16; ++r) s[r] = j + el(r) < x.lim ? s[r] : -INFINITY;
+    for (int r = 0; r < 16; ++r) s[r] = el(r) < left ? s[r] : -INFINITY;
     if (a.documents) {
 #pragma unroll
         for (int c = 0; c < 4; ++c) {

@@ -253,6 +253,13 @@ __device__ __forceinline__ void settle() {
     order();
 }
 
+// v, and nothing formed of it ahead of here: what only a branch needs is
+// otherwise computed in front of it.
+__device__ __forceinline__ int here(int v) {
+    asm volatile("" : "+v"(v));
+    return v;
+}
+
 __device__ __forceinline__ int wave_id() { return __builtin_amdgcn_readfirstlane(threadIdx.x >> 6); }
 
 // Kinds of call, each with kernels of its own: no bias and no documents, without
