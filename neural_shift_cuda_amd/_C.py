@@ -958,7 +958,7 @@ def _like(t: torch.Tensor, heads: int, tokens: int, width: int) -> torch.Tensor:
     return t.new_empty((B, heads, tokens, width))
 
 
-def _workspace(t: torch.Tensor, n: int) -> Optional[torch.Tensor]:
+def _scratch(t: torch.Tensor, n: int) -> Optional[torch.Tensor]:
     return torch.empty(n, dtype=torch.uint8, device=t.device) if n > 0 else None
 
 
@@ -1002,7 +1002,7 @@ def norm_rotary_backward(q, k, q_weight, k_weight, cos, sin, positions, eps, int
     a.grad_q, a.grad_k = grads[0].data_ptr(), grads[1].data_ptr()
     a.grad_q_weight, a.grad_k_weight = _ptr(wgrads[0]), _ptr(wgrads[1])
     if wgrads[0] is not None or wgrads[1] is not None:
-        ws = _workspace(q, int(_lib.nsh_norm_rotary_workspace_bytes(ctypes.byref(a))))
+        ws = _scratch(q, int(_lib.nsh_norm_rotary_workspace_bytes(ctypes.byref(a))))
         a.workspace, a.workspace_bytes = _ptr(ws), ws.numel() if ws is not None else 0
     _call_on(q, "nsh_norm_rotary_backward", ctypes.byref(a))
     return grads + wgrads
@@ -1029,7 +1029,7 @@ def position_bias_backward(grad_out, buckets, num_buckets):
     if not grad_out.numel():
         return grad.zero_()
     n = int(_lib.nsh_position_bias_workspace_bytes(H, q_len, k_len, reach))
-    ws = _workspace(grad_out, n)
+    ws = _scratch(grad_out, n)
     _call_on(grad_out, "nsh_position_bias_backward", grad_out.data_ptr(), buckets.data_ptr(), H,
              q_len, k_len, num_buckets, reach, code, grad.data_ptr(), _ptr(ws), n)
     return grad
@@ -1066,7 +1066,7 @@ def attention_forward(q, k, v, rules, want_degree, want_stats):
                 stats.zero_() if want_stats else None)
     a = _attention_args(q, k, v, out, degree, stats, rules)
     n = int(_lib.nsh_attention_workspace_bytes(ctypes.byref(a), 0))
-    ws = _workspace(q, n)
+    ws = _scratch(q, n)
     a.workspace, a.workspace_bytes = _ptr(ws), n
     _call_on(q, "nsh_attention_forward", ctypes.byref(a))
     return out, degree, stats
@@ -1087,7 +1087,7 @@ def attention_backward(q, k, v, out, row_stats, rules, grad_out, grad_log_degree
     a.gq_stride, a.gk_stride, a.gv_stride = (_strides(g) for g in grads)
     a.grad_bias_table = _ptr(gt)
     n = int(_lib.nsh_attention_workspace_bytes(ctypes.byref(a), 1))
-    ws = _workspace(q, n)
+    ws = _scratch(q, n)
     a.workspace, a.workspace_bytes = _ptr(ws), n
     _call_on(q, "nsh_attention_backward", ctypes.byref(a))
     return grads + [gt]
