@@ -486,9 +486,10 @@ NSH_API int nsh_stream_probe(int kind, const void* src, void* dst, int64_t bytes
  *   y = x * (mean(x^2) + eps)^(-1/2) * weight
  *   (a, b) -> (a cos - b sin, a sin + b cos) for the pairs of the first 2 * half
  *   elements: (i, i + half), or (2i, 2i + 1) if `interleaved`
- * cos, sin: float (rows, half); positions: int32, the row of each token.  A position outside [0, rows) gives NaN and reads nothing.  A NULL
- * weight is 1.  D <= 512, 2 * half <= D.  Outputs are contiguous
- * (B, heads, L, D) in `dtype`; q or k may have no heads.
+ * cos, sin: float (rows, half); positions: int32, the row of each token.  A
+ * position outside [0, rows) gives NaN and reads nothing.  A NULL weight is 1.
+ * D <= 512, 2 * half <= D.  Outputs are contiguous (B, heads, L, D) in `dtype`;
+ * q or k may have no heads.
  * Any alignment and strides. */
 typedef struct nsh_norm_rotary_args {
     const void *q, *k, *q_weight, *k_weight;
@@ -540,8 +541,9 @@ NSH_API int64_t nsh_position_bias_workspace_bytes(int64_t H, int64_t Lq, int64_t
  *   out = softmax(s) v,  log_degree = log sum exp s  (float, (B, Hq, Lq));
  * a row that sees nothing gives 0 and -inf.  Query head h reads key head
  * h / (Hq / Hk).  D <= 128, D a multiple of 8; the rows of q, k, v, out and of
- * the gradients start on 16 bytes.  Keys that a query does not see add
- * nothing to it, whatever they hold. */
+ * the gradients start on 16 bytes, those of q, k, v and grad_out 0 to 2^24 bytes
+ * apart from a token to the next.  Keys that a query does not see add nothing to
+ * it, whatever they hold. */
 typedef struct nsh_attention_args {
     const void *q, *k, *v;
     int64_t B, Hq, Hk, Lq, Lk, D;
@@ -557,7 +559,8 @@ typedef struct nsh_attention_args {
     void* out;
     float* log_degree; /* forward: NULL = not wanted */
     /* backward: `out`, and `row_stats` or `log_degree`, of the forward;
-     * grad_log_degree and grad_bias_table may be NULL.  grad_q has q's shape and gq_stride, ... */
+     * grad_log_degree and grad_bias_table may be NULL.  grad_q has q's shape and
+     * gq_stride, ... */
     const void* grad_out;
     const float* grad_log_degree;
     int64_t go_stride[3], gq_stride[3], gk_stride[3], gv_stride[3];
@@ -568,6 +571,10 @@ typedef struct nsh_attention_args {
      * units of log 2) and 1 / its sum.  Backward: used in log_degree's place,
      * which loses the sum of a row whose scores are beyond 2^20 or so. */
     float* row_stats;
+    /* (B, Hq, Lq, D) in `dtype`, 16-byte aligned, or NULL.  Forward: written,
+     * what was rounded off `out`.  Backward: added to it where the gradients
+     * take its product with grad_out. */
+    void* out_rest;
 } nsh_attention_args;
 NSH_API int nsh_attention_forward(const nsh_attention_args* args, void* stream);
 NSH_API int nsh_attention_backward(const nsh_attention_args* args, void* stream);

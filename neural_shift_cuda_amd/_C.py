@@ -32,6 +32,7 @@ from __future__ import annotations
 import ctypes
 import functools
 import os
+import struct
 import weakref
 from typing import List, Optional, Sequence
 
@@ -919,7 +920,7 @@ class _AttentionArgs(ctypes.Structure):
         ("log_degree", _P), ("grad_out", _P), ("grad_log_degree", _P), ("go_stride", _S3),
         ("gq_stride", _S3), ("gk_stride", _S3), ("gv_stride", _S3), ("grad_q", _P),
         ("grad_k", _P), ("grad_v", _P), ("grad_bias_table", _P), ("workspace", _P),
-        ("workspace_bytes", _I64), ("row_stats", _P)]
+        ("workspace_bytes", _I64), ("row_stats", _P), ("out_rest", _P)]
 
 
 for _name, _args, _res in (
@@ -949,13 +950,26 @@ def _strides(t: torch.Tensor):
     return t.stride()[:3]
 
 
-def _like(t: torch.Tensor, heads: int, tokens: int, width: int) -> torch.Tensor:
-    """A new (B, heads, tokens, width) tensor that keeps t's order of heads and
-    tokens in memory."""
-    B = t.shape[0]
+def _address(t) -> int:
+    return t.data_ptr() if t is not None else 0
+
+
+# The structs' fields in one call, those of the backward left zero (a keyword
+# for each field takes 8 us, this 4).
+_NORM_FIELDS = struct.Struct("7Pq7q6qdii128x")
+_ATTENTION_FIELDS = struct.Struct("3P6q12q6P2q2d2i2P160x2P")
+assert _NORM_FIELDS.size == ctypes.sizeof(_NormRotaryArgs)
+assert _ATTENTION_FIELDS.size == ctypes.sizeof(_AttentionArgs)
+
+
+def _like(t: torch.Tensor) -> torch.Tensor:
+    """A new tensor that keeps t's order of heads and tokens in memory."""
+    if t.is_contiguous():
+        return torch.empty_like(t)
     if t.stride(1) < t.stride(2):
+        B, heads, tokens, width = t.shape
         return t.new_empty((B, tokens, heads, width)).transpose(1, 2)
-    return t.new_empty((B, heads, tokens, width))
+    return t.new_empty(t.shape)
 
 
 def _scratch(t: torch.Tensor, n: int) -> Optional[torch.Tensor]:
@@ -964,13 +978,13 @@ def _scratch(t: torch.Tensor, n: int) -> Optional[torch.Tensor]:
 
 def _norm_rotary_args(op, q, k, q_weight, k_weight, cos, sin, positions, eps, interleaved):
     B, Hq, L, D = q.shape
-    return _NormRotaryArgs(
-        q=q.data_ptr(), k=k.data_ptr(), q_weight=_ptr(q_weight), k_weight=_ptr(k_weight),
-        cos=cos.data_ptr(), sin=sin.data_ptr(), positions=_ptr(positions),
-        position_stride=L if positions is not None and positions.dim() == 2 else 0,
-        B=B, Hq=Hq, Hk=k.shape[1], L=L, D=D, half=cos.shape[1], rows=cos.shape[0],
-        q_stride=_strides(q), k_stride=_strides(k), eps=eps, dtype=_heads_code(q, op),
-        interleaved=interleaved)
+    rows, half = cos.shape
+    return _NormRotaryArgs.from_buffer_copy(_NORM_FIELDS.pack(
+        q.data_ptr(), k.data_ptr(), _address(q_weight), _address(k_weight), cos.data_ptr(),
+        sin.data_ptr(), _address(positions),
+        L if positions is not None and positions.dim() == 2 else 0,
+        B, Hq, k.shape[1], L, D, half, rows, *_strides(q), *_strides(k), eps, _heads_code(q, op),
+        interleaved))
 
 
 def norm_rotary_forward(q, k, q_weight, k_weight, cos, sin, positions, eps, interleaved):
@@ -979,7 +993,7 @@ def norm_rotary_forward(q, k, q_weight, k_weight, cos, sin, positions, eps, inte
     float (rows, half); positions contiguous int32 (L) or (B, L), or None."""
     a = _norm_rotary_args("norm_rotary", q, k, q_weight, k_weight, cos, sin, positions, eps,
                           interleaved)
-    outs = [torch.empty(t.shape, dtype=t.dtype, device=t.device) for t in (q, k)]
+    outs = [q.new_empty(q.shape), k.new_empty(k.shape)]
     if a.B and a.L and a.D and (a.Hq or a.Hk):
         a.q_out, a.k_out = outs[0].data_ptr(), outs[1].data_ptr()
         _call_on(q, "nsh_norm_rotary_forward", ctypes.byref(a))
@@ -992,7 +1006,7 @@ def norm_rotary_backward(q, k, q_weight, k_weight, cos, sin, positions, eps, int
     the weights' gradients None where there is no weight, or not wanted."""
     a = _norm_rotary_args("norm_rotary", q, k, q_weight, k_weight, cos, sin, positions, eps,
                           interleaved)
-    grads = [torch.empty(t.shape, dtype=t.dtype, device=t.device) for t in (q, k)]
+    grads = [q.new_empty(q.shape), k.new_empty(k.shape)]
     wgrads = [torch.empty_like(w) if w is not None and need else None
               for w, need in zip((q_weight, k_weight), need_weights)]
     if not (a.B and a.L and a.D and (a.Hq or a.Hk)):
@@ -1035,52 +1049,55 @@ def position_bias_backward(grad_out, buckets, num_buckets):
     return grad
 
 
-def _attention_args(q, k, v, out, log_degree, row_stats, rules):
+def _attention_args(q, k, v, out, log_degree, kept, rules):
     B, Hq, Lq, D = q.shape
+    Hk, Lk = k.shape[1:3]
     table, buckets = rules["bias_table"], rules["buckets"]
-    return _AttentionArgs(
-        q=q.data_ptr(), k=k.data_ptr(), v=v.data_ptr(), B=B, Hq=Hq, Hk=k.shape[1], Lq=Lq,
-        Lk=k.shape[2], D=D, q_stride=_strides(q), k_stride=_strides(k), v_stride=_strides(v),
-        out_stride=_strides(out), lengths=_ptr(rules["lengths"]), prefix=_ptr(rules["prefix"]),
-        documents=_ptr(rules["documents"]), slopes=_ptr(rules["slopes"]), bias_table=_ptr(table),
-        buckets=_ptr(buckets), num_buckets=table.shape[0] if table is not None else 0,
-        reach=(buckets.numel() - 1) // 2 if table is not None else 0, scale=rules["scale"],
-        cap=rules["cap"], dtype=_heads_code(q, "attention"), causal=rules["causal"],
-        out=out.data_ptr(), log_degree=_ptr(log_degree), row_stats=_ptr(row_stats))
+    rest = row_stats = _address(kept)
+    if kept is not None:  # out_rest (16-bit types), then row_stats
+        rest, row_stats = (rest, rest + 2 * out.numel()) if q.element_size() == 2 else (0, rest)
+    return _AttentionArgs.from_buffer_copy(_ATTENTION_FIELDS.pack(
+        q.data_ptr(), k.data_ptr(), v.data_ptr(), B, Hq, Hk, Lq, Lk, D, *_strides(q), *_strides(k),
+        *_strides(v), *_strides(out), _address(rules["lengths"]), _address(rules["prefix"]),
+        _address(rules["documents"]), _address(rules["slopes"]), _address(table),
+        _address(buckets), table.shape[0] if table is not None else 0,
+        (buckets.numel() - 1) // 2 if table is not None else 0, rules["scale"], rules["cap"],
+        _heads_code(q, "attention"), rules["causal"], out.data_ptr(), _address(log_degree),
+        row_stats, rest))
 
 
-def attention_forward(q, k, v, rules, want_degree, want_stats):
-    """[out, log_degree or None, row_stats or None] (nsh_attention_forward):
+def attention_forward(q, k, v, rules, want_degree, keep):
+    """[out, log_degree or None, what the backward needs or None] (nsh_attention_forward):
     (B, heads, tokens, D) tensors with 16-byte rows; `rules` holds scale, cap,
     causal and the mask and bias tensors (or None) as the C ABI takes them."""
     B, Hq, Lq, D = q.shape
-    out = _like(q, Hq, Lq, D)
+    out = _like(q)
     degree = (torch.empty((B, Hq, Lq), dtype=torch.float32, device=q.device)
               if want_degree else None)
-    stats = (torch.empty((B, Hq, Lq, 2), dtype=torch.float32, device=q.device)
-             if want_stats else None)
+    # row_stats, two floats a row, behind out_rest
+    kept = (torch.empty(B * Hq * Lq * (2 + (D // 2 if q.element_size() == 2 else 0)),
+                        dtype=torch.float32, device=q.device) if keep else None)
     if not out.numel():
-        return out, degree, stats
+        return out, degree, kept
     if not k.numel():
         return (out.zero_(), degree.fill_(float("-inf")) if want_degree else None,
-                stats.zero_() if want_stats else None)
-    a = _attention_args(q, k, v, out, degree, stats, rules)
+                kept.zero_() if keep else None)
+    a = _attention_args(q, k, v, out, degree, kept, rules)
     n = int(_lib.nsh_attention_workspace_bytes(ctypes.byref(a), 0))
     ws = _scratch(q, n)
     a.workspace, a.workspace_bytes = _ptr(ws), n
     _call_on(q, "nsh_attention_forward", ctypes.byref(a))
-    return out, degree, stats
+    return out, degree, kept
 
 
-def attention_backward(q, k, v, out, row_stats, rules, grad_out, grad_log_degree, need_table):
+def attention_backward(q, k, v, out, kept, rules, grad_out, grad_log_degree, need_table):
     """[grad_q, grad_k, grad_v, grad_bias_table or None] (nsh_attention_backward)."""
-    B, Hq, Lq, D = q.shape
-    grads = [_like(q, Hq, Lq, D), _like(k, *k.shape[1:]), _like(v, *v.shape[1:])]
+    grads = [_like(q), _like(k), _like(v)]
     table = rules["bias_table"]
     gt = torch.empty_like(table) if need_table else None
     if not q.numel() or not k.numel():
         return [g.zero_() for g in grads] + [None if gt is None else gt.zero_()]
-    a = _attention_args(q, k, v, out, None, row_stats, rules)
+    a = _attention_args(q, k, v, out, None, kept, rules)
     a.grad_out, a.go_stride = grad_out.data_ptr(), _strides(grad_out)
     a.grad_log_degree = _ptr(grad_log_degree)
     a.grad_q, a.grad_k, a.grad_v = (g.data_ptr() for g in grads)

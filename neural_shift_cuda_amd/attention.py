@@ -112,6 +112,8 @@ def _whole(name: str, t: Optional[torch.Tensor], shape, like: torch.Tensor
     it at its ends: no row, bucket or length that the operators serve)."""
     if t is None:
         return None
+    if t.dtype is torch.int32 and t.shape == shape and t.device == like.device:
+        return t.contiguous()
     if t.is_floating_point() or t.is_complex() or t.dtype == torch.bool:
         raise TypeError(f"{name} must hold integers; got {t.dtype}")
     if tuple(t.shape) != tuple(shape):
@@ -173,9 +175,11 @@ def _check_buckets(table: torch.Tensor, buckets: Optional[torch.Tensor], name: s
 def _check_attention(q, k, v, scale, cap, causal, prefix, documents, lengths, slopes, bias_table,
                      buckets) -> dict:
     """The checked call, as the native functions take it."""
-    for name, t in (("q", q), ("k", k), ("v", v)):
-        _heads(t, name)
-        _same(name, t, q)
+    if not (q.dim() == k.dim() == v.dim() == 4 and q.dtype is k.dtype is v.dtype
+            and q.dtype.is_floating_point and q.device == k.device == v.device):
+        for name, t in (("q", q), ("k", k), ("v", v)):
+            _heads(t, name)
+            _same(name, t, q)
     B, Hq, Lq, D = q.shape
     Hk, Lk = k.shape[1:3]
     if k.shape != v.shape or k.shape[0] != B or k.shape[3] != D:
@@ -382,9 +386,9 @@ def _rows16(t: torch.Tensor) -> torch.Tensor:
     """t with rows that start on 16 bytes and a unit last stride, copied where
     they do not (their width is a multiple of 8 by then)."""
     bytes_ = t.element_size()
-    if (t.stride(3) == 1 and t.data_ptr() % 16 == 0
-            and all(s * bytes_ % 16 == 0 for s in t.stride()[:3])
-            and t.stride(2) * bytes_ <= 1 << 24):
+    b, h, n, one = t.stride()
+    if one == 1 and (t.data_ptr() | b * bytes_ | h * bytes_ | n * bytes_) % 16 == 0 \
+            and n * bytes_ <= 1 << 24:
         return t
     return t.clone(memory_format=torch.contiguous_format)
 
@@ -397,11 +401,10 @@ class _BiasedAttentionFn(torch.autograd.Function):
     def forward(ctx, q, k, v, bias_table, rules, want_degree):
         table = bias_table.contiguous() if bias_table is not None else None
         rules = {**rules, "bias_table": table}
-        # the gradients need every row's largest score and sum
         keep = any(ctx.needs_input_grad[:4])
-        out, degree, stats = _C.attention_forward(q, k, v, rules, want_degree, keep)
+        out, degree, kept = _C.attention_forward(q, k, v, rules, want_degree, keep)
         if keep:
-            ctx.save_for_backward(q, k, v, table, out, stats, *(rules[n] for n in _TENSOR_RULES))
+            ctx.save_for_backward(q, k, v, table, out, kept, *(rules[n] for n in _TENSOR_RULES))
             ctx.plain = {n: rules[n] for n in ("scale", "cap", "causal")}
         ctx.set_materialize_grads(False)
         return out, degree
@@ -409,10 +412,10 @@ class _BiasedAttentionFn(torch.autograd.Function):
     @staticmethod
     @once_differentiable
     def backward(ctx, grad_out, grad_degree):
-        q, k, v, table, out, stats, *rest = ctx.saved_tensors
+        q, k, v, table, out, kept, *rest = ctx.saved_tensors
         rules = {**ctx.plain, "bias_table": table, **dict(zip(_TENSOR_RULES, rest))}
         grad_out = torch.zeros_like(out) if grad_out is None else _rows16(grad_out)
-        grads = _C.attention_backward(q, k, v, out, stats, rules, grad_out,
+        grads = _C.attention_backward(q, k, v, out, kept, rules, grad_out,
                                       None if grad_degree is None else grad_degree.contiguous(),
                                       ctx.needs_input_grad[3])
         return (*grads, None, None)

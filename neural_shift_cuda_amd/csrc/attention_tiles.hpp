@@ -70,6 +70,14 @@ __device__ __forceinline__ void store4(T* p, f32x4 v) {
         *reinterpret_cast<bf16x4*>(p) = __builtin_convertvector(v, bf16x4);
 }
 
+// What store4 rounds off, stored in its place beside out.
+template <typename T>
+__device__ __forceinline__ void store4_rest(T* p, f32x4 v) {
+#pragma unroll
+    for (int e = 0; e < 4; ++e) v[e] = rounded_off<T>(v[e]);
+    store4<T>(p, v);
+}
+
 // Tile row of result element r, less the lane half's 4 g.
 __device__ __forceinline__ constexpr int el(int r) { return 8 * (r / 4) + r % 4; }
 

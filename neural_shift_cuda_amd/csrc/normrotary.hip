@@ -7,12 +7,20 @@
 // HBM streams: forward reads and writes every element once, backward reads x
 // and g and writes gx.  A row (one head of one token) belongs to a group of
 // lanes that holds it whole in registers, 16 bytes a lane where the rows allow
-// it; the sum of squares is a butterfly in the group and a rotated pair's other
-// half comes from its lane by a shuffle.  Rows run with the heads fastest, so a
-// token's cos and sin stay in the caches for all its heads.  Queries and keys
-// share the launch.  gw: each lane adds up its own columns over the rows it
-// walks, the groups of a workgroup add in order, and a second launch adds the
-// workgroups' sums in order.
+// it.  The sum of squares meets in the group, and a rotated pair's other half
+// comes from its lane, by DPP and row swaps: through LDS (shuffles) the forward
+// of 4 x 20 heads of 4096 tokens, width 128, bf16 took 51.5 us instead of 35 and
+// waited on LDS, not on memory.  A row's head, token and batch come from
+// multiplications by reciprocals.  Rows run with the heads fastest, so a token's
+// cos and sin stay in the caches for all its heads.  Queries and keys share the
+// launch.  gw: each lane adds up its own columns over the rows it walks, the
+// groups of a workgroup add in order, and a second launch adds the workgroups'
+// sums in order.
+//
+// At that size: forward 35 us (84 + 84 MB, 4.8 TB/s), backward 60.5 us (168 + 84
+// MB, 4.2 TB/s), the weights' sums 5 us; a copy of 84 MB, which the memory side
+// cache holds, runs at 7.0 TB/s, one of 268 MB at 5.4.  What bounds them is memory
+// latency behind a position's: its table rows can be asked for only then.
 #include <algorithm>
 #include <cmath>
 

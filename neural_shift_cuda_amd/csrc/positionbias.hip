@@ -15,6 +15,10 @@
 // sums per relative position go to a workspace, and one workgroup per head adds
 // them, first over the workgroups, then over each bucket's relative positions:
 // all in a fixed order.
+//
+// 16 heads, 2048 x 2048, fp32 (268 MB): forward 52 us (5.2 TB/s), backward 55.7
+// (4.8 TB/s) and 6.6 for the table's sums; a copy of 268 MB runs at 5.4 TB/s and a
+// library sum over as much at 4.9.  Both are bound by memory.
 #include <algorithm>
 
 #include "divisor.hpp"
