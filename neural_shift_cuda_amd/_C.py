@@ -23,9 +23,13 @@ trishitmg/neural_shift_cuda), so the guards in ``ops.py`` and
   shape (S*B, 1, H, W) used for every channel (``NSH_SHARED_WEIGHTS``); the
   weight gradient then still comes back per channel, (S*B, C, H, W).
 
-Importing this module raises ``OSError`` when the library has not been built
-(``python -m neural_shift_cuda_amd.build``); ``ops.py`` keeps that error and
-reports it when a GPU tensor reaches an op, instead of falling back.
+The token operators at the end have their host side in C++
+(``host/token_calls.cpp``, the extension module ``_token_calls``).
+
+Importing this module raises ``OSError`` or ``ImportError`` when the library
+has not been built (``python -m neural_shift_cuda_amd.build``); ``ops.py`` keeps
+that error and reports it when a GPU tensor reaches an op, instead of falling
+back.
 """
 from __future__ import annotations
 
@@ -40,6 +44,8 @@ import torch  # must precede the CDLL: the library binds to torch's HIP runtime
 
 _LIB_PATH = os.path.join(os.path.dirname(os.path.abspath(__file__)), "libneural_shift_hip.so")
 _lib = ctypes.CDLL(_LIB_PATH)
+
+from . import _token_calls  # noqa: E402  (linked to the library loaded above)
 
 _P = ctypes.c_void_p
 _I64 = ctypes.c_int64
@@ -954,99 +960,9 @@ def _address(t) -> int:
     return t.data_ptr() if t is not None else 0
 
 
-# The structs' fields in one call, those of the backward left zero (a keyword
-# for each field takes 8 us, this 4).
-_NORM_FIELDS = struct.Struct("7Pq7q6qdii128x")
+# The struct's fields in one call, those of the backward left zero.
 _ATTENTION_FIELDS = struct.Struct("3P6q12q6P2q2d2i2P160x2P")
-assert _NORM_FIELDS.size == ctypes.sizeof(_NormRotaryArgs)
 assert _ATTENTION_FIELDS.size == ctypes.sizeof(_AttentionArgs)
-
-
-def _like(t: torch.Tensor) -> torch.Tensor:
-    """A new tensor that keeps t's order of heads and tokens in memory."""
-    if t.is_contiguous():
-        return torch.empty_like(t)
-    if t.stride(1) < t.stride(2):
-        B, heads, tokens, width = t.shape
-        return t.new_empty((B, tokens, heads, width)).transpose(1, 2)
-    return t.new_empty(t.shape)
-
-
-def _scratch(t: torch.Tensor, n: int) -> Optional[torch.Tensor]:
-    return torch.empty(n, dtype=torch.uint8, device=t.device) if n > 0 else None
-
-
-def _norm_rotary_args(op, q, k, q_weight, k_weight, cos, sin, positions, eps, interleaved):
-    B, Hq, L, D = q.shape
-    rows, half = cos.shape
-    return _NormRotaryArgs.from_buffer_copy(_NORM_FIELDS.pack(
-        q.data_ptr(), k.data_ptr(), _address(q_weight), _address(k_weight), cos.data_ptr(),
-        sin.data_ptr(), _address(positions),
-        L if positions is not None and positions.dim() == 2 else 0,
-        B, Hq, k.shape[1], L, D, half, rows, *_strides(q), *_strides(k), eps, _heads_code(q, op),
-        interleaved))
-
-
-def norm_rotary_forward(q, k, q_weight, k_weight, cos, sin, positions, eps, interleaved):
-    """[q', k'] (nsh_norm_rotary_forward): (B, heads, L, D) tensors of any
-    strides with a unit last one; weights (D) or None; cos, sin contiguous
-    float (rows, half); positions contiguous int32 (L) or (B, L), or None."""
-    a = _norm_rotary_args("norm_rotary", q, k, q_weight, k_weight, cos, sin, positions, eps,
-                          interleaved)
-    outs = [q.new_empty(q.shape), k.new_empty(k.shape)]
-    if a.B and a.L and a.D and (a.Hq or a.Hk):
-        a.q_out, a.k_out = outs[0].data_ptr(), outs[1].data_ptr()
-        _call_on(q, "nsh_norm_rotary_forward", ctypes.byref(a))
-    return outs
-
-
-def norm_rotary_backward(q, k, q_weight, k_weight, cos, sin, positions, eps, interleaved, gq, gk,
-                         need_weights):
-    """[grad_q, grad_k, grad_q_weight, grad_k_weight] (nsh_norm_rotary_backward);
-    the weights' gradients None where there is no weight, or not wanted."""
-    a = _norm_rotary_args("norm_rotary", q, k, q_weight, k_weight, cos, sin, positions, eps,
-                          interleaved)
-    grads = [q.new_empty(q.shape), k.new_empty(k.shape)]
-    wgrads = [torch.empty_like(w) if w is not None and need else None
-              for w, need in zip((q_weight, k_weight), need_weights)]
-    if not (a.B and a.L and a.D and (a.Hq or a.Hk)):
-        return grads + [None if w is None else w.zero_() for w in wgrads]
-    a.grad_q_out, a.grad_k_out = gq.data_ptr(), gk.data_ptr()
-    a.gq_stride, a.gk_stride = _strides(gq), _strides(gk)
-    a.grad_q, a.grad_k = grads[0].data_ptr(), grads[1].data_ptr()
-    a.grad_q_weight, a.grad_k_weight = _ptr(wgrads[0]), _ptr(wgrads[1])
-    if wgrads[0] is not None or wgrads[1] is not None:
-        ws = _scratch(q, int(_lib.nsh_norm_rotary_workspace_bytes(ctypes.byref(a))))
-        a.workspace, a.workspace_bytes = _ptr(ws), ws.numel() if ws is not None else 0
-    _call_on(q, "nsh_norm_rotary_backward", ctypes.byref(a))
-    return grads + wgrads
-
-
-def position_bias_forward(table, buckets, q_len, k_len):
-    """(H, q_len, k_len) (nsh_position_bias_forward): table contiguous
-    (num_buckets, H), buckets contiguous int32 (2 * reach + 1)."""
-    code = _heads_code(table, "position_bias")
-    nb, H = table.shape
-    out = torch.empty((H, q_len, k_len), dtype=table.dtype, device=table.device)
-    if out.numel():
-        _call_on(table, "nsh_position_bias_forward", table.data_ptr(), buckets.data_ptr(), H,
-                 q_len, k_len, nb, (buckets.numel() - 1) // 2, code, out.data_ptr())
-    return out
-
-
-def position_bias_backward(grad_out, buckets, num_buckets):
-    """(num_buckets, H) from a contiguous (H, q_len, k_len) gradient."""
-    code = _heads_code(grad_out, "position_bias")
-    H, q_len, k_len = grad_out.shape
-    reach = (buckets.numel() - 1) // 2
-    grad = torch.empty((num_buckets, H), dtype=grad_out.dtype, device=grad_out.device)
-    if not grad_out.numel():
-        return grad.zero_()
-    n = int(_lib.nsh_position_bias_workspace_bytes(H, q_len, k_len, reach))
-    ws = _scratch(grad_out, n)
-    _call_on(grad_out, "nsh_position_bias_backward", grad_out.data_ptr(), buckets.data_ptr(), H,
-             q_len, k_len, num_buckets, reach, code, grad.data_ptr(), _ptr(ws), n)
-    return grad
 
 
 def _attention_args(q, k, v, out, log_degree, kept, rules):
@@ -1069,42 +985,15 @@ def _attention_args(q, k, v, out, log_degree, kept, rules):
 def attention_forward(q, k, v, rules, want_degree, keep):
     """[out, log_degree or None, what the backward needs or None] (nsh_attention_forward):
     (B, heads, tokens, D) tensors with 16-byte rows; `rules` holds scale, cap,
-    causal and the mask and bias tensors (or None) as the C ABI takes them."""
-    B, Hq, Lq, D = q.shape
-    out = _like(q)
-    degree = (torch.empty((B, Hq, Lq), dtype=torch.float32, device=q.device)
-              if want_degree else None)
-    # row_stats, two floats a row, behind out_rest
-    kept = (torch.empty(B * Hq * Lq * (2 + (D // 2 if q.element_size() == 2 else 0)),
-                        dtype=torch.float32, device=q.device) if keep else None)
-    if not out.numel():
-        return out, degree, kept
-    if not k.numel():
-        return (out.zero_(), degree.fill_(float("-inf")) if want_degree else None,
-                kept.zero_() if keep else None)
-    a = _attention_args(q, k, v, out, degree, kept, rules)
-    n = int(_lib.nsh_attention_workspace_bytes(ctypes.byref(a), 0))
-    ws = _scratch(q, n)
-    a.workspace, a.workspace_bytes = _ptr(ws), n
-    _call_on(q, "nsh_attention_forward", ctypes.byref(a))
-    return out, degree, kept
+    causal and the mask and bias tensors (or None) as the C ABI takes them.  No
+    graph is made: ``attention`` is the differentiable call."""
+    return _token_calls.attention_forward(
+        q, k, v, rules["bias_table"], rules["lengths"], rules["prefix"], rules["documents"],
+        rules["slopes"], rules["buckets"], rules["scale"], rules["cap"], rules["causal"],
+        want_degree, keep)
 
 
-def attention_backward(q, k, v, out, kept, rules, grad_out, grad_log_degree, need_table):
-    """[grad_q, grad_k, grad_v, grad_bias_table or None] (nsh_attention_backward)."""
-    grads = [_like(q), _like(k), _like(v)]
-    table = rules["bias_table"]
-    gt = torch.empty_like(table) if need_table else None
-    if not q.numel() or not k.numel():
-        return [g.zero_() for g in grads] + [None if gt is None else gt.zero_()]
-    a = _attention_args(q, k, v, out, None, kept, rules)
-    a.grad_out, a.go_stride = grad_out.data_ptr(), _strides(grad_out)
-    a.grad_log_degree = _ptr(grad_log_degree)
-    a.grad_q, a.grad_k, a.grad_v = (g.data_ptr() for g in grads)
-    a.gq_stride, a.gk_stride, a.gv_stride = (_strides(g) for g in grads)
-    a.grad_bias_table = _ptr(gt)
-    n = int(_lib.nsh_attention_workspace_bytes(ctypes.byref(a), 1))
-    ws = _scratch(q, n)
-    a.workspace, a.workspace_bytes = _ptr(ws), n
-    _call_on(q, "nsh_attention_backward", ctypes.byref(a))
-    return grads + [gt]
+# The differentiable calls, host/token_calls.cpp.
+norm_rotary = _token_calls.norm_rotary
+position_bias = _token_calls.position_bias
+attention = _token_calls.attention

@@ -13,8 +13,8 @@ and the tables a program makes once: ``rotary_table``, ``relative_buckets``.
 Tensors are (B, heads, tokens, width).  The conventions are those of the
 normalized accumulation: D = sum_j a_j v_j / sum_j a_j with a = exp(score),
 log_C the logarithm of the sum, and a row that sees nothing gives D = 0 and
-log_C = -inf.  GPU tensors go through the autograd Functions below into the HIP
-library (fp16, bf16, fp32; sums, norms and softmax statistics in fp32); CPU
+log_C = -inf.  GPU tensors go through autograd nodes in C++
+(host/token_calls.cpp) into the HIP library (fp16, bf16, fp32; sums, norms and softmax statistics in fp32); CPU
 tensors use the ``*_reference`` implementations (any floating type), which are
 also exported.  A GPU tensor never falls back to them.
 
@@ -28,7 +28,6 @@ import math
 from typing import Optional, Tuple
 
 import torch
-from torch.autograd.function import once_differentiable
 
 from . import ops
 
@@ -335,93 +334,6 @@ def biased_attention_reference(q, k, v, *, scale: Optional[float] = None,
 
 
 # ---------------------------------------------------------------------------
-# autograd Functions over the HIP library
-# ---------------------------------------------------------------------------
-
-def _unit(t: torch.Tensor) -> torch.Tensor:
-    """t with a unit last stride (a broadcast or transposed row is copied)."""
-    return t if t.stride(3) == 1 or t.shape[3] == 1 else t.contiguous()
-
-
-def _graph(*tensors: Optional[torch.Tensor]) -> bool:
-    """A gradient of one of them may be asked for."""
-    return torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in tensors)
-
-
-class _QkNormRotaryFn(torch.autograd.Function):
-    @staticmethod
-    def forward(ctx, q, k, q_weight, k_weight, cos, sin, positions, eps, interleaved):
-        q, k = _unit(q), _unit(k)
-        out = _C.norm_rotary_forward(q, k, q_weight, k_weight, cos, sin, positions, eps,
-                                     interleaved)
-        ctx.save_for_backward(q, k, q_weight, k_weight, cos, sin, positions)
-        ctx.rules = (eps, interleaved)
-        return out[0], out[1]
-
-    @staticmethod
-    @once_differentiable
-    def backward(ctx, gq, gk):
-        q, k, q_weight, k_weight, cos, sin, positions = ctx.saved_tensors
-        grads = _C.norm_rotary_backward(q, k, q_weight, k_weight, cos, sin, positions, *ctx.rules,
-                                        _unit(gq), _unit(gk), ctx.needs_input_grad[2:4])
-        return (*grads, None, None, None, None, None)
-
-
-class _PositionBiasFn(torch.autograd.Function):
-    @staticmethod
-    def forward(ctx, table, buckets, q_len, k_len):
-        ctx.save_for_backward(buckets)
-        ctx.num_buckets = table.shape[0]
-        return _C.position_bias_forward(table.contiguous(), buckets, q_len, k_len)
-
-    @staticmethod
-    @once_differentiable
-    def backward(ctx, grad_out):
-        (buckets,) = ctx.saved_tensors
-        return (_C.position_bias_backward(grad_out.contiguous(), buckets, ctx.num_buckets),
-                None, None, None)
-
-
-def _rows16(t: torch.Tensor) -> torch.Tensor:
-    """t with rows that start on 16 bytes and a unit last stride, copied where
-    they do not (their width is a multiple of 8 by then)."""
-    bytes_ = t.element_size()
-    b, h, n, one = t.stride()
-    if one == 1 and (t.data_ptr() | b * bytes_ | h * bytes_ | n * bytes_) % 16 == 0 \
-            and n * bytes_ <= 1 << 24:
-        return t
-    return t.clone(memory_format=torch.contiguous_format)
-
-
-_TENSOR_RULES = ("prefix", "documents", "lengths", "slopes", "buckets")
-
-
-class _BiasedAttentionFn(torch.autograd.Function):
-    @staticmethod
-    def forward(ctx, q, k, v, bias_table, rules, want_degree):
-        table = bias_table.contiguous() if bias_table is not None else None
-        rules = {**rules, "bias_table": table}
-        keep = any(ctx.needs_input_grad[:4])
-        out, degree, kept = _C.attention_forward(q, k, v, rules, want_degree, keep)
-        if keep:
-            ctx.save_for_backward(q, k, v, table, out, kept, *(rules[n] for n in _TENSOR_RULES))
-            ctx.plain = {n: rules[n] for n in ("scale", "cap", "causal")}
-        ctx.set_materialize_grads(False)
-        return out, degree
-
-    @staticmethod
-    @once_differentiable
-    def backward(ctx, grad_out, grad_degree):
-        q, k, v, table, out, kept, *rest = ctx.saved_tensors
-        rules = {**ctx.plain, "bias_table": table, **dict(zip(_TENSOR_RULES, rest))}
-        grad_out = torch.zeros_like(out) if grad_out is None else _rows16(grad_out)
-        grads = _C.attention_backward(q, k, v, out, kept, rules, grad_out,
-                                      None if grad_degree is None else grad_degree.contiguous(),
-                                      ctx.needs_input_grad[3])
-        return (*grads, None, None)
-
-
-# ---------------------------------------------------------------------------
 # Public API
 # ---------------------------------------------------------------------------
 
@@ -452,12 +364,8 @@ def qk_norm_rotary(q: torch.Tensor, k: torch.Tensor, q_weight: Optional[torch.Te
         raise ValueError(f"heads wider than 512 are not served on the GPU; got {q.shape[3]}")
     ops._require_cuda_ext("qk_norm_rotary")
     w = [None if t is None else t.contiguous() for t in (q_weight, k_weight)]
-    rest = (w[0], w[1], cos.float().contiguous(), sin.float().contiguous(), positions, float(eps),
-            bool(interleaved))
-    if not _graph(q, k, *w):
-        out = _C.norm_rotary_forward(_unit(q), _unit(k), *rest)
-        return out[0], out[1]
-    return _QkNormRotaryFn.apply(q, k, *rest)
+    return _C.norm_rotary(q, k, w[0], w[1], cos.float().contiguous(), sin.float().contiguous(),
+                          positions, eps, interleaved)
 
 
 def relative_position_bias(table: torch.Tensor, buckets: torch.Tensor, q_len: int, k_len: int
@@ -477,9 +385,7 @@ def relative_position_bias(table: torch.Tensor, buckets: torch.Tensor, q_len: in
         return relative_position_bias_reference(table, buckets, q_len, k_len)
     buckets = _check_buckets(table, buckets, "table")
     ops._require_cuda_ext("relative_position_bias")
-    if not _graph(table):
-        return _C.position_bias_forward(table.contiguous(), buckets, int(q_len), int(k_len))
-    return _PositionBiasFn.apply(table, buckets, int(q_len), int(k_len))
+    return _C.position_bias(table, buckets, q_len, k_len)
 
 
 def biased_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, *,
@@ -534,14 +440,9 @@ def biased_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, *,
     ops._require_cuda_ext("biased_attention")
     if D % 8:
         q, k, v = (torch.nn.functional.pad(t, (0, -D % 8)) for t in (q, k, v))
-    q, k, v = _rows16(q), _rows16(k), _rows16(v)
-    if _graph(q, k, v, bias_table):
-        del rules["bias_table"]
-        out, log_C = _BiasedAttentionFn.apply(q, k, v, bias_table, rules, bool(return_log_degree))
-    else:
-        if bias_table is not None:
-            rules["bias_table"] = bias_table.contiguous()
-        out, log_C, _ = _C.attention_forward(q, k, v, rules, bool(return_log_degree), False)
+    out, log_C = _C.attention(q, k, v, rules["bias_table"], rules["lengths"], rules["prefix"],
+                              rules["documents"], rules["slopes"], rules["buckets"],
+                              rules["scale"], rules["cap"], rules["causal"], return_log_degree)
     if D % 8:
         out = out[..., :D]
     return (out, log_C) if return_log_degree else out

@@ -1,4 +1,5 @@
-"""Build libneural_shift_hip.so for gfx950 with hipcc (no torch linkage).
+"""Build libneural_shift_hip.so for gfx950 with hipcc (no torch linkage), and
+the token operators' host side on torch tensors.
 
     python -m neural_shift_cuda_amd.build [--jobs N]
 
@@ -6,6 +7,10 @@ Every ``csrc/*.hip`` / ``csrc/*.cpp`` file is compiled to an object under
 ``neural_shift_cuda_amd/_build`` and linked into
 ``neural_shift_cuda_amd/libneural_shift_hip.so``.  The library exports only
 the C ABI declared in ``include/neural_shift_hip.h``.
+
+``host/token_calls.cpp`` (no device code) is compiled with the host compiler
+against the installed torch into ``neural_shift_cuda_amd/_token_calls.so``, an
+extension module that calls the library.
 """
 from __future__ import annotations
 
@@ -22,6 +27,7 @@ ROOT = os.path.dirname(PKG)
 CSRC = os.path.join(PKG, "csrc")
 BUILD = os.path.join(PKG, "_build")
 LIB = os.path.join(PKG, "libneural_shift_hip.so")
+CALLS = os.path.join(PKG, "_token_calls.so")
 INCLUDE = os.path.join(ROOT, "include")
 ARCH = "gfx950"
 
@@ -72,6 +78,37 @@ def _compile(src: str, flags) -> str:
     return obj
 
 
+def _compile_calls() -> str:
+    import sysconfig
+
+    import torch
+    obj = os.path.join(BUILD, "token_calls.o")
+    inc = os.path.join(os.path.dirname(torch.__file__), "include")
+    cmd = [os.environ.get("CXX", "g++"), "-O2", "-std=c++17", "-fPIC", "-fvisibility=hidden",
+           "-Wall", "-D__HIP_PLATFORM_AMD__=1", "-DUSE_ROCM=1", f"-I{INCLUDE}",
+           *(x for d in (inc, os.path.join(inc, "torch", "csrc", "api", "include"),
+                         sysconfig.get_paths()["include"], "/opt/rocm/include")
+             for x in ("-isystem", d)),
+           "-c", os.path.join(PKG, "host", "token_calls.cpp"), "-o", obj]
+    res = subprocess.run(cmd, capture_output=True, text=True)
+    if res.returncode != 0:
+        raise RuntimeError(f"compile failed: {' '.join(cmd)}\n{res.stdout}\n{res.stderr}")
+    return obj
+
+
+def _link_calls(obj: str) -> None:
+    import torch
+    tmp = CALLS + ".tmp"
+    cmd = [os.environ.get("CXX", "g++"), "-shared", "-o", tmp, obj,
+           "-L" + os.path.join(os.path.dirname(torch.__file__), "lib"), "-ltorch_python",
+           "-ltorch", "-ltorch_cpu", "-lc10", "-lc10_hip", f"-L{PKG}", "-lneural_shift_hip",
+           "-Wl,-rpath,$ORIGIN"]
+    res = subprocess.run(cmd, capture_output=True, text=True)
+    if res.returncode != 0:
+        raise RuntimeError(f"link failed: {' '.join(cmd)}\n{res.stdout}\n{res.stderr}")
+    os.replace(tmp, CALLS)
+
+
 def build(jobs: int = 0, verbose: bool = True) -> str:
     """Compile and link the library; returns its path."""
     os.makedirs(BUILD, exist_ok=True)
@@ -81,6 +118,7 @@ def build(jobs: int = 0, verbose: bool = True) -> str:
     jobs = jobs or min(len(srcs), max(1, (os.cpu_count() or 2)))
     t0 = time.time()
     with cf.ThreadPoolExecutor(max_workers=jobs) as ex:
+        calls = ex.submit(_compile_calls)
         objs = list(ex.map(lambda s: _compile(s, flags), srcs))
     tmp = LIB + ".tmp"
     cmd = [_hipcc(), f"--offload-arch={ARCH}", "-shared", "-fPIC", "-o", tmp, *objs,
@@ -89,6 +127,7 @@ def build(jobs: int = 0, verbose: bool = True) -> str:
     if res.returncode != 0:
         raise RuntimeError(f"link failed: {' '.join(cmd)}\n{res.stdout}\n{res.stderr}")
     os.replace(tmp, LIB)
+    _link_calls(calls.result())
     if verbose:
         print(f"[neural_shift_cuda_amd] built {LIB} ({len(srcs)} sources, "
               f"{time.time() - t0:.1f}s)")
