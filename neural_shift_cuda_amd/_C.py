@@ -993,7 +993,12 @@ def attention_forward(q, k, v, rules, want_degree, keep):
         want_degree, keep)
 
 
-# The differentiable calls, host/token_calls.cpp.
+# The differentiable calls, host/token_calls.cpp.  The ..._as_is ones take what
+# attention.py's functions take and return None unless all of it is in the types
+# and layouts of the C ABI; the others take what it has checked and converted.
+norm_rotary_as_is = _token_calls.norm_rotary_as_is
+position_bias_as_is = _token_calls.position_bias_as_is
+attention_as_is = _token_calls.attention_as_is
 norm_rotary = _token_calls.norm_rotary
 position_bias = _token_calls.position_bias
 attention = _token_calls.attention

@@ -359,6 +359,10 @@ def qk_norm_rotary(q: torch.Tensor, k: torch.Tensor, q_weight: Optional[torch.Te
     if not q.is_cuda:
         return qk_norm_rotary_reference(q, k, q_weight, k_weight, cos, sin, positions, eps=eps,
                                         interleaved=interleaved)
+    done = _C and _C.norm_rotary_as_is(q, k, q_weight, k_weight, cos, sin, positions, eps,
+                                       interleaved)
+    if done is not None:
+        return done
     positions = _check_norm(q, k, q_weight, k_weight, cos, sin, positions)
     if q.shape[3] > 512:
         raise ValueError(f"heads wider than 512 are not served on the GPU; got {q.shape[3]}")
@@ -383,6 +387,9 @@ def relative_position_bias(table: torch.Tensor, buckets: torch.Tensor, q_len: in
         raise ValueError(f"q_len and k_len must not be negative; got {q_len}, {k_len}")
     if not table.is_cuda:
         return relative_position_bias_reference(table, buckets, q_len, k_len)
+    done = _C and _C.position_bias_as_is(table, buckets, q_len, k_len)
+    if done is not None:
+        return done
     buckets = _check_buckets(table, buckets, "table")
     ops._require_cuda_ext("relative_position_bias")
     return _C.position_bias(table, buckets, q_len, k_len)
@@ -432,6 +439,10 @@ def biased_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, *,
             q, k, v, scale=scale, cap=cap, causal=causal, prefix=prefix, documents=documents,
             lengths=lengths, slopes=slopes, bias_table=bias_table, buckets=buckets,
             return_log_degree=return_log_degree)
+    done = _C and _C.attention_as_is(q, k, v, scale, cap, causal, prefix, documents, lengths,
+                                     slopes, bias_table, buckets, return_log_degree)
+    if done is not None:
+        return done if return_log_degree else done[0]
     rules = _check_attention(q, k, v, scale, cap, causal, prefix, documents, lengths, slopes,
                              bias_table, buckets)
     D = q.shape[3]

@@ -357,6 +357,68 @@ std::tuple<Tensor, Maybe> attention(const Tensor& q0, const Tensor& k0, const Te
     return {out, degree ? Maybe(log_degree) : Maybe()};
 }
 
+// ---------------------------------------------------------------------------
+// Calls as a program's loop makes them: every tensor already in the type and
+// layout that the entries take.  These look that over and run; anything else,
+// wrong or only to be converted, gives None, and attention.py's own checks say
+// what it is.  (They take 4 to 9 us in Python, as long as the rest of a call.)
+// ---------------------------------------------------------------------------
+
+bool served(const Tensor& t) {
+    const auto type = t.scalar_type();
+    return type == at::kHalf || type == at::kBFloat16 || type == at::kFloat;
+}
+
+bool alike(const Tensor& t, const Tensor& q) { return t.scalar_type() == q.scalar_type() && t.device() == q.device(); }
+
+// Not given, or contiguous in `type` and of this shape.
+bool plain(const Maybe& t, const Tensor& q, at::ScalarType type, at::IntArrayRef shape) {
+    return !t || (t->scalar_type() == type && t->device() == q.device() && t->sizes() == shape && t->is_contiguous());
+}
+
+bool map_of_buckets(const Tensor& table, const Maybe& buckets) {
+    return table.dim() == 2 && table.size(0) >= 1 && table.size(0) <= 4097 && buckets && buckets->dim() == 1 &&
+           buckets->size(0) % 2 == 1 && buckets->size(0) <= 4097 &&
+           plain(buckets, table, at::kInt, buckets->sizes());
+}
+
+std::optional<std::tuple<Tensor, Tensor>> norm_rotary_as_is(const Tensor& q, const Tensor& k, const Maybe& wq,
+                                                            const Maybe& wk, const Tensor& cos, const Tensor& sin,
+                                                            const Maybe& positions, double eps, bool interleaved) {
+    if (q.dim() != 4 || k.dim() != 4 || !served(q) || !alike(k, q)) return {};
+    const int64_t B = q.size(0), L = q.size(2), D = q.size(3);
+    if (k.size(0) != B || k.size(2) != L || k.size(3) != D || D > 512) return {};
+    if (!plain(wq, q, q.scalar_type(), {D}) || !plain(wk, q, q.scalar_type(), {D})) return {};
+    if (cos.dim() != 2 || 2 * cos.size(1) > D || cos.requires_grad() || sin.requires_grad()) return {};
+    if (!plain(cos, q, at::kFloat, cos.sizes()) || !plain(sin, q, at::kFloat, cos.sizes())) return {};
+    if (positions ? !plain(positions, q, at::kInt, {L}) && !plain(positions, q, at::kInt, {B, L}) : L > cos.size(0))
+        return {};
+    return norm_rotary(q, k, wq, wk, cos, sin, positions, eps, interleaved);
+}
+
+Maybe position_bias_as_is(const Tensor& table, const Maybe& buckets, int64_t Lq, int64_t Lk) {
+    if (Lq < 0 || Lk < 0 || !served(table) || !map_of_buckets(table, buckets)) return {};
+    return position_bias(table, *buckets, Lq, Lk);
+}
+
+std::optional<std::tuple<Tensor, Maybe>> attention_as_is(
+    const Tensor& q, const Tensor& k, const Tensor& v, std::optional<double> scale, std::optional<double> cap,
+    bool causal, const Maybe& prefix, const Maybe& documents, const Maybe& lengths, const Maybe& slopes,
+    const Maybe& table, const Maybe& buckets, bool degree) {
+    if (q.dim() != 4 || k.dim() != 4 || !served(q) || !alike(k, q) || !alike(v, q) || k.sizes() != v.sizes()) return {};
+    const int64_t B = q.size(0), Hq = q.size(1), D = q.size(3), Hk = k.size(1), Lk = k.size(2);
+    if (k.size(0) != B || k.size(3) != D || D < 8 || D > 128 || D % 8 || Hk < 1 || Hq % Hk) return {};
+    const double by = scale ? *scale : std::pow(static_cast<double>(D), -0.5), top = cap ? *cap : 0.0;
+    if (!std::isfinite(by) || !std::isfinite(top) || top < 0 || (prefix && !causal)) return {};
+    if (!plain(prefix, q, at::kInt, {B}) || !plain(lengths, q, at::kInt, {B}) ||
+        !plain(documents, q, at::kInt, {B, Lk}) || !plain(slopes, q, at::kFloat, {Hq}) ||
+        (slopes && slopes->requires_grad()))
+        return {};
+    if (table ? !alike(*table, q) || !map_of_buckets(*table, buckets) || table->size(1) != Hq : buckets.has_value())
+        return {};
+    return attention(q, k, v, table, lengths, prefix, documents, slopes, buckets, by, top, causal, degree);
+}
+
 std::tuple<Tensor, Maybe, Maybe> attention_plain(const Tensor& q, const Tensor& k, const Tensor& v, const Maybe& table,
                                                  const Maybe& lengths, const Maybe& prefix, const Maybe& documents,
                                                  const Maybe& slopes, const Maybe& buckets, double scale, double cap,
@@ -375,5 +437,8 @@ PYBIND11_MODULE(_token_calls, m) {
     m.def("norm_rotary", &norm_rotary, release());
     m.def("position_bias", &position_bias, release());
     m.def("attention", &attention, release());
+    m.def("norm_rotary_as_is", &norm_rotary_as_is, release());
+    m.def("position_bias_as_is", &position_bias_as_is, release());
+    m.def("attention_as_is", &attention_as_is, release());
     m.def("attention_forward", &attention_plain, release());
 }

@@ -137,3 +137,53 @@ def test_double_precision_is_refused(name):
     leaves, f = calls()[name]
     with pytest.raises(RuntimeError, match="not implemented"):
         f(*(t.double() for t in leaves))
+
+
+def test_refusals_on_the_gpu_are_the_checks_own():
+    q, k, v, table = calls()["attention"][0]
+    buckets = relative_buckets(8, 20).to(DEV)
+    for error, match, f in (
+            (ValueError, "multiple of the", lambda: biased_attention(q[:, :1], k, v)),
+            (ValueError, "prefix needs causal", lambda: biased_attention(
+                q, k, v, prefix=torch.zeros(1, dtype=torch.int32, device=DEV))),
+            (ValueError, "buckets come with", lambda: biased_attention(q, k, v, buckets=buckets)),
+            (ValueError, "finite", lambda: biased_attention(q, k, v, cap=float("nan"))),
+            (ValueError, "buckets must be", lambda: biased_attention(q, k, v, bias_table=table)),
+            (ValueError, "lengths must be", lambda: biased_attention(
+                q, k, v, lengths=torch.zeros(2, dtype=torch.int32, device=DEV))),
+            (ValueError, "lengths must be on", lambda: biased_attention(
+                q, k, v, lengths=torch.zeros(1, dtype=torch.int32))),
+            (TypeError, "must hold integers", lambda: biased_attention(
+                q, k, v, lengths=torch.zeros(1, device=DEV))),
+            (ValueError, "must not be negative", lambda: relative_position_bias(
+                table, buckets, -1, 3)),
+            (ValueError, "buckets must be", lambda: relative_position_bias(table, None, 3, 3)),
+            (ValueError, "rows for", lambda: qk_norm_rotary(
+                q, k, None, None, torch.ones(3, 4, device=DEV), torch.ones(3, 4, device=DEV))),
+            (ValueError, "half", lambda: qk_norm_rotary(
+                q, k, None, None, torch.ones(40, 9, device=DEV), torch.ones(40, 9, device=DEV)))):
+        with pytest.raises(error, match=match):
+            f()
+
+
+def test_converted_arguments_give_the_same():
+    """Masks in 64 bits, tables in double precision, a strided map: the same bits
+    as in the kernels' own types."""
+    q, k, v, table = calls()["attention"][0]
+    buckets = relative_buckets(8, 20).to(DEV)
+    docs = (torch.arange(40, device=DEV) // 15)[None]
+    lengths = torch.tensor([33], device=DEV)
+    slopes = torch.rand(2, device=DEV)
+    a = biased_attention(q, k, v, causal=True, documents=docs.int(), lengths=lengths.int(),
+                         slopes=slopes, bias_table=table, buckets=buckets)
+    b = biased_attention(q, k, v, causal=True, documents=docs, lengths=lengths,
+                         slopes=slopes.double(), bias_table=table,
+                         buckets=buckets.long().repeat_interleave(2)[::2])
+    assert torch.equal(a, b)
+    cos, sin = (t.to(DEV) for t in rotary_table(60, 16))
+    at = torch.arange(40, device=DEV) + 7
+    a = qk_norm_rotary(q, k, None, None, cos, sin, at.int())
+    b = qk_norm_rotary(q, k, None, None, cos.double(), sin.double(), at)
+    assert all(torch.equal(x, y) for x, y in zip(a, b))
+    assert torch.equal(relative_position_bias(table, buckets, 30, 40),
+                       relative_position_bias(table, buckets.long(), 30, 40))
