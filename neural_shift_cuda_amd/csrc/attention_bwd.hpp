@@ -103,8 +103,12 @@ __device__ __forceinline__ void row_gradient(const Att& a, const Cap& cap, const
     {
         RowFragments<T, DP> fk, fv;
         fk.read(K, by_row), fv.read(V, by_row);
-        order();
+        // here the vector work goes ahead of the other wave's products (2 x 16 heads of
+        // 4096, causal, capped: 291 us without, 267 with, 287 the other way round, as
+        // the forward has it; by keys neither changes anything)
+        priority<0>();
         s = fk.products(q), dp = fv.products(go);
+        priority<1>();
     }
     ColumnFragments<T, DP> f;
     f.read(K, by_col);
@@ -144,8 +148,9 @@ __device__ __forceinline__ void row_gradient(const Att& a, const Cap& cap, const
         if (ts) add_table(a, *ts, j0 - wr.first, least, most, l, dp);
         if (cap.mode != 0) dp *= y.w;
     }
-    order();
+    priority<0>();
     f.weigh_fine(dq, dp);
+    priority<1>();
     settle<T>();
 }
 

@@ -45,9 +45,13 @@ __device__ __forceinline__ void attend(const Att& a, const Cap& cap, const Bias&
         RowFragments<T, DP> f[NB];
 #pragma unroll
         for (int kb = 0; kb < NB; ++kb) f[kb].read(K, by_row, kb * 32);
-        order();
+        // a product issues in 4 cycles and takes 32: ahead of the other wave's vector
+        // work, which fills the rest (2 x 16 heads of 4096, causal, capped: 212 us
+        // without, 204 with, 219 the other way round; prompt of 8192: 262, 250, 267)
+        priority<1>();
 #pragma unroll
         for (int kb = 0; kb < NB; ++kb) s[kb] = f[kb].products(q);
+        priority<0>();
     }
     ColumnFragments<T, DP> f;
     const bool whole = j0 + NB * 32 <= wr.least && !(KIND == kGeneral && a.documents);
@@ -119,7 +123,9 @@ __device__ __forceinline__ void attend(const Att& a, const Cap& cap, const Bias&
     for (int kb = 0; kb < NB; ++kb) {
         ColumnFragments<T, DP> ahead;
         if (kb + 1 < NB) ahead.read(V, by_col, kb * 32 + 32);
+        priority<1>();
         f.weigh(st.o, s[kb]);
+        priority<0>();
         order();
         if (kb + 1 < NB) f = ahead;
     }

@@ -234,6 +234,15 @@ __device__ __forceinline__ void load_row(typename Eight<T>::V (&v)[DP / 16], con
 // their uses, one read and one wait at a time.
 __device__ __forceinline__ void order() { __builtin_amdgcn_sched_barrier(0); }
 
+// Which of a SIMD's waves issues first, from here on.  Without it the older wave
+// goes on with whatever it does, and the two tend to do the same.
+template <int P>
+__device__ __forceinline__ void priority() {
+    order();
+    __builtin_amdgcn_s_setprio(P);
+    order();
+}
+
 // Mixes a region's products into its other arithmetic: one product, V others,
 // N times.  A product keeps the matrix cores busy for 32 cycles after the wave
 // has gone on; in a row they would make it wait.
