@@ -67,10 +67,11 @@ static void cut_rows(Att& a, bool backward) {
 // Keys go key_block() to a workgroup.  `parts` workgroups share a key block's queries
 // where there are too few of them to go round, as long as each keeps two query
 // tiles; the third launch that adds up their sums costs more than it brings from
-// five workgroups to four CUs on.  4 x 12 heads, 1024 tokens, width 64, bf16 (384
-// workgroups): 86 us alone, 92 + 16 with two parts; 2 x 16 heads, 4 of keys, 4096
-// tokens, width 128, causal (256): 791 alone, 500 + 18; 2 x 5 heads, 333 over 517
-// tokens, fp32: 60 + 5 with four tiles kept, 38 + 5 with two, 48 + 8 with one.
+// five workgroups to four CUs on.  As the rule was set: 4 x 12 heads, 1024 tokens,
+// width 64, bf16 (384 workgroups, then of 128 keys): 86 us alone, 92 + 16 with two
+// parts; 2 x 16 heads, 4 of keys, 4096 tokens, width 128, causal (256): 791 alone,
+// 500 + 18 (now 402 + 18); 2 x 5 heads, 333 over 517 tokens, fp32: 60 + 5 with four
+// tiles kept, 38 + 5 with two, 48 + 8 with one.
 static void cut_keys(Att& a) {
     const int64_t cus = nsh_host::compute_units(), tile = a.wide ? 32 : 64;
     a.kblocks = static_cast<int>(nsh_host::ceil_div(a.Lk, key_block(a.wide ? 4 : 2, a.D)));

@@ -16,11 +16,11 @@
 //
 // What bounds them: as in the forward, the vector work of a score next to its
 // products (three by rows, four by keys).  2 x 16 heads, 4 of keys, 4096 tokens,
-// width 128, causal, capped, bf16: by rows 290 us, 710 TFLOP/s; by keys 434 us,
-// 630, and 18 for the join.  4 x 12 heads, 1024 tokens, width 64 with a learned bias, bf16:
-// 64 and 76 us, and 7 for the table.  The accumulators
-// fill half of the registers at width 128, which leaves one wave to a SIMD; by
-// keys, two fit with K and V in LDS instead (`kPaired`).
+// width 128, causal, capped, bf16: by rows 261 us, 790 TFLOP/s; by keys 402 us, 690,
+// and 18 for the join.  4 x 12 heads, 1024 tokens, width 64 with a learned bias, bf16:
+// 64 and 77 us, and 7 for the table.  The accumulators fill half of the registers at
+// width 128, which leaves one wave to a SIMD; by keys, two fit with K and V in LDS
+// instead (`kPaired`).
 #pragma once
 
 #include "attention_rows.hpp"

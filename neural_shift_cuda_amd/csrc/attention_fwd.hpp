@@ -11,13 +11,13 @@
 //     share a row block's keys (`splits`), and a second launch joins them.
 //
 // What bounds them: the vector work of a score (an exp2, with a cap another and
-// a reciprocal, and 6 to 10 more instructions) takes as much issue as its
-// products, and the two overlap only as far as the two waves of a SIMD are out of
-// step.  2 x 16 heads, 4 of keys, 4096 tokens, width 128, causal, capped, bf16: 221 us,
-// 620 TFLOP/s of the 1223 that a large library product reaches; 16 heads, 8 of keys,
-// 8192 tokens, width 96, a quarter of them a prefix: 240 us, 910.  One token
-// over 16 caches of up to 8192, 32 heads, 8 of keys: 78 + 5 us, 5.2 TB/s, which is
-// what memory gives.
+// a reciprocal, and 6 to 10 more instructions) takes more issue than its products
+// (at width 128, capped: 57% of the time and 32%), and the two overlap only as far
+// as the two waves of a SIMD are out of step.  2 x 16 heads, 4 of keys, 4096
+// tokens, width 128, causal, capped, bf16: 203 us, 680 TFLOP/s of the 1223 that a large
+// library product reaches; 16 heads, 8 of keys, 8192 tokens, width 96, a quarter of
+// them a prefix: 226 us, 970.  One token over 16 caches of up to 8192, 32 heads, 8 of
+// keys: 76 + 5 us, 5.3 TB/s, which is what memory gives.
 #pragma once
 
 #include "attention_rows.hpp"
