@@ -14,9 +14,10 @@ Tensors are (B, heads, tokens, width).  The conventions are those of the
 normalized accumulation: D = sum_j a_j v_j / sum_j a_j with a = exp(score),
 log_C the logarithm of the sum, and a row that sees nothing gives D = 0 and
 log_C = -inf.  GPU tensors go through autograd nodes in C++
-(host/token_calls.cpp) into the HIP library (fp16, bf16, fp32; sums, norms and softmax statistics in fp32); CPU
-tensors use the ``*_reference`` implementations (any floating type), which are
-also exported.  A GPU tensor never falls back to them.
+(host/token_calls.cpp) into the HIP library (fp16, bf16, fp32; sums, norms and
+softmax statistics in fp32); CPU tensors use the ``*_reference`` implementations
+(any floating type), which are also exported.  A GPU tensor never falls back to
+them.
 
 Where tokens stand: the Lq queries are the last of the n filled keys (n = Lk,
 or ``lengths[b]``), so query i has position i + n - Lq.  A training step has
