@@ -578,6 +578,10 @@ typedef struct nsh_attention_args {
 } nsh_attention_args;
 NSH_API int nsh_attention_forward(const nsh_attention_args* args, void* stream);
 NSH_API int nsh_attention_backward(const nsh_attention_args* args, void* stream);
+/* Document numbers (B, L) of any 64-bit size as the int32 that `documents`
+ * takes: each becomes the first place in its row that holds it, a negative one -1. */
+NSH_API int nsh_document_ids(const int64_t* documents, int64_t B, int64_t L, int32_t* out,
+                             void* stream);
 NSH_API int64_t nsh_attention_workspace_bytes(const nsh_attention_args* args, int backward);
 
 #ifdef __cplusplus

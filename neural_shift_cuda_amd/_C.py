@@ -937,6 +937,7 @@ for _name, _args, _res in (
         ("nsh_position_bias_backward", [_P, _P, _I64, _I64, _I64, _I64, _I64, _I, _P, _P, _I64,
                                         _P], _I),
         ("nsh_position_bias_workspace_bytes", [_I64, _I64, _I64, _I64], _I64),
+        ("nsh_document_ids", [_P, _I64, _I64, _P, _P], _I),
         ("nsh_attention_forward", [_P, _P], _I),
         ("nsh_attention_backward", [_P, _P], _I),
         ("nsh_attention_workspace_bytes", [_P, _I], _I64)):
@@ -991,6 +992,19 @@ def attention_forward(q, k, v, rules, want_degree, keep):
         q, k, v, rules["bias_table"], rules["lengths"], rules["prefix"], rules["documents"],
         rules["slopes"], rules["buckets"], rules["scale"], rules["cap"], rules["causal"],
         want_degree, keep)
+
+
+def document_ids(documents: torch.Tensor) -> torch.Tensor:
+    """int64 document numbers (B, L) as int32 with the same ones equal, and -1
+    for the negative ones (nsh_document_ids)."""
+    _cuda(documents, "documents")
+    _contig(documents, "documents")
+    _check(documents.dtype is torch.int64 and documents.dim() == 2,
+           "documents must be int64 (B, L)")
+    out = torch.empty(documents.shape, dtype=torch.int32, device=documents.device)
+    if out.numel():
+        _call_on(out, "nsh_document_ids", documents.data_ptr(), *documents.shape, out.data_ptr())
+    return out
 
 
 # The differentiable calls, host/token_calls.cpp.  The ..._as_is ones take what

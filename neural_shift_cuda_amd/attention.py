@@ -106,6 +106,14 @@ def _same(name: str, t: torch.Tensor, like: torch.Tensor, dtype: bool = True) ->
         raise ValueError(f"{name} must have dtype {like.dtype}; got {t.dtype}")
 
 
+def _integers(name: str, t: torch.Tensor, shape, like: torch.Tensor) -> None:
+    if t.is_floating_point() or t.is_complex() or t.dtype == torch.bool:
+        raise TypeError(f"{name} must hold integers; got {t.dtype}")
+    if tuple(t.shape) != tuple(shape):
+        raise ValueError(f"{name} must be {tuple(shape)}; got {tuple(t.shape)}")
+    _same(name, t, like, dtype=False)
+
+
 def _whole(name: str, t: Optional[torch.Tensor], shape, like: torch.Tensor
            ) -> Optional[torch.Tensor]:
     """An integer tensor of a given shape as contiguous int32 (values beyond
@@ -114,14 +122,28 @@ def _whole(name: str, t: Optional[torch.Tensor], shape, like: torch.Tensor
         return None
     if t.dtype is torch.int32 and t.shape == shape and t.device == like.device:
         return t.contiguous()
-    if t.is_floating_point() or t.is_complex() or t.dtype == torch.bool:
-        raise TypeError(f"{name} must hold integers; got {t.dtype}")
-    if tuple(t.shape) != tuple(shape):
-        raise ValueError(f"{name} must be {tuple(shape)}; got {tuple(t.shape)}")
-    _same(name, t, like, dtype=False)
+    _integers(name, t, shape, like)
+    if t.dtype == torch.uint64:  # the upper half has no place among the signed
+        t = t.view(torch.int64)
+        t = torch.where(t < 0, (1 << 31) - 1, t)
+    elif t.dtype == torch.uint32:
+        t = t.long()
     if t.dtype == torch.int64:
         t = t.clamp(-(1 << 31), (1 << 31) - 1)
     return t.to(torch.int32).contiguous()
+
+
+def _documents(t: Optional[torch.Tensor], shape, like: torch.Tensor) -> Optional[torch.Tensor]:
+    """Document numbers, contiguous: as int32, or, where the type holds more, as
+    int64.  Only which are equal and which are negative counts, so no two may
+    fall together as ``_whole`` lets them."""
+    if t is None:
+        return None
+    _integers("documents", t, shape, like)
+    if t.dtype == torch.uint64:  # numbered anew: the upper half would turn negative
+        t = torch.unique(t.view(torch.int64), return_inverse=True)[1]
+    wide = t.dtype in (torch.int64, torch.uint32)
+    return t.to(torch.int64 if wide else torch.int32).contiguous()
 
 
 def _acc(t: torch.Tensor) -> torch.dtype:
@@ -213,7 +235,7 @@ def _check_attention(q, k, v, scale, cap, causal, prefix, documents, lengths, sl
         raise ValueError("buckets come with a bias_table")
     return {"scale": scale, "cap": cap, "causal": bool(causal),
             "prefix": _whole("prefix", prefix, (B,), q),
-            "documents": _whole("documents", documents, (B, Lk), q),
+            "documents": _documents(documents, (B, Lk), q),
             "lengths": _whole("lengths", lengths, (B,), q), "slopes": slopes,
             "bias_table": bias_table, "buckets": buckets}
 
@@ -420,7 +442,8 @@ def biased_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, *,
       every query sees.
     * documents (B, Lk): several sequences in one row; a query sees the keys of
       its own position's document only, and a negative one (padding) sees nothing
-      and is not seen.
+      and is not seen.  Any integers: int32 is taken as it is, 64-bit numbers are
+      written anew as int32 in every call (one small launch).
     * slopes (Hq,): linear distance bias, no gradient.
     * bias_table (num_buckets, Hq) with buckets (2 * reach + 1,): a learned bias
       by buckets of the relative position, as ``relative_position_bias`` writes
@@ -450,10 +473,13 @@ def biased_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, *,
     if D > 128:
         raise ValueError(f"heads wider than 128 are not served on the GPU; got {D}")
     ops._require_cuda_ext("biased_attention")
+    docs = rules["documents"]
+    if docs is not None and docs.dtype is not torch.int32:
+        docs = _C.document_ids(docs)
     if D % 8:
         q, k, v = (torch.nn.functional.pad(t, (0, -D % 8)) for t in (q, k, v))
     out, log_C = _C.attention(q, k, v, rules["bias_table"], rules["lengths"], rules["prefix"],
-                              rules["documents"], rules["slopes"], rules["buckets"],
+                              docs, rules["slopes"], rules["buckets"],
                               rules["scale"], rules["cap"], rules["causal"], return_log_degree)
     if D % 8:
         out = out[..., :D]

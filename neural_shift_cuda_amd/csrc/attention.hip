@@ -30,6 +30,43 @@ static int ranges_launch(const Att& a, hipStream_t st) {
     return nsh_host::check_launch("attention_ranges");
 }
 
+// Document numbers of any 64-bit size as int32: each becomes the place where it
+// first stands in its row, so equal ones stay equal, the rising numbers of packed
+// rows stay rising, and the ranges above stay narrow; negative ones become -1.  A
+// wave takes 64 places and looks up their numbers, one after the other, from the
+// row's start on, 256 places a step.
+constexpr int kLookups = 4;  // loads under way
+__global__ __launch_bounds__(kAttThreads) void document_ids_kernel(const int64_t* __restrict__ ids, int64_t B, int64_t L,
+                                                                   int64_t waves, int32_t* __restrict__ out) {
+    const int l = threadIdx.x & 63;
+    for (int64_t w = static_cast<int64_t>(blockIdx.x) * kAttWaves + (threadIdx.x >> 6); w < B * waves;
+         w += static_cast<int64_t>(gridDim.x) * kAttWaves) {
+        const int64_t b = w / waves, j = (w - b * waves) * 64 + l;
+        const int64_t* row = ids + b * L;
+        const int64_t mine = j < L ? row[j] : -1;
+        int64_t first = -1;
+        for (unsigned long long open = __ballot(mine >= 0); open;) {
+            const int64_t id = __shfl(mine, __builtin_ctzll(open));
+            const unsigned long long same = __ballot(mine == id);
+            int64_t at = -1;
+            for (int64_t i0 = 0; at < 0; i0 += 64 * kLookups) {  // its own place ends the search
+                int64_t v[kLookups];
+#pragma unroll
+                for (int c = 0; c < kLookups; ++c) v[c] = i0 + c * 64 + l < L ? row[i0 + c * 64 + l] : -1;
+#pragma unroll
+                for (int c = 0; c < kLookups; ++c) {
+                    const unsigned long long hit = __ballot(v[c] == id);
+                    if (hit && at < 0) at = i0 + c * 64 + __builtin_ctzll(hit);
+                }
+                if (i0 > L) break;
+            }
+            if (same >> l & 1) first = at;
+            open &= ~same;
+        }
+        if (j < L) out[b * L + j] = static_cast<int32_t>(first);
+    }
+}
+
 // The cut of a call, from its sizes alone (workspace sizes come from here too).
 //
 // Rows go 128 to a workgroup where that gives every CU one; otherwise 32, and
@@ -187,6 +224,18 @@ extern "C" int64_t nsh_attention_workspace_bytes(const nsh_attention_args* g, in
         case NSH_DTYPE_BFLOAT16: { using T = nsh::bf16; __VA_ARGS__ } break; \
         default: { using T = float; __VA_ARGS__ } break;                     \
     }
+
+extern "C" int nsh_document_ids(const int64_t* documents, int64_t B, int64_t L, int32_t* out, void* stream) {
+    constexpr int64_t kMost = int64_t(1) << 30;
+    if (B < 1 || L < 1) return fail(NSH_ERR_INVALID, "document_ids: empty tensor");
+    if (B > kMost || L > kMost) return fail(NSH_ERR_INVALID, "document_ids: a size exceeds 2^30");
+    if (!documents || !out) return fail(NSH_ERR_INVALID, "document_ids: null pointer argument");
+    const int64_t waves = nsh_host::ceil_div(L, 64);
+    const int64_t blocks = std::min<int64_t>(nsh_host::ceil_div(B * waves, nsh::kAttWaves), 1 << 20);
+    nsh::document_ids_kernel<<<static_cast<unsigned>(blocks), nsh::kAttThreads, 0, static_cast<hipStream_t>(stream)>>>(
+        documents, B, L, waves, out);
+    return check_launch("document_ids");
+}
 
 extern "C" int nsh_attention_forward(const nsh_attention_args* g, void* stream) {
     nsh::Att a;
