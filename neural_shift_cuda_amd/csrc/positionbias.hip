@@ -137,9 +137,8 @@ __device__ __forceinline__ void far_sums(const T* g, uint32_t n, int Lk, Divisor
             }
         }
     };
-    const uint32_t step = gridDim.x * kWay * kBiasThreads;
-    for (uint32_t at = blockIdx.x * kWay * kBiasThreads; at < whole; at += step) {
-        const uint32_t k = at + threadIdx.x;
+    for (Turns turn = Turns::of(blockIdx.x, gridDim.x, kWay * kBiasThreads); turn.at < whole; turn.at += turn.step) {
+        const uint32_t at = static_cast<uint32_t>(turn.at), k = at + threadIdx.x;
         if (at + kWay * kBiasThreads <= whole) {
             Pack<T, VEC> p[kWay];
 #pragma unroll
