@@ -711,6 +711,9 @@ void att_bwd_key_kernel(Att a) {
         if (now.u < u1) step(tiles1[0], tiles0[0], 1);
     }
     if constexpr (QP == 2) {  // the second waves' sums join the first's
+        // a part without a unit (late keys of a causal call have few) has not waited
+        // for its K and V, whose place the sums take
+        if (PAIRED) __builtin_amdgcn_s_waitcnt(0x0f70);  // vmcnt(0)
         float* const room = reinterpret_cast<float*>(PAIRED ? &kv[0][0] : &tiles0[0][0]);
         float* sums = room + (kw * DP + 4 * g) * 32 + (l & 31);  // [keys][column][key]
         static_assert((PAIRED ? sizeof(kv) : sizeof(tiles0)) >= KG * DP * 32 * 4, "the sums of dk take the tiles' place");
