@@ -596,38 +596,6 @@ void att_bwd_key_kernel(Att a) {
         cq.weigh_fine(dk, dp);
         settle<T>();
     };
-    // Both parts of a 64-row tile: one part's products run under the other's
-    // weights.  (One path for all tiles, with the masks in branches of their
-    // own: where the sums were updated on several, they were copied each time.)
-    auto both = [&](const char* tile, int buf, bool whole0, bool whole1) {
-        constexpr int V = KIND == kPlain ? 6 : 11;
-        RowFragments<T, DP> fq, fg;
-        fq.read(tile, by_row), fg.read(tile + HALF, by_row);
-        order();
-        f32x16 s0 = fq.products(k), dp0 = fg.products(v);
-        const RowInfo x0 = row_info(buf, 0);
-        order();
-        fq.read(tile, by_row, 32), fg.read(tile + HALF, by_row, 32);
-        order();
-        f32x16 s1 = fq.products(k), dp1 = fg.products(v);
-        weights(x0, s0, dp0);
-        mix<2 * DP / 16, V>();
-        settle<T>();
-        if (!whole0) unsee(buf, 0, s0, dp0);
-        ColumnFragments<T, DP> cg, cq;
-        cg.read(tile + HALF, by_col), cq.read(tile, by_col);
-        const RowInfo x1 = row_info(buf, 1);
-        order();
-        cg.weigh(dv, s0), cq.weigh_fine(dk, dp0);
-        weights(x1, s1, dp1);
-        mix<(__is_same(T, f16) ? 6 : 4) * DP / 32, V>();
-        settle<T>();
-        if (!whole1) unsee(buf, 1, s1, dp1);
-        cg.read(tile + HALF, by_col, 32), cq.read(tile, by_col, 32);
-        order();
-        cg.weigh(dv, s1), cq.weigh_fine(dk, dp1);
-        settle<T>();
-    };
     auto paired = [&](const char* tile, int buf, int qb, bool whole) {
         // formed anew for each tile: kept, the reads' addresses would be spilled
         const int rows = here(by_row), cols = here(by_col), keys = rows + key_off;
@@ -666,9 +634,6 @@ void att_bwd_key_kernel(Att a) {
             if constexpr (KIND == kGeneral) general(tile, buf, qb, pf, whole);
             else if constexpr (PAIRED) paired(tile, buf, qb, whole);
             else simple(tile, buf, qb, whole);
-        } else if constexpr (KIND != kGeneral && NB == 2) {
-            if (j0 < ends(p0 + min(a.Lq - i0, 64) - 1))
-                both(tile, buf, j0 + 32 <= ends(p0), j0 + 32 <= ends(p0 + 32));
         } else {
 #pragma unroll 1
             for (int qb = 0; qb < NB; ++qb) {

@@ -243,18 +243,6 @@ __device__ __forceinline__ void priority() {
     order();
 }
 
-// Mixes a region's products into its other arithmetic: one product, V others,
-// N times.  A product keeps the matrix cores busy for 32 cycles after the wave
-// has gone on; in a row they would make it wait.
-template <int N, int V>
-__device__ __forceinline__ void mix() {
-#pragma unroll
-    for (int i = 0; i < N; ++i) {
-        __builtin_amdgcn_sched_group_barrier(0x008, 1, 0);
-        __builtin_amdgcn_sched_group_barrier(0x402, V, 0);
-    }
-}
-
 // Ends a run of products ahead of a branch.  Their results may be read 12 wait
 // states (18 for the fp32 products) after the last one at the earliest, and the
 // hardware does not wait by itself; the compiler counts the states, but has
