@@ -114,15 +114,16 @@ __device__ __forceinline__ void row_gradient(const Att& a, const Cap& cap, const
     f.read(K, by_col);
     if (KIND != kGeneral) {
         order();
-        // p's two constants in one: 1 / sum joins the exponent
-        const float up = __builtin_amdgcn_logf(stat.y) - stat.x + (KIND == kCapped ? cap.top : 0.f);
+        // 1 / sum goes to the other factor: in the exponent, next to a maximum of
+        // thousands, it would lose its last places
+        const float up = (KIND == kCapped ? cap.top : 0.f) - stat.x, d = delta * stat.y;
 #pragma unroll
         for (int r = 0; r < 16; ++r) {
             if (KIND == kPlain) {
-                dp[r] = __builtin_amdgcn_exp2f(fma_acc(s[r], cap.c, up)) * (dp[r] - delta);
+                dp[r] = __builtin_amdgcn_exp2f(fma_acc(s[r], cap.c, up)) * fma_acc(dp[r], stat.y, -d);
             } else {
                 const float c = quick_r(s[r], cap.k);
-                dp[r] = __builtin_amdgcn_exp2f(fma_acc(c, -2.f * cap.top, up)) * (dp[r] - delta) *
+                dp[r] = __builtin_amdgcn_exp2f(fma_acc(c, -2.f * cap.top, up)) * fma_acc(dp[r], stat.y, -d) *
                         (4.f * fma_acc(-c, c, c));
             }
         }
@@ -355,18 +356,28 @@ __global__ __launch_bounds__(kAttThreads, SPLIT || DP * sizeof(T) > (KIND == kGe
 //            and one wave waits for its own products
 enum Share { kAlone, kTwin, kPaired };
 
+// A row's log 2 of weight over score this far from 0 is off by less than 2^-15 of
+// the weight, a sixteenth of an fp16 weight's own half step.
+constexpr float kNear = 1024.f;
+
 template <typename T, int DP, Kind KIND, Share SHARE>
 __global__ __launch_bounds__(SHARE == kPaired ? 512 : kAttThreads, SHARE != kPaired && DP * sizeof(T) < 256 ? 2 : 1)
 void att_bwd_key_kernel(Att a) {
     constexpr int KG = SHARE == kTwin ? 2 : 4, QP = SHARE == kAlone ? 1 : 2;
     constexpr bool PAIRED = SHARE == kPaired;
+    // fp32 results show the places that 1 / sum loses in the exponent from the first
+    // score on: there it is a factor of its own
+    constexpr bool kApart = sizeof(T) == 4;
     using L = Tile<T, DP>;
     constexpr int QT = BwdShape<T, DP>::KT, NB = QT / 32, HALF = QT * L::ROW;
     constexpr int KV = PAIRED ? 128 * L::ROW : 16;
     __shared__ __attribute__((aligned(1024))) char kv[2][KV];
     __shared__ __attribute__((aligned(1024))) char tiles0[2][HALF];
     __shared__ __attribute__((aligned(1024))) char tiles1[2][HALF];
-    __shared__ __attribute__((aligned(256))) float info[2][6][QT];  // log 2 of weight over score, maximum, 1 / sum, delta, key end, document
+    // log 2 of weight over score, maximum, 1 / sum (without a bias: what that log 2
+    // leaves of it), delta, key end, document
+    __shared__ __attribute__((aligned(256))) float info[2][6][QT];
+    __shared__ int far[2];
     extern __shared__ float line[];
     const int l = threadIdx.x & 63, wave = wave_id(), g = l >> 5, kw = wave % KG;
     int bg, rest;
@@ -469,8 +480,18 @@ void att_bwd_key_kernel(Att a) {
     auto put = [&](int buf) {
         const int x = threadIdx.x;
         if (x >= QT) return;
-        info[buf][0][x] = __builtin_amdgcn_logf(r_stat.y) - r_stat.x + (cap.mode == 1 ? cap.top : 0.f);
-        info[buf][1][x] = r_stat.x, info[buf][2][x] = r_stat.y, info[buf][3][x] = r_delta;
+        if (KIND == kGeneral) {
+            info[buf][1][x] = r_stat.x, info[buf][2][x] = r_stat.y;
+        } else {
+            // 1 / sum joins the exponent; next to a large maximum that loses its last
+            // places, and the weights take what it lost as a factor
+            const float up = __builtin_amdgcn_logf(r_stat.y) - r_stat.x;
+            info[buf][0][x] = kApart ? -r_stat.x : up + (KIND == kCapped ? cap.top : 0.f);
+            info[buf][2][x] = kApart || r_stat.y == 0.f ? r_stat.y : r_stat.y * __builtin_amdgcn_exp2f(-r_stat.x - up);
+            const bool beyond = __any(r_stat.y != 0.f && fabsf(up) > kNear);
+            if (x == 0) far[buf] = beyond;
+        }
+        info[buf][3][x] = r_delta;
         info[buf][4][x] = __int_as_float(r_lim);
         if (KIND == kGeneral) info[buf][5][x] = __int_as_float(r_doc);
     };
@@ -541,7 +562,7 @@ void att_bwd_key_kernel(Att a) {
     };
     // The weights p (in place of the products s) and dx, without a bias.
     struct RowInfo {
-        f32x4 up[4], del[4];
+        f32x4 up[4], del[4], inv[kApart ? 4 : 1];
     };
     auto row_info = [&](int buf, int qb) {
         const float* rows = &info[buf][0][qb * 32 + 4 * g];
@@ -550,6 +571,7 @@ void att_bwd_key_kernel(Att a) {
         for (int c = 0; c < 4; ++c) {
             x.up[c] = *reinterpret_cast<const f32x4*>(rows + 8 * c);
             x.del[c] = *reinterpret_cast<const f32x4*>(rows + 3 * QT + 8 * c);
+            if (kApart) x.inv[c] = *reinterpret_cast<const f32x4*>(rows + 2 * QT + 8 * c);
         }
         return x;
     };
@@ -558,6 +580,7 @@ void att_bwd_key_kernel(Att a) {
         for (int r = 0; r < 16; ++r) {
             if constexpr (KIND == kPlain) {
                 s[r] = __builtin_amdgcn_exp2f(fma_acc(s[r], cap.c, x.up[r / 4][r % 4]));
+                if constexpr (kApart) s[r] *= x.inv[r / 4][r % 4];
                 dp[r] = s[r] * (dp[r] - x.del[r / 4][r % 4]);
             } else {
                 const float q = quick_r(s[r], cap.k);
@@ -566,15 +589,18 @@ void att_bwd_key_kernel(Att a) {
             }
         }
     };
-    auto unsee = [&](int buf, int qb, f32x16& s, f32x16& dp) {
+    // Unseen pairs to 0, and far rows' weights to their last places.
+    auto mend = [&](int buf, int qb, f32x16& s, f32x16& dp) {
         const float* rows = &info[buf][4][qb * 32 + 4 * g];
 #pragma unroll
         for (int c = 0; c < 4; ++c) {
             const i32x4 lim = *reinterpret_cast<const i32x4*>(rows + 8 * c);
+            f32x4 by = {1.f, 1.f, 1.f, 1.f};
+            if (KIND == kPlain && !kApart) by = *reinterpret_cast<const f32x4*>(rows - 2 * QT + 8 * c);
 #pragma unroll
             for (int e = 0; e < 4; ++e) {
                 const int r = 4 * c + e;
-                s[r] = j < lim[e] ? s[r] : 0.f, dp[r] = j < lim[e] ? dp[r] : 0.f;
+                s[r] = j < lim[e] ? s[r] * by[e] : 0.f, dp[r] = j < lim[e] ? dp[r] * by[e] : 0.f;
             }
         }
     };
@@ -589,7 +615,7 @@ void att_bwd_key_kernel(Att a) {
         const RowInfo x = row_info(buf, qb);
         settle<T>();
         weights(x, s, dp);
-        if (!whole) unsee(buf, qb, s, dp);
+        if (!whole) mend(buf, qb, s, dp);
         cq.read(part, by_col);
         order();
         cg.weigh(dv, s);
@@ -616,7 +642,7 @@ void att_bwd_key_kernel(Att a) {
         weights(row_info(buf, qb), s, dp);
         ColumnFragments<T, DP> cg, cq;
         cg.read(tile + HALF, cols);
-        if (!whole) unsee(buf, qb, s, dp);
+        if (!whole) mend(buf, qb, s, dp);
         cq.read(tile, cols);
         order();
         cg.weigh(dv, s);
@@ -627,10 +653,11 @@ void att_bwd_key_kernel(Att a) {
         const int i0 = now.i0, p0 = i0 + off;
         // the rows' key ends rise with their position
         auto ends = [&](int p) { return a.causal ? min(n, max(p + 1, prefix)) : n; };
+        auto rows_far = [&](int buf) { return KIND == kPlain && !kApart && __builtin_amdgcn_readfirstlane(far[buf]); };
         if constexpr (QP == 2) {
             const int qb = wave / KG, pf = p0 + qb * 32, count = min(a.Lq - i0 - qb * 32, 32);
             if (count <= 0 || j0 >= ends(pf + count - 1)) return;
-            const bool whole = j0 + 32 <= ends(pf) && !(KIND == kGeneral && a.documents);
+            const bool whole = j0 + 32 <= ends(pf) && !(KIND == kGeneral && a.documents) && !rows_far(buf);
             if constexpr (KIND == kGeneral) general(tile, buf, qb, pf, whole);
             else if constexpr (PAIRED) paired(tile, buf, qb, whole);
             else simple(tile, buf, qb, whole);
