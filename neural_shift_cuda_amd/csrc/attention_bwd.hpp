@@ -98,7 +98,7 @@ __device__ __forceinline__ void row_gradient(const Att& a, const Cap& cap, const
                                              const WaveRows& wr, const typename Eight<T>::V (&q)[DP / 16],
                                              const typename Eight<T>::V (&go)[DP / 16], float2 stat, float delta,
                                              const char* K, const char* V, int by_row, int by_col, const int* kd, int j0, int l,
-                                             TableSums* ts, f32x16 (&dq)[DP / 32]) {
+                                             TableSums* ts, float& by, f32x16 (&dq)[DP / 32]) {
     f32x16 s, dp;
     {
         RowFragments<T, DP> fk, fv;
@@ -116,14 +116,15 @@ __device__ __forceinline__ void row_gradient(const Att& a, const Cap& cap, const
         order();
         // 1 / sum goes to the other factor: in the exponent, next to a maximum of
         // thousands, it would lose its last places
-        const float up = (KIND == kCapped ? cap.top : 0.f) - stat.x, d = delta * stat.y;
+        const float up = (KIND == kCapped ? cap.top : 0.f) - stat.x;
+        const float y = kNarrow<T> ? stat.y * by : stat.y, d = delta * y;
 #pragma unroll
         for (int r = 0; r < 16; ++r) {
             if (KIND == kPlain) {
-                dp[r] = __builtin_amdgcn_exp2f(fma_acc(s[r], cap.c, up)) * fma_acc(dp[r], stat.y, -d);
+                dp[r] = __builtin_amdgcn_exp2f(fma_acc(s[r], cap.c, up)) * fma_acc(dp[r], y, -d);
             } else {
                 const float c = quick_r(s[r], cap.k);
-                dp[r] = __builtin_amdgcn_exp2f(fma_acc(c, -2.f * cap.top, up)) * fma_acc(dp[r], stat.y, -d) *
+                dp[r] = __builtin_amdgcn_exp2f(fma_acc(c, -2.f * cap.top, up)) * fma_acc(dp[r], y, -d) *
                         (4.f * fma_acc(-c, c, c));
             }
         }
@@ -139,16 +140,17 @@ __device__ __forceinline__ void row_gradient(const Att& a, const Cap& cap, const
         s = add_bias<1>(a, bs, rel0, least, most, y.s);
         const bool whole = j0 + 32 <= wr.least && !a.documents;
         if (!whole) s = mask_keys(a, x, j0, kd, l, s);
-        const float d = delta * stat.y;
+        const float w = kNarrow<T> ? stat.y * by : stat.y, d = delta * w;
 #pragma unroll
-        for (int r = 0; r < 16; ++r) dp[r] = __builtin_amdgcn_exp2f(s[r] - stat.x) * fma_acc(dp[r], stat.y, -d);
+        for (int r = 0; r < 16; ++r) dp[r] = __builtin_amdgcn_exp2f(s[r] - stat.x) * fma_acc(dp[r], w, -d);
         if (!whole) {
 #pragma unroll
             for (int r = 0; r < 16; ++r) dp[r] = s[r] == -INFINITY ? 0.f : dp[r];
         }
-        if (ts) add_table(a, *ts, j0 - wr.first, least, most, l, dp);
+        if (ts) add_table(a, *ts, j0 - wr.first, least, most, l, kNarrow<T> ? dp * (1.f / by) : dp);
         if (cap.mode != 0) dp *= y.w;
     }
+    dp = fit<T>(by, dp, dq);
     priority<0>();
     f.weigh_fine(dq, dp);
     priority<1>();
@@ -241,6 +243,7 @@ __global__ __launch_bounds__(kAttThreads, SPLIT || DP * sizeof(T) > (KIND == kGe
     };
     Needed<decltype(wanted)> need{wanted};
     f32x16 dq[L::ND] = {};
+    float by = kFitFirst;  // what dq's weights are times
     int t = need.next(begin, end);
     TableSums* const ts = KIND == kGeneral && a.gtable ? &sums : nullptr;
     const int by_row = L::row_base(0, l), by_col = L::col_base(0, l);
@@ -251,7 +254,7 @@ __global__ __launch_bounds__(kAttThreads, SPLIT || DP * sizeof(T) > (KIND == kGe
             const int j0 = t * KT + kb * 32;
             if (j0 >= wr.most) break;
             row_gradient<T, DP, KIND>(a, cap, bs, x.r, wr, q, go, stat, delta, tile + kb * 32 * L::ROW,
-                                      tile + HALF + kb * 32 * L::ROW, by_row, by_col, docs + kb * 32, j0, l, ts, dq);
+                                      tile + HALF + kb * 32 * L::ROW, by_row, by_col, docs + kb * 32, j0, l, ts, by, dq);
         }
     };
     auto step = [&](char* tile, int* docs, char* ahead, int* docs_ahead) {
@@ -273,10 +276,11 @@ __global__ __launch_bounds__(kAttThreads, SPLIT || DP * sizeof(T) > (KIND == kGe
         if (NBUF == 2 && t < end) step(tiles1[NBUF == 2 ? mine : 0][0], docs1[mine], tiles0[mine][0], docs0[mine]);
     }
     float bad = 0.f;
+    const float last = kNarrow<T> ? a.scale / by : a.scale;
 #pragma unroll
     for (int d = 0; d < L::ND; ++d)
 #pragma unroll
-        for (int r = 0; r < 16; ++r) dq[d][r] *= a.scale, bad = fma_acc(dq[d][r], 0.f, bad);
+        for (int r = 0; r < 16; ++r) dq[d][r] *= last, bad = fma_acc(dq[d][r], 0.f, bad);
     if constexpr (SPLIT) {
         // the waves' sums in their order, half of the columns at a time
         float* part = reinterpret_cast<float*>(&tiles0[0][0][0]);  // [wave][column][row]
@@ -481,12 +485,12 @@ void att_bwd_key_kernel(Att a) {
         const int x = threadIdx.x;
         if (x >= QT) return;
         if (KIND == kGeneral) {
-            info[buf][1][x] = r_stat.x, info[buf][2][x] = r_stat.y;
+            info[buf][1][x] = r_stat.x, info[buf][2][x] = r_stat.y * kRoom<T>;
         } else {
             // 1 / sum joins the exponent; next to a large maximum that loses its last
             // places, and the weights take what it lost as a factor
             const float up = __builtin_amdgcn_logf(r_stat.y) - r_stat.x;
-            info[buf][0][x] = kApart ? -r_stat.x : up + (KIND == kCapped ? cap.top : 0.f);
+            info[buf][0][x] = kApart ? -r_stat.x : up + ((KIND == kCapped ? cap.top : 0.f) + (kNarrow<T> ? 15.f : 0.f));
             info[buf][2][x] = kApart || r_stat.y == 0.f ? r_stat.y : r_stat.y * __builtin_amdgcn_exp2f(-r_stat.x - up);
             const bool beyond = __any(r_stat.y != 0.f && fabsf(up) > kNear);
             if (x == 0) far[buf] = beyond;
@@ -496,6 +500,7 @@ void att_bwd_key_kernel(Att a) {
         if (KIND == kGeneral) info[buf][5][x] = __int_as_float(r_doc);
     };
     f32x16 dk[L::ND] = {}, dv[L::ND] = {};
+    float by = kFitFirst / kRoom<T>;  // what dk's weights are times, besides kRoom
     Unit now{need.next(u0, u1), 0, 0};
     if (now.u < u1) now.h = hk * a.per + now.u / (t1 - t0), now.i0 = (t0 + now.u % (t1 - t0)) * QT;
     int staged = -1;
@@ -548,6 +553,7 @@ void att_bwd_key_kernel(Att a) {
             }
         }
         if (cap.mode != 0) dp *= y.w;
+        if (kNarrow<T>) dp *= by;
         if (!whole) {  // 0 times what an unseen pair holds is not always 0
 #pragma unroll
             for (int r = 0; r < 16; ++r) dp[r] = s[r] == 0.f ? 0.f : dp[r];
@@ -555,6 +561,7 @@ void att_bwd_key_kernel(Att a) {
         order();
         if (DP > 64) cg.read(part + HALF, by_col);
         if (DP <= 64) cq.read(part, by_col);
+        dp = fit<T>(by, dp, dk);
         cg.weigh(dv, s);
         if (DP > 64) cq.read(part, by_col);
         cq.weigh_fine(dk, dp);
@@ -582,10 +589,11 @@ void att_bwd_key_kernel(Att a) {
                 s[r] = __builtin_amdgcn_exp2f(fma_acc(s[r], cap.c, x.up[r / 4][r % 4]));
                 if constexpr (kApart) s[r] *= x.inv[r / 4][r % 4];
                 dp[r] = s[r] * (dp[r] - x.del[r / 4][r % 4]);
+                if constexpr (kNarrow<T>) dp[r] *= by;
             } else {
                 const float q = quick_r(s[r], cap.k);
                 s[r] = __builtin_amdgcn_exp2f(fma_acc(q, -2.f * cap.top, x.up[r / 4][r % 4]));
-                dp[r] = s[r] * (dp[r] - x.del[r / 4][r % 4]) * (4.f * fma_acc(-q, q, q));
+                dp[r] = s[r] * (dp[r] - x.del[r / 4][r % 4]) * ((kNarrow<T> ? 4.f * by : 4.f) * fma_acc(-q, q, q));
             }
         }
     };
@@ -595,12 +603,12 @@ void att_bwd_key_kernel(Att a) {
 #pragma unroll
         for (int c = 0; c < 4; ++c) {
             const i32x4 lim = *reinterpret_cast<const i32x4*>(rows + 8 * c);
-            f32x4 by = {1.f, 1.f, 1.f, 1.f};
-            if (KIND == kPlain && !kApart) by = *reinterpret_cast<const f32x4*>(rows - 2 * QT + 8 * c);
+            f32x4 fix = {1.f, 1.f, 1.f, 1.f};
+            if (KIND == kPlain && !kApart) fix = *reinterpret_cast<const f32x4*>(rows - 2 * QT + 8 * c);
 #pragma unroll
             for (int e = 0; e < 4; ++e) {
                 const int r = 4 * c + e;
-                s[r] = j < lim[e] ? s[r] * by[e] : 0.f, dp[r] = j < lim[e] ? dp[r] * by[e] : 0.f;
+                s[r] = j < lim[e] ? s[r] * fix[e] : 0.f, dp[r] = j < lim[e] ? dp[r] * fix[e] : 0.f;
             }
         }
     };
@@ -617,6 +625,7 @@ void att_bwd_key_kernel(Att a) {
         weights(x, s, dp);
         if (!whole) mend(buf, qb, s, dp);
         cq.read(part, by_col);
+        dp = fit<T>(by, dp, dk);
         order();
         cg.weigh(dv, s);
         cq.weigh_fine(dk, dp);
@@ -644,6 +653,7 @@ void att_bwd_key_kernel(Att a) {
         cg.read(tile + HALF, cols);
         if (!whole) mend(buf, qb, s, dp);
         cq.read(tile, cols);
+        dp = fit<T>(by, dp, dk);
         order();
         cg.weigh(dv, s);
         cq.weigh_fine(dk, dp);
@@ -701,6 +711,11 @@ void att_bwd_key_kernel(Att a) {
     while (now.u < u1) {
         step(tiles0[0], tiles1[0], 0);
         if (now.u < u1) step(tiles1[0], tiles0[0], 1);
+    }
+    if constexpr (kNarrow<T>) {
+        const float back = 1.f / (by * kRoom<T>);
+#pragma unroll
+        for (int d = 0; d < L::ND; ++d) dk[d] *= back, dv[d] *= 1.f / kRoom<T>;
     }
     if constexpr (QP == 2) {  // the second waves' sums join the first's
         // a part without a unit (late keys of a causal call have few) has not waited

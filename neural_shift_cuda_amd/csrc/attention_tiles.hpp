@@ -309,8 +309,9 @@ struct ColumnFragments {  // 32 tile rows, `row` rows on from the base's, by col
     // cancel: in fp16, which is chosen for its 11 bits, w goes in two parts, what
     // the type takes of it and of the rest (errors of those gradients 3.4e-4 to
     // 2.9e-4 at 2500 tokens of width 64, where the result's own rounding makes
-    // 2.1e-4; 5% of the gradients' time).  In bf16 one part's rounding, at most
-    // 2^-9 of every dx, is of the size of the results' own; two would cost 15%.
+    // 2.1e-4; 5% of the gradients' time), brought into its range by fit().  In
+    // bf16 one part's rounding, at most 2^-9 of every dx, is of the size of the
+    // results' own; two would cost 15%.
     __device__ __forceinline__ void weigh_fine(f32x16 (&acc)[DP / 32], const f32x16& w) const {
         if constexpr (!__is_same(T, f16)) return weigh(acc, w);
         using V = typename Eight<T>::V;
@@ -329,6 +330,37 @@ struct ColumnFragments {  // 32 tile rows, `row` rows on from the base's, by col
         for (int d = 0; d < DP / 32; ++d) acc[d] = Eight<T>::mma(f[d][1], hi2, acc[d]);
     }
 };
+
+// fp16 has its 11 bits from 2^-14 to 2^16 alone, where the gradients' weights lie
+// anywhere: a mean loss sends dO of 1e-5, and p is 1 / count.  The products take
+// both times powers of two, which the sums are rid of at the end: p (1 at most)
+// times kRoom, dx times a factor of the lane's own row or key, kept as the running
+// maximum of a softmax is: a tile whose largest dx passes kFitMost brings that
+// down to kFitTo, and the sums with it.  It starts where the smallest dx that an
+// fp16 result can show is still a normal number.  (2500 tokens, width 64, causal,
+// dO of 2^-10: dq and dk off by 2.8e-4 and 3.0e-4, their own rounding, and 1.1e-3
+// without; documents in rows of 2500, training: 143 us without, 151 with.)
+template <typename T> constexpr bool kNarrow = __is_same(T, f16);
+template <typename T> constexpr float kRoom = kNarrow<T> ? 32768.f : 1.f;
+constexpr float kFitMost = 32768.f, kFitFirst = 1.0995116e12f;  // 2^40
+constexpr int kFitTo = 8;                                       // the largest below 2^8
+
+template <typename T, int ND>
+__device__ __forceinline__ f32x16 fit(float& by, f32x16 dx, f32x16 (&acc)[ND]) {
+    if constexpr (!kNarrow<T>) return dx;
+    float top = 0.f;
+#pragma unroll
+    for (int r = 0; r < 16; ++r) top = fmaxf(top, fabsf(dx[r]));
+    top = halves_max(top);
+    if (__any(top > kFitMost)) {
+        const float down = top > kFitMost ? ldexpf(1.f, kFitTo - __builtin_amdgcn_frexp_expf(top)) : 1.f;
+        by *= down;
+        dx *= down;
+#pragma unroll
+        for (int d = 0; d < ND; ++d) acc[d] *= down;
+    }
+    return dx;
+}
 
 // ---------------------------------------------------------------------------
 // Scores, in units of log 2.
