@@ -489,10 +489,10 @@ void att_bwd_key_kernel(Att a) {
         } else {
             // 1 / sum joins the exponent; next to a large maximum that loses its last
             // places, and the weights take what it lost as a factor
-            const float up = __builtin_amdgcn_logf(r_stat.y) - r_stat.x;
-            info[buf][0][x] = kApart ? -r_stat.x : up + ((KIND == kCapped ? cap.top : 0.f) + (kNarrow<T> ? 15.f : 0.f));
-            info[buf][2][x] = kApart || r_stat.y == 0.f ? r_stat.y : r_stat.y * __builtin_amdgcn_exp2f(-r_stat.x - up);
-            const bool beyond = __any(r_stat.y != 0.f && fabsf(up) > kNear);
+            const float y = r_stat.y * kRoom<T>, up = __builtin_amdgcn_logf(y) - r_stat.x;
+            info[buf][0][x] = kApart ? -r_stat.x : up + (KIND == kCapped ? cap.top : 0.f);
+            info[buf][2][x] = kApart || y == 0.f ? y : y * __builtin_amdgcn_exp2f(-r_stat.x - up);
+            const bool beyond = __any(y != 0.f && fabsf(up) > kNear);
             if (x == 0) far[buf] = beyond;
         }
         info[buf][3][x] = r_delta;
