@@ -473,7 +473,8 @@ void att_bwd_key_kernel(Att a) {
         const int x = threadIdx.x;
         if (x >= QT) return;
         const int i = y.i0 + x;
-        r_stat = make_float2(0.f, 0.f), r_delta = 0.f, r_lim = 0, r_doc = -1;
+        // a row past the end has a maximum that no bias comes near: exp2 of its scores is 0
+        r_stat = make_float2(__FLT_MAX__, 0.f), r_delta = 0.f, r_lim = 0, r_doc = -1;
         if (i < a.Lq) {
             const int64_t at = (static_cast<int64_t>(b) * a.Hq + y.h) * a.Lq + i;
             const Row r = row_of(a, b, i, n, prefix);

@@ -267,7 +267,7 @@ __device__ __forceinline__ int here(int v) {
 
 __device__ __forceinline__ int wave_id() { return __builtin_amdgcn_readfirstlane(threadIdx.x >> 6); }
 
-// Kinds of call, each with kernels of its own: no bias and no documents, without
+// Kinds of call, each with kernels of its own: no bias, no documents and a scale, without
 // a cap (kPlain) or with the quick one (kCapped), whose tiles take no branch; or
 // whatever a call may hold (kGeneral), at a cost in registers.
 enum Kind { kPlain, kCapped, kGeneral };
@@ -376,7 +376,8 @@ struct Cap {
 
 template <typename T>
 inline Kind kind_of(const Att& a) {
-    if (a.slopes || a.table || a.documents) return kGeneral;
+    // a scale of 0 too: the others mask their products ahead of it, and -inf times 0 is none
+    if (a.slopes || a.table || a.documents || a.scale == 0.f) return kGeneral;
     return a.cap <= 0.f ? kPlain : sizeof(T) == 2 && a.cap <= kQuickCap ? kCapped : kGeneral;
 }
 
