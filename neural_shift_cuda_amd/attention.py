@@ -25,6 +25,7 @@ Lq = Lk, a single new token Lq = 1.
 """
 from __future__ import annotations
 
+import functools
 import math
 from typing import Optional, Tuple
 
@@ -357,6 +358,44 @@ def biased_attention_reference(q, k, v, *, scale: Optional[float] = None,
 
 
 # ---------------------------------------------------------------------------
+# Calls under torch.jit.trace
+# ---------------------------------------------------------------------------
+
+class _TracedCall(torch.autograd.Function):
+    """A call as one step of a trace, which records a Python function as what is to
+    be run again, but nothing of what C++ does with the tensors' memory."""
+
+    @staticmethod
+    def forward(ctx, call, *tensors):
+        ctx.set_materialize_grads(False)
+        with torch.enable_grad():
+            ctx.leaves = [t if t is None else t.detach().requires_grad_(t.requires_grad)
+                          for t in tensors]
+            out = call(*ctx.leaves)
+        ctx.out = out if isinstance(out, tuple) else (out,)
+        out = tuple(t.detach() for t in ctx.out)
+        return out if len(out) > 1 else out[0]
+
+    @staticmethod
+    @torch.autograd.function.once_differentiable
+    def backward(ctx, *upstream):
+        want = [n for n, t in enumerate(ctx.leaves) if t is not None and t.requires_grad]
+        outs = [(t, g) for t, g in zip(ctx.out, upstream) if g is not None]
+        got = torch.autograd.grad([t for t, _ in outs], [ctx.leaves[n] for n in want],
+                                  [g for _, g in outs], retain_graph=True, allow_unused=True)
+        grads = [None] * len(ctx.leaves)
+        for n, g in zip(want, got):
+            grads[n] = g
+        return (None, *grads)
+
+
+def _traceable(call, tensors, **rules):
+    if not torch.jit.is_tracing():
+        return call(*tensors, **rules)
+    return _TracedCall.apply(functools.partial(call, **rules), *tensors)
+
+
+# ---------------------------------------------------------------------------
 # Public API
 # ---------------------------------------------------------------------------
 
@@ -386,6 +425,11 @@ def qk_norm_rotary(q: torch.Tensor, k: torch.Tensor, q_weight: Optional[torch.Te
                                        interleaved)
     if done is not None:
         return done
+    return _traceable(_norm_rotary, (q, k, q_weight, k_weight, cos, sin, positions), eps=eps,
+                      interleaved=interleaved)
+
+
+def _norm_rotary(q, k, q_weight, k_weight, cos, sin, positions, *, eps, interleaved):
     positions = _check_norm(q, k, q_weight, k_weight, cos, sin, positions)
     if q.shape[3] > 512:
         raise ValueError(f"heads wider than 512 are not served on the GPU; got {q.shape[3]}")
@@ -413,6 +457,10 @@ def relative_position_bias(table: torch.Tensor, buckets: torch.Tensor, q_len: in
     done = _C and _C.position_bias_as_is(table, buckets, q_len, k_len)
     if done is not None:
         return done
+    return _traceable(_position_bias, (table, buckets), q_len=q_len, k_len=k_len)
+
+
+def _position_bias(table, buckets, *, q_len, k_len):
     buckets = _check_buckets(table, buckets, "table")
     ops._require_cuda_ext("relative_position_bias")
     return _C.position_bias(table, buckets, q_len, k_len)
@@ -467,6 +515,12 @@ def biased_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, *,
                                      slopes, bias_table, buckets, return_log_degree)
     if done is not None:
         return done if return_log_degree else done[0]
+    return _traceable(_attention, (q, k, v, prefix, documents, lengths, slopes, bias_table, buckets),
+                      scale=scale, cap=cap, causal=causal, return_log_degree=return_log_degree)
+
+
+def _attention(q, k, v, prefix, documents, lengths, slopes, bias_table, buckets, *, scale, cap,
+               causal, return_log_degree):
     rules = _check_attention(q, k, v, scale, cap, causal, prefix, documents, lengths, slopes,
                              bias_table, buckets)
     D = q.shape[3]

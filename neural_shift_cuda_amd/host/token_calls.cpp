@@ -8,7 +8,9 @@
 // for the backward in the autograd thread, whose caches are cold for the
 // interpreter; here 96.  One token over a short cache: 17 us, here 10.
 #include <c10/hip/HIPStream.h>
+#include <c10/core/AutogradState.h>
 #include <torch/csrc/autograd/functions/basic_ops.h>
+#include <torch/csrc/jit/frontend/tracer.h>
 #include <torch/extension.h>
 
 #include <cmath>
@@ -80,6 +82,14 @@ variable_list once(variable_list grads) {
         "trying to differentiate twice a token operator, whose gradients are not differentiable",
         static_cast<int64_t>(grads.size()));
     return (*error)(std::move(grads));
+}
+
+// A tangent would be dropped without a word: what the kernels write has none.
+void no_tangents(const char* op, std::initializer_list<const Tensor*> tensors) {
+    if (!c10::AutogradState::get_tls_state().get_fw_grad_mode()) return;
+    for (const Tensor* t : tensors)
+        TORCH_CHECK_NOT_IMPLEMENTED(!t->defined() || !t->_fw_grad(0).defined(), op,
+                                    ": forward-mode derivatives are not implemented");
 }
 
 bool graph(std::initializer_list<const Tensor*> tensors) {
@@ -177,6 +187,7 @@ std::tuple<Tensor, Tensor> norm_rotary(const Tensor& q, const Tensor& k, const M
                                        double eps, bool interleaved) {
     c10::DeviceGuard on(q.device());
     const Tensor w0 = given(wq), w1 = given(wk);
+    no_tangents("norm_rotary", {&q, &k, &w0, &w1, &cos, &sin});
     const variable_list out =
         graph({&q, &k, &w0, &w1})
             ? NormNode::apply(q, k, wq, wk, cos, sin, positions, NormRules{eps, interleaved})
@@ -230,6 +241,7 @@ struct BiasNode : torch::autograd::Function<BiasNode> {
 
 Tensor position_bias(const Tensor& table, const Tensor& buckets, int64_t Lq, int64_t Lk) {
     c10::DeviceGuard on(table.device());
+    no_tangents("position_bias", {&table});
     return graph({&table}) ? BiasNode::apply(table, buckets, Lq, Lk)
                            : bias_forward(table.contiguous(), buckets, Lq, Lk);
 }
@@ -347,6 +359,7 @@ std::tuple<Tensor, Maybe> attention(const Tensor& q0, const Tensor& k0, const Te
     c10::DeviceGuard on(q0.device());
     const Tensor q = rows16(q0), k = rows16(k0), v = rows16(v0), t = given(table);
     const Masks m{given(lengths), given(prefix), given(documents), given(slopes), given(buckets)};
+    no_tangents("attention", {&q, &k, &v, &t, &m.slopes});
     const Rules r{scale, cap, causal, degree};
     if (graph({&q, &k, &v, &t})) {
         const variable_list out = AttentionNode::apply(q, k, v, table, m, r);
@@ -361,7 +374,8 @@ std::tuple<Tensor, Maybe> attention(const Tensor& q0, const Tensor& k0, const Te
 // Calls as a program's loop makes them: every tensor already in the type and
 // layout that the entries take.  These look that over and run; anything else,
 // wrong or only to be converted, gives None, and attention.py's own checks say
-// what it is.  (They take 4 to 9 us in Python, as long as the rest of a call.)
+// what it is.  So does a call under torch.jit.trace, which would record the
+// allocations here and no kernel.  (They take 4 to 9 us in Python, as long as the rest of a call.)
 // ---------------------------------------------------------------------------
 
 bool served(const Tensor& t) {
@@ -385,6 +399,7 @@ bool map_of_buckets(const Tensor& table, const Maybe& buckets) {
 std::optional<std::tuple<Tensor, Tensor>> norm_rotary_as_is(const Tensor& q, const Tensor& k, const Maybe& wq,
                                                             const Maybe& wk, const Tensor& cos, const Tensor& sin,
                                                             const Maybe& positions, double eps, bool interleaved) {
+    if (torch::jit::tracer::isTracing()) return {};
     if (q.dim() != 4 || k.dim() != 4 || !served(q) || !alike(k, q)) return {};
     const int64_t B = q.size(0), L = q.size(2), D = q.size(3);
     if (k.size(0) != B || k.size(2) != L || k.size(3) != D || D > 512) return {};
@@ -397,6 +412,7 @@ std::optional<std::tuple<Tensor, Tensor>> norm_rotary_as_is(const Tensor& q, con
 }
 
 Maybe position_bias_as_is(const Tensor& table, const Maybe& buckets, int64_t Lq, int64_t Lk) {
+    if (torch::jit::tracer::isTracing()) return {};
     if (Lq < 0 || Lk < 0 || !served(table) || !map_of_buckets(table, buckets)) return {};
     return position_bias(table, *buckets, Lq, Lk);
 }
@@ -405,6 +421,7 @@ std::optional<std::tuple<Tensor, Maybe>> attention_as_is(
     const Tensor& q, const Tensor& k, const Tensor& v, std::optional<double> scale, std::optional<double> cap,
     bool causal, const Maybe& prefix, const Maybe& documents, const Maybe& lengths, const Maybe& slopes,
     const Maybe& table, const Maybe& buckets, bool degree) {
+    if (torch::jit::tracer::isTracing()) return {};
     if (q.dim() != 4 || k.dim() != 4 || !served(q) || !alike(k, q) || !alike(v, q) || k.sizes() != v.sizes()) return {};
     const int64_t B = q.size(0), Hq = q.size(1), D = q.size(3), Hk = k.size(1), Lk = k.size(2);
     if (k.size(0) != B || k.size(3) != D || D < 8 || D > 128 || D % 8 || Hk < 1 || Hq % Hk) return {};
