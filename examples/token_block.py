@@ -6,7 +6,8 @@ documents and then run token by token over a cache.
 Queries and keys are normed per head and rotated by position
 (``qk_norm_rotary``); the attention (``biased_attention``) caps its scores, adds
 a learned bias by buckets of the distance, keeps documents apart in training and
-reads a cache of mixed lengths in decoding.  The task is to repeat the token that
+reads a cache of mixed lengths in decoding.  What the bias has learned is read off
+it written out (``relative_position_bias``).  The task is to repeat the token that
 stood `lag` places earlier in the same document.
 """
 from __future__ import annotations
@@ -22,7 +23,7 @@ from torch.nn import functional as F
 sys.path.insert(0, os.path.dirname(os.path.dirname(os.path.abspath(__file__))))
 
 from neural_shift_cuda import (biased_attention, qk_norm_rotary, relative_buckets,  # noqa: E402
-                               rotary_table)
+                               relative_position_bias, rotary_table)
 
 
 class TokenBlock(nn.Module):
@@ -55,6 +56,11 @@ class TokenBlock(nn.Module):
         y = biased_attention(q, k, v, cap=self.cap, causal=True, bias_table=self.bias,
                              buckets=self.buckets, **masks)
         return self.out(y.transpose(1, 2).flatten(2))
+
+    @torch.no_grad()
+    def bias_by_distance(self, reach):
+        """(heads, reach + 1): the bias of a key 0, 1, .. reach places back."""
+        return relative_position_bias(self.bias, self.buckets, 1, reach + 1)[:, 0].flip(1)
 
     def forward(self, tokens, documents=None):
         positions = torch.arange(tokens.shape[1], device=tokens.device)
@@ -112,6 +118,9 @@ def main(argv=None) -> float:
         opt.step()
         if step % 10 == 0 or step + 1 == a.steps:
             print(f"step {step:3d}  loss {loss.item():.4f}", flush=True)
+    bias = block.bias_by_distance(8).float().cpu()
+    print("learned bias by distance, mean of the heads: "
+          + " ".join(f"{b:+.3f}" for b in bias.mean(0).tolist()))
     # token by token gives what the whole sequence gives
     tokens = batch_of(gen, 4, 24, 32, 3, a.device)[0]
     cache = Cache(block, 4, 64)
