@@ -540,7 +540,8 @@ NSH_API int64_t nsh_position_bias_workspace_bytes(int64_t H, int64_t Lq, int64_t
  * query with p outside [0, n) sees nothing.
  *   out = softmax(s) v,  log_degree = log sum exp s  (float, (B, Hq, Lq));
  * a row that sees nothing gives 0 and -inf.  Query head h reads key head
- * h / (Hq / Hk).  D <= 128, D a multiple of 8; the rows of q, k, v, out and of
+ * h / (Hq / Hk).  scale is finite in fp32, cap 0 or 2^-60 to 2^60.  D <= 128, D a
+ * multiple of 8; the rows of q, k, v, out and of
  * the gradients start on 16 bytes, those of q, k, v and grad_out 0 to 2^24 bytes
  * apart from a token to the next.  Keys that a query does not see add nothing to
  * it, whatever they hold. */

@@ -505,7 +505,8 @@ def biased_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, *,
     (D, log_C) with return_log_degree, log_C fp32 (B, Hq, Lq).  Differentiable in
     q, k, v and bias_table; the gradients are summed in a fixed order.  The GPU
     serves fp16, bf16 and fp32 with D <= 128 (a width that is no multiple of 8,
-    or rows that do not start on 16 bytes, are copied first)."""
+    or rows that do not start on 16 bytes, are copied first), a scale within fp32 and
+    caps of 2^-60 to 2^60."""
     if not q.is_cuda:
         return biased_attention_reference(
             q, k, v, scale=scale, cap=cap, causal=causal, prefix=prefix, documents=documents,

@@ -154,6 +154,10 @@ static int attention_check(const char* op, const nsh_attention_args* g, nsh::Att
         return fail(NSH_ERR_INVALID, "%s: the head width must be a multiple of 8 up to 128", op);
     if (!(g->cap >= 0.0) || !std::isfinite(g->cap) || !std::isfinite(g->scale))
         return fail(NSH_ERR_INVALID, "%s: scale and cap must be finite, cap not negative", op);
+    // the kernels hold both in fp32, with the cap's reciprocal
+    if (!std::isfinite(static_cast<float>(g->scale)) ||
+        (g->cap != 0.0 && (g->cap < std::ldexp(1.0, -60) || g->cap > std::ldexp(1.0, 60))))
+        return fail(NSH_ERR_INVALID, "%s: a scale within fp32 and a cap of 2^-60 to 2^60, or none, are served", op);
     if (g->prefix && !g->causal) return fail(NSH_ERR_INVALID, "%s: a prefix needs causal", op);
     if (g->bias_table &&
         (!g->buckets || g->reach < 0 || g->reach > 2048 || g->num_buckets < 1 || g->num_buckets > 4097))
