@@ -107,7 +107,7 @@ static void cut_rows(Att& a, bool backward) {
 // five workgroups to four CUs on.  As the rule was set: 4 x 12 heads, 1024 tokens,
 // width 64, bf16 (384 workgroups, then of 128 keys): 86 us alone, 92 + 16 with two
 // parts; 2 x 16 heads, 4 of keys, 4096 tokens, width 128, causal (256): 791 alone,
-// 500 + 18 (now 402 + 18); 2 x 5 heads, 333 over 517 tokens, fp32: 60 + 5 with four
+// 500 + 18 (now 324 + 17); 2 x 5 heads, 333 over 517 tokens, fp32: 60 + 5 with four
 // tiles kept, 38 + 5 with two, 48 + 8 with one.
 static void cut_keys(Att& a) {
     const int64_t cus = nsh_host::compute_units(), tile = a.wide ? 32 : 64;

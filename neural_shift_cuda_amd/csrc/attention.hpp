@@ -151,8 +151,8 @@ __device__ __forceinline__ int wave_max(int v) {
 // One row by one wave, pair by pair: a pair that is not seen takes part in
 // nothing.  The matrix products of the tiles give such a pair the weight 0,
 // which is no help against an infinity or a NaN in the other factor, so a row
-// whose tiles end in one of those is computed again here.  Sound data never
-// come this way.
+// whose tiles end in one of those is computed again here.  Data without them, and
+// whose sums fp32 holds, never come this way (it takes some fifty times as long).
 // ---------------------------------------------------------------------------
 
 template <typename T>

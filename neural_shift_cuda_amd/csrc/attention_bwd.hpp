@@ -14,13 +14,16 @@
 //      workgroups, or their loads uneven, `parts` workgroups share a key
 //      block's queries and a third launch adds their sums.
 //
-// What bounds them: as in the forward, the vector work of a score next to its
-// products (three by rows, four by keys).  2 x 16 heads, 4 of keys, 4096 tokens,
-// width 128, causal, capped, bf16: by rows 261 us, 790 TFLOP/s; by keys 402 us, 690,
-// and 18 for the join.  4 x 12 heads, 1024 tokens, width 64 with a learned bias, bf16:
-// 64 and 77 us, and 7 for the table.  The accumulators fill half of the registers at
+// What bounds them (times as in the forward): by rows as there the vector work of a
+// score next to its products, 60% and 40% of the time: 2 x 16 heads, 4 of keys, 4096
+// tokens, width 128, causal, capped, bf16: 231 us, 890 TFLOP/s.  By keys, 324 us, 850,
+// and 17 for the join, vector work is 44%, products 34%, LDS reads 30% (2.3 for each
+// product: K and V come from there again for every 32 rows), and the waves wait 28% of
+// their time: no one unit is full.  The accumulators fill half of the registers at
 // width 128, which leaves one wave to a SIMD; by keys, two fit with K and V in LDS
-// instead (`kPaired`).
+// instead (`kPaired`).  4 x 12 heads, 1024 tokens, width 64 with a learned bias, bf16:
+// 58 and 70 us, and 7 for the table; documents in rows of 2500, 2 x 12 heads, fp16: 55
+// and 59: waves wait 40 to 47% of their time, one to a SIMD on average.
 #pragma once
 
 #include "attention_rows.hpp"
@@ -103,9 +106,9 @@ __device__ __forceinline__ void row_gradient(const Att& a, const Cap& cap, const
     {
         RowFragments<T, DP> fk, fv;
         fk.read(K, by_row), fv.read(V, by_row);
-        // here the vector work goes ahead of the other wave's products (2 x 16 heads of
-        // 4096, causal, capped: 291 us without, 267 with, 287 the other way round, as
-        // the forward has it; by keys neither changes anything)
+        // here the vector work goes ahead of the other wave's products (first dozen
+        // launches, 2 x 16 heads of 4096, causal, capped: 291 us without, 267 with, 287
+        // the other way round, as the forward has it; by keys neither changes anything)
         priority<0>();
         s = fk.products(q), dp = fv.products(go);
         priority<1>();

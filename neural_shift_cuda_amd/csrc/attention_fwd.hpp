@@ -10,14 +10,17 @@
 //     each, with tiles of their own and no barrier; several workgroups may
 //     share a row block's keys (`splits`), and a second launch joins them.
 //
-// What bounds them: the vector work of a score (an exp2, with a cap another and
-// a reciprocal, and 6 to 10 more instructions) takes more issue than its products
-// (at width 128, capped: 57% of the time and 32%), and the two overlap only as far
-// as the two waves of a SIMD are out of step.  2 x 16 heads, 4 of keys, 4096
-// tokens, width 128, causal, capped, bf16: 203 us, 680 TFLOP/s of the 1223 that a large
-// library product reaches; 16 heads, 8 of keys, 8192 tokens, width 96, a quarter of
-// them a prefix: 226 us, 970.  One token over 16 caches of up to 8192, 32 heads, 8 of
-// keys: 76 + 5 us, 5.3 TB/s, which is what memory gives.
+// What bounds them (times: medians of many launches with inputs in turn): the
+// vector work of a score (an exp2, with a cap another and a reciprocal, and 6 to 10
+// more instructions) takes more issue than its products (at width 128, capped: 60%
+// of the time and 34%), and the two overlap only as far as the two waves of a SIMD
+// are out of step.  2 x 16 heads, 4 of keys, 4096 tokens, width 128, causal, capped,
+// bf16: 176 us, 780 TFLOP/s of the 1223 that a large library product reaches; 16
+// heads, 8 of keys, 8192 tokens, width 96, a quarter of them a prefix: 231 us, 950.
+// One token over 16 caches of up to 8192, 32 heads, 8 of keys: 78 + 5 us, 5.2 TB/s,
+// near what a copy reaches.  With a learned bias (4 x 12 heads, 1024 tokens, width 64:
+// 40 us) or documents (2 x 12 heads, rows of 2500: 38 us) neither is busy: vector 32%
+// and 23%, products 11% and 5%, with one wave to a SIMD or less.
 #pragma once
 
 #include "attention_rows.hpp"
@@ -46,8 +49,9 @@ __device__ __forceinline__ void attend(const Att& a, const Cap& cap, const Bias&
 #pragma unroll
         for (int kb = 0; kb < NB; ++kb) f[kb].read(K, by_row, kb * 32);
         // a product issues in 4 cycles and takes 32: ahead of the other wave's vector
-        // work, which fills the rest (2 x 16 heads of 4096, causal, capped: 212 us
-        // without, 204 with, 219 the other way round; prompt of 8192: 262, 250, 267)
+        // work, which fills the rest (first dozen launches, 2 x 16 heads of 4096, causal,
+        // capped: 212 us without, 204 with, 219 the other way round; prompt of 8192:
+        // 262, 250, 267)
         priority<1>();
 #pragma unroll
         for (int kb = 0; kb < NB; ++kb) s[kb] = f[kb].products(q);

@@ -296,7 +296,11 @@ struct ColumnFragments {  // 32 tile rows, `row` rows on from the base's, by col
         for (int d = 0; d < DP / 32; ++d)
             f[d][0] = Tile<T, DP>::col(lds, base, row, d), f[d][1] = Tile<T, DP>::col(lds, base, row + 16, d);
     }
-    // acc += their columns times the weights w
+    // acc += their columns times the weights w, rounded to T as the matrix
+    // instructions want them: in 16 bits half a step of each weight, of the size of
+    // the result's own rounding and not shared by a row's pairs (errors 0.0017 to
+    // 0.0024 of the whole in bf16, 2.1e-4 to 2.9e-4 in fp16; a second product for what
+    // the rounding left would take that away for half as much matrix time again)
     __device__ __forceinline__ void weigh(f32x16 (&acc)[DP / 32], const f32x16& w) const {
         const typename Eight<T>::V lo = Eight<T>::pack(__builtin_shufflevector(w, w, 0, 1, 2, 3, 4, 5, 6, 7));
         const typename Eight<T>::V hi = Eight<T>::pack(__builtin_shufflevector(w, w, 8, 9, 10, 11, 12, 13, 14, 15));

@@ -17,10 +17,12 @@
 // groups of a workgroup add in order, and a second launch adds the workgroups'
 // sums in order.
 //
-// At that size: forward 35 us (84 + 84 MB, 4.8 TB/s), backward 60.5 us (168 + 84
-// MB, 4.2 TB/s), the weights' sums 5 us; a copy of 84 MB, which the memory side
-// cache holds, runs at 7.0 TB/s, one of 268 MB at 5.4.  What bounds them is memory
-// latency behind a position's: its table rows can be asked for only then.
+// At that size: forward 40 us (84 + 84 MB, 4.2 TB/s; 35 where the inputs are the
+// same each time and the memory side cache has some of them), backward 59 us (168 +
+// 84 MB, 4.3 TB/s), the weights' sums 5 us; a copy of 84 MB runs at 7.0 TB/s from that
+// cache and at 5.1 without.  What bounds them is memory latency behind a position's:
+// its table rows can be asked for only then.  The root is the reciprocal square root
+// instruction's, off by 2^-23 of the row (fp32 errors 1.4e-7 to 2.0e-7).
 #include <algorithm>
 #include <cmath>
 
@@ -371,8 +373,9 @@ static int norm_launch(NormArgs a, bool bwd, hipStream_t st) {
 }
 
 // Two rows at once, forward, where that leaves no CU without work (4 x 20 heads
-// of 4096 tokens, bf16: 38.7 us with one, 35.1 with two, 40.1 with four).  The
-// backward has two tensors' loads under way with one (60.5 us, 67.9 with two).
+// of 4096 tokens, bf16, the same inputs each time: 38.7 us with one, 35.1 with two,
+// 40.1 with four).  The backward has two tensors' loads under way with one (60.5 us,
+// 67.9 with two).
 template <typename T, int G>
 static int norm_rows(const NormArgs& a, bool bwd, hipStream_t st) {
     constexpr int V = 16 / sizeof(T);

@@ -16,9 +16,13 @@
 // them, first over the workgroups, then over each bucket's relative positions:
 // all in a fixed order.
 //
-// 16 heads, 2048 x 2048, fp32 (268 MB): forward 52 us (5.2 TB/s), backward 55.7
-// (4.8 TB/s) and 6.6 for the table's sums; a copy of 268 MB runs at 5.4 TB/s and a
-// library sum over as much at 4.9.  Both are bound by memory.
+// 16 heads, 2048 x 2048, fp32 (268 MB): forward 51 us (5.3 TB/s), backward 72
+// (3.7 TB/s; 54 where the upstream gradient is the same each time and the memory
+// side cache has some of it) and 6.5 for the table's sums; a copy of 268 MB runs at
+// 5.4 TB/s, a library sum over as much at 3.6, a plain read at 6.2.  Both are bound by
+// memory; the backward's second reads, along the diagonals, cost it the rest.  Its
+// sums are fp32 throughout (off by 1.8e-7 of the whole, where rounding the result
+// alone makes 2.2e-8).
 #include <algorithm>
 
 #include "divisor.hpp"
