@@ -310,8 +310,8 @@ constexpr float kQuickCap = 256.f;
 
 // Keys of a workgroup of the gradients by keys.  16-bit heads up to 64 wide take
 // 64, two waves to a group of 32 keys, each with one half of a query tile: rows
-// of 2500 tokens in documents, 2 x 12 heads, fp16, 57 us, and 76 with 128 keys, one
-// wave to each 32.
+// of 2500 tokens in documents, 2 x 12 heads, fp16, 57 us as the rule was set (59 now),
+// and 76 with 128 keys, one wave to each 32.
 constexpr int key_block(int bytes, int D) { return bytes == 2 && D <= 64 ? 64 : 128; }
 
 // Launches of one type's kernels (attention_fwd_*.hip, attention_bwd_*.hip).
