@@ -207,6 +207,7 @@ static int64_t plan(nsh::Att& a, bool backward, char* ws) {
     }
     nsh::cut_keys(a);
     a.delta = reinterpret_cast<float*>(take_bytes(rows * 4));
+    a.far = reinterpret_cast<int*>(take_bytes(static_cast<int64_t>(a.B) * a.Hq * a.rblocks * nsh::kAttWaves * 4));
     if (a.parts > 1)
         a.part = reinterpret_cast<float*>(take_bytes(2 * a.parts * static_cast<int64_t>(a.B) * a.Hk * a.Lk * a.D * 4));
     if (a.gtable)

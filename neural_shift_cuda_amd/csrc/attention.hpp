@@ -42,6 +42,7 @@ struct Att {
     int nranges;   // document ranges of a batch
     const int2* ranges;
     float *part, *delta, *bins;
+    int* far;      // by row block and wave of the gradients by rows: some row's weights need care
 };
 
 __device__ __forceinline__ int filled_keys(const Att& a, int b) {

@@ -88,6 +88,13 @@ __device__ __forceinline__ void add_table(const Att& a, TableSums& ts, int rel0,
     ts.next = rel0 + 32;
 }
 
+// The gradients by keys of a plain 16-bit call have 1 / sum in the exponent next to
+// the maximum.  A row whose two come to less than this is off by less than 2^-15 of
+// its weights, a sixteenth of an fp16 weight's own half step; the launch by rows
+// notes, wave by wave, where some row is beyond.
+constexpr float kNear = 1024.f;
+template <typename T, Kind KIND> constexpr bool kNotes = KIND == kPlain && sizeof(T) == 2;
+
 template <typename T, int DP>
 struct BwdShape {
     using L = Tile<T, DP>;
@@ -216,6 +223,10 @@ __global__ __launch_bounds__(kAttThreads, SPLIT || DP * sizeof(T) > (KIND == kGe
     // rows that see nothing, and lanes that stand in for no row, weigh nothing
     float2 stat = get_stats(a, at);
     if (!x.live) stat.y = 0.f;
+    if constexpr (kNotes<T, KIND>) {
+        const int beyond = __any(stat.y != 0.f && fabsf(__builtin_amdgcn_logf(stat.y * kRoom<T>) - stat.x) > kNear);
+        if (l == 0) a.far[((static_cast<int64_t>(b) * a.Hq + h) * a.rblocks + rb) * kAttWaves + wave] = beyond;
+    }
 
     Loader<T, DP, KT, SPLIT ? 1 : kAttWaves> lk, lv;
     lk.init(SPLIT ? l : threadIdx.x, a.ks[2], a.D);
@@ -363,9 +374,6 @@ __global__ __launch_bounds__(kAttThreads, SPLIT || DP * sizeof(T) > (KIND == kGe
 //            and one wave waits for its own products
 enum Share { kAlone, kTwin, kPaired };
 
-// A row's log 2 of weight over score this far from 0 is off by less than 2^-15 of
-// the weight, a sixteenth of an fp16 weight's own half step.
-constexpr float kNear = 1024.f;
 
 template <typename T, int DP, Kind KIND, Share SHARE>
 __global__ __launch_bounds__(SHARE == kPaired ? 512 : kAttThreads, SHARE != kPaired && DP * sizeof(T) < 256 ? 2 : 1)
@@ -384,7 +392,6 @@ void att_bwd_key_kernel(Att a) {
     // log 2 of weight over score, maximum, 1 / sum (without a bias: what that log 2
     // leaves of it), delta, key end, document
     __shared__ __attribute__((aligned(256))) float info[2][6][QT];
-    __shared__ int far[2];
     extern __shared__ float line[];
     const int l = threadIdx.x & 63, wave = wave_id(), g = l >> 5, kw = wave % KG;
     int bg, rest;
@@ -411,6 +418,16 @@ void att_bwd_key_kernel(Att a) {
         load_row<T, DP>(k, row_at<T>(a.k, a.ks, b, hk, j), a.D, l);
         load_row<T, DP>(v, row_at<T>(a.v, a.vs, b, hk, j), a.D, l);
     }
+
+    // Whether some row of these heads is far (kNear): asked for here, the first of
+    // the answers looked at with the first rows' own values.
+    bool far = false;
+    constexpr int kAsk = 8;
+    const int notes = kNotes<T, KIND> ? a.per * a.rblocks * kAttWaves : 0;
+    const int* const note = a.far + static_cast<int64_t>(b * a.Hq + hk * a.per) * a.rblocks * kAttWaves;
+    int noted[kAsk];
+#pragma unroll
+    for (int c = 0; c < kAsk; ++c) noted[c] = c * 64 + l < notes ? note[c * 64 + l] : 0;
 
     // the queries that see any of the block's keys: all of them, or those from
     // the first key's position on
@@ -443,7 +460,7 @@ void att_bwd_key_kernel(Att a) {
     };
     Needed<decltype(wanted)> need{wanted};
 
-    Loader<T, DP, QT, 4> lq, lg;
+    Loader<T, DP, QT, 4, PAIRED> lq, lg;
     lq.init(threadIdx.x & 255, second ? a.gos[2] : a.qs[2], a.D);
     if (!PAIRED) lg.init(threadIdx.x, a.gos[2], a.D);
     // a unit's head and first row, kept up by addition
@@ -495,9 +512,8 @@ void att_bwd_key_kernel(Att a) {
             // places, and the weights take what it lost as a factor
             const float y = r_stat.y * kRoom<T>, up = __builtin_amdgcn_logf(y) - r_stat.x;
             info[buf][0][x] = kApart ? -r_stat.x : up + (KIND == kCapped ? cap.top : 0.f);
-            info[buf][2][x] = kApart || y == 0.f ? y : y * __builtin_amdgcn_exp2f(-r_stat.x - up);
-            const bool beyond = __any(y != 0.f && fabsf(up) > kNear);
-            if (x == 0) far[buf] = beyond;
+            if (kApart) info[buf][2][x] = y;
+            if (far) info[buf][2][x] = y == 0.f ? y : y * __builtin_amdgcn_exp2f(-r_stat.x - up);
         }
         info[buf][3][x] = r_delta;
         info[buf][4][x] = __int_as_float(r_lim);
@@ -608,7 +624,7 @@ void att_bwd_key_kernel(Att a) {
         for (int c = 0; c < 4; ++c) {
             const i32x4 lim = *reinterpret_cast<const i32x4*>(rows + 8 * c);
             f32x4 fix = {1.f, 1.f, 1.f, 1.f};
-            if (KIND == kPlain && !kApart) fix = *reinterpret_cast<const f32x4*>(rows - 2 * QT + 8 * c);
+            if (far) fix = *reinterpret_cast<const f32x4*>(rows - 2 * QT + 8 * c);
 #pragma unroll
             for (int e = 0; e < 4; ++e) {
                 const int r = 4 * c + e;
@@ -667,11 +683,10 @@ void att_bwd_key_kernel(Att a) {
         const int i0 = now.i0, p0 = i0 + off;
         // the rows' key ends rise with their position
         auto ends = [&](int p) { return a.causal ? min(n, max(p + 1, prefix)) : n; };
-        auto rows_far = [&](int buf) { return KIND == kPlain && !kApart && __builtin_amdgcn_readfirstlane(far[buf]); };
         if constexpr (QP == 2) {
             const int qb = wave / KG, pf = p0 + qb * 32, count = min(a.Lq - i0 - qb * 32, 32);
             if (count <= 0 || j0 >= ends(pf + count - 1)) return;
-            const bool whole = j0 + 32 <= ends(pf) && !(KIND == kGeneral && a.documents) && !rows_far(buf);
+            const bool whole = j0 + 32 <= ends(pf) && !(KIND == kGeneral && a.documents) && !far;
             if constexpr (KIND == kGeneral) general(tile, buf, qb, pf, whole);
             else if constexpr (PAIRED) paired(tile, buf, qb, whole);
             else simple(tile, buf, qb, whole);
@@ -710,6 +725,13 @@ void att_bwd_key_kernel(Att a) {
     if (now.u < u1) {
         fetch(now);
         load(now, tiles0[0]);
+        if constexpr (kNotes<T, KIND>) {
+            int any = 0;
+#pragma unroll
+            for (int c = 0; c < kAsk; ++c) any |= noted[c];
+            for (int i = kAsk * 64 + l; i < notes; i += 64) any |= note[i];
+            far = __any(any);
+        }
         put(0);
     }
     while (now.u < u1) {

@@ -162,6 +162,13 @@ struct Tile {
     }
 };
 
+// v, and nothing formed of it ahead of here: what only a branch needs is
+// otherwise computed in front of it.
+__device__ __forceinline__ int here(int v) {
+    asm volatile("" : "+v"(v));
+    return v;
+}
+
 // BYTES a lane from its offset in the buffer to LDS, the lanes side by side
 // from `lds` on; nothing passes through registers.
 template <int BYTES>
@@ -177,16 +184,20 @@ __device__ __forceinline__ void to_lds(__amdgpu_buffer_rsrc_t rs, void* lds, uin
 // Tile rows [0, ROWS) of a tensor from global memory straight into LDS by NW
 // waves.  Rows past the tensor's end, and columns past D, arrive as zeros (the
 // buffer's range check): nothing behind a cache's filled part is read.
-template <typename T, int DP, int ROWS, int NW>
+//
+// LEAN keeps one offset in a register and forms the others of it at each load,
+// where an instruction covers whole sets of 16 rows, whose chunks' order repeats.
+template <typename T, int DP, int ROWS, int NW, bool LEAN = false>
 struct Loader {
     using L = Tile<T, DP>;
     static constexpr int NI = ROWS * L::NC / (NW * 64);
     static_assert(NI * NW * 64 == ROWS * L::NC, "whole instructions");
-    uint32_t off[NI];
+    static constexpr bool kOne = LEAN && NW * 64 % (16 * L::NC) == 0;
+    uint32_t off[kOne ? 1 : NI];
 
     __device__ __forceinline__ void init(int id, int64_t stride, int D) {
 #pragma unroll
-        for (int i = 0; i < NI; ++i) {
+        for (int i = 0; i < (kOne ? 1 : NI); ++i) {
             const int x = i * NW * 64 + id, r = x / L::NC, c = (x % L::NC) ^ L::turn(r);
             off[i] = c * L::CE < D ? static_cast<uint32_t>(r) * static_cast<uint32_t>(stride * sizeof(T)) + c * 16 : 0x80000000u;
         }
@@ -201,9 +212,11 @@ struct Loader {
         const __amdgpu_buffer_rsrc_t rs = __builtin_amdgcn_make_buffer_rsrc(
             const_cast<char*>(reinterpret_cast<const char*>(base) + static_cast<uint64_t>(static_cast<uint32_t>(first)) * bytes),
             static_cast<short>(0), static_cast<int>(size), 0x00020000);
+        // (columns past D are at 2^31, and 112 rows of 2^24 bytes on past any size still)
+        const uint32_t one = kOne ? static_cast<uint32_t>(here(static_cast<int>(off[0]))) : 0u;
 #pragma unroll
         for (int i = 0; i < NI; ++i)
-            to_lds<16>(rs, lds + (i * NW + wave) * 1024, off[i]);
+            to_lds<16>(rs, lds + (i * NW + wave) * 1024, kOne ? one + i * (NW * 64 / L::NC) * bytes : off[i]);
     }
 };
 
@@ -256,13 +269,6 @@ __device__ __forceinline__ void settle() {
     else
         asm volatile("s_nop 11");
     order();
-}
-
-// v, and nothing formed of it ahead of here: what only a branch needs is
-// otherwise computed in front of it.
-__device__ __forceinline__ int here(int v) {
-    asm volatile("" : "+v"(v));
-    return v;
 }
 
 __device__ __forceinline__ int wave_id() { return __builtin_amdgcn_readfirstlane(threadIdx.x >> 6); }
@@ -343,7 +349,7 @@ struct ColumnFragments {  // 32 tile rows, `row` rows on from the base's, by col
 // down to kFitTo, and the sums with it.  It starts where the smallest dx that an
 // fp16 result can show is still a normal number.  (2500 tokens, width 64, causal,
 // dO of 2^-10: dq and dk off by 2.8e-4 and 3.0e-4, their own rounding, and 1.1e-3
-// without; documents in rows of 2500, training: 143 us without, 151 with.)
+// without; by keys at 2 x 16 heads, 4096 tokens, width 128: 339 us without, 357 with.)
 template <typename T> constexpr bool kNarrow = __is_same(T, f16);
 template <typename T> constexpr float kRoom = kNarrow<T> ? 32768.f : 1.f;
 constexpr float kFitMost = 32768.f, kFitFirst = 1.0995116e12f;  // 2^40
