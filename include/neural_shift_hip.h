@@ -585,6 +585,63 @@ NSH_API int nsh_document_ids(const int64_t* documents, int64_t B, int64_t L, int
                              void* stream);
 NSH_API int64_t nsh_attention_workspace_bytes(const nsh_attention_args* args, int backward);
 
+/* Layer norm of `rows` rows of n, of x or of its sum with a residual stream:
+ *   s = x + residual, rounded to `dtype` and written (x alone without one)
+ *   h = (s - mean(s)) * (var(s) + eps)^(-1/2);  y = h * weight + bias
+ *   grad_x = grad_s + d(y), of x and of the residual alike
+ * A NULL weight is 1, a NULL bias 0.  Inputs have a unit last stride, the given
+ * strides from row to row (elements) and any alignment; outputs are contiguous. */
+typedef struct nsh_layer_norm_args {
+    const void *x, *residual, *weight, *bias; /* backward: x is what was normed, s with a residual */
+    int64_t rows, n, x_stride, residual_stride;
+    double eps;
+    int32_t dtype;
+    void *y, *s;  /* forward; s comes with a residual */
+    float* stats; /* (rows, 2) or NULL: written by the forward, read by the backward */
+    /* backward: grad_s, grad_weight, grad_bias and grad_x may be NULL (not all of
+     * the last three) */
+    const void *grad_y, *grad_s;
+    int64_t gy_stride, gs_stride;
+    void *grad_x, *grad_weight, *grad_bias;
+    void* workspace; /* nsh_layer_norm_workspace_bytes, 4-byte aligned; for the weights' gradients */
+    int64_t workspace_bytes;
+} nsh_layer_norm_args;
+NSH_API int nsh_layer_norm_forward(const nsh_layer_norm_args* args, void* stream);
+NSH_API int nsh_layer_norm_backward(const nsh_layer_norm_args* args, void* stream);
+NSH_API int64_t nsh_layer_norm_workspace_bytes(const nsh_layer_norm_args* args);
+
+/* The gated projections of a feed-forward:
+ *   g = x gate^T,  u = x up^T,  h = act(g) * u
+ * x (rows, K), gate and up (F, K) with a unit last stride and the given strides from row
+ * to row (elements), any alignment (rows that do not start on 16 bytes, or whose width is
+ * no multiple of 16 bytes, are copied into the workspace first).  K, F <= 2^20.  Products,
+ * the activation and all sums are float; dg and du are rounded to `dtype` (fp16: times a
+ * power of two that the call chooses) as operands of the gradients' products. */
+#define NSH_ACTIVATION_SILU 1
+#define NSH_ACTIVATION_GELU 2      /* g * Phi(g) */
+#define NSH_ACTIVATION_GELU_TANH 3 /* its form with a hyperbolic tangent */
+#define NSH_ACTIVATION_RELU 4
+#define NSH_ACTIVATION_SIGMOID 5
+typedef struct nsh_gated_linear_args {
+    const void *x, *gate_weight, *up_weight;
+    int64_t rows, K, F, x_stride, gate_stride, up_stride;
+    int32_t dtype, activation;
+    void* h; /* forward: (rows, F), contiguous */
+    /* nsh_gated_linear_kept_bytes, 16-byte aligned, or NULL.  Forward: written, what
+     * the backward needs.  Backward: read. */
+    float* kept;
+    const void* grad_h; /* backward, with its stride; gradients contiguous, NULL = not wanted */
+    int64_t gh_stride;
+    void *grad_x, *grad_gate, *grad_up;
+    void* workspace; /* nsh_gated_linear_workspace_bytes, 16-byte aligned */
+    int64_t workspace_bytes;
+} nsh_gated_linear_args;
+NSH_API int nsh_gated_linear_forward(const nsh_gated_linear_args* args, void* stream);
+NSH_API int nsh_gated_linear_backward(const nsh_gated_linear_args* args, void* stream);
+/* (of arguments whose pointers and strides are set: the alignment decides on copies) */
+NSH_API int64_t nsh_gated_linear_workspace_bytes(const nsh_gated_linear_args* args, int backward);
+NSH_API int64_t nsh_gated_linear_kept_bytes(const nsh_gated_linear_args* args);
+
 #ifdef __cplusplus
 }
 #endif

@@ -10,13 +10,14 @@
 import sys as _sys
 
 import neural_shift_cuda_amd as _impl
-from neural_shift_cuda_amd import attention, metropolis, ops  # noqa: F401
+from neural_shift_cuda_amd import attention, feedforward, metropolis, ops  # noqa: F401
 from neural_shift_cuda_amd import *  # noqa: F401,F403
 from neural_shift_cuda_amd import __all__, __version__  # noqa: F401
 
 _sys.modules[__name__ + ".ops"] = _impl.ops
 _sys.modules[__name__ + ".metropolis"] = _impl.metropolis
 _sys.modules[__name__ + ".attention"] = _impl.attention
+_sys.modules[__name__ + ".feedforward"] = _impl.feedforward
 
 # model installers: neural_shift_cuda.integration and its patch modules
 from neural_shift_cuda_amd import integration  # noqa: E402,F401

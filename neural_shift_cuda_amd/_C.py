@@ -24,7 +24,7 @@ trishitmg/neural_shift_cuda), so the guards in ``ops.py`` and
   weight gradient then still comes back per channel, (S*B, C, H, W).
 
 The token operators at the end have their host side in C++
-(``host/token_calls.cpp``, the extension module ``_token_calls``).
+(``host/*.cpp``, the extension module ``_token_calls``).
 
 Importing this module raises ``OSError`` or ``ImportError`` when the library
 has not been built (``python -m neural_shift_cuda_amd.build``); ``ops.py`` keeps
@@ -929,6 +929,24 @@ class _AttentionArgs(ctypes.Structure):
         ("workspace_bytes", _I64), ("row_stats", _P), ("out_rest", _P)]
 
 
+class _LayerNormArgs(ctypes.Structure):
+    _fields_ = [
+        ("x", _P), ("residual", _P), ("weight", _P), ("bias", _P), ("rows", _I64), ("n", _I64),
+        ("x_stride", _I64), ("residual_stride", _I64), ("eps", _F64), ("dtype", _I32), ("y", _P),
+        ("s", _P), ("stats", _P), ("grad_y", _P), ("grad_s", _P), ("gy_stride", _I64),
+        ("gs_stride", _I64), ("grad_x", _P), ("grad_weight", _P), ("grad_bias", _P),
+        ("workspace", _P), ("workspace_bytes", _I64)]
+
+
+class _GatedLinearArgs(ctypes.Structure):
+    _fields_ = [
+        ("x", _P), ("gate_weight", _P), ("up_weight", _P), ("rows", _I64), ("K", _I64),
+        ("F", _I64), ("x_stride", _I64), ("gate_stride", _I64), ("up_stride", _I64),
+        ("dtype", _I32), ("activation", _I32), ("h", _P), ("kept", _P), ("grad_h", _P),
+        ("gh_stride", _I64), ("grad_x", _P), ("grad_gate", _P), ("grad_up", _P),
+        ("workspace", _P), ("workspace_bytes", _I64)]
+
+
 for _name, _args, _res in (
         ("nsh_norm_rotary_forward", [_P, _P], _I),
         ("nsh_norm_rotary_backward", [_P, _P], _I),
@@ -940,7 +958,14 @@ for _name, _args, _res in (
         ("nsh_document_ids", [_P, _I64, _I64, _P, _P], _I),
         ("nsh_attention_forward", [_P, _P], _I),
         ("nsh_attention_backward", [_P, _P], _I),
-        ("nsh_attention_workspace_bytes", [_P, _I], _I64)):
+        ("nsh_attention_workspace_bytes", [_P, _I], _I64),
+        ("nsh_layer_norm_forward", [_P, _P], _I),
+        ("nsh_layer_norm_backward", [_P, _P], _I),
+        ("nsh_layer_norm_workspace_bytes", [_P], _I64),
+        ("nsh_gated_linear_forward", [_P, _P], _I),
+        ("nsh_gated_linear_backward", [_P, _P], _I),
+        ("nsh_gated_linear_workspace_bytes", [_P, _I], _I64),
+        ("nsh_gated_linear_kept_bytes", [_P], _I64)):
     _fn = getattr(_lib, _name)
     _fn.argtypes = _args
     _fn.restype = _res
@@ -1016,3 +1041,8 @@ attention_as_is = _token_calls.attention_as_is
 norm_rotary = _token_calls.norm_rotary
 position_bias = _token_calls.position_bias
 attention = _token_calls.attention
+# host/block_calls.cpp, the same for feedforward.py's
+layer_norm_as_is = _token_calls.layer_norm_as_is
+gated_linear_as_is = _token_calls.gated_linear_as_is
+layer_norm = _token_calls.layer_norm
+gated_linear = _token_calls.gated_linear

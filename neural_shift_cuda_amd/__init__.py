@@ -28,6 +28,12 @@ from .attention import (
     relative_position_bias_reference,
     rotary_table,
 )
+from .feedforward import (
+    gated_linear,
+    gated_linear_reference,
+    layer_norm,
+    layer_norm_reference,
+)
 
 __version__ = "0.12.0"
 __all__ = [
@@ -47,7 +53,11 @@ __all__ = [
     "relative_position_bias",
     "relative_buckets",
     "rotary_table",
+    "layer_norm",
+    "gated_linear",
     "biased_attention_reference",
     "qk_norm_rotary_reference",
     "relative_position_bias_reference",
+    "layer_norm_reference",
+    "gated_linear_reference",
 ]

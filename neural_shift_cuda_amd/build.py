@@ -8,9 +8,9 @@ Every ``csrc/*.hip`` / ``csrc/*.cpp`` file is compiled to an object under
 ``neural_shift_cuda_amd/libneural_shift_hip.so``.  The library exports only
 the C ABI declared in ``include/neural_shift_hip.h``.
 
-``host/token_calls.cpp`` (no device code) is compiled with the host compiler
-against the installed torch into ``neural_shift_cuda_amd/_token_calls.so``, an
-extension module that calls the library.
+``host/*.cpp`` (no device code) is compiled with the host compiler against the
+installed torch into ``neural_shift_cuda_amd/_token_calls.so``, an extension
+module that calls the library.
 """
 from __future__ import annotations
 
@@ -78,28 +78,33 @@ def _compile(src: str, flags) -> str:
     return obj
 
 
-def _compile_calls() -> str:
+def _call_sources():
+    host = os.path.join(PKG, "host")
+    return sorted(os.path.join(host, f) for f in os.listdir(host) if f.endswith(".cpp"))
+
+
+def _compile_calls(src: str) -> str:
     import sysconfig
 
     import torch
-    obj = os.path.join(BUILD, "token_calls.o")
+    obj = os.path.join(BUILD, os.path.splitext(os.path.basename(src))[0] + ".o")
     inc = os.path.join(os.path.dirname(torch.__file__), "include")
     cmd = [os.environ.get("CXX", "g++"), "-O2", "-std=c++17", "-fPIC", "-fvisibility=hidden",
            "-Wall", "-D__HIP_PLATFORM_AMD__=1", "-DUSE_ROCM=1", f"-I{INCLUDE}",
            *(x for d in (inc, os.path.join(inc, "torch", "csrc", "api", "include"),
                          sysconfig.get_paths()["include"], "/opt/rocm/include")
              for x in ("-isystem", d)),
-           "-c", os.path.join(PKG, "host", "token_calls.cpp"), "-o", obj]
+           "-c", src, "-o", obj]
     res = subprocess.run(cmd, capture_output=True, text=True)
     if res.returncode != 0:
         raise RuntimeError(f"compile failed: {' '.join(cmd)}\n{res.stdout}\n{res.stderr}")
     return obj
 
 
-def _link_calls(obj: str) -> None:
+def _link_calls(objs) -> None:
     import torch
     tmp = CALLS + ".tmp"
-    cmd = [os.environ.get("CXX", "g++"), "-shared", "-o", tmp, obj,
+    cmd = [os.environ.get("CXX", "g++"), "-shared", "-o", tmp, *objs,
            "-L" + os.path.join(os.path.dirname(torch.__file__), "lib"), "-ltorch_python",
            "-ltorch", "-ltorch_cpu", "-lc10", "-lc10_hip", f"-L{PKG}", "-lneural_shift_hip",
            "-Wl,-rpath,$ORIGIN"]
@@ -118,7 +123,7 @@ def build(jobs: int = 0, verbose: bool = True) -> str:
     jobs = jobs or min(len(srcs), max(1, (os.cpu_count() or 2)))
     t0 = time.time()
     with cf.ThreadPoolExecutor(max_workers=jobs) as ex:
-        calls = ex.submit(_compile_calls)
+        calls = [ex.submit(_compile_calls, s) for s in _call_sources()]
         objs = list(ex.map(lambda s: _compile(s, flags), srcs))
     tmp = LIB + ".tmp"
     cmd = [_hipcc(), f"--offload-arch={ARCH}", "-shared", "-fPIC", "-o", tmp, *objs,
@@ -127,7 +132,7 @@ def build(jobs: int = 0, verbose: bool = True) -> str:
     if res.returncode != 0:
         raise RuntimeError(f"link failed: {' '.join(cmd)}\n{res.stdout}\n{res.stderr}")
     os.replace(tmp, LIB)
-    _link_calls(calls.result())
+    _link_calls([c.result() for c in calls])
     if verbose:
         print(f"[neural_shift_cuda_amd] built {LIB} ({len(srcs)} sources, "
               f"{time.time() - t0:.1f}s)")

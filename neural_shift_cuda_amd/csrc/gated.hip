@@ -1,0 +1,314 @@
+// gated.hip -- the gated projections' entries: checks, workspaces, and the passes
+// around the products of gated.hpp (copies of rows that do not start on 16 bytes,
+// dg and du with fp16's factor, the join of split sums).
+#include <algorithm>
+#include <cmath>
+
+#include "gated.hpp"
+
+namespace nsh {
+
+NSH_GATED_ENTRIES(extern, f16)
+NSH_GATED_ENTRIES(extern, bf16)
+NSH_GATED_ENTRIES(extern, float)
+
+constexpr int kPassThreads = 256;
+
+// Rows copied to a length of whole 16 bytes, zeros behind them: up to three matrices.
+struct CopyArgs {
+    struct Side {
+        const void* from;
+        void* to;
+        int64_t rows, stride;  // stride in elements
+    } side[3];
+    int n, np;
+};
+
+template <typename T>
+__global__ __launch_bounds__(kPassThreads) void gated_copy_kernel(CopyArgs a) {
+    const CopyArgs::Side& s = a.side[blockIdx.y];
+    const int each = a.np / kVec<T>;
+    const int64_t all = s.rows * each, step = static_cast<int64_t>(gridDim.x) * kPassThreads;
+    for (int64_t i = static_cast<int64_t>(blockIdx.x) * kPassThreads + threadIdx.x; i < all; i += step) {
+        const int64_t row = i / each;
+        const int c = static_cast<int>(i - row * each) * kVec<T>;
+        const ux4 v = load_bits(static_cast<const T*>(s.from) + row * s.stride, c, a.n);
+        *reinterpret_cast<ux4*>(static_cast<T*>(s.to) + row * a.np + c) = v;
+    }
+}
+
+struct SlopeArgs {
+    const void* gh;
+    int64_t gh_stride, rows;
+    const float* kept;
+    void* dgu;
+    int F, Fk, Fp;
+    const float* scale;
+};
+
+// dg and du, a workgroup a row and 256 parts of it.
+template <typename T>
+__global__ __launch_bounds__(kPassThreads) void gated_slope_kernel(SlopeArgs a) {
+    constexpr int V = kVec<T>;
+    const int c = (blockIdx.x * kPassThreads + threadIdx.x) * V;
+    if (c >= a.Fp) return;
+    const float by = __is_same(T, f16) && a.scale ? a.scale[0] : 1.f;
+    for (int64_t m = blockIdx.y; m < a.rows; m += gridDim.y) {
+        float d[V], s[V] = {}, h[V] = {};
+        unpack<T>(load_bits(static_cast<const T*>(a.gh) + m * a.gh_stride, c, a.F), d);
+        const float* k = a.kept + m * 2 * a.Fk + c;
+        if (c < a.F) {
+#pragma unroll
+            for (int e = 0; e < V; e += 4) {
+                load_acc<float, 4>(k + e, *reinterpret_cast<float(*)[4]>(&s[e]));
+                load_acc<float, 4>(k + a.Fk + e, *reinterpret_cast<float(*)[4]>(&h[e]));
+            }
+        }
+#pragma unroll
+        for (int e = 0; e < V; ++e) {
+            const bool in = c + e < a.F;
+            s[e] = in ? d[e] * by * s[e] : 0.f;
+            h[e] = in ? d[e] * by * h[e] : 0.f;
+        }
+        T* to = static_cast<T*>(a.dgu) + m * 2 * a.Fp + c;
+        *reinterpret_cast<ux4*>(to) = pack<T>(s);
+        *reinterpret_cast<ux4*>(to + a.Fp) = pack<T>(h);
+    }
+}
+
+// fp16's numbers end at 2^-24 and lose bits from 2^-14 down, where the gradients of a
+// mean loss are.  dg and du are multiplied by a power of two, of the largest dh and the
+// largest factor, that brings them just under 2^15 and that the sums are divided by: what is
+// rounded off is then below 2^-39 of the largest wherever it is not half a step.
+constexpr int kMostBlocks = 512;
+
+__device__ __forceinline__ float workgroup_max(float v, float* lds) {
+    lds[threadIdx.x] = v;
+    __syncthreads();
+    for (int n = kPassThreads / 2; n >= 1; n /= 2) {
+        if (static_cast<int>(threadIdx.x) < n) lds[threadIdx.x] = fmaxf(lds[threadIdx.x], lds[threadIdx.x + n]);
+        __syncthreads();
+    }
+    const float r = lds[0];
+    __syncthreads();
+    return r;
+}
+
+__global__ __launch_bounds__(kPassThreads) void gated_most_kernel(const f16* gh, int64_t stride, int64_t rows, int F,
+                                                                  float* out) {
+    __shared__ float lds[kPassThreads];
+    const int each = (F + 7) / 8;
+    const int64_t all = rows * each, step = static_cast<int64_t>(gridDim.x) * kPassThreads;
+    float most = 0.f;
+    for (int64_t i = static_cast<int64_t>(blockIdx.x) * kPassThreads + threadIdx.x; i < all; i += step) {
+        const int64_t row = i / each;
+        float d[8];
+        unpack<f16>(load_bits(gh + row * stride, static_cast<int>(i - row * each) * 8, F), d);
+#pragma unroll
+        for (int e = 0; e < 8; ++e) most = fmaxf(most, fabsf(d[e]) < INFINITY ? fabsf(d[e]) : 0.f);
+    }
+    most = workgroup_max(most, lds);
+    if (threadIdx.x == 0) out[blockIdx.x] = most;
+}
+
+__global__ __launch_bounds__(kPassThreads) void gated_scale_kernel(const float* gh, int n, const float* kept, int nk,
+                                                                   float* scale) {
+    __shared__ float lds[kPassThreads];
+    float x = 0.f, y = 0.f;
+    for (int i = threadIdx.x; i < n; i += kPassThreads) x = fmaxf(x, gh[i]);
+    for (int i = threadIdx.x; i < nk; i += kPassThreads) y = fmaxf(y, kept[i]);
+    x = workgroup_max(x, lds);
+    y = workgroup_max(y, lds);
+    if (threadIdx.x) return;
+    int e = 0;
+    if (x > 0.f && y > 0.f) {
+        int ex, ey;
+        frexpf(x, &ex);
+        frexpf(y, &ey);  // x < 2^ex, y < 2^ey
+        e = min(max(15 - ex - ey, -100), 100);
+    }
+    scale[0] = ldexpf(1.f, e);
+    scale[1] = ldexpf(1.f, -e);
+}
+
+template <typename T>
+__global__ __launch_bounds__(kPassThreads) void gated_join_kernel(const float* part, int splits, int64_t n, T* out) {
+    const int64_t i = static_cast<int64_t>(blockIdx.x) * kPassThreads + threadIdx.x;
+    if (i >= n) return;
+    float s = 0.f;
+    for (int k = 0; k < splits; ++k) s += part[k * n + i];
+    out[i] = from_acc<T>(s);
+}
+
+}  // namespace nsh
+
+using nsh_host::ceil_div;
+using nsh_host::fail;
+
+namespace {
+
+constexpr int64_t kWidest = int64_t(1) << 20;
+constexpr int64_t kStep = int64_t(1) << 23;  // bytes from a row to the next that a panel's 32-bit offsets take
+
+struct Plan {
+    int64_t esz, Kp, Fp, Fk;
+    bool copy[3];       // x, gate, up
+    int64_t copies[3];  // offsets in the workspace
+    int64_t dgu, scale, most, part, bytes;
+    nsh::Cut cut;
+    int splits;
+};
+
+int64_t up(int64_t v, int64_t to) { return ceil_div(v, to) * to; }
+
+Plan plan_of(const nsh_gated_linear_args* g, bool bwd) {
+    Plan p{};
+    p.esz = g->dtype == NSH_DTYPE_FLOAT32 ? 4 : 2;
+    const int64_t vec = 16 / p.esz;
+    p.Kp = up(g->K, vec), p.Fp = up(g->F, 128 / p.esz), p.Fk = up(g->F, 8);
+    const void* at[3] = {g->x, g->gate_weight, g->up_weight};
+    const int64_t stride[3] = {g->x_stride, g->gate_stride, g->up_stride}, rows[3] = {g->rows, g->F, g->F};
+    for (int i = 0; i < 3; ++i) {
+        // (a single row has no step to the next)
+        const bool steps = rows[i] == 1 || (stride[i] % vec == 0 && stride[i] >= g->K && stride[i] * p.esz <= kStep);
+        p.copy[i] = g->K % vec != 0 || !nsh_host::aligned(at[i], 16) || !steps;
+        p.copies[i] = p.bytes;
+        if (p.copy[i]) p.bytes += up(rows[i] * p.Kp * p.esz, 256);
+    }
+    if (!bwd) return p;
+    p.dgu = p.bytes;
+    p.bytes += up(g->rows * 2 * p.Fp * p.esz, 256);
+    p.scale = p.bytes, p.bytes += 256;
+    p.most = p.bytes, p.bytes += up(nsh::kMostBlocks * 4, 256);
+    p.part = p.bytes, p.splits = 1;
+    p.cut = nsh::cut_of(g->rows, g->K, p.esz == 4, false, 1);
+    // few tiles: workgroups share a tile's sum over the hidden columns, eight panels each or more
+    const int64_t panels = 2 * p.Fp * p.esz / 128, tiles = p.cut.tiles(), cus = nsh_host::compute_units();
+    if (tiles < cus) p.splits = static_cast<int>(std::max<int64_t>(1, std::min({ceil_div(2 * cus, tiles), panels / 8, int64_t(16)})));
+    if (p.splits > 1) p.bytes += up(p.splits * g->rows * g->K * 4, 256);
+    return p;
+}
+
+int64_t forward_blocks(const nsh_gated_linear_args* g) {
+    return nsh::cut_of(g->rows, g->F, g->dtype == NSH_DTYPE_FLOAT32, true, 1).tiles();
+}
+
+int check(const char* op, const nsh_gated_linear_args* g, bool bwd) {
+    if (!g) return fail(NSH_ERR_INVALID, "%s: null arguments", op);
+    if (g->dtype < NSH_DTYPE_FLOAT16 || g->dtype > NSH_DTYPE_FLOAT32)
+        return fail(NSH_ERR_INVALID, "%s: unsupported dtype code %d", op, g->dtype);
+    if (g->rows < 1 || g->K < 1 || g->F < 1) return fail(NSH_ERR_INVALID, "%s: empty tensor", op);
+    if (g->K > kWidest || g->F > kWidest || g->rows > (int64_t(1) << 30))
+        return fail(NSH_ERR_INVALID, "%s: width or hidden size above 2^20, or more than 2^30 rows", op);
+    if (g->activation < NSH_ACTIVATION_SILU || g->activation > NSH_ACTIVATION_SIGMOID)
+        return fail(NSH_ERR_INVALID, "%s: unknown activation code %d", op, g->activation);
+    if (!g->x || !g->gate_weight || !g->up_weight ||
+        (bwd ? !g->kept || !g->grad_h || (!g->grad_x && !g->grad_gate && !g->grad_up) : !g->h))
+        return fail(NSH_ERR_INVALID, "%s: null pointer argument", op);
+    if (g->kept && !nsh_host::aligned(g->kept, 16)) return fail(NSH_ERR_INVALID, "%s: misaligned kept", op);
+    return NSH_OK;
+}
+
+template <typename T>
+int copy_rows(const nsh_gated_linear_args* g, const Plan& p, nsh::GatedArgs& a, char* ws, hipStream_t st) {
+    nsh::CopyArgs c{};
+    int n = 0;
+    int64_t most = 0;
+    const void** at[3] = {&a.x, &a.wg, &a.wu};
+    uint32_t* stride[3] = {&a.x_stride, &a.wg_stride, &a.wu_stride};
+    const int64_t steps[3] = {g->x_stride, g->gate_stride, g->up_stride}, rows[3] = {g->rows, g->F, g->F};
+    for (int i = 0; i < 3; ++i) {
+        *stride[i] = static_cast<uint32_t>(rows[i] == 1 ? p.Kp * p.esz : steps[i] * p.esz);
+        if (!p.copy[i]) continue;
+        c.side[n++] = {*at[i], ws + p.copies[i], rows[i], steps[i]};
+        *at[i] = ws + p.copies[i];
+        *stride[i] = static_cast<uint32_t>(p.Kp * p.esz);
+        most = std::max(most, rows[i] * (p.Kp * p.esz / 16));
+    }
+    if (!n) return NSH_OK;
+    c.n = static_cast<int>(g->K), c.np = static_cast<int>(p.Kp);
+    const int64_t blocks = std::min<int64_t>(ceil_div(most, nsh::kPassThreads), nsh_host::compute_units() * 16);
+    nsh::gated_copy_kernel<T><<<dim3(static_cast<unsigned>(blocks), n), nsh::kPassThreads, 0, st>>>(c);
+    return nsh_host::check_launch("gated_linear");
+}
+
+template <typename T>
+int backward(const nsh_gated_linear_args* g, const Plan& p, nsh::GatedArgs a, char* ws, hipStream_t st) {
+    float* scale = nullptr;
+    if constexpr (__is_same(T, nsh::f16)) {
+        scale = reinterpret_cast<float*>(ws + p.scale);
+        float* most = reinterpret_cast<float*>(ws + p.most);
+        const int n = static_cast<int>(std::min<int64_t>(ceil_div(g->rows * ceil_div(g->F, 8), nsh::kPassThreads), nsh::kMostBlocks));
+        nsh::gated_most_kernel<<<n, nsh::kPassThreads, 0, st>>>(static_cast<const nsh::f16*>(g->grad_h), g->gh_stride, g->rows, a.F, most);
+        nsh::gated_scale_kernel<<<1, nsh::kPassThreads, 0, st>>>(most, n, g->kept + g->rows * 2 * p.Fk, static_cast<int>(forward_blocks(g)), scale);
+    }
+    a.scale = scale, a.dgu = ws + p.dgu;
+    const nsh::SlopeArgs s{g->grad_h, g->gh_stride, g->rows, g->kept, a.dgu, a.F, a.Fk, a.Fp, scale};
+    const unsigned across = static_cast<unsigned>(ceil_div(a.Fp, nsh::kPassThreads * nsh::kVec<T>));
+    nsh::gated_slope_kernel<T><<<dim3(across, static_cast<unsigned>(std::min<int64_t>(g->rows, 32768))), nsh::kPassThreads, 0, st>>>(s);
+    if (g->grad_x) {
+        a.splits = p.splits;
+        a.part = p.splits > 1 ? reinterpret_cast<float*>(ws + p.part) : nullptr;
+        const int rc = nsh::gated_input_gradient<T>(a, p.cut, st);
+        if (rc != NSH_OK) return rc;
+        if (a.part) {
+            const int64_t n = g->rows * g->K;
+            nsh::gated_join_kernel<T><<<static_cast<unsigned>(ceil_div(n, nsh::kPassThreads)), nsh::kPassThreads, 0, st>>>(
+                a.part, p.splits, n, static_cast<T*>(a.dx));
+        }
+    }
+    if (g->grad_gate || g->grad_up) return nsh::gated_weight_gradient<T>(a, st);
+    return nsh_host::check_launch("gated_linear_backward");
+}
+
+template <typename T>
+int run(const nsh_gated_linear_args* g, const Plan& p, bool bwd, hipStream_t st) {
+    nsh::GatedArgs a{};
+    char* ws = static_cast<char*>(g->workspace);
+    a.x = g->x, a.wg = g->gate_weight, a.wu = g->up_weight;
+    a.rows = g->rows, a.K = static_cast<int>(g->K), a.F = static_cast<int>(g->F);
+    a.Kp = static_cast<int>(p.Kp), a.Fp = static_cast<int>(p.Fp), a.Fk = static_cast<int>(p.Fk);
+    a.activation = g->activation - NSH_ACTIVATION_SILU;
+    a.h = g->h, a.dx = g->grad_x, a.dwg = g->grad_gate, a.dwu = g->grad_up;
+    const int rc = copy_rows<T>(g, p, a, ws, st);
+    if (rc != NSH_OK) return rc;
+    if (bwd) return backward<T>(g, p, a, ws, st);
+    a.kept = g->kept;
+    if (__is_same(T, nsh::f16) && a.kept) a.most = a.kept + a.rows * 2 * a.Fk;
+    return nsh::gated_forward<T>(a, st);
+}
+
+int gated_linear(const char* op, const nsh_gated_linear_args* g, bool bwd, void* stream) {
+    const int rc = check(op, g, bwd);
+    if (rc != NSH_OK) return rc;
+    const Plan p = plan_of(g, bwd);
+    if (p.bytes > 0 && (!g->workspace || g->workspace_bytes < p.bytes))
+        return fail(NSH_ERR_INVALID, "%s: workspace smaller than nsh_gated_linear_workspace_bytes", op);
+    if (p.bytes > 0 && !nsh_host::aligned(g->workspace, 16)) return fail(NSH_ERR_INVALID, "%s: misaligned workspace", op);
+    hipStream_t st = static_cast<hipStream_t>(stream);
+    switch (g->dtype) {
+        case NSH_DTYPE_FLOAT16: return run<nsh::f16>(g, p, bwd, st);
+        case NSH_DTYPE_BFLOAT16: return run<nsh::bf16>(g, p, bwd, st);
+        default: return run<float>(g, p, bwd, st);
+    }
+}
+
+}  // namespace
+
+extern "C" int64_t nsh_gated_linear_workspace_bytes(const nsh_gated_linear_args* g, int backward) {
+    if (!g || g->rows < 1 || g->K < 1 || g->F < 1) return -1;
+    return plan_of(g, backward != 0).bytes;
+}
+
+extern "C" int64_t nsh_gated_linear_kept_bytes(const nsh_gated_linear_args* g) {
+    if (!g || g->rows < 1 || g->K < 1 || g->F < 1) return -1;
+    return (g->rows * 2 * up(g->F, 8) + (g->dtype == NSH_DTYPE_FLOAT16 ? forward_blocks(g) : 0)) * 4;
+}
+
+extern "C" int nsh_gated_linear_forward(const nsh_gated_linear_args* g, void* stream) {
+    return gated_linear("gated_linear_forward", g, false, stream);
+}
+
+extern "C" int nsh_gated_linear_backward(const nsh_gated_linear_args* g, void* stream) {
+    return gated_linear("gated_linear_backward", g, true, stream);
+}

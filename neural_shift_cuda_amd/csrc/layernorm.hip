@@ -1,0 +1,527 @@
+// layernorm.hip -- layer norm of rows, alone or of their sum with a residual
+// stream, and its gradients, on gfx950.
+//
+//   s = x + residual (rounded to the type, and written)     h = (s - mean) / sqrt(var + eps)
+//   y = h w + b
+//   g' = gy w,  gx = gs + (g' - mean(g') - h mean(g' h)) / sqrt(var + eps)
+//   gw = sum gy h,  gb = sum gy
+//
+// HBM streams: every input is read and every output written once.  A row belongs
+// to a group of lanes that holds it whole in registers, 16 bytes a lane and part:
+// up to 64 lanes of a wave, then a workgroup of 256 or 512.  So mean and variance
+// are two sums over the same registers, the variance about the mean (as a
+// difference of squares it would lose what the mean is larger than the deviations).
+// Rows wider than a workgroup holds are read again for each sum.
+//
+// gw and gb: a lane adds up its own columns over the rows that its group walks, the
+// groups of a workgroup add in order, and a second launch adds the workgroups'
+// sums in order.
+#include <algorithm>
+#include <cmath>
+
+#include "rows.hpp"
+
+namespace nsh {
+
+struct LayerNormArgs {
+    const void *x, *residual, *weight, *bias, *grad_y, *grad_s;
+    int64_t x_stride, residual_stride, gy_stride, gs_stride;
+    void *y, *s, *gx, *gw, *gb;
+    float* stats;    // (rows, 2): mean and 1 / sqrt(var + eps), or NULL
+    float* partial;  // (blocks, 2, N)
+    int64_t rows;
+    int n, blocks;
+    float eps, inv_n;
+};
+
+// Groups of G lanes; several waves meet through LDS, `turn` telling two sums in a
+// row apart.
+template <int G>
+struct Group {
+    static constexpr int kThreads = G > 64 ? G : 256;
+    static constexpr int kGroups = kThreads / G;
+    static constexpr int kWaves = G > 64 ? G / 64 : 1;
+    float* lds;  // 2 turns of two values a wave
+    int turn = 0;
+
+    __device__ __forceinline__ void sum(float& a, float& b) {
+        a = lanes_sum<(G < 64 ? G : 64)>(a);
+        b = lanes_sum<(G < 64 ? G : 64)>(b);
+        if constexpr (kWaves > 1) {
+            float* at = lds + turn * 2 * kWaves;
+            turn ^= 1;
+            if ((threadIdx.x & 63) == 0) {
+                at[threadIdx.x / 64] = a;
+                at[kWaves + threadIdx.x / 64] = b;
+            }
+            lds_barrier();
+            a = b = 0.f;
+#pragma unroll
+            for (int w = 0; w < kWaves; ++w) a += at[w], b += at[kWaves + w];
+        }
+    }
+    __device__ __forceinline__ float sum(float a) {
+        float b = 0.f;
+        if constexpr (kWaves > 1) {
+            sum(a, b);
+        } else {
+            a = lanes_sum<G>(a);
+        }
+        return a;
+    }
+};
+
+// Of a row's deviations from its mean as first summed: 1 / sqrt(var + eps), and their own
+// mean, what that sum's rounding left (rows of one value would otherwise come out as its
+// last place over sqrt(eps)).
+template <typename Gr>
+__device__ __forceinline__ float variance(Gr& group, float square, float off, const LayerNormArgs& a, float& by) {
+    group.sum(square, off);
+    const float rest = off * a.inv_n, var = square * a.inv_n;
+    // (squares beyond fp32 leave infinity, and a row of zeros, as the formula does)
+    by = __builtin_amdgcn_rsqf(var - (var < INFINITY ? rest * rest : 0.f) + a.eps);
+    return rest;
+}
+
+template <typename T, int G, int NV>
+__global__ __launch_bounds__(Group<G>::kThreads) void layer_norm_forward_kernel(LayerNormArgs a) {
+    using Gr = Group<G>;
+    constexpr int V = kVec<T>;
+    __shared__ float meet[Gr::kWaves > 1 ? 4 * Gr::kWaves : 1];
+    Gr group{meet};
+    const int lane = threadIdx.x % G, own = threadIdx.x / G;
+    ux4 w[NV], b[NV];
+#pragma unroll
+    for (int i = 0; i < NV; ++i) {
+        const int c = (i * G + lane) * V;
+        if (a.weight) w[i] = load_bits(static_cast<const T*>(a.weight), c, a.n);
+        if (a.bias) b[i] = load_bits(static_cast<const T*>(a.bias), c, a.n);
+    }
+    // every lane of the workgroup takes every turn: the groups meet in lane exchanges
+    for (int64_t r0 = static_cast<int64_t>(blockIdx.x) * Gr::kGroups; r0 < a.rows;
+         r0 += static_cast<int64_t>(a.blocks) * Gr::kGroups) {
+        const bool live = r0 + own < a.rows;
+        const int64_t row = live ? r0 + own : 0;
+        const T* x = static_cast<const T*>(a.x) + row * a.x_stride;
+        ux4 bits[NV], more[NV];
+#pragma unroll
+        for (int i = 0; i < NV; ++i) bits[i] = load_bits(x, (i * G + lane) * V, a.n);
+        if (a.residual) {
+            const T* r = static_cast<const T*>(a.residual) + row * a.residual_stride;
+#pragma unroll
+            for (int i = 0; i < NV; ++i) more[i] = load_bits(r, (i * G + lane) * V, a.n);
+        }
+        float v[NV][V], total = 0.f;
+#pragma unroll
+        for (int i = 0; i < NV; ++i) {
+            const int c = (i * G + lane) * V;
+            unpack<T>(bits[i], v[i]);
+            if (a.residual) {
+                float m[V];
+                unpack<T>(more[i], m);
+#pragma unroll
+                for (int k = 0; k < V; ++k) v[i][k] += m[k];
+                bits[i] = pack<T>(v[i]);
+                unpack<T>(bits[i], v[i]);
+                if (live) store_bits(static_cast<T*>(a.s) + row * a.n, c, a.n, bits[i]);
+            }
+#pragma unroll
+            for (int k = 0; k < V; ++k) total += v[i][k];
+        }
+        const float mean = group.sum(total) * a.inv_n;
+        float square = 0.f, off = 0.f;
+#pragma unroll
+        for (int i = 0; i < NV; ++i) {
+            const int c = (i * G + lane) * V;
+#pragma unroll
+            for (int k = 0; k < V; ++k) {
+                v[i][k] = c + k < a.n ? v[i][k] - mean : 0.f;
+                square = fma_acc(v[i][k], v[i][k], square);
+                off += v[i][k];
+            }
+        }
+        float by;
+        const float rest = variance(group, square, off, a, by);
+        if (!live) continue;
+        if (a.stats && lane == 0) a.stats[2 * row] = mean + rest, a.stats[2 * row + 1] = by;
+#pragma unroll
+        for (int i = 0; i < NV; ++i) {
+            const int c = (i * G + lane) * V;
+            float m[V];
+#pragma unroll
+            for (int k = 0; k < V; ++k) v[i][k] = (v[i][k] - rest) * by;
+            if (a.weight) {
+                unpack<T>(w[i], m);
+#pragma unroll
+                for (int k = 0; k < V; ++k) v[i][k] *= m[k];
+            }
+            if (a.bias) {
+                unpack<T>(b[i], m);
+#pragma unroll
+                for (int k = 0; k < V; ++k) v[i][k] += m[k];
+            }
+            store_bits(static_cast<T*>(a.y) + row * a.n, c, a.n, pack<T>(v[i]));
+        }
+    }
+}
+
+// Sums over the rows of a workgroup's groups, in their order, to its partial sums.
+template <int G, int NV, int V>
+__device__ __forceinline__ void add_groups(const float (&sum)[NV][V], float* to, int n, float* lds) {
+    using Gr = Group<G>;
+    if constexpr (Gr::kGroups == 1) {
+#pragma unroll
+        for (int i = 0; i < NV; ++i)
+#pragma unroll
+            for (int k = 0; k < V; ++k) {
+                const int c = (i * G + threadIdx.x) * V + k;
+                if (c < n) to[c] = sum[i][k];
+            }
+    } else {
+        const int lane = threadIdx.x % G, own = threadIdx.x / G;
+        __syncthreads();
+#pragma unroll
+        for (int i = 0; i < NV; ++i)
+#pragma unroll
+            for (int k = 0; k < V; ++k) lds[own * (G * NV * V) + (i * G + lane) * V + k] = sum[i][k];
+        __syncthreads();
+        for (int c = threadIdx.x; c < n; c += Gr::kThreads) {
+            float s = 0.f;
+            for (int i = 0; i < Gr::kGroups; ++i) s += lds[i * (G * NV * V) + c];
+            to[c] = s;
+        }
+    }
+}
+
+template <typename T, int G, int NV>
+__global__ __launch_bounds__(Group<G>::kThreads) void layer_norm_backward_kernel(LayerNormArgs a) {
+    using Gr = Group<G>;
+    constexpr int V = kVec<T>;
+    __shared__ float lds[Gr::kGroups > 1 ? Gr::kThreads * NV * V : 4 * Gr::kWaves];
+    Gr group{lds};
+    const int lane = threadIdx.x % G, own = threadIdx.x / G;
+    ux4 w[NV];
+    float gw[NV][V], gb[NV][V];
+#pragma unroll
+    for (int i = 0; i < NV; ++i) {
+        if (a.weight) w[i] = load_bits(static_cast<const T*>(a.weight), (i * G + lane) * V, a.n);
+#pragma unroll
+        for (int k = 0; k < V; ++k) gw[i][k] = gb[i][k] = 0.f;
+    }
+    for (int64_t r0 = static_cast<int64_t>(blockIdx.x) * Gr::kGroups; r0 < a.rows;
+         r0 += static_cast<int64_t>(a.blocks) * Gr::kGroups) {
+        const bool live = r0 + own < a.rows;
+        const int64_t row = live ? r0 + own : 0;
+        const T* x = static_cast<const T*>(a.x) + row * a.x_stride;
+        const T* g = static_cast<const T*>(a.grad_y) + row * a.gy_stride;
+        ux4 xs[NV], gs[NV], more[NV];
+#pragma unroll
+        for (int i = 0; i < NV; ++i) {
+            xs[i] = load_bits(x, (i * G + lane) * V, a.n);
+            gs[i] = load_bits(g, (i * G + lane) * V, a.n);
+        }
+        if (a.grad_s) {
+            const T* s = static_cast<const T*>(a.grad_s) + row * a.gs_stride;
+#pragma unroll
+            for (int i = 0; i < NV; ++i) more[i] = load_bits(s, (i * G + lane) * V, a.n);
+        }
+        const float mean = a.stats[2 * row], by = a.stats[2 * row + 1];
+        float h[NV][V], d[NV][V], s1 = 0.f, s2 = 0.f;
+#pragma unroll
+        for (int i = 0; i < NV; ++i) {
+            const int c = (i * G + lane) * V;
+            float m[V];
+            unpack<T>(xs[i], h[i]);
+            unpack<T>(gs[i], d[i]);
+            if (a.weight) unpack<T>(w[i], m);
+#pragma unroll
+            for (int k = 0; k < V; ++k) {
+                // past the row's end nothing: there x is 0, and less the mean no number
+                // that 0 would take away where the mean is none
+                h[i][k] = c + k < a.n ? (h[i][k] - mean) * by : 0.f;
+                if (live) {
+                    gw[i][k] = fma_acc(d[i][k], h[i][k], gw[i][k]);
+                    gb[i][k] += d[i][k];
+                }
+                if (a.weight) d[i][k] *= m[k];
+                s1 += d[i][k];
+                s2 = fma_acc(d[i][k], h[i][k], s2);
+            }
+        }
+        group.sum(s1, s2);
+        s1 *= a.inv_n, s2 *= a.inv_n;
+        if (!live || !a.gx) continue;
+#pragma unroll
+        for (int i = 0; i < NV; ++i) {
+            float m[V];
+            if (a.grad_s) unpack<T>(more[i], m);
+#pragma unroll
+            for (int k = 0; k < V; ++k) {
+                d[i][k] = (d[i][k] - s1 - h[i][k] * s2) * by;
+                if (a.grad_s) d[i][k] += m[k];
+            }
+            store_bits(static_cast<T*>(a.gx) + row * a.n, (i * G + lane) * V, a.n, pack<T>(d[i]));
+        }
+    }
+    if (!a.partial) return;
+    float* to = a.partial + static_cast<int64_t>(blockIdx.x) * 2 * a.n;
+    add_groups<G, NV, V>(gw, to, a.n, lds);
+    add_groups<G, NV, V>(gb, to + a.n, a.n, lds);
+}
+
+// ---------------------------------------------------------------------------
+// Rows wider than a workgroup holds
+// ---------------------------------------------------------------------------
+
+constexpr int kWideThreads = 1024;
+using WideGroup = Group<kWideThreads>;
+
+template <typename T>
+__device__ __forceinline__ void wide_values(const LayerNormArgs& a, int64_t row, int c, bool summed, float (&v)[kVec<T>]) {
+    unpack<T>(load_bits(static_cast<const T*>(a.x) + row * a.x_stride, c, a.n), v);
+    if (summed && a.residual) {
+        float m[kVec<T>];
+        unpack<T>(load_bits(static_cast<const T*>(a.residual) + row * a.residual_stride, c, a.n), m);
+#pragma unroll
+        for (int k = 0; k < kVec<T>; ++k) v[k] += m[k];
+        unpack<T>(pack<T>(v), v);
+    }
+}
+
+template <typename T>
+__global__ __launch_bounds__(kWideThreads) void layer_norm_wide_forward_kernel(LayerNormArgs a) {
+    constexpr int V = kVec<T>, kStep = kWideThreads * V;
+    __shared__ float meet[4 * WideGroup::kWaves];
+    WideGroup group{meet};
+    for (int64_t row = blockIdx.x; row < a.rows; row += a.blocks) {
+        float v[V], m[V], total = 0.f, square = 0.f, off = 0.f;
+        for (int c = threadIdx.x * V; c < a.n; c += kStep) {
+            wide_values<T>(a, row, c, true, v);
+            if (a.residual) store_bits(static_cast<T*>(a.s) + row * a.n, c, a.n, pack<T>(v));
+#pragma unroll
+            for (int k = 0; k < V; ++k) total += v[k];
+        }
+        const float mean = group.sum(total) * a.inv_n;
+        for (int c = threadIdx.x * V; c < a.n; c += kStep) {
+            wide_values<T>(a, row, c, true, v);
+#pragma unroll
+            for (int k = 0; k < V; ++k)
+                if (c + k < a.n) square = fma_acc(v[k] - mean, v[k] - mean, square), off += v[k] - mean;
+        }
+        float by;
+        const float rest = variance(group, square, off, a, by);
+        if (a.stats && threadIdx.x == 0) a.stats[2 * row] = mean + rest, a.stats[2 * row + 1] = by;
+        for (int c = threadIdx.x * V; c < a.n; c += kStep) {
+            wide_values<T>(a, row, c, true, v);
+#pragma unroll
+            for (int k = 0; k < V; ++k) v[k] = (v[k] - mean - rest) * by;
+            if (a.weight) {
+                unpack<T>(load_bits(static_cast<const T*>(a.weight), c, a.n), m);
+#pragma unroll
+                for (int k = 0; k < V; ++k) v[k] *= m[k];
+            }
+            if (a.bias) {
+                unpack<T>(load_bits(static_cast<const T*>(a.bias), c, a.n), m);
+#pragma unroll
+                for (int k = 0; k < V; ++k) v[k] += m[k];
+            }
+            store_bits(static_cast<T*>(a.y) + row * a.n, c, a.n, pack<T>(v));
+        }
+    }
+}
+
+template <typename T>
+__global__ __launch_bounds__(kWideThreads) void layer_norm_wide_backward_kernel(LayerNormArgs a) {
+    constexpr int V = kVec<T>, kStep = kWideThreads * V;
+    __shared__ float meet[4 * WideGroup::kWaves];
+    WideGroup group{meet};
+    for (int64_t row = blockIdx.x; row < a.rows; row += a.blocks) {
+        const float mean = a.stats[2 * row], by = a.stats[2 * row + 1];
+        const T* g = static_cast<const T*>(a.grad_y) + row * a.gy_stride;
+        float h[V], d[V], m[V], s1 = 0.f, s2 = 0.f;
+        for (int turn = 0; turn < 2; ++turn) {
+            for (int c = threadIdx.x * V; c < a.n; c += kStep) {
+                wide_values<T>(a, row, c, false, h);
+                unpack<T>(load_bits(g, c, a.n), d);
+                if (a.weight) {
+                    unpack<T>(load_bits(static_cast<const T*>(a.weight), c, a.n), m);
+#pragma unroll
+                    for (int k = 0; k < V; ++k) d[k] *= m[k];
+                }
+#pragma unroll
+                for (int k = 0; k < V; ++k) h[k] = c + k < a.n ? (h[k] - mean) * by : 0.f;
+                if (turn == 0) {
+#pragma unroll
+                    for (int k = 0; k < V; ++k) s1 += d[k], s2 = fma_acc(d[k], h[k], s2);
+                    continue;
+                }
+#pragma unroll
+                for (int k = 0; k < V; ++k) d[k] = (d[k] - s1 - h[k] * s2) * by;
+                if (a.grad_s) {
+                    unpack<T>(load_bits(static_cast<const T*>(a.grad_s) + row * a.gs_stride, c, a.n), m);
+#pragma unroll
+                    for (int k = 0; k < V; ++k) d[k] += m[k];
+                }
+                store_bits(static_cast<T*>(a.gx) + row * a.n, c, a.n, pack<T>(d));
+            }
+            if (turn == 0) {
+                group.sum(s1, s2);
+                s1 *= a.inv_n, s2 *= a.inv_n;
+            }
+        }
+    }
+}
+
+// 512 columns (256 in fp32) of every gridDim.y-th row for each wave.
+template <typename T>
+__global__ __launch_bounds__(64) void layer_norm_columns_kernel(LayerNormArgs a) {
+    constexpr int V = kVec<T>;
+    const int c = (blockIdx.x * 64 + threadIdx.x) * V;
+    float gw[V] = {}, gb[V] = {};
+    for (int64_t row = blockIdx.y; row < a.rows; row += gridDim.y) {
+        const float mean = a.stats[2 * row], by = a.stats[2 * row + 1];
+        float h[V], d[V];
+        wide_values<T>(a, row, c, false, h);
+        unpack<T>(load_bits(static_cast<const T*>(a.grad_y) + row * a.gy_stride, c, a.n), d);
+#pragma unroll
+        for (int k = 0; k < V; ++k) {
+            gw[k] = fma_acc(d[k], (h[k] - mean) * by, gw[k]);
+            gb[k] += d[k];
+        }
+    }
+    float* to = a.partial + static_cast<int64_t>(blockIdx.y) * 2 * a.n;
+#pragma unroll
+    for (int k = 0; k < V; ++k)
+        if (c + k < a.n) to[c + k] = gw[k], to[a.n + c + k] = gb[k];
+}
+
+// 32 columns per workgroup, 32 runs of blocks each: gw (blockIdx.y 0) or gb.
+template <typename T>
+__global__ __launch_bounds__(1024) void layer_norm_weights_kernel(LayerNormArgs a) {
+    __shared__ float part[32][32];
+    void* out = blockIdx.y ? a.gb : a.gw;
+    if (!out) return;
+    const int col = threadIdx.x % 32, run = threadIdx.x / 32;
+    const int64_t c = static_cast<int64_t>(blockIdx.x) * 32 + col;
+    const float* at = a.partial + (blockIdx.y ? a.n : 0);
+    const int len = (a.blocks + 31) / 32, end = min(a.blocks, (run + 1) * len);
+    float s = 0.f;
+    if (c < a.n) {
+#pragma unroll 8
+        for (int i = run * len; i < end; ++i) s += at[static_cast<int64_t>(i) * 2 * a.n + c];
+    }
+    part[run][col] = s;
+    __syncthreads();
+    if (run == 0 && c < a.n) {
+        for (int i = 1; i < 32; ++i) s += part[i][col];
+        static_cast<T*>(out)[c] = from_acc<T>(s);
+    }
+}
+
+// Workgroups that walk the rows: enough to fill the card; in the backward few
+// enough that their sums of the weights' gradients stay small next to the rows.
+static int norm_row_blocks(int64_t rows, int per, bool bwd) {
+    const int64_t most = static_cast<int64_t>(nsh_host::compute_units()) * (bwd ? 2 : 8);
+    return static_cast<int>(std::min(nsh_host::ceil_div(rows, per), most));
+}
+
+template <typename T, int G, int NV>
+static int layer_norm_launch(LayerNormArgs a, bool bwd, hipStream_t st) {
+    using Gr = Group<G>;
+    a.blocks = norm_row_blocks(a.rows, Gr::kGroups, bwd);
+    if (!bwd) {
+        layer_norm_forward_kernel<T, G, NV><<<a.blocks, Gr::kThreads, 0, st>>>(a);
+        return nsh_host::check_launch("layer_norm_forward");
+    }
+    layer_norm_backward_kernel<T, G, NV><<<a.blocks, Gr::kThreads, 0, st>>>(a);
+    if (a.partial) layer_norm_weights_kernel<T><<<dim3((a.n + 31) / 32, 2), 1024, 0, st>>>(a);
+    return nsh_host::check_launch("layer_norm_backward");
+}
+
+template <typename T>
+static int layer_norm_wide(LayerNormArgs a, bool bwd, hipStream_t st) {
+    a.blocks = norm_row_blocks(a.rows, 1, bwd);
+    if (!bwd) {
+        layer_norm_wide_forward_kernel<T><<<a.blocks, kWideThreads, 0, st>>>(a);
+        return nsh_host::check_launch("layer_norm_forward");
+    }
+    if (a.gx) layer_norm_wide_backward_kernel<T><<<a.blocks, kWideThreads, 0, st>>>(a);
+    if (a.partial) {
+        constexpr int kCols = 64 * kVec<T>;
+        layer_norm_columns_kernel<T><<<dim3((a.n + kCols - 1) / kCols, a.blocks), 64, 0, st>>>(a);
+        layer_norm_weights_kernel<T><<<dim3((a.n + 31) / 32, 2), 1024, 0, st>>>(a);
+    }
+    return nsh_host::check_launch("layer_norm_backward");
+}
+
+// Lanes a row: as few as hold it in one part of 16 bytes each, up to a wave with four
+// parts; then a workgroup.  Where that leaves most CUs without a row, the workgroup
+// takes rows that a wave would hold.
+template <typename T>
+static int layer_norm_dispatch(const LayerNormArgs& a, bool bwd, hipStream_t st) {
+    const int64_t parts = nsh_host::ceil_div(a.n, kVec<T>);
+    if (parts <= 8) return layer_norm_launch<T, 8, 1>(a, bwd, st);
+    if (parts <= 16) return layer_norm_launch<T, 16, 1>(a, bwd, st);
+    if (parts <= 32) return layer_norm_launch<T, 32, 1>(a, bwd, st);
+    if (parts <= 64) return layer_norm_launch<T, 64, 1>(a, bwd, st);
+    if (parts <= 256 && a.rows <= nsh_host::compute_units()) return layer_norm_launch<T, 256, 1>(a, bwd, st);
+    if (parts <= 128) return layer_norm_launch<T, 64, 2>(a, bwd, st);
+    if (parts <= 256) return layer_norm_launch<T, 64, 4>(a, bwd, st);
+    if (parts <= 512) return layer_norm_launch<T, 256, 2>(a, bwd, st);
+    if (parts <= 1024) return layer_norm_launch<T, 256, 4>(a, bwd, st);
+    if (parts <= 2048) return layer_norm_launch<T, 512, 4>(a, bwd, st);
+    return layer_norm_wide<T>(a, bwd, st);
+}
+
+}  // namespace nsh
+
+using nsh_host::fail;
+
+extern "C" int64_t nsh_layer_norm_workspace_bytes(const nsh_layer_norm_args* g) {
+    if (!g || g->rows < 1 || g->n < 1) return -1;
+    return static_cast<int64_t>(nsh::norm_row_blocks(g->rows, 1, true)) * 2 * g->n * 4;
+}
+
+static int layer_norm(const char* op, const nsh_layer_norm_args* g, bool bwd, void* stream) {
+    if (!g) return fail(NSH_ERR_INVALID, "%s: null arguments", op);
+    if (g->dtype < NSH_DTYPE_FLOAT16 || g->dtype > NSH_DTYPE_FLOAT32)
+        return fail(NSH_ERR_INVALID, "%s: unsupported dtype code %d", op, g->dtype);
+    if (g->rows < 1 || g->n < 1) return fail(NSH_ERR_INVALID, "%s: empty tensor", op);
+    if (g->n > (int64_t(1) << 30) || g->rows > (int64_t(1) << 40))
+        return fail(NSH_ERR_INVALID, "%s: rows wider than 2^30 or more than 2^40", op);
+    if (!(g->eps >= 0) || std::isinf(g->eps)) return fail(NSH_ERR_INVALID, "%s: eps must be finite and not negative", op);
+    if (bwd ? !g->x || !g->grad_y || !g->stats || (!g->grad_x && !g->grad_weight && !g->grad_bias)
+            : !g->x || !g->y || !g->residual != !g->s)
+        return fail(NSH_ERR_INVALID, "%s: null pointer argument", op);
+    nsh::LayerNormArgs a{};
+    a.x = g->x, a.weight = g->weight, a.x_stride = g->x_stride;
+    a.stats = g->stats, a.rows = g->rows, a.n = static_cast<int>(g->n);
+    a.eps = static_cast<float>(g->eps), a.inv_n = 1.f / static_cast<float>(a.n);
+    if (bwd) {
+        a.grad_y = g->grad_y, a.gy_stride = g->gy_stride, a.grad_s = g->grad_s, a.gs_stride = g->gs_stride;
+        a.gx = g->grad_x, a.gw = g->grad_weight, a.gb = g->grad_bias;
+        if (a.gw || a.gb) {
+            if (!g->workspace || g->workspace_bytes < nsh_layer_norm_workspace_bytes(g))
+                return fail(NSH_ERR_INVALID, "%s: workspace smaller than nsh_layer_norm_workspace_bytes", op);
+            if (!nsh_host::aligned(g->workspace, 4)) return fail(NSH_ERR_INVALID, "%s: misaligned workspace", op);
+            a.partial = static_cast<float*>(g->workspace);
+        }
+    } else {
+        a.residual = g->residual, a.residual_stride = g->residual_stride, a.bias = g->bias;
+        a.y = g->y, a.s = g->s;
+    }
+    hipStream_t st = static_cast<hipStream_t>(stream);
+    switch (g->dtype) {
+        case NSH_DTYPE_FLOAT16: return nsh::layer_norm_dispatch<nsh::f16>(a, bwd, st);
+        case NSH_DTYPE_BFLOAT16: return nsh::layer_norm_dispatch<nsh::bf16>(a, bwd, st);
+        default: return nsh::layer_norm_dispatch<float>(a, bwd, st);
+    }
+}
+
+extern "C" int nsh_layer_norm_forward(const nsh_layer_norm_args* g, void* stream) {
+    return layer_norm("layer_norm_forward", g, false, stream);
+}
+
+extern "C" int nsh_layer_norm_backward(const nsh_layer_norm_args* g, void* stream) {
+    return layer_norm("layer_norm_backward", g, true, stream);
+}

@@ -1,0 +1,253 @@
+// panels.hpp -- products of two matrices by panels in LDS, for fp16, bf16 and
+// fp32, whichever way each of them runs in memory.
+//
+//   out[m][n] = sum_k second[m][k] first[n][k]
+//
+// A workgroup owns BM x BN of the result.  Of both matrices it takes 128 bytes of the
+// contraction at a time (BK elements) straight from memory to LDS, two panels ahead
+// of each other: with the contraction running along the rows (`kAlong`, one LDS row
+// for each row of the result) or across them (`kAcross`, one LDS row for each
+// contraction step, read by columns).  The chunk order within an LDS row is
+// attention_tiles.hpp's, free of bank conflicts both ways.
+//
+// A wave has WM x WN of the result in 32 x 32 products with `first` on their first
+// side, so a lane holds one row m and, of every 32 columns n, four times four next to
+// each other.  The operands of a step are read while the products of the step before
+// run, those of a panel's first step too: the panels change hands (one barrier) ahead
+// of a panel's last products.
+#pragma once
+
+#include "attention_tiles.hpp"
+#include "rows.hpp"
+
+namespace nsh {
+
+enum Run { kAlong, kAcross };
+
+// How the lane's operands lie in a panel: DP is the LDS row's length.
+template <typename T, int DP, Run RUN>
+struct Operand {
+    using L = Tile<T, DP>;
+    using V = typename Eight<T>::V;
+
+    // first: the wave's first row (or column) of the panel, a multiple of 32 (of
+    // the wave's own width, if across)
+    static __device__ __forceinline__ int base(int first, int l) {
+        if constexpr (RUN == kAlong) {
+            return L::at(first + (l & 31), (l >> 5));
+        } else if constexpr (sizeof(T) == 2) {
+            // a transposing read takes four rows by 16 columns from 16 lanes; a lane
+            // half has eight contraction steps in a row, as along
+            const int i = l & 15, d = first + (l & 16) + 4 * (i & 3);
+            return L::at(8 * (l >> 5) + (i >> 2), d / 8) + (d & 7) * 2;
+        } else {
+            const int d = first + (l & 31);
+            return L::at(4 * (l >> 5), d / 4) + (d & 3) * 4;
+        }
+    }
+
+    // Step s (16 of the contraction) of the 32 rows or columns `on` further.
+    static __device__ __forceinline__ V read(const char* lds, int base, int on, int s) {
+        if constexpr (RUN == kAlong && sizeof(T) == 2) {
+            return *reinterpret_cast<const V*>(lds + L::moved(base, 32 * s, on));
+        } else if constexpr (RUN == kAlong) {  // steps 4 g .. and 8 + 4 g .., as across
+            const f32x4 a = *reinterpret_cast<const f32x4*>(lds + L::moved(base, 64 * s, on));
+            const f32x4 b = *reinterpret_cast<const f32x4*>(lds + L::moved(base, 64 * s + 32, on));
+            return __builtin_shufflevector(a, b, 0, 1, 2, 3, 4, 5, 6, 7);
+        } else if constexpr (sizeof(T) == 2) {
+            const s16x4 a = __builtin_amdgcn_ds_read_tr16_b64_v4i16((NSH_LDS s16x4*)(lds + L::moved(base, on * 2, 16 * s)));
+            const s16x4 b = __builtin_amdgcn_ds_read_tr16_b64_v4i16((NSH_LDS s16x4*)(lds + L::moved(base, on * 2, 16 * s + 4)));
+            return __builtin_bit_cast(V, __builtin_shufflevector(a, b, 0, 1, 2, 3, 4, 5, 6, 7));
+        } else {
+            return L::col(lds, base, 16 * s, on / 32);
+        }
+    }
+};
+
+// A matrix's panel, from memory straight to LDS by NT lanes.  Rows past the matrix's end
+// arrive as zeros (the buffer's range check), and along, columns past its end too.
+template <typename T, int ROWS, int DP, int NT, Run RUN>
+struct Panel {
+    using L = Tile<T, DP>;
+    static constexpr int NI = ROWS * L::NC / NT;
+    static_assert(NI * NT == ROWS * L::NC, "whole instructions");
+    // along, a lane has the same chunk of every row it loads
+    static_assert(RUN == kAcross || (NT / L::NC) % 16 == 0, "whole sets of 16 rows");
+    uint32_t off[NI];
+    int chunk;
+
+    __device__ __forceinline__ void init(uint32_t stride) {
+        chunk = ((threadIdx.x % L::NC) ^ L::turn(threadIdx.x / L::NC)) * 16;
+#pragma unroll
+        for (int i = 0; i < NI; ++i) {
+            const int x = i * NT + threadIdx.x, r = x / L::NC;
+            off[i] = static_cast<uint32_t>(r) * stride + ((x % L::NC) ^ L::turn(r)) * 16;
+        }
+    }
+    // from: the panel's first row; rows: how many are left, from there; left: bytes
+    // left of a row
+    __device__ __forceinline__ void load(char* lds, const char* from, uint32_t stride, int rows, int64_t left, int wave) const {
+        const uint32_t n = static_cast<uint32_t>(max(min(rows, ROWS), 0));
+        const uint32_t last = static_cast<uint32_t>(left < DP * static_cast<int>(sizeof(T)) ? left : DP * sizeof(T));
+        const __amdgpu_buffer_rsrc_t rs = __builtin_amdgcn_make_buffer_rsrc(
+            const_cast<char*>(from), static_cast<short>(0), static_cast<int>(n ? (n - 1) * stride + last : 0u), 0x00020000);
+        if (RUN == kAlong && left < DP * static_cast<int>(sizeof(T))) {
+            const bool past = chunk >= static_cast<int>(left);
+#pragma unroll
+            for (int i = 0; i < NI; ++i) to_lds<16>(rs, lds + (i * (NT / 64) + wave) * 1024, past ? 0x80000000u : off[i]);
+        } else {
+#pragma unroll
+            for (int i = 0; i < NI; ++i) to_lds<16>(rs, lds + (i * (NT / 64) + wave) * 1024, off[i]);
+        }
+    }
+};
+
+// PAIRED: the wave's columns come in equal parts from the two halves of BN.
+template <typename T_, int BM_, int BN_, int WAVES_M, int WAVES_N, Run FIRST, Run SECOND, bool PAIRED_>
+struct Product {
+    using T = T_;
+    using V = typename Eight<T>::V;
+    static constexpr int BM = BM_, BN = BN_, BK = 128 / sizeof(T), STEPS = BK / 16;
+    static constexpr int NT = 64 * WAVES_M * WAVES_N, WM = BM / WAVES_M, WN = BN / WAVES_N;
+    static constexpr int MT = WM / 32, NB = WN / 32;
+    static constexpr bool PAIRED = PAIRED_;
+    using First = Operand<T, FIRST == kAlong ? BK : BN, FIRST>;
+    using Second = Operand<T, SECOND == kAlong ? BK : BM, SECOND>;
+    using FirstPanel = Panel<T, FIRST == kAlong ? (PAIRED ? BN / 2 : BN) : BK, FIRST == kAlong ? BK : BN, NT, FIRST>;
+    using SecondPanel = Panel<T, SECOND == kAlong ? BM : BK, SECOND == kAlong ? BK : BM, NT, SECOND>;
+    static constexpr int FIRST_BYTES = BN * 128, SECOND_BYTES = BM * 128;
+    static_assert(STEPS % 2 == 0 && (!PAIRED || (FIRST == kAlong && NB % 2 == 0)), "");
+
+    f32x16 acc[MT][NB];
+    int by_first, by_second;
+    struct Step {
+        V f[NB], s[MT];
+    };
+
+    static __device__ __forceinline__ int wave_m() { return wave_id() % WAVES_M; }
+    static __device__ __forceinline__ int wave_n() { return wave_id() / WAVES_M; }
+    // Where the wave's columns b start in the tile (PAIRED: b < NB / 2, in each half).
+    static __device__ __forceinline__ int column(int b) { return wave_n() * (PAIRED ? WN / 2 : WN) + b * 32; }
+    // The lane's row of block i.
+    static __device__ __forceinline__ int row(int i) { return wave_m() * WM + i * 32 + (threadIdx.x & 31); }
+
+    __device__ __forceinline__ void init() {
+        const int l = threadIdx.x & 63;
+        by_first = First::base(column(0), l);
+        by_second = Second::base(wave_m() * WM, l);
+#pragma unroll
+        for (int i = 0; i < MT; ++i)
+#pragma unroll
+            for (int b = 0; b < NB; ++b) acc[i][b] = f32x16{};
+    }
+    __device__ __forceinline__ void read(Step& x, const char* first, const char* second, int s) const {
+#pragma unroll
+        for (int b = 0; b < NB; ++b)
+            x.f[b] = First::read(first, by_first, PAIRED && b >= NB / 2 ? BN / 2 + (b - NB / 2) * 32 : b * 32, s);
+#pragma unroll
+        for (int i = 0; i < MT; ++i) x.s[i] = Second::read(second, by_second, i * 32, s);
+    }
+    __device__ __forceinline__ void multiply(const Step& x) {
+#pragma unroll
+        for (int i = 0; i < MT; ++i)
+#pragma unroll
+            for (int b = 0; b < NB; ++b) acc[i][b] = Eight<T>::mma(x.f[b], x.s[i], acc[i][b]);
+    }
+
+    // All n panels (n >= 1); load(i, first, second) asks for panel i.
+    template <typename Load>
+    __device__ __forceinline__ void run(int n, char (&f0)[FIRST_BYTES], char (&s0)[SECOND_BYTES], char (&f1)[FIRST_BYTES],
+                                        char (&s1)[SECOND_BYTES], const Load& load) {
+        Step x, y;
+        load(0, f0, s0);
+        landed();
+        if (n > 1) load(1, f1, s1);
+        read(x, f0, s0, 0);
+        auto panel = [&](int i, char (&f)[FIRST_BYTES], char (&s)[SECOND_BYTES], char (&fn)[FIRST_BYTES], char (&sn)[SECOND_BYTES]) {
+#pragma unroll
+            for (int st = 0; st + 2 < STEPS; st += 2) {
+                read(y, f, s, st + 1);
+                order();
+                multiply(x);
+                order();
+                read(x, f, s, st + 2);
+                order();
+                multiply(y);
+                order();
+            }
+            read(y, f, s, STEPS - 1);
+            order();
+            multiply(x);
+            order();
+            landed();
+            if (i + 2 < n) load(i + 2, f, s);
+            if (i + 1 < n) read(x, fn, sn, 0);
+            order();
+            multiply(y);
+            order();
+        };
+        for (int i = 0; i < n; i += 2) {
+            panel(i, f0, s0, f1, s1);
+            if (i + 1 < n) panel(i + 1, f1, s1, f0, s0);
+        }
+        settle<T>();
+    }
+
+    // Every wave's loads have landed, and every wave has read what it needs of the
+    // panel before.
+    static __device__ __forceinline__ void landed() {
+        __builtin_amdgcn_s_waitcnt(0x0070);  // vmcnt(0), lgkmcnt(0)
+        __syncthreads();
+    }
+};
+
+// The order of result tiles: every XCD has a run of its own, in which `rows` rows of
+// tiles advance together, so that its L2 serves both matrices.
+struct TileOrder {
+    int m, n;
+    __device__ __forceinline__ TileOrder(int64_t id, int64_t count, int tiles_m, int tiles_n, int rows) {
+        const int64_t t = xcd_tile(id, count);
+        const int64_t band = static_cast<int64_t>(rows) * tiles_n;
+        const int first = static_cast<int>(t / band) * rows, deep = min(tiles_m - first, rows);
+        const int in = static_cast<int>(t % band);
+        m = first + in % deep;
+        n = in / deep;
+    }
+};
+
+// The lane's values of 32 columns from `c` on (the first of them the block's), rounded
+// to T, to its row of n columns.
+template <typename T>
+__device__ __forceinline__ void store_block(T* row, int64_t c, int64_t n, const f32x16& v) {
+    const int g = (threadIdx.x >> 5) & 1;
+    if constexpr (sizeof(T) == 4) {
+#pragma unroll
+        for (int q = 0; q < 4; ++q) {
+            const int64_t at = c + 8 * q + 4 * g;
+            if (at < n)
+                store_bits(row + at, 0, static_cast<int>(min(n - at, int64_t(4))),
+                           __builtin_bit_cast(ux4, (f32x4{v[4 * q], v[4 * q + 1], v[4 * q + 2], v[4 * q + 3]})));
+        }
+    } else {
+        // a lane half has four columns of each eight: halves exchange, eight a lane
+        typedef uint32_t ux2 __attribute__((ext_vector_type(2)));
+#pragma unroll
+        for (int q = 0; q < 4; q += 2) {
+            ux2 p[2];
+#pragma unroll
+            for (int e = 0; e < 2; ++e) {
+                const f32x4 x = {v[4 * (q + e)], v[4 * (q + e) + 1], v[4 * (q + e) + 2], v[4 * (q + e) + 3]};
+                if constexpr (__is_same(T, f16))
+                    p[e] = __builtin_bit_cast(ux2, __builtin_convertvector(x, f16x4));
+                else
+                    p[e] = __builtin_bit_cast(ux2, __builtin_convertvector(x, bf16x4));
+            }
+            const auto a = __builtin_amdgcn_permlane32_swap(p[0][0], p[1][0], false, false);
+            const auto b = __builtin_amdgcn_permlane32_swap(p[0][1], p[1][1], false, false);
+            const int64_t at = c + 8 * q + 8 * g;
+            if (at < n) store_bits(row + at, 0, static_cast<int>(min(n - at, int64_t(8))), ux4{a[0], b[0], a[1], b[1]});
+        }
+    }
+}
+
+}  // namespace nsh

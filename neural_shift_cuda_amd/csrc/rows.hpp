@@ -1,0 +1,92 @@
+// rows.hpp -- 16 bytes of a row at a time, whatever it is aligned to, and sums
+// over groups of lanes.
+#pragma once
+
+#include "nsh_common.hpp"
+
+namespace nsh {
+
+typedef float fx8 __attribute__((ext_vector_type(8)));
+typedef float fx4 __attribute__((ext_vector_type(4)));
+typedef uint32_t ux4 __attribute__((ext_vector_type(4)));
+
+template <typename T> constexpr int kVec = 16 / sizeof(T);
+
+// Columns c .. c + kVec - 1 of a row of n, those past its end as zeros.  Rows need
+// no alignment beyond an element's: gfx950 splits a load that crosses a line.
+template <typename T>
+__device__ __forceinline__ ux4 load_bits(const T* row, int c, int n) {
+    ux4 r = {0, 0, 0, 0};
+    if (c + kVec<T> <= n) {
+        __builtin_memcpy(&r, row + c, 16);
+    } else if (c < n) {
+        T e[kVec<T>] = {};
+#pragma unroll
+        for (int k = 0; k < kVec<T>; ++k)
+            if (c + k < n) e[k] = row[c + k];
+        __builtin_memcpy(&r, e, 16);
+    }
+    return r;
+}
+
+template <typename T>
+__device__ __forceinline__ void unpack(ux4 r, float (&o)[kVec<T>]) {
+    const Pack<T, kVec<T>> v = __builtin_bit_cast(Pack<T, kVec<T>>, r);
+#pragma unroll
+    for (int k = 0; k < kVec<T>; ++k) o[k] = to_acc(v.e[k]);
+}
+
+// Rounded to nearest even by the conversion instructions.
+template <typename T>
+__device__ __forceinline__ ux4 pack(const float (&v)[kVec<T>]) {
+    if constexpr (__is_same(T, float)) {
+        return __builtin_bit_cast(ux4, (fx4{v[0], v[1], v[2], v[3]}));
+    } else {
+        const fx8 f = {v[0], v[1], v[2], v[3], v[4], v[5], v[6], v[7]};
+        if constexpr (__is_same(T, bf16)) {
+            typedef __bf16 V __attribute__((ext_vector_type(8)));
+            return __builtin_bit_cast(ux4, __builtin_convertvector(f, V));
+        } else {
+            typedef _Float16 V __attribute__((ext_vector_type(8)));
+            return __builtin_bit_cast(ux4, __builtin_convertvector(f, V));
+        }
+    }
+}
+
+template <typename T>
+__device__ __forceinline__ void store_bits(T* row, int c, int n, ux4 r) {
+    if (c + kVec<T> <= n) {
+        __builtin_memcpy(row + c, &r, 16);
+    } else if (c < n) {
+        T e[kVec<T>];
+        __builtin_memcpy(e, &r, 16);
+#pragma unroll
+        for (int k = 0; k < kVec<T>; ++k)
+            if (c + k < n) row[c + k] = e[k];
+    }
+}
+
+template <int CTRL>
+__device__ __forceinline__ float lane_moved(float v) {
+    return __int_as_float(__builtin_amdgcn_mov_dpp(__float_as_int(v), CTRL, 0xf, 0xf, true));
+}
+
+// Over G lanes that stand side by side, in every one of them (no LDS).
+template <int G>
+__device__ __forceinline__ float lanes_sum(float v) {
+    v += lane_moved<0xB1>(v);   // lane ^ 1
+    v += lane_moved<0x4E>(v);   // lane ^ 2
+    v += lane_moved<0x141>(v);  // mirrored in eight lanes, whose fours agree
+    if constexpr (G >= 16) v += lane_moved<0x140>(v);  // mirrored in 16
+    if constexpr (G >= 32) {
+        const auto r = __builtin_amdgcn_permlane16_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+        v = __uint_as_float(r[0]) + __uint_as_float(r[1]);
+    }
+    if constexpr (G >= 64) {
+        const auto r = __builtin_amdgcn_permlane32_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+        v = __uint_as_float(r[0]) + __uint_as_float(r[1]);
+    }
+    return v;
+}
+
+}  // namespace nsh

@@ -7,60 +7,20 @@
 // the norm (3 x 12 heads, 1025 tokens, 28 us of kernels) took 175 us, 50 of them
 // for the backward in the autograd thread, whose caches are cold for the
 // interpreter; here 96.  One token over a short cache: 17 us, here 10.
-#include <c10/hip/HIPStream.h>
-#include <c10/core/AutogradState.h>
-#include <torch/csrc/autograd/functions/basic_ops.h>
-#include <torch/csrc/jit/frontend/tracer.h>
-#include <torch/extension.h>
+#include "calls.hpp"
 
-#include <cmath>
-#include <stdexcept>
-
-#include "neural_shift_hip.h"
+// the operators of block_calls.cpp
+void block_calls(pybind11::module_& m);
 
 namespace {
 
-using at::Tensor;
-using torch::autograd::AutogradContext;
-using torch::autograd::variable_list;
-using Maybe = std::optional<Tensor>;
-
-template <typename T = void>
-T* address(const Tensor& t) {
-    return t.defined() ? static_cast<T*>(t.data_ptr()) : nullptr;
-}
-Tensor given(const Maybe& t) { return t ? *t : Tensor(); }
-
-void strides(int64_t (&to)[3], const Tensor& t) {
-    for (int i = 0; i < 3; ++i) to[i] = t.stride(i);
-}
-
-int32_t code(const Tensor& t, const char* op) {
-    switch (t.scalar_type()) {
-        case at::kHalf: return NSH_DTYPE_FLOAT16;
-        case at::kBFloat16: return NSH_DTYPE_BFLOAT16;
-        case at::kFloat: return NSH_DTYPE_FLOAT32;
-        default:
-            throw std::runtime_error(std::string("\"") + op + "\" not implemented for '" +
-                                     c10::toString(t.scalar_type()) + "'");
-    }
-}
-
-void* stream(const Tensor& t) { return c10::hip::getCurrentHIPStream(t.get_device()).stream(); }
-
-void done(int rc) {
-    if (rc != NSH_OK) throw std::runtime_error(nsh_last_error());
-}
+using namespace nsh_calls;
 
 // A new tensor that keeps t's order of heads and tokens in memory.
 Tensor like(const Tensor& t) {
     if (!t.is_contiguous() && t.stride(1) < t.stride(2))
         return at::empty({t.size(0), t.size(2), t.size(1), t.size(3)}, t.options()).transpose(1, 2);
     return at::empty(t.sizes(), t.options());
-}
-
-Tensor scratch(const Tensor& t, int64_t bytes) {
-    return bytes > 0 ? at::empty({bytes}, t.options().dtype(at::kByte)) : Tensor();
 }
 
 // Rows with a unit last stride, in whole (`rows16`) 16-byte pieces.
@@ -71,32 +31,6 @@ Tensor rows16(const Tensor& t) {
         t.stride(2) * e <= int64_t(1) << 24)
         return t;
     return t.clone(at::MemoryFormat::Contiguous);
-}
-
-// Gradients of gradients are refused where they are asked for.
-variable_list once(variable_list grads) {
-    if (!at::GradMode::is_enabled()) return grads;
-    for (auto& g : grads)
-        if (g.defined()) g = g.detach().requires_grad_();
-    auto error = std::make_shared<torch::autograd::DelayedError>(
-        "trying to differentiate twice a token operator, whose gradients are not differentiable",
-        static_cast<int64_t>(grads.size()));
-    return (*error)(std::move(grads));
-}
-
-// A tangent would be dropped without a word: what the kernels write has none.
-void no_tangents(const char* op, std::initializer_list<const Tensor*> tensors) {
-    if (!c10::AutogradState::get_tls_state().get_fw_grad_mode()) return;
-    for (const Tensor* t : tensors)
-        TORCH_CHECK_NOT_IMPLEMENTED(!t->defined() || !t->_fw_grad(0).defined(), op,
-                                    ": forward-mode derivatives are not implemented");
-}
-
-bool graph(std::initializer_list<const Tensor*> tensors) {
-    if (!at::GradMode::is_enabled()) return false;
-    for (const Tensor* t : tensors)
-        if (t->defined() && t->requires_grad()) return true;
-    return false;
 }
 
 // ---------------------------------------------------------------------------
@@ -378,18 +312,6 @@ std::tuple<Tensor, Maybe> attention(const Tensor& q0, const Tensor& k0, const Te
 // allocations here and no kernel.  (They take 4 to 9 us in Python, as long as the rest of a call.)
 // ---------------------------------------------------------------------------
 
-bool served(const Tensor& t) {
-    const auto type = t.scalar_type();
-    return type == at::kHalf || type == at::kBFloat16 || type == at::kFloat;
-}
-
-bool alike(const Tensor& t, const Tensor& q) { return t.scalar_type() == q.scalar_type() && t.device() == q.device(); }
-
-// Not given, or contiguous in `type` and of this shape.
-bool plain(const Maybe& t, const Tensor& q, at::ScalarType type, at::IntArrayRef shape) {
-    return !t || (t->scalar_type() == type && t->device() == q.device() && t->sizes() == shape && t->is_contiguous());
-}
-
 bool map_of_buckets(const Tensor& table, const Maybe& buckets) {
     return table.dim() == 2 && table.size(0) >= 1 && table.size(0) <= 4097 && buckets && buckets->dim() == 1 &&
            buckets->size(0) % 2 == 1 && buckets->size(0) <= 4097 &&
@@ -458,4 +380,5 @@ PYBIND11_MODULE(_token_calls, m) {
     m.def("position_bias_as_is", &position_bias_as_is, release());
     m.def("attention_as_is", &attention_as_is, release());
     m.def("attention_forward", &attention_plain, release());
+    block_calls(m);
 }
