@@ -628,8 +628,8 @@ typedef struct nsh_gated_linear_args {
     int32_t dtype, activation;
     void* h; /* forward: (rows, F), contiguous */
     /* nsh_gated_linear_kept_bytes, 16-byte aligned, or NULL.  Forward: written, what
-     * the backward needs.  Backward: read. */
-    float* kept;
+     * the backward needs.  Backward: read, with the forward's rows, F and dtype. */
+    void* kept;
     const void* grad_h; /* backward, with its stride; gradients contiguous, NULL = not wanted */
     int64_t gh_stride;
     void *grad_x, *grad_gate, *grad_up;

@@ -39,40 +39,46 @@ __global__ __launch_bounds__(kPassThreads) void gated_copy_kernel(CopyArgs a) {
 
 struct SlopeArgs {
     const void* gh;
-    int64_t gh_stride, rows;
-    const float* kept;
+    int64_t gh_stride, rows, dgu_stride;  // elements
+    char* kept;
     void* dgu;
-    int F, Fk, Fp;
+    int F, Fp;
+    uint32_t across;  // workgroups a row of blocks
     const float* scale;
 };
 
-// dg and du, a workgroup a row and 256 parts of it.
+// dg and du: a wave has 32 rows and 128 bytes of each, blocks of what was kept.
 template <typename T>
 __global__ __launch_bounds__(kPassThreads) void gated_slope_kernel(SlopeArgs a) {
-    constexpr int V = kVec<T>;
-    const int c = (blockIdx.x * kPassThreads + threadIdx.x) * V;
-    if (c >= a.Fp) return;
+    constexpr int COLS = 128 / sizeof(T), BLOCKS = COLS / 32;
+    using S = Stage<T, 32, COLS>;
+    __shared__ __attribute__((aligned(256))) char stages[kPassThreads / 64][S::BYTES];
+    char* stage = stages[wave_id()];
+    const uint32_t down = blockIdx.x / a.across, across = blockIdx.x - down * a.across;
+    const int c0 = (across * (kPassThreads / 64) + wave_id()) * COLS;
+    if (c0 >= a.Fp) return;
+    const int64_t m0 = static_cast<int64_t>(down) * 32, rows = a.rows - m0;
     const float by = __is_same(T, f16) && a.scale ? a.scale[0] : 1.f;
-    for (int64_t m = blockIdx.y; m < a.rows; m += gridDim.y) {
-        float d[V], s[V] = {}, h[V] = {};
-        unpack<T>(load_bits(static_cast<const T*>(a.gh) + m * a.gh_stride, c, a.F), d);
-        const float* k = a.kept + m * 2 * a.Fk + c;
-        if (c < a.F) {
+    Kept<T> k[BLOCKS];
 #pragma unroll
-            for (int e = 0; e < V; e += 4) {
-                load_acc<float, 4>(k + e, *reinterpret_cast<float(*)[4]>(&s[e]));
-                load_acc<float, 4>(k + a.Fk + e, *reinterpret_cast<float(*)[4]>(&h[e]));
-            }
-        }
+    for (int b = 0; b < BLOCKS; ++b)
+        if (c0 + 32 * b < a.F) k[b].load(Kept<T>::block(a.kept, m0, c0 + 32 * b, a.F));
+    S::load(stage, static_cast<const T*>(a.gh) + m0 * a.gh_stride + c0, a.gh_stride, rows, a.F - c0);
+    wave_exchange();
+    f32x16 d[BLOCKS], x[BLOCKS];
 #pragma unroll
-        for (int e = 0; e < V; ++e) {
-            const bool in = c + e < a.F;
-            s[e] = in ? d[e] * by * s[e] : 0.f;
-            h[e] = in ? d[e] * by * h[e] : 0.f;
-        }
-        T* to = static_cast<T*>(a.dgu) + m * 2 * a.Fp + c;
-        *reinterpret_cast<ux4*>(to) = pack<T>(s);
-        *reinterpret_cast<ux4*>(to + a.Fp) = pack<T>(h);
+    for (int b = 0; b < BLOCKS; ++b) d[b] = S::get(stage, 0, b) * by;
+#pragma unroll
+    for (int side = 0; side < 2; ++side) {
+        // (dh past F is 0, and what was kept of places past it in the last block is the
+        // activation at 0, a number)
+#pragma unroll
+        for (int b = 0; b < BLOCKS; ++b) x[b] = c0 + 32 * b < a.F ? d[b] * k[b].factor(side) : f32x16{};
+        wave_exchange();
+#pragma unroll
+        for (int b = 0; b < BLOCKS; ++b) S::put(stage, 0, b, x[b]);
+        wave_exchange();
+        S::store(stage, static_cast<T*>(a.dgu) + m0 * a.dgu_stride + side * a.Fp + c0, a.dgu_stride, rows, COLS);
     }
 }
 
@@ -97,16 +103,14 @@ __device__ __forceinline__ float workgroup_max(float v, float* lds) {
 __global__ __launch_bounds__(kPassThreads) void gated_most_kernel(const f16* gh, int64_t stride, int64_t rows, int F,
                                                                   float* out) {
     __shared__ float lds[kPassThreads];
-    const int each = (F + 7) / 8;
-    const int64_t all = rows * each, step = static_cast<int64_t>(gridDim.x) * kPassThreads;
     float most = 0.f;
-    for (int64_t i = static_cast<int64_t>(blockIdx.x) * kPassThreads + threadIdx.x; i < all; i += step) {
-        const int64_t row = i / each;
-        float d[8];
-        unpack<f16>(load_bits(gh + row * stride, static_cast<int>(i - row * each) * 8, F), d);
+    for (int64_t row = blockIdx.x; row < rows; row += gridDim.x)
+        for (int c = threadIdx.x * 8; c < F; c += kPassThreads * 8) {
+            float d[8];
+            unpack<f16>(load_bits(gh + row * stride, c, F), d);
 #pragma unroll
-        for (int e = 0; e < 8; ++e) most = fmaxf(most, fabsf(d[e]) < INFINITY ? fabsf(d[e]) : 0.f);
-    }
+            for (int e = 0; e < 8; ++e) most = fmaxf(most, fabsf(d[e]) < INFINITY ? fabsf(d[e]) : 0.f);
+        }
     most = workgroup_max(most, lds);
     if (threadIdx.x == 0) out[blockIdx.x] = most;
 }
@@ -151,7 +155,7 @@ constexpr int64_t kWidest = int64_t(1) << 20;
 constexpr int64_t kStep = int64_t(1) << 23;  // bytes from a row to the next that a panel's 32-bit offsets take
 
 struct Plan {
-    int64_t esz, Kp, Fp, Fk;
+    int64_t esz, Kp, Fp;
     bool copy[3];       // x, gate, up
     int64_t copies[3];  // offsets in the workspace
     int64_t dgu, scale, most, part, bytes;
@@ -165,7 +169,7 @@ Plan plan_of(const nsh_gated_linear_args* g, bool bwd) {
     Plan p{};
     p.esz = g->dtype == NSH_DTYPE_FLOAT32 ? 4 : 2;
     const int64_t vec = 16 / p.esz;
-    p.Kp = up(g->K, vec), p.Fp = up(g->F, 128 / p.esz), p.Fk = up(g->F, 8);
+    p.Kp = up(g->K, vec), p.Fp = up(g->F, 64);
     const void* at[3] = {g->x, g->gate_weight, g->up_weight};
     const int64_t stride[3] = {g->x_stride, g->gate_stride, g->up_stride}, rows[3] = {g->rows, g->F, g->F};
     for (int i = 0; i < 3; ++i) {
@@ -177,7 +181,7 @@ Plan plan_of(const nsh_gated_linear_args* g, bool bwd) {
     }
     if (!bwd) return p;
     p.dgu = p.bytes;
-    p.bytes += up(g->rows * 2 * p.Fp * p.esz, 256);
+    p.bytes += up(g->rows * (2 * p.Fp * p.esz + 128), 256);
     p.scale = p.bytes, p.bytes += 256;
     p.most = p.bytes, p.bytes += up(nsh::kMostBlocks * 4, 256);
     p.part = p.bytes, p.splits = 1;
@@ -191,6 +195,13 @@ Plan plan_of(const nsh_gated_linear_args* g, bool bwd) {
 
 int64_t forward_blocks(const nsh_gated_linear_args* g) {
     return nsh::cut_of(g->rows, g->F, g->dtype == NSH_DTYPE_FLOAT32, true, 1).tiles();
+}
+
+int64_t kept_blocks(const nsh_gated_linear_args* g) {
+    const int64_t each = g->dtype == NSH_DTYPE_FLOAT32    ? nsh::Kept<float>::BYTES
+                         : g->dtype == NSH_DTYPE_BFLOAT16 ? nsh::Kept<nsh::bf16>::BYTES
+                                                          : nsh::Kept<nsh::f16>::BYTES;
+    return ceil_div(g->rows, 32) * ceil_div(g->F, 32) * each;
 }
 
 int check(const char* op, const nsh_gated_linear_args* g, bool bwd) {
@@ -238,14 +249,14 @@ int backward(const nsh_gated_linear_args* g, const Plan& p, nsh::GatedArgs a, ch
     if constexpr (__is_same(T, nsh::f16)) {
         scale = reinterpret_cast<float*>(ws + p.scale);
         float* most = reinterpret_cast<float*>(ws + p.most);
-        const int n = static_cast<int>(std::min<int64_t>(ceil_div(g->rows * ceil_div(g->F, 8), nsh::kPassThreads), nsh::kMostBlocks));
+        const int n = static_cast<int>(std::min<int64_t>(g->rows, nsh::kMostBlocks));
         nsh::gated_most_kernel<<<n, nsh::kPassThreads, 0, st>>>(static_cast<const nsh::f16*>(g->grad_h), g->gh_stride, g->rows, a.F, most);
-        nsh::gated_scale_kernel<<<1, nsh::kPassThreads, 0, st>>>(most, n, g->kept + g->rows * 2 * p.Fk, static_cast<int>(forward_blocks(g)), scale);
+        nsh::gated_scale_kernel<<<1, nsh::kPassThreads, 0, st>>>(most, n, reinterpret_cast<const float*>(a.kept + kept_blocks(g)), static_cast<int>(forward_blocks(g)), scale);
     }
     a.scale = scale, a.dgu = ws + p.dgu;
-    const nsh::SlopeArgs s{g->grad_h, g->gh_stride, g->rows, g->kept, a.dgu, a.F, a.Fk, a.Fp, scale};
-    const unsigned across = static_cast<unsigned>(ceil_div(a.Fp, nsh::kPassThreads * nsh::kVec<T>));
-    nsh::gated_slope_kernel<T><<<dim3(across, static_cast<unsigned>(std::min<int64_t>(g->rows, 32768))), nsh::kPassThreads, 0, st>>>(s);
+    const uint32_t across = static_cast<uint32_t>(ceil_div(a.Fp, nsh::kPassThreads / 64 * 128 / p.esz));
+    const nsh::SlopeArgs s{g->grad_h, g->gh_stride, g->rows, 2 * p.Fp + 128 / p.esz, a.kept, a.dgu, a.F, a.Fp, across, scale};
+    nsh::gated_slope_kernel<T><<<static_cast<unsigned>(across * ceil_div(g->rows, 32)), nsh::kPassThreads, 0, st>>>(s);
     if (g->grad_x) {
         a.splits = p.splits;
         a.part = p.splits > 1 ? reinterpret_cast<float*>(ws + p.part) : nullptr;
@@ -267,14 +278,14 @@ int run(const nsh_gated_linear_args* g, const Plan& p, bool bwd, hipStream_t st)
     char* ws = static_cast<char*>(g->workspace);
     a.x = g->x, a.wg = g->gate_weight, a.wu = g->up_weight;
     a.rows = g->rows, a.K = static_cast<int>(g->K), a.F = static_cast<int>(g->F);
-    a.Kp = static_cast<int>(p.Kp), a.Fp = static_cast<int>(p.Fp), a.Fk = static_cast<int>(p.Fk);
+    a.Kp = static_cast<int>(p.Kp), a.Fp = static_cast<int>(p.Fp);
     a.activation = g->activation - NSH_ACTIVATION_SILU;
     a.h = g->h, a.dx = g->grad_x, a.dwg = g->grad_gate, a.dwu = g->grad_up;
     const int rc = copy_rows<T>(g, p, a, ws, st);
     if (rc != NSH_OK) return rc;
+    a.kept = static_cast<char*>(g->kept);
     if (bwd) return backward<T>(g, p, a, ws, st);
-    a.kept = g->kept;
-    if (__is_same(T, nsh::f16) && a.kept) a.most = a.kept + a.rows * 2 * a.Fk;
+    if (__is_same(T, nsh::f16) && a.kept) a.most = reinterpret_cast<float*>(a.kept + kept_blocks(g));
     return nsh::gated_forward<T>(a, st);
 }
 
@@ -302,7 +313,7 @@ extern "C" int64_t nsh_gated_linear_workspace_bytes(const nsh_gated_linear_args*
 
 extern "C" int64_t nsh_gated_linear_kept_bytes(const nsh_gated_linear_args* g) {
     if (!g || g->rows < 1 || g->K < 1 || g->F < 1) return -1;
-    return (g->rows * 2 * up(g->F, 8) + (g->dtype == NSH_DTYPE_FLOAT16 ? forward_blocks(g) : 0)) * 4;
+    return kept_blocks(g) + (g->dtype == NSH_DTYPE_FLOAT16 ? forward_blocks(g) * 4 : 0);
 }
 
 extern "C" int nsh_gated_linear_forward(const nsh_gated_linear_args* g, void* stream) {

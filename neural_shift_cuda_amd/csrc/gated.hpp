@@ -7,9 +7,9 @@
 // Three products over panels (panels.hpp).  Forward: both weights' rows stand side by
 // side in one panel, so a lane has g and u of the same place and the activation and
 // the product never leave its registers.  Training keeps u act'(g) and act(g), the
-// factors that dh takes, in fp32: rounded to 16 bits they would bring a third rounding
-// next to dg's and the result's (errors of the gradients 1.7 times the result's own
-// rounding instead of 1.4).  Backward: one pass forms dg and du, as one matrix
+// factors that dh takes, finer than the type (struct Kept): rounded to it they would bring
+// a third rounding next to dg's and the result's (errors of the gradients 1.7 times the
+// result's own rounding instead of 1.4).  Backward: one pass forms dg and du, as one matrix
 // (rows, 2, Fp) of the operands' type (a matrix instruction takes no other; each is off by
 // half a step, of the size of the result's own rounding and not shared by a sum's
 // terms), then dx takes both in one sum over 2 F, and one product gives both weights'
@@ -24,12 +24,12 @@ struct GatedArgs {
     const void *x, *wg, *wu;
     uint32_t x_stride, wg_stride, wu_stride;  // bytes from row to row
     int64_t rows;
-    int K, F, Kp, Fp, Fk;  // Kp: columns of x and the weights as they lie; Fp, Fk: row lengths of dgu and kept
+    int K, F, Kp, Fp;     // Kp: columns of x and the weights as they lie; Fp: F in whole panels
     int activation;
     void* h;
-    float* kept;           // (rows, 2, Fk) or NULL
-    float* most;           // fp16 training: largest |kept| of every workgroup
-    void* dgu;             // (rows, 2, Fp)
+    char* kept;            // blocks of 32 x 32 (struct Kept), or NULL
+    float* most;           // fp16 training: largest factor of every workgroup
+    void* dgu;             // (rows, 2, Fp) and a panel's width of nothing
     const float* scale;    // fp16: what dgu was multiplied by, and its inverse
     void *dx, *dwg, *dwu;
     float* part;           // (splits, rows, K): sums of dx that a second launch joins
@@ -38,52 +38,180 @@ struct GatedArgs {
 
 enum Activation { kSilu, kGelu, kGeluTanh, kRelu, kSigmoid };
 
-// The activation at g and its slope there.
-__device__ __forceinline__ float2 activate(int kind, float g) {
-    switch (kind) {
-        case kSilu: {
-            const float s = 1.f / (1.f + __expf(-g));
-            return make_float2(g * s, s * fma_acc(g, 1.f - s, 1.f));
-        }
-        case kGelu: {
-            // erfc, whose small values near -inf keep their places
-            const float below = 0.5f * erfcf(g * -0.70710678118654752f);
-            return make_float2(g * below, fma_acc(g * 0.3989422804014327f, __expf(-0.5f * g * g), below));
-        }
-        case kGeluTanh: {
-            constexpr float a = 1.5957691216057308f, b = 0.044715f;  // 2 sqrt(2 / pi)
-            const float s = 1.f / (1.f + __expf(-a * g * fma_acc(b * g, g, 1.f)));
-            return make_float2(g * s, fma_acc(g * s * (1.f - s), a * fma_acc(3.f * b * g, g, 1.f), s));
-        }
-        case kRelu: return g > 0.f ? make_float2(g, 1.f) : make_float2(g == g ? 0.f : g, 0.f);
-        default: {
-            const float s = 1.f / (1.f + __expf(-g));
-            return make_float2(s, s * (1.f - s));
-        }
+// The activation at g and its slope there, by instructions of one place in the last or so:
+// next to the sums' roundings nothing, and a third of the library functions' time.
+__device__ __forceinline__ float sigmoid(float x) {
+    return __builtin_amdgcn_rcpf(1.f + __builtin_amdgcn_exp2f(-kLog2e * x));
+}
+template <Activation KIND>
+__device__ __forceinline__ float2 activate(float g) {
+    if constexpr (KIND == kSilu) {
+        const float s = sigmoid(g);
+        return make_float2(g * s, s * fma_acc(g, 1.f - s, 1.f));
+    } else if constexpr (KIND == kGelu) {
+        // Phi(-|g|) = exp(-g^2 / 2) erfcx(|g| / sqrt 2) / 2, whose small values keep their
+        // places; erfcx(z) / t as a polynomial in t = 1 / (1 + 0.4 z), by least squares with
+        // weights towards the smallest largest error: 6e-9 of it, 1e-7 with fp32's roundings
+        const float z = fabsf(g), t = __builtin_amdgcn_rcpf(fma_acc(0.28284271247461901f, z, 1.f));
+        const float e = __builtin_amdgcn_exp2f(z * z * (-0.5f * kLog2e));
+        float p = -0.0292149931f;
+        p = fma_acc(p, t, 0.140446082f);
+        p = fma_acc(p, t, -0.235525861f);
+        p = fma_acc(p, t, 0.137559712f);
+        p = fma_acc(p, t, -0.0468939133f);
+        p = fma_acc(p, t, 0.0839158222f);
+        p = fma_acc(p, t, 0.119008467f);
+        p = fma_acc(p, t, 0.17173925f);
+        p = fma_acc(p, t, 0.207613736f);
+        p = fma_acc(p, t, 0.225675866f);
+        p = fma_acc(p, t, 0.225675836f);
+        const float tail = 0.5f * e * (p * t), below = g > 0.f ? 1.f - tail : tail;
+        return make_float2(g * below, fma_acc(g * 0.3989422804014327f, e, below));
+    } else if constexpr (KIND == kGeluTanh) {
+        constexpr float a = 1.5957691216057308f, b = 0.044715f;  // 2 sqrt(2 / pi)
+        const float s = sigmoid(a * g * fma_acc(b * g, g, 1.f));
+        return make_float2(g * s, fma_acc(g * s * (1.f - s), a * fma_acc(3.f * b * g, g, 1.f), s));
+    } else if constexpr (KIND == kRelu) {
+        return g > 0.f ? make_float2(g, 1.f) : make_float2(g == g ? 0.f : g, 0.f);
+    } else {
+        const float s = sigmoid(g);
+        return make_float2(s, s * (1.f - s));
     }
 }
 
-// h, and what the gradients need, of the lane's 16 places from column c on.
-template <typename T>
-__device__ __forceinline__ float gate_block(const GatedArgs& a, int64_t m, int c, const f32x16& g, const f32x16& u) {
-    f32x16 h, s;
+// v and slope of N places.
+template <int N, typename V>
+__device__ __forceinline__ void activate(int kind, const V& g, V& v, V& slope) {
+    auto all = [&](auto one) {
 #pragma unroll
-    for (int r = 0; r < 16; ++r) {
-        const float2 f = activate(a.activation, g[r]);
-        h[r] = f.x;
-        s[r] = u[r] * f.y;
+        for (int r = 0; r < N; ++r) {
+            const float2 f = one(g[r]);
+            v[r] = f.x, slope[r] = f.y;
+        }
+    };
+    switch (kind) {
+        case kSilu: return all([](float x) { return activate<kSilu>(x); });
+        case kGelu: return all([](float x) { return activate<kGelu>(x); });
+        case kGeluTanh: return all([](float x) { return activate<kGeluTanh>(x); });
+        case kRelu: return all([](float x) { return activate<kRelu>(x); });
+        default: return all([](float x) { return activate<kSigmoid>(x); });
     }
-    float most = 0.f;
-    if (a.kept && m < a.rows) {
-        float* to = a.kept + m * 2 * a.Fk;
+}
+
+// What training keeps of a block of 32 x 32 places: the two factors as the lanes have
+// them, so that every store and load is 1 KB in one piece (rows of their own, 16 bytes a
+// lane apart, took the forward 8192 x 2048 -> 8192 from 480 to 1017 us).
+//   bf16: fp16 times a power of two of each lane's largest, which leaves 11 bits of all
+//     that is not below 2^-29 of it, and 2^-40 of it of the rest
+//   fp16: the upper 24 bits of fp32
+//   fp32: itself
+template <typename T>
+struct Kept {
+    static constexpr int BYTES = sizeof(T) == 4 ? 8192 : __is_same(T, bf16) ? 4096 + 256 : 6144;
+
+    static __device__ __forceinline__ char* block(char* kept, int64_t m, int c, int F) {
+        return kept + ((m >> 5) * ((F + 31) >> 5) + (c >> 5)) * BYTES;
+    }
+    static __device__ __forceinline__ ux4* part(char* at, int n) {
+        return reinterpret_cast<ux4*>(at + n * 1024) + (threadIdx.x & 63);
+    }
+
+    // The exponent field of the largest number of a lane's 16 (15 at the least).
+    static __device__ __forceinline__ uint32_t field(const f32x16& v) {
+        float most = 0.f;
 #pragma unroll
-        for (int q = 0; q < 4; ++q) {
-            const int at = c + 8 * q + 4 * ((threadIdx.x >> 5) & 1);
-            if (at < a.Fk) {
-                *reinterpret_cast<f32x4*>(to + at) = f32x4{s[4 * q], s[4 * q + 1], s[4 * q + 2], s[4 * q + 3]};
-                *reinterpret_cast<f32x4*>(to + a.Fk + at) = f32x4{h[4 * q], h[4 * q + 1], h[4 * q + 2], h[4 * q + 3]};
+        for (int r = 0; r < 16; ++r) most = fmaxf(most, fabsf(v[r]));
+        if (!(most < INFINITY)) {  // an infinity says nothing of the others
+            most = 0.f;
+#pragma unroll
+            for (int r = 0; r < 16; ++r) most = fmaxf(most, fabsf(v[r]) < INFINITY ? fabsf(v[r]) : 0.f);
+        }
+        return max(__float_as_uint(most) >> 23, 15u);
+    }
+
+    static __device__ __forceinline__ void store(char* at, const f32x16& s, const f32x16& h) {
+        const f32x16* both[2] = {&s, &h};
+        uint32_t fields[2];
+#pragma unroll
+        for (int n = 0; n < 2; ++n) {
+            const f32x16& v = *both[n];
+            if constexpr (sizeof(T) == 4) {
+#pragma unroll
+                for (int q = 0; q < 4; ++q)
+                    *part(at, 4 * n + q) = __builtin_bit_cast(ux4, (f32x4{v[4 * q], v[4 * q + 1], v[4 * q + 2], v[4 * q + 3]}));
+            } else if constexpr (__is_same(T, bf16)) {
+                fields[n] = field(v);
+                const f32x16 x = v * __uint_as_float((268u - fields[n]) << 23);  // to 2^14 .. 2^15
+#pragma unroll
+                for (int q = 0; q < 2; ++q) {
+                    const f32x8 y = {x[8 * q], x[8 * q + 1], x[8 * q + 2], x[8 * q + 3],
+                                     x[8 * q + 4], x[8 * q + 5], x[8 * q + 6], x[8 * q + 7]};
+                    *part(at, 2 * n + q) = __builtin_bit_cast(ux4, __builtin_convertvector(y, f16x8));
+                }
+            } else {
+                uint32_t b[16];
+#pragma unroll
+                for (int r = 0; r < 16; ++r) b[r] = __float_as_uint(v[r]) + 0x80u;
+#pragma unroll
+                for (int q = 0; q < 2; ++q) {
+                    ux4 x;
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) x[e] = b[8 * q + 2 * e] >> 16 | (b[8 * q + 2 * e + 1] & 0xffff0000u);
+                    *part(at, 2 * n + q) = x;
+                }
+                ux4 x;
+#pragma unroll
+                for (int e = 0; e < 4; ++e)
+                    x[e] = (b[4 * e] >> 8 & 0xffu) | (b[4 * e + 1] & 0xff00u) | (b[4 * e + 2] & 0xff00u) << 8 |
+                           (b[4 * e + 3] & 0xff00u) << 16;
+                *part(at, 4 + n) = x;
             }
         }
+        if constexpr (__is_same(T, bf16))
+            reinterpret_cast<uint32_t*>(at + 4096)[threadIdx.x & 63] = fields[0] | fields[1] << 16;
+    }
+
+    // As loaded, and its numbers.
+    ux4 bits[BYTES / 1024];
+    uint32_t fields;
+    __device__ __forceinline__ void load(char* at) {
+#pragma unroll
+        for (int n = 0; n < BYTES / 1024; ++n) bits[n] = *part(at, n);
+        if constexpr (__is_same(T, bf16)) fields = reinterpret_cast<const uint32_t*>(at + 4096)[threadIdx.x & 63];
+    }
+    __device__ __forceinline__ f32x16 factor(int n) const {
+        f32x16 v;
+        if constexpr (sizeof(T) == 4) {
+#pragma unroll
+            for (int r = 0; r < 16; ++r) v[r] = __uint_as_float(bits[4 * n + r / 4][r % 4]);
+        } else if constexpr (__is_same(T, bf16)) {
+            const uint32_t f = n ? fields >> 16 : fields & 0xffffu;
+#pragma unroll
+            for (int q = 0; q < 2; ++q) {
+                const f32x8 x = __builtin_convertvector(__builtin_bit_cast(f16x8, bits[2 * n + q]), f32x8);
+#pragma unroll
+                for (int e = 0; e < 8; ++e) v[8 * q + e] = x[e];
+            }
+            v *= __uint_as_float((f - 14u) << 23);
+        } else {
+#pragma unroll
+            for (int r = 0; r < 16; ++r) {
+                const uint32_t hi = bits[2 * n + r / 8][r / 2 % 4], lo = bits[4 + n][r / 4] >> 8 * (r % 4) & 0xffu;
+                v[r] = __uint_as_float((r % 2 ? hi & 0xffff0000u : hi << 16) | lo << 8);
+            }
+        }
+        return v;
+    }
+};
+
+// h of the lane's 16 places from column c on, and what the gradients need.
+template <typename T>
+__device__ __forceinline__ f32x16 gate_block(const GatedArgs& a, int64_t m, int c, const f32x16& g, const f32x16& u, float& most) {
+    f32x16 h, s;
+    activate<16>(a.activation, g, h, s);
+    if (a.kept && (m & ~int64_t(31)) < a.rows && c < a.F) {
+        s *= u;
+        Kept<T>::store(Kept<T>::block(a.kept, m, c, a.F), s, h);
         if constexpr (__is_same(T, f16)) {
 #pragma unroll
             for (int r = 0; r < 16; ++r) {
@@ -93,12 +221,14 @@ __device__ __forceinline__ float gate_block(const GatedArgs& a, int64_t m, int c
             }
         }
     }
-#pragma unroll
-    for (int r = 0; r < 16; ++r) h[r] *= u[r];
-    // (the exchange of lane halves is every lane's)
-    const int64_t row = m < a.rows ? m : a.rows - 1;
-    store_block<T>(static_cast<T*>(a.h) + row * a.F, c, m < a.rows ? a.F : 0, h);
-    return most;
+    return h * u;
+}
+
+// Bytes of a row of dgu: not a power of two, which would have every row's same place in
+// one channel of the caches.
+template <typename T>
+__device__ __forceinline__ uint32_t dgu_stride(const GatedArgs& a) {
+    return 2 * a.Fp * static_cast<uint32_t>(sizeof(T)) + 128;
 }
 
 template <typename T, int BM, int BN, int WAVES_M, int WAVES_N>
@@ -128,14 +258,16 @@ __global__ __launch_bounds__(64 * WAVES_M * WAVES_N) void gated_forward_kernel(G
         rows.load(s, x + at, a.x_stride, left_m, wide - at, wave);
     });
     float most = 0.f;
-#pragma unroll
-    for (int i = 0; i < P::MT; ++i)
-#pragma unroll
-        for (int b = 0; b < P::NB / 2; ++b)
-            most = fmaxf(most, gate_block<T>(a, m0 + P::row(i), c0 + P::column(b), p.acc[i][b], p.acc[i][b + P::NB / 2]));
+    const int64_t m = m0 + P::wave_m() * P::WM;
+    const int c = c0 + P::column(0);
+    __syncthreads();  // the panels' place is free
+    store_tile<T, P::WM, P::WN / 2>(P::stage(f0, s0, f1, s1), static_cast<T*>(a.h) + m * a.F + c, a.F, a.rows - m, a.F - c,
+                                    [&](int i, int b) {
+                                        return gate_block<T>(a, m0 + P::row(i), c0 + P::column(b), p.acc[i][b],
+                                                             p.acc[i][b + P::NB / 2], most);
+                                    });
     if constexpr (__is_same(T, f16)) {
         if (!a.most) return;
-        // the panels' place is free once every wave is past its products
         float* meet = reinterpret_cast<float*>(f0);
         __syncthreads();
         meet[threadIdx.x] = most;
@@ -164,7 +296,7 @@ __global__ __launch_bounds__(64 * WAVES_M * WAVES_N) void gated_input_gradient_k
     typename P::SecondPanel rows;
     gate.init(a.wg_stride);
     up.init(a.wu_stride);
-    const uint32_t stride = 2 * a.Fp * static_cast<uint32_t>(sizeof(T));
+    const uint32_t stride = dgu_stride<T>(a);
     rows.init(stride);
     const char* d = static_cast<const char*>(a.dgu) + m0 * stride;
     const char* wg = static_cast<const char*>(a.wg) + c0 * static_cast<int64_t>(sizeof(T));
@@ -185,19 +317,14 @@ __global__ __launch_bounds__(64 * WAVES_M * WAVES_N) void gated_input_gradient_k
         rows.load(s, d + static_cast<int64_t>(at) * 128, stride, left_m, 128, wave);
     });
     const float by = __is_same(T, f16) && a.scale ? a.scale[1] : 1.f;
-#pragma unroll
-    for (int i = 0; i < P::MT; ++i) {
-        const int64_t m = m0 + P::row(i), row = m < a.rows ? m : a.rows - 1;
-#pragma unroll
-        for (int b = 0; b < P::NB; ++b) {
-            const f32x16 v = p.acc[i][b] * by;
-            const int64_t c = c0 + P::column(b), n = m < a.rows ? a.K : 0;
-            if (a.part)
-                store_block<float>(a.part + (split * a.rows + row) * a.K, c, n, v);
-            else
-                store_block<T>(static_cast<T*>(a.dx) + row * a.K, c, n, v);
-        }
-    }
+    const int64_t m = m0 + P::wave_m() * P::WM, c = c0 + P::column(0);
+    __syncthreads();  // the panels' place is free
+    char* stage = P::stage(f0, s0, f1, s1);
+    const auto value = [&](int i, int b) { return p.acc[i][b] * by; };
+    if (a.part)
+        store_tile<float, P::WM, P::WN>(stage, a.part + (split * a.rows + m) * a.K + c, a.K, a.rows - m, a.K - c, value);
+    else
+        store_tile<T, P::WM, P::WN>(stage, static_cast<T*>(a.dx) + m * a.K + c, a.K, a.rows - m, a.K - c, value);
 }
 
 // Both weights' gradients: tiles of hidden rows of the one, then of the other.
@@ -217,7 +344,7 @@ __global__ __launch_bounds__(64 * WAVES_M * WAVES_N) void gated_weight_gradient_
     typename P::FirstPanel in;
     typename P::SecondPanel d;
     in.init(a.x_stride);
-    const uint32_t stride = 2 * a.Fp * static_cast<uint32_t>(sizeof(T));
+    const uint32_t stride = dgu_stride<T>(a);
     d.init(stride);
     const char* x = static_cast<const char*>(a.x) + c0 * static_cast<int64_t>(sizeof(T));
     const char* dgu = static_cast<const char*>(a.dgu) + (static_cast<int64_t>(side) * a.Fp + f_first) * static_cast<int64_t>(sizeof(T));
@@ -232,13 +359,10 @@ __global__ __launch_bounds__(64 * WAVES_M * WAVES_N) void gated_weight_gradient_
         d.load(s, dgu + at * stride, stride, left, left_f, wave);
     });
     const float by = __is_same(T, f16) && a.scale ? a.scale[1] : 1.f;
-#pragma unroll
-    for (int i = 0; i < P::MT; ++i) {
-        const int f = f_first + P::row(i), row = f < a.F ? f : a.F - 1;
-#pragma unroll
-        for (int b = 0; b < P::NB; ++b)
-            store_block<T>(out + static_cast<int64_t>(row) * a.K, c0 + P::column(b), f < a.F ? a.K : 0, p.acc[i][b] * by);
-    }
+    const int64_t f = f_first + P::wave_m() * P::WM, c = c0 + P::column(0);
+    __syncthreads();  // the panels' place is free
+    store_tile<T, P::WM, P::WN>(P::stage(f0, s0, f1, s1), out + f * a.K + c, a.K, a.F - f, a.K - c,
+                                [&](int i, int b) { return p.acc[i][b] * by; });
 }
 
 // ---------------------------------------------------------------------------
@@ -335,9 +459,11 @@ __global__ __launch_bounds__(256) void gated_rows_kernel(GatedArgs a) {
         for (int w = 0; w < 4; ++w) g += meet[w][i][j][0][l], u += meet[w][i][j][1][l];
         if (m >= rows || f >= a.F) continue;
         T* out = static_cast<T*>(a.h) + static_cast<int64_t>(m) * a.F + f;
+        f32x4 h, slope;
+        activate<4>(a.activation, g, h, slope);
 #pragma unroll
         for (int e = 0; e < 4; ++e)
-            if (f + e < a.F) out[e] = from_acc<T>(activate(a.activation, g[e]).x * u[e]);
+            if (f + e < a.F) out[e] = from_acc<T>(h[e] * u[e]);
     }
 }
 

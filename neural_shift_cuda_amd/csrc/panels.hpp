@@ -193,6 +193,17 @@ struct Product {
         settle<T>();
     }
 
+    // A place of the wave's own in the panels, 32 rows of its tile in fp32 at the most.
+    static __device__ __forceinline__ char* stage(char (&f0)[FIRST_BYTES], char (&s0)[SECOND_BYTES], char (&f1)[FIRST_BYTES],
+                                                  char (&s1)[SECOND_BYTES]) {
+        constexpr int BYTES = 32 * WN * 4, IN_F = FIRST_BYTES / BYTES, IN_S = SECOND_BYTES / BYTES;
+        static_assert(2 * (IN_F + IN_S) >= NT / 64, "a place for every wave");
+        const int w = wave_id();
+        return w < IN_F ? f0 + w * BYTES
+               : w < 2 * IN_F ? f1 + (w - IN_F) * BYTES
+               : w < 2 * IN_F + IN_S ? s0 + (w - 2 * IN_F) * BYTES : s1 + (w - 2 * IN_F - IN_S) * BYTES;
+    }
+
     // Every wave's loads have landed, and every wave has read what it needs of the
     // panel before.
     static __device__ __forceinline__ void landed() {
@@ -215,38 +226,94 @@ struct TileOrder {
     }
 };
 
-// The lane's values of 32 columns from `c` on (the first of them the block's), rounded
-// to T, to its row of n columns.
-template <typename T>
-__device__ __forceinline__ void store_block(T* row, int64_t c, int64_t n, const f32x16& v) {
-    const int g = (threadIdx.x >> 5) & 1;
-    if constexpr (sizeof(T) == 4) {
+// Lanes that wrote to LDS and read what others of their wave wrote.
+__device__ __forceinline__ void wave_exchange() {
+    __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+    __builtin_amdgcn_wave_barrier();
+}
+
+// ROWS x COLS of a wave in LDS, between the products' order (a lane: row l % 32 of 32, and
+// of 32 columns four times four) and rows of memory, 16 bytes a lane and as much of a row
+// side by side as there is: stored from the products' order, 32 rows are 32 pieces of 32
+// bytes.  The chunks of a row are permuted so that no bank is asked twice either way.
+template <typename T, int ROWS, int COLS>
+struct Stage {
+    static constexpr int CHUNKS = COLS * sizeof(T) / 16, ROW = CHUNKS * 16, BYTES = ROWS * ROW;
+    static constexpr int PER = CHUNKS < 16 ? 16 / CHUNKS : 1;  // rows that share 256 bytes
+    static constexpr int TURNS = ROWS * CHUNKS / 64;
+    static_assert(TURNS * 64 == ROWS * CHUNKS && CHUNKS >= 4, "whole instructions");
+
+    static __device__ __forceinline__ int at(int row, int chunk) {
+        return row * ROW + ((chunk ^ (row / PER % (CHUNKS < 16 ? CHUNKS : 16))) * 16);
+    }
+    // Block (i, b) of 32 x 32.
+    static __device__ __forceinline__ void put(char* lds, int i, int b, const f32x16& v) {
+        const int l = threadIdx.x & 63, row = i * 32 + (l & 31);
 #pragma unroll
         for (int q = 0; q < 4; ++q) {
-            const int64_t at = c + 8 * q + 4 * g;
-            if (at < n)
-                store_bits(row + at, 0, static_cast<int>(min(n - at, int64_t(4))),
-                           __builtin_bit_cast(ux4, (f32x4{v[4 * q], v[4 * q + 1], v[4 * q + 2], v[4 * q + 3]})));
+            const f32x4 x = {v[4 * q], v[4 * q + 1], v[4 * q + 2], v[4 * q + 3]};
+            if constexpr (sizeof(T) == 4)
+                *reinterpret_cast<f32x4*>(lds + at(row, b * 8 + 2 * q + (l >> 5))) = x;
+            else
+                store4<T>(reinterpret_cast<T*>(lds + at(row, b * 4 + q) + (l >> 5) * 8), x);
         }
-    } else {
-        // a lane half has four columns of each eight: halves exchange, eight a lane
-        typedef uint32_t ux2 __attribute__((ext_vector_type(2)));
+    }
+    static __device__ __forceinline__ f32x16 get(const char* lds, int i, int b) {
+        const int l = threadIdx.x & 63, row = i * 32 + (l & 31);
+        f32x16 v;
 #pragma unroll
-        for (int q = 0; q < 4; q += 2) {
-            ux2 p[2];
+        for (int q = 0; q < 4; ++q) {
+            if constexpr (sizeof(T) == 4) {
+                const f32x4 x = *reinterpret_cast<const f32x4*>(lds + at(row, b * 8 + 2 * q + (l >> 5)));
 #pragma unroll
-            for (int e = 0; e < 2; ++e) {
-                const f32x4 x = {v[4 * (q + e)], v[4 * (q + e) + 1], v[4 * (q + e) + 2], v[4 * (q + e) + 3]};
-                if constexpr (__is_same(T, f16))
-                    p[e] = __builtin_bit_cast(ux2, __builtin_convertvector(x, f16x4));
-                else
-                    p[e] = __builtin_bit_cast(ux2, __builtin_convertvector(x, bf16x4));
+                for (int e = 0; e < 4; ++e) v[4 * q + e] = x[e];
+            } else {
+                float x[4];
+                load_acc<T, 4>(reinterpret_cast<const T*>(lds + at(row, b * 4 + q) + (l >> 5) * 8), x);
+#pragma unroll
+                for (int e = 0; e < 4; ++e) v[4 * q + e] = x[e];
             }
-            const auto a = __builtin_amdgcn_permlane32_swap(p[0][0], p[1][0], false, false);
-            const auto b = __builtin_amdgcn_permlane32_swap(p[0][1], p[1][1], false, false);
-            const int64_t at = c + 8 * q + 8 * g;
-            if (at < n) store_bits(row + at, 0, static_cast<int>(min(n - at, int64_t(8))), ux4{a[0], b[0], a[1], b[1]});
         }
+        return v;
+    }
+    // To and from memory: `rows` rows of `cols` columns (more than there are, or none).
+    static __device__ __forceinline__ void store(const char* lds, T* to, int64_t stride, int64_t rows, int64_t cols) {
+        const int l = threadIdx.x & 63, n = static_cast<int>(min(cols, int64_t(COLS)));
+#pragma unroll
+        for (int t = 0; t < TURNS; ++t) {
+            const int x = t * 64 + l, row = x / CHUNKS, chunk = x % CHUNKS;
+            const ux4 v = *reinterpret_cast<const ux4*>(lds + at(row, chunk));
+            if (row < rows) store_bits(to + row * stride, chunk * kVec<T>, n, v);
+        }
+    }
+    static __device__ __forceinline__ void load(char* lds, const T* from, int64_t stride, int64_t rows, int64_t cols) {
+        const int l = threadIdx.x & 63, n = static_cast<int>(min(cols, int64_t(COLS)));
+        ux4 v[TURNS];
+#pragma unroll
+        for (int t = 0; t < TURNS; ++t) {
+            const int x = t * 64 + l, row = x / CHUNKS;
+            v[t] = ux4{0, 0, 0, 0};
+            if (row < rows) v[t] = load_bits(from + row * stride, x % CHUNKS * kVec<T>, n);
+        }
+#pragma unroll
+        for (int t = 0; t < TURNS; ++t) {
+            const int x = t * 64 + l;
+            *reinterpret_cast<ux4*>(lds + at(x / CHUNKS, x % CHUNKS)) = v[t];
+        }
+    }
+};
+
+// A wave's tile to memory, 32 rows of it at a time through LDS (Stage<T, 32, COLS>'s bytes).
+template <typename T, int ROWS, int COLS, typename Value>
+__device__ __forceinline__ void store_tile(char* lds, T* to, int64_t stride, int64_t rows, int64_t cols, const Value& value) {
+    using S = Stage<T, 32, COLS>;
+#pragma unroll
+    for (int i = 0; i < ROWS / 32; ++i) {
+#pragma unroll
+        for (int b = 0; b < COLS / 32; ++b) S::put(lds, 0, b, value(i, b));
+        wave_exchange();
+        S::store(lds, to + i * 32 * stride, stride, rows - i * 32, cols);
+        wave_exchange();
     }
 }
 

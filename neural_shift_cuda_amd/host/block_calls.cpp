@@ -151,7 +151,7 @@ std::tuple<Tensor, Tensor> gated_forward(const Tensor& x0, const Tensor& gate0, 
     if (!h.numel()) return {h, kept};
     if (!x.size(1)) return {h.zero_(), kept};  // act(0) * 0
     if (keep) kept = scratch(x, nsh_gated_linear_kept_bytes(&a));
-    a.h = address(h), a.kept = address<float>(kept);
+    a.h = address(h), a.kept = address(kept);
     a.workspace_bytes = nsh_gated_linear_workspace_bytes(&a, 0);
     const Tensor ws = scratch(x, a.workspace_bytes);
     a.workspace = address(ws);
@@ -184,7 +184,7 @@ struct GatedNode : torch::autograd::Function<GatedNode> {
                     if (g.defined()) g.zero_();
             } else if (grads[0].defined() || grads[1].defined() || grads[2].defined()) {
                 nsh_gated_linear_args a = gated_args(x, gate, up, ctx->saved_data["activation"].toInt());
-                a.kept = address<float>(kept);
+                a.kept = address(kept);
                 a.grad_h = address(gh), a.gh_stride = step(gh);
                 a.grad_x = address(grads[0]), a.grad_gate = address(grads[1]), a.grad_up = address(grads[2]);
                 a.workspace_bytes = nsh_gated_linear_workspace_bytes(&a, 1);
