@@ -231,9 +231,9 @@ __device__ __forceinline__ uint32_t dgu_stride(const GatedArgs& a) {
     return 2 * a.Fp * static_cast<uint32_t>(sizeof(T)) + 128;
 }
 
-template <typename T, int BM, int BN, int WAVES_M, int WAVES_N>
-__global__ __launch_bounds__(64 * WAVES_M * WAVES_N) void gated_forward_kernel(GatedArgs a) {
-    using P = Product<T, BM, BN, WAVES_M, WAVES_N, kAlong, kAlong, true>;
+template <typename T, int BM, int BN, int WAVES_M, int WAVES_N, int KB>
+__global__ __launch_bounds__(64 * WAVES_M * WAVES_N, 2) void gated_forward_kernel(GatedArgs a) {
+    using P = Product<T, BM, BN, WAVES_M, WAVES_N, KB, kAlong, kAlong, true>;
     __shared__ __attribute__((aligned(1024))) char f0[P::FIRST_BYTES], s0[P::SECOND_BYTES];
     __shared__ __attribute__((aligned(1024))) char f1[P::FIRST_BYTES], s1[P::SECOND_BYTES];
     const TileOrder t(blockIdx.x, gridDim.x, a.tiles_m, a.tiles_n, 8);
@@ -251,11 +251,13 @@ __global__ __launch_bounds__(64 * WAVES_M * WAVES_N) void gated_forward_kernel(G
     const int left_m = static_cast<int>(min(a.rows - m0, int64_t(BM)));
     P p;
     p.init();
-    p.run((a.Kp + P::BK - 1) / P::BK, f0, s0, f1, s1, [&](int i, char* f, char* s) {
-        const int64_t at = static_cast<int64_t>(i) * 128;
-        gate.load(f, wg + at, a.wg_stride, a.F - c0, wide - at, wave);
-        up.load(f + P::FIRST_BYTES / 2, wu + at, a.wu_stride, a.F - c0, wide - at, wave);
-        rows.load(s, x + at, a.x_stride, left_m, wide - at, wave);
+    const int n = (a.Kp + P::BK - 1) / P::BK;
+    p.run(n, f0, s0, f1, s1, [&](int i, char* f, char* s) {
+        const int64_t at = static_cast<int64_t>(i) * KB;
+        const int left_f = i < n ? a.F - c0 : 0;
+        gate.load(f, wg + at, a.wg_stride, left_f, wide - at, wave);
+        up.load(f + P::FIRST_BYTES / 2, wu + at, a.wu_stride, left_f, wide - at, wave);
+        rows.load(s, x + at, a.x_stride, i < n ? left_m : 0, wide - at, wave);
     });
     float most = 0.f;
     const int64_t m = m0 + P::wave_m() * P::WM;
@@ -281,14 +283,14 @@ __global__ __launch_bounds__(64 * WAVES_M * WAVES_N) void gated_forward_kernel(G
 }
 
 // dx: over the hidden columns of dg, then of du.
-template <typename T, int BM, int BN, int WAVES_M, int WAVES_N>
-__global__ __launch_bounds__(64 * WAVES_M * WAVES_N) void gated_input_gradient_kernel(GatedArgs a) {
-    using P = Product<T, BM, BN, WAVES_M, WAVES_N, kAcross, kAlong, false>;
+template <typename T, int BM, int BN, int WAVES_M, int WAVES_N, int KB>
+__global__ __launch_bounds__(64 * WAVES_M * WAVES_N, 2) void gated_input_gradient_kernel(GatedArgs a) {
+    using P = Product<T, BM, BN, WAVES_M, WAVES_N, KB, kAcross, kAlong, false>;
     __shared__ __attribute__((aligned(1024))) char f0[P::FIRST_BYTES], s0[P::SECOND_BYTES];
     __shared__ __attribute__((aligned(1024))) char f1[P::FIRST_BYTES], s1[P::SECOND_BYTES];
-    const int64_t tiles = static_cast<int64_t>(a.tiles_m) * a.tiles_n;
-    const int split = static_cast<int>(blockIdx.x / tiles);
-    const TileOrder t(blockIdx.x % tiles, tiles, a.tiles_m, a.tiles_n, 8);
+    const uint32_t tiles = static_cast<uint32_t>(a.tiles_m) * a.tiles_n;
+    const int split = TileOrder::uniform(blockIdx.x / tiles);
+    const TileOrder t(blockIdx.x - split * tiles, tiles, a.tiles_m, a.tiles_n, 8);
     const int64_t m0 = static_cast<int64_t>(t.m) * BM;
     const int64_t c0 = static_cast<int64_t>(t.n) * BN;
     const int wave = wave_id();
@@ -304,17 +306,17 @@ __global__ __launch_bounds__(64 * WAVES_M * WAVES_N) void gated_input_gradient_k
     const int left_m = static_cast<int>(min(a.rows - m0, int64_t(BM)));
     const int64_t left_c = (a.Kp - c0) * static_cast<int64_t>(sizeof(T));
     const int half = a.Fp / P::BK, all = 2 * half;
-    const int begin = static_cast<int>(static_cast<int64_t>(all) * split / a.splits);
-    const int end = static_cast<int>(static_cast<int64_t>(all) * (split + 1) / a.splits);
+    const int begin = TileOrder::uniform(all * static_cast<uint32_t>(split) / a.splits);
+    const int end = TileOrder::uniform(all * static_cast<uint32_t>(split + 1) / a.splits);
     P p;
     p.init();
     p.run(end - begin, f0, s0, f1, s1, [&](int i, char* f, char* s) {
         const int at = begin + i, in = at < half ? at : at - half;
-        if (at < half)
-            gate.load(f, wg + static_cast<int64_t>(in) * P::BK * a.wg_stride, a.wg_stride, a.F - in * P::BK, left_c, wave);
-        else
-            up.load(f, wu + static_cast<int64_t>(in) * P::BK * a.wu_stride, a.wu_stride, a.F - in * P::BK, left_c, wave);
-        rows.load(s, d + static_cast<int64_t>(at) * 128, stride, left_m, 128, wave);
+        const bool one = at < half;
+        const uint32_t step = one ? a.wg_stride : a.wu_stride;
+        P::FirstPanel::either(one, gate, up).load(f, (one ? wg : wu) + static_cast<int64_t>(in) * P::BK * step, step,
+                                                  at < end ? a.F - in * P::BK : 0, left_c, wave);
+        rows.load(s, d + static_cast<int64_t>(at) * KB, stride, at < end ? left_m : 0, KB, wave);
     });
     const float by = __is_same(T, f16) && a.scale ? a.scale[1] : 1.f;
     const int64_t m = m0 + P::wave_m() * P::WM, c = c0 + P::column(0);
@@ -328,9 +330,9 @@ __global__ __launch_bounds__(64 * WAVES_M * WAVES_N) void gated_input_gradient_k
 }
 
 // Both weights' gradients: tiles of hidden rows of the one, then of the other.
-template <typename T, int BM, int BN, int WAVES_M, int WAVES_N>
-__global__ __launch_bounds__(64 * WAVES_M * WAVES_N) void gated_weight_gradient_kernel(GatedArgs a) {
-    using P = Product<T, BM, BN, WAVES_M, WAVES_N, kAcross, kAcross, false>;
+template <typename T, int BM, int BN, int WAVES_M, int WAVES_N, int KB>
+__global__ __launch_bounds__(64 * WAVES_M * WAVES_N, 2) void gated_weight_gradient_kernel(GatedArgs a) {
+    using P = Product<T, BM, BN, WAVES_M, WAVES_N, KB, kAcross, kAcross, false>;
     __shared__ __attribute__((aligned(1024))) char f0[P::FIRST_BYTES], s0[P::SECOND_BYTES];
     __shared__ __attribute__((aligned(1024))) char f1[P::FIRST_BYTES], s1[P::SECOND_BYTES];
     const int each = a.tiles_m / 2;
@@ -354,7 +356,7 @@ __global__ __launch_bounds__(64 * WAVES_M * WAVES_N) void gated_weight_gradient_
     p.init();
     p.run(static_cast<int>((a.rows + P::BK - 1) / P::BK), f0, s0, f1, s1, [&](int i, char* f, char* s) {
         const int64_t at = static_cast<int64_t>(i) * P::BK;
-        const int left = static_cast<int>(min(a.rows - at, int64_t(P::BK)));
+        const int left = static_cast<int>(max(min(a.rows - at, int64_t(P::BK)), int64_t(0)));
         in.load(f, x + at * a.x_stride, a.x_stride, left, left_c, wave);
         d.load(s, dgu + at * stride, stride, left, left_f, wave);
     });
@@ -510,9 +512,9 @@ int gated_forward(GatedArgs a, hipStream_t st) {
     a.tiles_m = c.tiles_m, a.tiles_n = c.tiles_n;
     const unsigned grid = static_cast<unsigned>(c.tiles());
     if constexpr (sizeof(T) == 2)
-        if (c.bm == 256) gated_forward_kernel<T, 256, 256, 4, 2><<<grid, 512, 0, st>>>(a);
-    if (c.bm == 128) gated_forward_kernel<T, 128, 128, 2, 2><<<grid, 256, 0, st>>>(a);
-    if (c.bm == 64) gated_forward_kernel<T, 64, 128, 2, 2><<<grid, 256, 0, st>>>(a);
+        if (c.bm == 256) gated_forward_kernel<T, 256, 256, 4, 2, 128><<<grid, 512, 0, st>>>(a);
+    if (c.bm == 128) gated_forward_kernel<T, 128, 128, 2, 2, 128><<<grid, 256, 0, st>>>(a);
+    if (c.bm == 64) gated_forward_kernel<T, 64, 128, 2, 2, 128><<<grid, 256, 0, st>>>(a);
     return nsh_host::check_launch("gated_linear_forward");
 }
 
@@ -521,9 +523,9 @@ int gated_input_gradient(GatedArgs a, const Cut& c, hipStream_t st) {
     a.tiles_m = c.tiles_m, a.tiles_n = c.tiles_n;
     const unsigned grid = static_cast<unsigned>(c.tiles() * a.splits);
     if constexpr (sizeof(T) == 2)
-        if (c.bm == 256) gated_input_gradient_kernel<T, 256, 256, 4, 2><<<grid, 512, 0, st>>>(a);
-    if (c.bm == 128) gated_input_gradient_kernel<T, 128, 128, 2, 2><<<grid, 256, 0, st>>>(a);
-    if (c.bm == 64) gated_input_gradient_kernel<T, 64, 128, 2, 2><<<grid, 256, 0, st>>>(a);
+        if (c.bm == 256) gated_input_gradient_kernel<T, 256, 256, 4, 2, 128><<<grid, 512, 0, st>>>(a);
+    if (c.bm == 128) gated_input_gradient_kernel<T, 128, 128, 2, 2, 128><<<grid, 256, 0, st>>>(a);
+    if (c.bm == 64) gated_input_gradient_kernel<T, 64, 128, 2, 2, 128><<<grid, 256, 0, st>>>(a);
     return nsh_host::check_launch("gated_linear_backward");
 }
 
@@ -533,9 +535,9 @@ int gated_weight_gradient(GatedArgs a, hipStream_t st) {
     a.tiles_m = c.tiles_m, a.tiles_n = c.tiles_n;
     const unsigned grid = static_cast<unsigned>(c.tiles());
     if constexpr (sizeof(T) == 2)
-        if (c.bm == 256) gated_weight_gradient_kernel<T, 256, 256, 4, 2><<<grid, 512, 0, st>>>(a);
-    if (c.bm == 128) gated_weight_gradient_kernel<T, 128, 128, 2, 2><<<grid, 256, 0, st>>>(a);
-    if (c.bm == 64) gated_weight_gradient_kernel<T, 64, 128, 2, 2><<<grid, 256, 0, st>>>(a);
+        if (c.bm == 256) gated_weight_gradient_kernel<T, 256, 256, 4, 2, 128><<<grid, 512, 0, st>>>(a);
+    if (c.bm == 128) gated_weight_gradient_kernel<T, 128, 128, 2, 2, 128><<<grid, 256, 0, st>>>(a);
+    if (c.bm == 64) gated_weight_gradient_kernel<T, 64, 128, 2, 2, 128><<<grid, 256, 0, st>>>(a);
     return nsh_host::check_launch("gated_linear_backward");
 }
 

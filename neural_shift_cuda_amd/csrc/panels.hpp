@@ -3,7 +3,7 @@
 //
 //   out[m][n] = sum_k second[m][k] first[n][k]
 //
-// A workgroup owns BM x BN of the result.  Of both matrices it takes 128 bytes of the
+// A workgroup owns BM x BN of the result.  Of both matrices it takes KB bytes of the
 // contraction at a time (BK elements) straight from memory to LDS, two panels ahead
 // of each other: with the contraction running along the rows (`kAlong`, one LDS row
 // for each row of the result) or across them (`kAcross`, one LDS row for each
@@ -29,6 +29,7 @@ template <typename T, int DP, Run RUN>
 struct Operand {
     using L = Tile<T, DP>;
     using V = typename Eight<T>::V;
+    static constexpr int READS = RUN == kAlong ? sizeof(T) / 2 : sizeof(T) == 2 ? 2 : 8;  // instructions of a read()
 
     // first: the wave's first row (or column) of the panel, a multiple of 32 (of
     // the wave's own width, if across)
@@ -84,30 +85,32 @@ struct Panel {
             off[i] = static_cast<uint32_t>(r) * stride + ((x % L::NC) ^ L::turn(r)) * 16;
         }
     }
-    // from: the panel's first row; rows: how many are left, from there; left: bytes
-    // left of a row
+    static __device__ __forceinline__ Panel either(bool first, const Panel& a, const Panel& b) {
+        Panel p;
+        p.chunk = a.chunk;
+#pragma unroll
+        for (int i = 0; i < NI; ++i) p.off[i] = first ? a.off[i] : b.off[i];
+        return p;
+    }
+    // from: the panel's first row; rows: how many are left, from there (none: nothing is
+    // read); left: bytes left of a row
     __device__ __forceinline__ void load(char* lds, const char* from, uint32_t stride, int rows, int64_t left, int wave) const {
         const uint32_t n = static_cast<uint32_t>(max(min(rows, ROWS), 0));
-        const uint32_t last = static_cast<uint32_t>(left < DP * static_cast<int>(sizeof(T)) ? left : DP * sizeof(T));
+        const uint32_t last = static_cast<uint32_t>(min(left, static_cast<int64_t>(DP * sizeof(T))));
         const __amdgpu_buffer_rsrc_t rs = __builtin_amdgcn_make_buffer_rsrc(
             const_cast<char*>(from), static_cast<short>(0), static_cast<int>(n ? (n - 1) * stride + last : 0u), 0x00020000);
-        if (RUN == kAlong && left < DP * static_cast<int>(sizeof(T))) {
-            const bool past = chunk >= static_cast<int>(left);
+        const bool past = RUN == kAlong && chunk >= static_cast<int>(last);
 #pragma unroll
-            for (int i = 0; i < NI; ++i) to_lds<16>(rs, lds + (i * (NT / 64) + wave) * 1024, past ? 0x80000000u : off[i]);
-        } else {
-#pragma unroll
-            for (int i = 0; i < NI; ++i) to_lds<16>(rs, lds + (i * (NT / 64) + wave) * 1024, off[i]);
-        }
+        for (int i = 0; i < NI; ++i) to_lds<16>(rs, lds + (i * (NT / 64) + wave) * 1024, past ? 0x80000000u : off[i]);
     }
 };
 
 // PAIRED: the wave's columns come in equal parts from the two halves of BN.
-template <typename T_, int BM_, int BN_, int WAVES_M, int WAVES_N, Run FIRST, Run SECOND, bool PAIRED_>
+template <typename T_, int BM_, int BN_, int WAVES_M, int WAVES_N, int KB_, Run FIRST, Run SECOND, bool PAIRED_>
 struct Product {
     using T = T_;
     using V = typename Eight<T>::V;
-    static constexpr int BM = BM_, BN = BN_, BK = 128 / sizeof(T), STEPS = BK / 16;
+    static constexpr int BM = BM_, BN = BN_, KB = KB_, BK = KB / sizeof(T), STEPS = BK / 16;
     static constexpr int NT = 64 * WAVES_M * WAVES_N, WM = BM / WAVES_M, WN = BN / WAVES_N;
     static constexpr int MT = WM / 32, NB = WN / 32;
     static constexpr bool PAIRED = PAIRED_;
@@ -115,7 +118,7 @@ struct Product {
     using Second = Operand<T, SECOND == kAlong ? BK : BM, SECOND>;
     using FirstPanel = Panel<T, FIRST == kAlong ? (PAIRED ? BN / 2 : BN) : BK, FIRST == kAlong ? BK : BN, NT, FIRST>;
     using SecondPanel = Panel<T, SECOND == kAlong ? BM : BK, SECOND == kAlong ? BK : BM, NT, SECOND>;
-    static constexpr int FIRST_BYTES = BN * 128, SECOND_BYTES = BM * 128;
+    static constexpr int FIRST_BYTES = BN * KB, SECOND_BYTES = BM * KB;
     static_assert(STEPS % 2 == 0 && (!PAIRED || (FIRST == kAlong && NB % 2 == 0)), "");
 
     f32x16 acc[MT][NB];
@@ -147,43 +150,54 @@ struct Product {
 #pragma unroll
         for (int i = 0; i < MT; ++i) x.s[i] = Second::read(second, by_second, i * 32, s);
     }
+    template <int FROM, int TO>
     __device__ __forceinline__ void multiply(const Step& x) {
 #pragma unroll
-        for (int i = 0; i < MT; ++i)
+        for (int i = FROM; i < TO; ++i)
 #pragma unroll
             for (int b = 0; b < NB; ++b) acc[i][b] = Eight<T>::mma(x.f[b], x.s[i], acc[i][b]);
+    }
+
+    // The region's products with reads between them: a product issues in 4 cycles and
+    // takes 32, and what stands in front of a run of them keeps it waiting.
+    template <int ALL, int READS>
+    static __device__ __forceinline__ void mix() {
+#pragma unroll
+        for (int i = 0; i < ALL; ++i) {
+            __builtin_amdgcn_sched_group_barrier(0x008, 1, 0);
+            constexpr int R = (READS + ALL - 1) / ALL;
+            if (i * R < READS) __builtin_amdgcn_sched_group_barrier(0x100, R, 0);
+        }
+        order();
     }
 
     // All n panels (n >= 1); load(i, first, second) asks for panel i.
     template <typename Load>
     __device__ __forceinline__ void run(int n, char (&f0)[FIRST_BYTES], char (&s0)[SECOND_BYTES], char (&f1)[FIRST_BYTES],
                                         char (&s1)[SECOND_BYTES], const Load& load) {
+        constexpr int READS = NB * First::READS + MT * Second::READS;
+        constexpr int ROW = NB * (sizeof(T) == 4 ? 8 : 1);  // products of 32 rows
         Step x, y;
         load(0, f0, s0);
         landed();
         if (n > 1) load(1, f1, s1);
         read(x, f0, s0, 0);
+        order();
         auto panel = [&](int i, char (&f)[FIRST_BYTES], char (&s)[SECOND_BYTES], char (&fn)[FIRST_BYTES], char (&sn)[SECOND_BYTES]) {
 #pragma unroll
-            for (int st = 0; st + 2 < STEPS; st += 2) {
-                read(y, f, s, st + 1);
-                order();
-                multiply(x);
-                order();
-                read(x, f, s, st + 2);
-                order();
-                multiply(y);
-                order();
+            for (int st = 0; st + 1 < STEPS; ++st) {
+                read(st % 2 ? x : y, f, s, st + 1);
+                multiply<0, MT>(st % 2 ? y : x);
+                mix<MT * ROW, READS>();
             }
-            read(y, f, s, STEPS - 1);
-            order();
-            multiply(x);
-            order();
             landed();
-            if (i + 2 < n) load(i + 2, f, s);
-            if (i + 1 < n) read(x, fn, sn, 0);
             order();
-            multiply(y);
+            read(x, fn, sn, 0);  // (behind the last panel nothing that is used)
+            multiply<0, (MT + 1) / 2>(y);
+            mix<(MT + 1) / 2 * ROW, READS>();
+            if (i + 2 < n) load(i + 2, f, s);
+            order();
+            multiply<(MT + 1) / 2, MT>(y);
             order();
         };
         for (int i = 0; i < n; i += 2) {
@@ -193,10 +207,10 @@ struct Product {
         settle<T>();
     }
 
-    // A place of the wave's own in the panels, 32 rows of its tile in fp32 at the most.
+    // A place of the wave's own in the panels, for 32 x 64 in fp32.
     static __device__ __forceinline__ char* stage(char (&f0)[FIRST_BYTES], char (&s0)[SECOND_BYTES], char (&f1)[FIRST_BYTES],
                                                   char (&s1)[SECOND_BYTES]) {
-        constexpr int BYTES = 32 * WN * 4, IN_F = FIRST_BYTES / BYTES, IN_S = SECOND_BYTES / BYTES;
+        constexpr int BYTES = 32 * 64 * 4, IN_F = FIRST_BYTES / BYTES, IN_S = SECOND_BYTES / BYTES;
         static_assert(2 * (IN_F + IN_S) >= NT / 64, "a place for every wave");
         const int w = wave_id();
         return w < IN_F ? f0 + w * BYTES
@@ -216,14 +230,16 @@ struct Product {
 // tiles advance together, so that its L2 serves both matrices.
 struct TileOrder {
     int m, n;
-    __device__ __forceinline__ TileOrder(int64_t id, int64_t count, int tiles_m, int tiles_n, int rows) {
-        const int64_t t = xcd_tile(id, count);
-        const int64_t band = static_cast<int64_t>(rows) * tiles_n;
-        const int first = static_cast<int>(t / band) * rows, deep = min(tiles_m - first, rows);
-        const int in = static_cast<int>(t % band);
-        m = first + in % deep;
-        n = in / deep;
+    __device__ __forceinline__ TileOrder(uint32_t id, uint32_t count, int tiles_m, int tiles_n, int rows) {
+        const uint32_t xcd = id % kXcds, local = id / kXcds, per = count / kXcds, rem = count % kXcds;
+        const uint32_t t = xcd * per + min(xcd, rem) + local, band = static_cast<uint32_t>(rows) * tiles_n;
+        const uint32_t group = t / band, in = t - group * band;
+        const uint32_t first = group * rows, deep = min(static_cast<uint32_t>(tiles_m) - first, static_cast<uint32_t>(rows));
+        n = uniform(in / deep);
+        m = uniform(first + in % deep);
     }
+    // (divisions come out of vector registers, and a load's buffer has to be in scalar ones)
+    static __device__ __forceinline__ int uniform(uint32_t v) { return __builtin_amdgcn_readfirstlane(v); }
 };
 
 // Lanes that wrote to LDS and read what others of their wave wrote.
@@ -303,18 +319,21 @@ struct Stage {
     }
 };
 
-// A wave's tile to memory, 32 rows of it at a time through LDS (Stage<T, 32, COLS>'s bytes).
+// A wave's tile to memory, 32 rows and 64 columns of it at a time through LDS.
 template <typename T, int ROWS, int COLS, typename Value>
 __device__ __forceinline__ void store_tile(char* lds, T* to, int64_t stride, int64_t rows, int64_t cols, const Value& value) {
-    using S = Stage<T, 32, COLS>;
+    constexpr int PART = COLS < 64 ? COLS : 64;
+    using S = Stage<T, 32, PART>;
 #pragma unroll
-    for (int i = 0; i < ROWS / 32; ++i) {
+    for (int i = 0; i < ROWS / 32; ++i)
 #pragma unroll
-        for (int b = 0; b < COLS / 32; ++b) S::put(lds, 0, b, value(i, b));
-        wave_exchange();
-        S::store(lds, to + i * 32 * stride, stride, rows - i * 32, cols);
-        wave_exchange();
-    }
+        for (int c = 0; c < COLS; c += PART) {
+#pragma unroll
+            for (int b = 0; b < PART / 32; ++b) S::put(lds, 0, b, value(i, c / 32 + b));
+            wave_exchange();
+            S::store(lds, to + i * 32 * stride + c, stride, rows - i * 32, cols - c);
+            wave_exchange();
+        }
 }
 
 }  // namespace nsh
