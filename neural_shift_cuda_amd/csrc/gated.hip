@@ -86,7 +86,7 @@ __global__ __launch_bounds__(kPassThreads) void gated_slope_kernel(SlopeArgs a) 
 // mean loss are.  dg and du are multiplied by a power of two, of the largest dh and the
 // largest factor, that brings them just under 2^15 and that the sums are divided by: what is
 // rounded off is then below 2^-39 of the largest wherever it is not half a step.
-constexpr int kMostBlocks = 512;
+constexpr int kMostBlocks = 2048;
 
 __device__ __forceinline__ float workgroup_max(float v, float* lds) {
     lds[threadIdx.x] = v;
@@ -100,19 +100,31 @@ __device__ __forceinline__ float workgroup_max(float v, float* lds) {
     return r;
 }
 
-__global__ __launch_bounds__(kPassThreads) void gated_most_kernel(const f16* gh, int64_t stride, int64_t rows, int F,
+// Over rows of n, four parts of 16 bytes a lane at once.
+__global__ __launch_bounds__(kPassThreads) void gated_most_kernel(const f16* gh, int64_t stride, int64_t rows, int64_t n,
                                                                   float* out) {
+    constexpr int kParts = 4;
     __shared__ float lds[kPassThreads];
     float most = 0.f;
-    for (int64_t row = blockIdx.x; row < rows; row += gridDim.x)
-        for (int c = threadIdx.x * 8; c < F; c += kPassThreads * 8) {
-            float d[8];
-            unpack<f16>(load_bits(gh + row * stride, c, F), d);
+    for (int64_t row = blockIdx.y; row < rows; row += gridDim.y)
+        for (int64_t c = static_cast<int64_t>(blockIdx.x) * (kPassThreads * 8 * kParts) + threadIdx.x * 8; c < n;
+             c += static_cast<int64_t>(gridDim.x) * (kPassThreads * 8 * kParts)) {
+            ux4 v[kParts];
 #pragma unroll
-            for (int e = 0; e < 8; ++e) most = fmaxf(most, fabsf(d[e]) < INFINITY ? fabsf(d[e]) : 0.f);
+            for (int i = 0; i < kParts; ++i) {
+                const int64_t at = c + i * kPassThreads * 8;
+                v[i] = load_bits(gh + row * stride + (at < n ? at : 0), 0, static_cast<int>(max(min(n - at, int64_t(8)), int64_t(0))));
+            }
+#pragma unroll
+            for (int i = 0; i < kParts; ++i) {
+                float d[8];
+                unpack<f16>(v[i], d);
+#pragma unroll
+                for (int e = 0; e < 8; ++e) most = fmaxf(most, fabsf(d[e]) < INFINITY ? fabsf(d[e]) : 0.f);
+            }
         }
     most = workgroup_max(most, lds);
-    if (threadIdx.x == 0) out[blockIdx.x] = most;
+    if (threadIdx.x == 0) out[blockIdx.y * gridDim.x + blockIdx.x] = most;
 }
 
 __global__ __launch_bounds__(kPassThreads) void gated_scale_kernel(const float* gh, int n, const float* kept, int nk,
@@ -135,13 +147,51 @@ __global__ __launch_bounds__(kPassThreads) void gated_scale_kernel(const float* 
     scale[1] = ldexpf(1.f, -e);
 }
 
+// The workgroups' sums, in order, four places of a row a lane, all of them asked for before
+// the first is waited for.
+template <typename T, int SPLITS>
+__global__ __launch_bounds__(kPassThreads) void gated_join_kernel(const float* part, int64_t rows, int K, int Kq, T* out) {
+    const int c = (blockIdx.x * kPassThreads + threadIdx.x) * 4;
+    if (c >= K) return;
+    for (int64_t m = blockIdx.y; m < rows; m += gridDim.y) {
+        float s[4] = {}, v[SPLITS][4];
+#pragma unroll
+        for (int k = 0; k < SPLITS; ++k) load_acc<float, 4>(part + (k * rows + m) * Kq + c, v[k]);
+#pragma unroll
+        for (int k = 0; k < SPLITS; ++k)
+#pragma unroll
+            for (int e = 0; e < 4; ++e) s[e] += v[k][e];
+        T e[4];
+#pragma unroll
+        for (int k = 0; k < 4; ++k) e[k] = from_acc<T>(s[k]);
+        if (c + 4 <= K) {
+            __builtin_memcpy(out + m * K + c, e, sizeof(e));
+        } else {
+#pragma unroll
+            for (int k = 0; k < 4; ++k)
+                if (c + k < K) out[m * K + c + k] = e[k];
+        }
+    }
+}
+
 template <typename T>
-__global__ __launch_bounds__(kPassThreads) void gated_join_kernel(const float* part, int splits, int64_t n, T* out) {
-    const int64_t i = static_cast<int64_t>(blockIdx.x) * kPassThreads + threadIdx.x;
-    if (i >= n) return;
-    float s = 0.f;
-    for (int k = 0; k < splits; ++k) s += part[k * n + i];
-    out[i] = from_acc<T>(s);
+int gated_join(const GatedArgs& a, int splits, hipStream_t st) {
+    const dim3 grid(static_cast<unsigned>(nsh_host::ceil_div(a.K, 4 * kPassThreads)),
+                    static_cast<unsigned>(std::min<int64_t>(a.rows, 32768)));
+    auto go = [&](auto n) {
+        gated_join_kernel<T, decltype(n)::value><<<grid, kPassThreads, 0, st>>>(a.part, a.rows, a.K, a.Kq, static_cast<T*>(a.dx));
+    };
+    switch (splits) {
+        case 2: go(std::integral_constant<int, 2>{}); break;
+        case 3: go(std::integral_constant<int, 3>{}); break;
+        case 4: go(std::integral_constant<int, 4>{}); break;
+        case 6: go(std::integral_constant<int, 6>{}); break;
+        case 8: go(std::integral_constant<int, 8>{}); break;
+        case 12: go(std::integral_constant<int, 12>{}); break;
+        case 16: go(std::integral_constant<int, 16>{}); break;
+        default: return nsh_host::fail(NSH_ERR_INVALID, "gated_linear_backward: no join of %d sums", splits);
+    }
+    return nsh_host::check_launch("gated_linear_backward");
 }
 
 }  // namespace nsh
@@ -160,7 +210,6 @@ struct Plan {
     int64_t copies[3];  // offsets in the workspace
     int64_t dgu, scale, most, part, bytes;
     nsh::Cut cut;
-    int splits;
 };
 
 int64_t up(int64_t v, int64_t to) { return ceil_div(v, to) * to; }
@@ -184,17 +233,15 @@ Plan plan_of(const nsh_gated_linear_args* g, bool bwd) {
     p.bytes += up(g->rows * (2 * p.Fp * p.esz + 128), 256);
     p.scale = p.bytes, p.bytes += 256;
     p.most = p.bytes, p.bytes += up(nsh::kMostBlocks * 4, 256);
-    p.part = p.bytes, p.splits = 1;
-    p.cut = nsh::cut_of(g->rows, g->K, p.esz == 4, false, 1);
-    // few tiles: workgroups share a tile's sum over the hidden columns, eight panels each or more
-    const int64_t panels = 2 * p.Fp * p.esz / 128, tiles = p.cut.tiles(), cus = nsh_host::compute_units();
-    if (tiles < cus) p.splits = static_cast<int>(std::max<int64_t>(1, std::min({ceil_div(2 * cus, tiles), panels / 8, int64_t(16)})));
-    if (p.splits > 1) p.bytes += up(p.splits * g->rows * g->K * 4, 256);
+    p.part = p.bytes;
+    p.cut = nsh::gradient_cut(g->rows, g->K, p.Fp, g->F, p.esz == 4, g->grad_x != nullptr, g->grad_gate || g->grad_up);
+    if (p.cut.splits > 1) p.bytes += up(p.cut.splits * g->rows * up(g->K, 4) * 4, 256);
     return p;
 }
 
 int64_t forward_blocks(const nsh_gated_linear_args* g) {
-    return nsh::cut_of(g->rows, g->F, g->dtype == NSH_DTYPE_FLOAT32, true, 1).tiles();
+    const bool wide = g->dtype == NSH_DTYPE_FLOAT32;
+    return nsh::forward_cut(g->rows, g->F, up(g->K, wide ? 4 : 8), wide).tiles();
 }
 
 int64_t kept_blocks(const nsh_gated_linear_args* g) {
@@ -249,27 +296,23 @@ int backward(const nsh_gated_linear_args* g, const Plan& p, nsh::GatedArgs a, ch
     if constexpr (__is_same(T, nsh::f16)) {
         scale = reinterpret_cast<float*>(ws + p.scale);
         float* most = reinterpret_cast<float*>(ws + p.most);
-        const int n = static_cast<int>(std::min<int64_t>(g->rows, nsh::kMostBlocks));
-        nsh::gated_most_kernel<<<n, nsh::kPassThreads, 0, st>>>(static_cast<const nsh::f16*>(g->grad_h), g->gh_stride, g->rows, a.F, most);
-        nsh::gated_scale_kernel<<<1, nsh::kPassThreads, 0, st>>>(most, n, reinterpret_cast<const float*>(a.kept + kept_blocks(g)), static_cast<int>(forward_blocks(g)), scale);
+        const bool flat = g->gh_stride == g->F;
+        const int64_t rows = flat ? 1 : g->rows, cols = flat ? g->rows * g->F : g->F;
+        const int64_t x = std::min<int64_t>(ceil_div(cols, nsh::kPassThreads * 32), nsh::kMostBlocks);
+        const int64_t y = std::min<int64_t>(rows, nsh::kMostBlocks / x), n = x * y;
+        nsh::gated_most_kernel<<<dim3(static_cast<unsigned>(x), static_cast<unsigned>(y)), nsh::kPassThreads, 0, st>>>(
+            static_cast<const nsh::f16*>(g->grad_h), g->gh_stride, rows, cols, most);
+        nsh::gated_scale_kernel<<<1, nsh::kPassThreads, 0, st>>>(most, static_cast<int>(n), reinterpret_cast<const float*>(a.kept + kept_blocks(g)), static_cast<int>(forward_blocks(g)), scale);
     }
     a.scale = scale, a.dgu = ws + p.dgu;
     const uint32_t across = static_cast<uint32_t>(ceil_div(a.Fp, nsh::kPassThreads / 64 * 128 / p.esz));
     const nsh::SlopeArgs s{g->grad_h, g->gh_stride, g->rows, 2 * p.Fp + 128 / p.esz, a.kept, a.dgu, a.F, a.Fp, across, scale};
     nsh::gated_slope_kernel<T><<<static_cast<unsigned>(across * ceil_div(g->rows, 32)), nsh::kPassThreads, 0, st>>>(s);
-    if (g->grad_x) {
-        a.splits = p.splits;
-        a.part = p.splits > 1 ? reinterpret_cast<float*>(ws + p.part) : nullptr;
-        const int rc = nsh::gated_input_gradient<T>(a, p.cut, st);
-        if (rc != NSH_OK) return rc;
-        if (a.part) {
-            const int64_t n = g->rows * g->K;
-            nsh::gated_join_kernel<T><<<static_cast<unsigned>(ceil_div(n, nsh::kPassThreads)), nsh::kPassThreads, 0, st>>>(
-                a.part, p.splits, n, static_cast<T*>(a.dx));
-        }
-    }
-    if (g->grad_gate || g->grad_up) return nsh::gated_weight_gradient<T>(a, st);
-    return nsh_host::check_launch("gated_linear_backward");
+    a.Kq = static_cast<int>(up(g->K, 4));
+    a.part = p.cut.splits > 1 ? reinterpret_cast<float*>(ws + p.part) : nullptr;
+    const int rc = nsh::gated_gradients<T>(a, p.cut, st);
+    if (rc != NSH_OK || !a.part) return rc;
+    return nsh::gated_join<T>(a, p.cut.splits, st);
 }
 
 template <typename T>

@@ -16,6 +16,11 @@
 // gradients.
 #pragma once
 
+#include <algorithm>
+#include <cmath>
+#include <type_traits>
+#include <utility>
+
 #include "panels.hpp"
 
 namespace nsh {
@@ -32,8 +37,13 @@ struct GatedArgs {
     void* dgu;             // (rows, 2, Fp) and a panel's width of nothing
     const float* scale;    // fp16: what dgu was multiplied by, and its inverse
     void *dx, *dwg, *dwu;
-    float* part;           // (splits, rows, K): sums of dx that a second launch joins
-    int tiles_m, tiles_n, splits;
+    float* part;           // (splits, rows, Kq): sums of dx that a second launch joins, Kq a multiple of 4
+    int Kq;
+    int tiles_m, tiles_n;  // of h, or of dx
+    int splits;            // workgroups that share a tile of dx
+    int weight_m, weight_n;  // tiles of the weights' gradients, both sides
+    int first;             // workgroups of the part that comes first
+    bool weights_first;
 };
 
 enum Activation { kSilu, kGelu, kGeluTanh, kRelu, kSigmoid };
@@ -283,16 +293,15 @@ __global__ __launch_bounds__(64 * WAVES_M * WAVES_N, 2) void gated_forward_kerne
 }
 
 // dx: over the hidden columns of dg, then of du.
-template <typename T, int BM, int BN, int WAVES_M, int WAVES_N, int KB>
-__global__ __launch_bounds__(64 * WAVES_M * WAVES_N, 2) void gated_input_gradient_kernel(GatedArgs a) {
-    using P = Product<T, BM, BN, WAVES_M, WAVES_N, KB, kAcross, kAlong, false>;
-    __shared__ __attribute__((aligned(1024))) char f0[P::FIRST_BYTES], s0[P::SECOND_BYTES];
-    __shared__ __attribute__((aligned(1024))) char f1[P::FIRST_BYTES], s1[P::SECOND_BYTES];
+template <typename P>
+__device__ __forceinline__ void input_gradient(const GatedArgs& a, uint32_t id, char (&f0)[P::FIRST_BYTES], char (&s0)[P::SECOND_BYTES],
+                                               char (&f1)[P::FIRST_BYTES], char (&s1)[P::SECOND_BYTES]) {
+    using T = typename P::T;
     const uint32_t tiles = static_cast<uint32_t>(a.tiles_m) * a.tiles_n;
-    const int split = TileOrder::uniform(blockIdx.x / tiles);
-    const TileOrder t(blockIdx.x - split * tiles, tiles, a.tiles_m, a.tiles_n, 8);
-    const int64_t m0 = static_cast<int64_t>(t.m) * BM;
-    const int64_t c0 = static_cast<int64_t>(t.n) * BN;
+    const int split = TileOrder::uniform(id / tiles);
+    const TileOrder t(id - split * tiles, tiles, a.tiles_m, a.tiles_n, 8);
+    const int64_t m0 = static_cast<int64_t>(t.m) * P::BM;
+    const int64_t c0 = static_cast<int64_t>(t.n) * P::BN;
     const int wave = wave_id();
     typename P::FirstPanel gate, up;
     typename P::SecondPanel rows;
@@ -303,7 +312,7 @@ __global__ __launch_bounds__(64 * WAVES_M * WAVES_N, 2) void gated_input_gradien
     const char* d = static_cast<const char*>(a.dgu) + m0 * stride;
     const char* wg = static_cast<const char*>(a.wg) + c0 * static_cast<int64_t>(sizeof(T));
     const char* wu = static_cast<const char*>(a.wu) + c0 * static_cast<int64_t>(sizeof(T));
-    const int left_m = static_cast<int>(min(a.rows - m0, int64_t(BM)));
+    const int left_m = static_cast<int>(min(a.rows - m0, int64_t(P::BM)));
     const int64_t left_c = (a.Kp - c0) * static_cast<int64_t>(sizeof(T));
     const int half = a.Fp / P::BK, all = 2 * half;
     const int begin = TileOrder::uniform(all * static_cast<uint32_t>(split) / a.splits);
@@ -316,7 +325,7 @@ __global__ __launch_bounds__(64 * WAVES_M * WAVES_N, 2) void gated_input_gradien
         const uint32_t step = one ? a.wg_stride : a.wu_stride;
         P::FirstPanel::either(one, gate, up).load(f, (one ? wg : wu) + static_cast<int64_t>(in) * P::BK * step, step,
                                                   at < end ? a.F - in * P::BK : 0, left_c, wave);
-        rows.load(s, d + static_cast<int64_t>(at) * KB, stride, at < end ? left_m : 0, KB, wave);
+        rows.load(s, d + static_cast<int64_t>(at) * P::KB, stride, at < end ? left_m : 0, P::KB, wave);
     });
     const float by = __is_same(T, f16) && a.scale ? a.scale[1] : 1.f;
     const int64_t m = m0 + P::wave_m() * P::WM, c = c0 + P::column(0);
@@ -324,24 +333,23 @@ __global__ __launch_bounds__(64 * WAVES_M * WAVES_N, 2) void gated_input_gradien
     char* stage = P::stage(f0, s0, f1, s1);
     const auto value = [&](int i, int b) { return p.acc[i][b] * by; };
     if (a.part)
-        store_tile<float, P::WM, P::WN>(stage, a.part + (split * a.rows + m) * a.K + c, a.K, a.rows - m, a.K - c, value);
+        store_tile<float, P::WM, P::WN>(stage, a.part + (split * a.rows + m) * a.Kq + c, a.Kq, a.rows - m, a.K - c, value);
     else
         store_tile<T, P::WM, P::WN>(stage, static_cast<T*>(a.dx) + m * a.K + c, a.K, a.rows - m, a.K - c, value);
 }
 
 // Both weights' gradients: tiles of hidden rows of the one, then of the other.
-template <typename T, int BM, int BN, int WAVES_M, int WAVES_N, int KB>
-__global__ __launch_bounds__(64 * WAVES_M * WAVES_N, 2) void gated_weight_gradient_kernel(GatedArgs a) {
-    using P = Product<T, BM, BN, WAVES_M, WAVES_N, KB, kAcross, kAcross, false>;
-    __shared__ __attribute__((aligned(1024))) char f0[P::FIRST_BYTES], s0[P::SECOND_BYTES];
-    __shared__ __attribute__((aligned(1024))) char f1[P::FIRST_BYTES], s1[P::SECOND_BYTES];
-    const int each = a.tiles_m / 2;
-    const TileOrder t(blockIdx.x, gridDim.x, a.tiles_m, a.tiles_n, 8);
+template <typename P>
+__device__ __forceinline__ void weight_gradient(const GatedArgs& a, uint32_t id, char (&f0)[P::FIRST_BYTES], char (&s0)[P::SECOND_BYTES],
+                                                char (&f1)[P::FIRST_BYTES], char (&s1)[P::SECOND_BYTES]) {
+    using T = typename P::T;
+    const int each = a.weight_m / 2;
+    const TileOrder t(id, static_cast<uint32_t>(a.weight_m) * a.weight_n, a.weight_m, a.weight_n, 8);
     const int side = t.m >= each;
     T* out = static_cast<T*>(side ? a.dwu : a.dwg);
     if (!out) return;
-    const int f_first = (side ? t.m - each : t.m) * BM;
-    const int64_t c0 = static_cast<int64_t>(t.n) * BN;
+    const int f_first = (side ? t.m - each : t.m) * P::BM;
+    const int64_t c0 = static_cast<int64_t>(t.n) * P::BN;
     const int wave = wave_id();
     typename P::FirstPanel in;
     typename P::SecondPanel d;
@@ -367,6 +375,23 @@ __global__ __launch_bounds__(64 * WAVES_M * WAVES_N, 2) void gated_weight_gradie
                                 [&](int i, int b) { return p.acc[i][b] * by; });
 }
 
+// Both, in one launch: neither alone fills the card but for large calls.  Whichever has the
+// longer workgroups comes first.
+template <typename T, int BM, int BN, int WAVES_M, int WAVES_N, int KB>
+__global__ __launch_bounds__(64 * WAVES_M * WAVES_N, 2) void gated_gradients_kernel(GatedArgs a) {
+    using In = Product<T, BM, BN, WAVES_M, WAVES_N, KB, kAcross, kAlong, false>;
+    using Weights = Product<T, BM, BN, WAVES_M, WAVES_N, KB, kAcross, kAcross, false>;
+    __shared__ __attribute__((aligned(1024))) char f0[In::FIRST_BYTES], s0[In::SECOND_BYTES];
+    __shared__ __attribute__((aligned(1024))) char f1[In::FIRST_BYTES], s1[In::SECOND_BYTES];
+    const uint32_t first = a.first;
+    const bool second = blockIdx.x >= first;
+    const uint32_t id = second ? blockIdx.x - first : blockIdx.x;
+    if (second == a.weights_first)
+        input_gradient<In>(a, id, f0, s0, f1, s1);
+    else
+        weight_gradient<Weights>(a, id, f0, s0, f1, s1);
+}
+
 // ---------------------------------------------------------------------------
 // Few rows: the weights are read once, past the LDS
 // ---------------------------------------------------------------------------
@@ -386,79 +411,95 @@ __device__ __forceinline__ f32x4 multiply16(ux4 first, ux4 second, f32x4 c) {
     }
 }
 
-// FG groups of 16 hidden columns and MG of 16 rows a workgroup, whose four waves take
-// turns in 256 bytes of the contraction: a lane (row l % 16) reads 16 bytes of each 64.
-template <typename T, int FG, int MG>
-__global__ __launch_bounds__(256) void gated_rows_kernel(GatedArgs a) {
-    constexpr int kBlock = 256, kSteps = 4;
-    __shared__ f32x4 meet[4][FG][MG][2][64];
-    const int l = threadIdx.x & 63, wave = wave_id(), f0 = blockIdx.x * (16 * FG);
+// 16 hidden columns and MG groups of 16 rows a workgroup, whose waves take turns in KB
+// bytes of the contraction, each with panels of its own in LDS and no barrier.  (Straight to
+// registers a lane would load 16 bytes of its own row, and lanes side by side other
+// rows: 45 rows, 4096 -> 11000, took 65 us, four times the caches' requests.)
+template <typename T, int MG, int WAVES, int KB>
+__global__ __launch_bounds__(64 * WAVES) void gated_rows_kernel(GatedArgs a) {
+    using L = Tile<T, KB / sizeof(T)>;
+    constexpr int SIZE = 16 * KB, NI = KB / 64, STEPS = KB / 64, LOADS = NI * (2 + MG);
+    __shared__ __attribute__((aligned(1024))) char panels0[WAVES][(2 + MG) * SIZE], panels1[WAVES][(2 + MG) * SIZE];
+    static_assert(sizeof(panels0) >= WAVES * MG * 1024, "the waves' sums take the panels' place");
+    const int l = threadIdx.x & 63, wave = wave_id(), f0 = blockIdx.x * 16;
     const int row_bytes = a.Kp * static_cast<int>(sizeof(T));
-    auto matrix = [&](const void* base, uint32_t stride, int64_t first, int rows) {
+    const int left = min(a.F - f0, 16), rows = static_cast<int>(a.rows);
+    auto matrix = [&](const void* base, uint32_t stride, int64_t first, int n) {
         return __builtin_amdgcn_make_buffer_rsrc(
             const_cast<char*>(static_cast<const char*>(base) + first * stride), static_cast<short>(0),
-            static_cast<int>((rows - 1) * stride + row_bytes), 0x00020000);
+            static_cast<int>((n - 1) * stride + row_bytes), 0x00020000);
     };
-    const int left = min(a.F - f0, 16 * FG), rows = static_cast<int>(a.rows);
     const __amdgpu_buffer_rsrc_t rg = matrix(a.wg, a.wg_stride, f0, left), ru = matrix(a.wu, a.wu_stride, f0, left);
     const __amdgpu_buffer_rsrc_t rx = matrix(a.x, a.x_stride, 0, rows);
-    struct Block {
-        ux4 g[FG][kSteps], u[FG][kSteps], x[MG][kSteps];
-    };
-    const int r = l & 15, part = (l >> 4) * 16;
-    auto read = [&](Block& b, int k) {
+    // the chunk that the lane loads of its row, and where that row starts (a row that is none
+    // lies past any buffer: zeros)
+    uint32_t og[NI], ou[NI], ox[MG][NI];
+    int chunk[NI];
 #pragma unroll
-        for (int s = 0; s < kSteps; ++s) {
-            const int at = k + s * 64 + part;
-            const bool in = at < row_bytes;
-            auto get = [&](__amdgpu_buffer_rsrc_t rs, int row, int most, uint32_t stride) {
-                const uint32_t off = in && row < most ? static_cast<uint32_t>(row) * stride + at : 0x80000000u;
-                return __builtin_bit_cast(ux4, __builtin_amdgcn_raw_buffer_load_b128(rs, off, 0, 0));
-            };
+    for (int i = 0; i < NI; ++i) {
+        const int x = i * 64 + l, r = x / L::NC;
+        chunk[i] = ((x % L::NC) ^ L::turn(r)) * 16;
+        og[i] = r < left ? r * a.wg_stride + chunk[i] : 0x80000000u;
+        ou[i] = r < left ? r * a.wu_stride + chunk[i] : 0x80000000u;
 #pragma unroll
-            for (int i = 0; i < FG; ++i) {
-                b.g[i][s] = get(rg, 16 * i + r, left, a.wg_stride);
-                b.u[i][s] = get(ru, 16 * i + r, left, a.wu_stride);
-            }
+        for (int j = 0; j < MG; ++j) ox[j][i] = 16 * j + r < rows ? (16 * j + r) * a.x_stride + chunk[i] : 0x80000000u;
+    }
+    auto load = [&](char* to, int k) {
 #pragma unroll
-            for (int i = 0; i < MG; ++i) b.x[i][s] = get(rx, 16 * i + r, rows, a.x_stride);
+        for (int i = 0; i < NI; ++i) {
+            const bool past = k + chunk[i] >= row_bytes;
+            to_lds<16>(rg, to + i * 1024, past ? 0x80000000u : og[i] + k);
+            to_lds<16>(ru, to + SIZE + i * 1024, past ? 0x80000000u : ou[i] + k);
+#pragma unroll
+            for (int j = 0; j < MG; ++j) to_lds<16>(rx, to + (2 + j) * SIZE + i * 1024, past ? 0x80000000u : ox[j][i] + k);
         }
     };
-    f32x4 acc[FG][MG][2] = {};
-    auto multiply = [&](const Block& b) {
+    f32x4 acc[MG][2] = {};
+    auto multiply = [&](const char* from) {
+        ux4 v[STEPS][2 + MG];
 #pragma unroll
-        for (int s = 0; s < kSteps; ++s)
+        for (int s = 0; s < STEPS; ++s)
 #pragma unroll
-            for (int i = 0; i < FG; ++i)
+            for (int n = 0; n < 2 + MG; ++n)
+                v[s][n] = *reinterpret_cast<const ux4*>(from + n * SIZE + L::at(l & 15, s * 4 + (l >> 4)));
 #pragma unroll
-                for (int j = 0; j < MG; ++j) {
-                    acc[i][j][0] = multiply16<T>(b.g[i][s], b.x[j][s], acc[i][j][0]);
-                    acc[i][j][1] = multiply16<T>(b.u[i][s], b.x[j][s], acc[i][j][1]);
-                }
+        for (int s = 0; s < STEPS; ++s)
+#pragma unroll
+            for (int j = 0; j < MG; ++j) {
+                acc[j][0] = multiply16<T>(v[s][0], v[s][2 + j], acc[j][0]);
+                acc[j][1] = multiply16<T>(v[s][1], v[s][2 + j], acc[j][1]);
+            }
     };
-    Block p, q;
-    int k = wave * kBlock;
-    if (k < row_bytes) read(p, k);
-    while (k < row_bytes) {
-        const int next = k + 4 * kBlock, after = k + 8 * kBlock;
-        if (next < row_bytes) read(q, next);
+    char *p = panels0[wave], *q = panels1[wave];
+    const int turns = (row_bytes + WAVES * KB - 1) / (WAVES * KB);
+    auto place = [&](int i) { return (i * WAVES + wave) * KB; };
+    // (turns past the end load zeros, and nothing from memory)
+    load(p, place(0));
+    load(q, place(1));
+    for (int i = 0; i < turns; i += 2) {
+        __builtin_amdgcn_s_waitcnt(0x0f70 | LOADS);  // all but the other panels'
+        order();
         multiply(p);
-        if (next >= row_bytes) break;
-        if (after < row_bytes) read(p, after);
+        order();
+        load(p, place(i + 2));
+        __builtin_amdgcn_s_waitcnt(0x0f70 | LOADS);
+        order();
         multiply(q);
-        k = after;
+        order();
+        load(q, place(i + 3));
     }
     settle<float>();
-#pragma unroll
-    for (int i = 0; i < FG; ++i)
-#pragma unroll
-        for (int j = 0; j < MG; ++j) meet[wave][i][j][0][l] = acc[i][j][0], meet[wave][i][j][1][l] = acc[i][j][1];
+    __builtin_amdgcn_s_waitcnt(0x0f70);  // the zeros have landed, and the panels' place is free
     __syncthreads();
-    for (int n = wave; n < FG * MG; n += 4) {
-        const int i = n / MG, j = n % MG, m = 16 * j + r, f = f0 + 16 * i + 4 * (l >> 4);
+    f32x4 *meet_g = reinterpret_cast<f32x4*>(panels0), *meet_u = reinterpret_cast<f32x4*>(panels1);  // (wave, group, lane)
+#pragma unroll
+    for (int j = 0; j < MG; ++j) meet_g[(wave * MG + j) * 64 + l] = acc[j][0], meet_u[(wave * MG + j) * 64 + l] = acc[j][1];
+    __syncthreads();
+    for (int j = wave; j < MG; j += WAVES) {
+        const int m = 16 * j + (l & 15), f = f0 + 4 * (l >> 4);
         f32x4 g = {}, u = {};
 #pragma unroll
-        for (int w = 0; w < 4; ++w) g += meet[w][i][j][0][l], u += meet[w][i][j][1][l];
+        for (int w = 0; w < WAVES; ++w) g += meet_g[(w * MG + j) * 64 + l], u += meet_u[(w * MG + j) * 64 + l];
         if (m >= rows || f >= a.F) continue;
         T* out = static_cast<T*>(a.h) + static_cast<int64_t>(m) * a.F + f;
         f32x4 h, slope;
@@ -475,75 +516,140 @@ __global__ __launch_bounds__(256) void gated_rows_kernel(GatedArgs a) {
 
 constexpr int kFewRows = 64;
 
-struct Cut {
-    int bm, bn;  // of the result
-    int tiles_m, tiles_n;
-    int64_t tiles() const { return static_cast<int64_t>(tiles_m) * tiles_n; }
+// Workgroup tiles, and the microseconds that a panel takes where one, two or three of
+// them share a CU (measured at sizes that leave the clock alone; `setup`: what a workgroup
+// takes besides, in panels).
+struct Shape {
+    int bm, bn, most;
+    float along[3], across[3], wide[3];
+    float setup;
+};
+constexpr Shape kShapes[3] = {{256, 256, 1, {1.42f}, {1.5f}, {0.f}, 5.f},
+                              {128, 128, 2, {0.72f, 1.12f}, {0.73f, 1.15f}, {1.9f, 3.5f}, 5.f},
+                              {64, 128, 3, {0.55f, 0.65f, 0.85f}, {0.57f, 0.9f, 1.25f}, {0.98f, 1.8f, 2.65f}, 5.f}};
+
+// n workgroups of `length` panels, on as many CUs as there are.
+struct Part {
+    int64_t n, length;
 };
 
-// Tiles of 256 x 256 where they fill the card, of 128 x 128, or of 64 x 128 (`paired`: a
-// tile has half as many columns, of both matrices).
-inline Cut cut_of(int64_t rows, int64_t cols, bool wide, bool paired, int sides) {
-    static constexpr int kSizes[3][2] = {{256, 256}, {128, 128}, {64, 128}};
-    const int cus = nsh_host::compute_units();
-    Cut c{};
+// Panels until the last of two parts' workgroups is done, the longer ones first.
+inline double panels_until_done(Part a, Part b, double setup, int64_t slots) {
+    if (a.length < b.length) std::swap(a, b);
+    const int64_t turns = a.n / slots, over = a.n % slots;
+    const double la = static_cast<double>(a.length) + setup, lb = static_cast<double>(b.length) + setup;
+    const double late = static_cast<double>(turns + 1) * la, early = static_cast<double>(turns) * la;
+    double done = over ? late : early;
+    if (!b.n) return done;
+    auto room = [&](double t) {
+        return static_cast<double>(over) * std::max(0.0, std::floor((t - late) / lb)) +
+               static_cast<double>(slots - over) * std::max(0.0, std::floor((t - early) / lb));
+    };
+    double t = (static_cast<double>(a.n) * la + static_cast<double>(b.n) * lb) / static_cast<double>(slots);
+    while (room(t) < static_cast<double>(b.n)) t += lb / 8;
+    return std::max(done, t);
+}
+
+struct Cut {
+    int shape, tiles_m, tiles_n, splits, weight_m, weight_n;
+    int64_t tiles() const { return static_cast<int64_t>(tiles_m) * tiles_n; }
+    int64_t weights() const { return static_cast<int64_t>(weight_m) * weight_n; }
+};
+
+inline double time_of(const Shape& s, const float (&rate)[3], Part a, Part b) {
+    const int64_t cus = nsh_host::compute_units();
+    const int share = static_cast<int>(std::min<int64_t>(s.most, nsh_host::ceil_div(a.n + b.n, cus)));
+    return panels_until_done(a, b, s.setup, cus * share) * rate[share - 1];
+}
+
+inline Cut forward_cut(int64_t rows, int64_t F, int64_t Kp, bool wide) {
+    Cut best{};
+    double least = 0;
     for (int i = wide ? 1 : 0; i < 3; ++i) {
-        c.bm = kSizes[i][0], c.bn = kSizes[i][1];
-        c.tiles_m = static_cast<int>(nsh_host::ceil_div(rows, c.bm)) * sides;
-        c.tiles_n = static_cast<int>(nsh_host::ceil_div(cols, paired ? c.bn / 2 : c.bn));
-        if (c.tiles() >= (i == 0 ? cus * 3 / 4 : cus)) break;
+        const Shape& s = kShapes[i];
+        Cut c{i, static_cast<int>(nsh_host::ceil_div(rows, s.bm)), static_cast<int>(nsh_host::ceil_div(F, s.bn / 2)), 1, 0, 0};
+        const double t = time_of(s, wide ? s.wide : s.along, {c.tiles(), nsh_host::ceil_div(Kp, wide ? 32 : 64)}, {0, 0});
+        if (least == 0 || t < least) least = t, best = c;
     }
-    return c;
+    return best;
+}
+
+// Of dx, of the weights' gradients, or of both in one launch: with few tiles of dx,
+// workgroups share a tile's sum over the hidden columns, and another launch joins them
+// (4 us, and their sums' bytes at 3.5 TB/s).
+inline Cut gradient_cut(int64_t rows, int64_t K, int64_t Fp, int64_t F, bool wide, bool input, bool weights) {
+    Cut best{};
+    double least = 0;
+    const int64_t bk = wide ? 32 : 64;
+    for (int i = wide ? 1 : 0; i < 3; ++i) {
+        const Shape& s = kShapes[i];
+        Cut c{i, 0, 0, 1, 0, 0};
+        if (input) c.tiles_m = static_cast<int>(nsh_host::ceil_div(rows, s.bm)), c.tiles_n = static_cast<int>(nsh_host::ceil_div(K, s.bn));
+        if (weights) c.weight_m = 2 * static_cast<int>(nsh_host::ceil_div(F, s.bm)), c.weight_n = static_cast<int>(nsh_host::ceil_div(K, s.bn));
+        const int64_t panels = 2 * Fp / bk;
+        for (const int splits : {1, 2, 3, 4, 6, 8, 12, 16}) {  // (those that the join knows)
+            if (splits > 1 && (!input || panels / splits < 4)) break;
+            c.splits = splits;
+            double t = time_of(s, wide ? s.wide : s.across, {c.tiles() * splits, nsh_host::ceil_div(panels, splits)},
+                               {c.weights(), nsh_host::ceil_div(rows, bk)});
+            if (splits > 1) t += 4 + static_cast<double>(splits * rows * K) * 4 / 3.5e6;
+            if (least == 0 || t < least) least = t, best = c;
+        }
+    }
+    return best;
 }
 
 template <typename T>
 int gated_forward(GatedArgs a, hipStream_t st) {
     if (a.rows <= kFewRows && !a.kept) {
-        const unsigned one = (a.F + 15) / 16, two = (a.F + 31) / 32;
+        // twice the waves a workgroup where there are too few for two on every CU
+        const unsigned grid = (a.F + 15) / 16;
+        const bool more = grid < 2u * nsh_host::compute_units();
+        auto go = [&](auto groups) {
+            // (45 rows, 4096 -> 11000: 58 us by 64 bytes, 44 by 128; eight waves' panels of
+            // those fit the LDS up to 32 rows)
+            constexpr int MG = decltype(groups)::value;
+            if (more)
+                gated_rows_kernel<T, MG, 8, MG < 3 ? 128 : 64><<<grid, 512, 0, st>>>(a);
+            else
+                gated_rows_kernel<T, MG, 4, 128><<<grid, 256, 0, st>>>(a);
+        };
         if (a.rows <= 16)
-            gated_rows_kernel<T, 1, 1><<<one, 256, 0, st>>>(a);
+            go(std::integral_constant<int, 1>{});
         else if (a.rows <= 32)
-            gated_rows_kernel<T, 2, 2><<<two, 256, 0, st>>>(a);
+            go(std::integral_constant<int, 2>{});
+        else if (a.rows <= 48)
+            go(std::integral_constant<int, 3>{});
         else
-            gated_rows_kernel<T, 2, 4><<<two, 256, 0, st>>>(a);
+            go(std::integral_constant<int, 4>{});
         return nsh_host::check_launch("gated_linear_forward");
     }
-    const Cut c = cut_of(a.rows, a.F, sizeof(T) == 4, true, 1);
+    const Cut c = forward_cut(a.rows, a.F, a.Kp, sizeof(T) == 4);
     a.tiles_m = c.tiles_m, a.tiles_n = c.tiles_n;
     const unsigned grid = static_cast<unsigned>(c.tiles());
     if constexpr (sizeof(T) == 2)
-        if (c.bm == 256) gated_forward_kernel<T, 256, 256, 4, 2, 128><<<grid, 512, 0, st>>>(a);
-    if (c.bm == 128) gated_forward_kernel<T, 128, 128, 2, 2, 128><<<grid, 256, 0, st>>>(a);
-    if (c.bm == 64) gated_forward_kernel<T, 64, 128, 2, 2, 128><<<grid, 256, 0, st>>>(a);
+        if (c.shape == 0) gated_forward_kernel<T, 256, 256, 4, 2, 128><<<grid, 512, 0, st>>>(a);
+    if (c.shape == 1) gated_forward_kernel<T, 128, 128, 2, 2, 128><<<grid, 256, 0, st>>>(a);
+    if (c.shape == 2) gated_forward_kernel<T, 64, 128, 2, 2, 128><<<grid, 256, 0, st>>>(a);
     return nsh_host::check_launch("gated_linear_forward");
 }
 
 template <typename T>
-int gated_input_gradient(GatedArgs a, const Cut& c, hipStream_t st) {
-    a.tiles_m = c.tiles_m, a.tiles_n = c.tiles_n;
-    const unsigned grid = static_cast<unsigned>(c.tiles() * a.splits);
+int gated_gradients(GatedArgs a, const Cut& c, hipStream_t st) {
+    a.tiles_m = c.tiles_m, a.tiles_n = c.tiles_n, a.splits = c.splits, a.weight_m = c.weight_m, a.weight_n = c.weight_n;
+    const int64_t in = c.tiles() * c.splits, all = in + c.weights();
+    a.weights_first = 2 * a.Fp / c.splits < a.rows;
+    a.first = static_cast<int>(a.weights_first ? c.weights() : in);
+    const unsigned grid = static_cast<unsigned>(all);
     if constexpr (sizeof(T) == 2)
-        if (c.bm == 256) gated_input_gradient_kernel<T, 256, 256, 4, 2, 128><<<grid, 512, 0, st>>>(a);
-    if (c.bm == 128) gated_input_gradient_kernel<T, 128, 128, 2, 2, 128><<<grid, 256, 0, st>>>(a);
-    if (c.bm == 64) gated_input_gradient_kernel<T, 64, 128, 2, 2, 128><<<grid, 256, 0, st>>>(a);
+        if (c.shape == 0) gated_gradients_kernel<T, 256, 256, 4, 2, 128><<<grid, 512, 0, st>>>(a);
+    if (c.shape == 1) gated_gradients_kernel<T, 128, 128, 2, 2, 128><<<grid, 256, 0, st>>>(a);
+    if (c.shape == 2) gated_gradients_kernel<T, 64, 128, 2, 2, 128><<<grid, 256, 0, st>>>(a);
     return nsh_host::check_launch("gated_linear_backward");
 }
 
-template <typename T>
-int gated_weight_gradient(GatedArgs a, hipStream_t st) {
-    const Cut c = cut_of(a.F, a.K, sizeof(T) == 4, false, 2);
-    a.tiles_m = c.tiles_m, a.tiles_n = c.tiles_n;
-    const unsigned grid = static_cast<unsigned>(c.tiles());
-    if constexpr (sizeof(T) == 2)
-        if (c.bm == 256) gated_weight_gradient_kernel<T, 256, 256, 4, 2, 128><<<grid, 512, 0, st>>>(a);
-    if (c.bm == 128) gated_weight_gradient_kernel<T, 128, 128, 2, 2, 128><<<grid, 256, 0, st>>>(a);
-    if (c.bm == 64) gated_weight_gradient_kernel<T, 64, 128, 2, 2, 128><<<grid, 256, 0, st>>>(a);
-    return nsh_host::check_launch("gated_linear_backward");
-}
-
-#define NSH_GATED_ENTRIES(EXTERN, T)                                                       \
-    EXTERN template int gated_forward<T>(GatedArgs, hipStream_t);                          \
-    EXTERN template int gated_input_gradient<T>(GatedArgs, const Cut&, hipStream_t);       \
-    EXTERN template int gated_weight_gradient<T>(GatedArgs, hipStream_t);
+#define NSH_GATED_ENTRIES(EXTERN, T)                               \
+    EXTERN template int gated_forward<T>(GatedArgs, hipStream_t); \
+    EXTERN template int gated_gradients<T>(GatedArgs, const Cut&, hipStream_t);
 
 }  // namespace nsh
