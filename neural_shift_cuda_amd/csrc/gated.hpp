@@ -108,6 +108,19 @@ __device__ __forceinline__ void activate(int kind, const V& g, V& v, V& slope) {
     }
 }
 
+// The largest magnitude of a lane's 16 numbers: an infinity says nothing of the others.
+__device__ __forceinline__ float largest(const f32x16& v) {
+    float most = 0.f;
+#pragma unroll
+    for (int r = 0; r < 16; ++r) most = fmaxf(most, fabsf(v[r]));
+    if (!(most < INFINITY)) {
+        most = 0.f;
+#pragma unroll
+        for (int r = 0; r < 16; ++r) most = fmaxf(most, fabsf(v[r]) < INFINITY ? fabsf(v[r]) : 0.f);
+    }
+    return most;
+}
+
 // What training keeps of a block of 32 x 32 places: the two factors as the lanes have
 // them, so that every store and load is 1 KB in one piece (rows of their own, 16 bytes a
 // lane apart, took the forward 8192 x 2048 -> 8192 from 480 to 1017 us).
@@ -127,17 +140,7 @@ struct Kept {
     }
 
     // The exponent field of the largest number of a lane's 16 (15 at the least).
-    static __device__ __forceinline__ uint32_t field(const f32x16& v) {
-        float most = 0.f;
-#pragma unroll
-        for (int r = 0; r < 16; ++r) most = fmaxf(most, fabsf(v[r]));
-        if (!(most < INFINITY)) {  // an infinity says nothing of the others
-            most = 0.f;
-#pragma unroll
-            for (int r = 0; r < 16; ++r) most = fmaxf(most, fabsf(v[r]) < INFINITY ? fabsf(v[r]) : 0.f);
-        }
-        return max(__float_as_uint(most) >> 23, 15u);
-    }
+    static __device__ __forceinline__ uint32_t field(const f32x16& v) { return max(__float_as_uint(largest(v)) >> 23, 15u); }
 
     static __device__ __forceinline__ void store(char* at, const f32x16& s, const f32x16& h) {
         const f32x16* both[2] = {&s, &h};
@@ -164,16 +167,16 @@ struct Kept {
                 for (int r = 0; r < 16; ++r) b[r] = __float_as_uint(v[r]) + 0x80u;
 #pragma unroll
                 for (int q = 0; q < 2; ++q) {
-                    ux4 x;
+                    ux4 x;  // upper halves of two
 #pragma unroll
-                    for (int e = 0; e < 4; ++e) x[e] = b[8 * q + 2 * e] >> 16 | (b[8 * q + 2 * e + 1] & 0xffff0000u);
+                    for (int e = 0; e < 4; ++e) x[e] = __builtin_amdgcn_perm(b[8 * q + 2 * e + 1], b[8 * q + 2 * e], 0x07060302);
                     *part(at, 2 * n + q) = x;
                 }
-                ux4 x;
+                ux4 x;  // second bytes of four
 #pragma unroll
                 for (int e = 0; e < 4; ++e)
-                    x[e] = (b[4 * e] >> 8 & 0xffu) | (b[4 * e + 1] & 0xff00u) | (b[4 * e + 2] & 0xff00u) << 8 |
-                           (b[4 * e + 3] & 0xff00u) << 16;
+                    x[e] = __builtin_amdgcn_perm(__builtin_amdgcn_perm(b[4 * e + 3], b[4 * e + 2], 0x05010501),
+                                                 __builtin_amdgcn_perm(b[4 * e + 1], b[4 * e], 0x05010501), 0x05040100);
                 *part(at, 4 + n) = x;
             }
         }
@@ -222,14 +225,7 @@ __device__ __forceinline__ f32x16 gate_block(const GatedArgs& a, int64_t m, int 
     if (a.kept && (m & ~int64_t(31)) < a.rows && c < a.F) {
         s *= u;
         Kept<T>::store(Kept<T>::block(a.kept, m, c, a.F), s, h);
-        if constexpr (__is_same(T, f16)) {
-#pragma unroll
-            for (int r = 0; r < 16; ++r) {
-                // (numbers only: an infinity says nothing of the others)
-                const float x = fabsf(s[r]), y = fabsf(h[r]);
-                most = fmaxf(most, fmaxf(x < INFINITY ? x : 0.f, y < INFINITY ? y : 0.f));
-            }
-        }
+        if constexpr (__is_same(T, f16)) most = fmaxf(most, fmaxf(largest(s), largest(h)));
     }
     return h * u;
 }

@@ -83,19 +83,24 @@ __device__ __forceinline__ float variance(Gr& group, float square, float off, co
     return rest;
 }
 
-template <typename T, int G, int NV>
+template <typename T, int G, int NV, bool WHOLE>
 __global__ __launch_bounds__(Group<G>::kThreads) void layer_norm_forward_kernel(LayerNormArgs a) {
     using Gr = Group<G>;
     constexpr int V = kVec<T>;
     __shared__ float meet[Gr::kWaves > 1 ? 4 * Gr::kWaves : 1];
     Gr group{meet};
+    // Groups of a wave keep the weights for all their rows; a workgroup has one row, and
+    // reads them at its end: registers for more workgroups at once instead.
+    constexpr bool KEEP = G <= 64;
     const int lane = threadIdx.x % G, own = threadIdx.x / G;
-    ux4 w[NV], b[NV];
+    ux4 w[KEEP ? NV : 1], b[KEEP ? NV : 1];
+    if constexpr (KEEP) {
 #pragma unroll
-    for (int i = 0; i < NV; ++i) {
-        const int c = (i * G + lane) * V;
-        if (a.weight) w[i] = load_bits(static_cast<const T*>(a.weight), c, a.n);
-        if (a.bias) b[i] = load_bits(static_cast<const T*>(a.bias), c, a.n);
+        for (int i = 0; i < NV; ++i) {
+            const int c = (i * G + lane) * V;
+            if (a.weight) w[i] = load_bits<T, WHOLE>(static_cast<const T*>(a.weight), c, a.n);
+            if (a.bias) b[i] = load_bits<T, WHOLE>(static_cast<const T*>(a.bias), c, a.n);
+        }
     }
     // every lane of the workgroup takes every turn: the groups meet in lane exchanges
     for (int64_t r0 = static_cast<int64_t>(blockIdx.x) * Gr::kGroups; r0 < a.rows;
@@ -105,11 +110,11 @@ __global__ __launch_bounds__(Group<G>::kThreads) void layer_norm_forward_kernel(
         const T* x = static_cast<const T*>(a.x) + row * a.x_stride;
         ux4 bits[NV], more[NV];
 #pragma unroll
-        for (int i = 0; i < NV; ++i) bits[i] = load_bits(x, (i * G + lane) * V, a.n);
+        for (int i = 0; i < NV; ++i) bits[i] = load_bits<T, WHOLE>(x, (i * G + lane) * V, a.n);
         if (a.residual) {
             const T* r = static_cast<const T*>(a.residual) + row * a.residual_stride;
 #pragma unroll
-            for (int i = 0; i < NV; ++i) more[i] = load_bits(r, (i * G + lane) * V, a.n);
+            for (int i = 0; i < NV; ++i) more[i] = load_bits<T, WHOLE>(r, (i * G + lane) * V, a.n);
         }
         float v[NV][V], total = 0.f;
 #pragma unroll
@@ -123,7 +128,7 @@ __global__ __launch_bounds__(Group<G>::kThreads) void layer_norm_forward_kernel(
                 for (int k = 0; k < V; ++k) v[i][k] += m[k];
                 bits[i] = pack<T>(v[i]);
                 unpack<T>(bits[i], v[i]);
-                if (live) store_bits(static_cast<T*>(a.s) + row * a.n, c, a.n, bits[i]);
+                if (live) store_bits<T, WHOLE>(static_cast<T*>(a.s) + row * a.n, c, a.n, bits[i]);
             }
 #pragma unroll
             for (int k = 0; k < V; ++k) total += v[i][k];
@@ -135,7 +140,7 @@ __global__ __launch_bounds__(Group<G>::kThreads) void layer_norm_forward_kernel(
             const int c = (i * G + lane) * V;
 #pragma unroll
             for (int k = 0; k < V; ++k) {
-                v[i][k] = c + k < a.n ? v[i][k] - mean : 0.f;
+                v[i][k] = (WHOLE ? c : c + k) < a.n ? v[i][k] - mean : 0.f;
                 square = fma_acc(v[i][k], v[i][k], square);
                 off += v[i][k];
             }
@@ -151,17 +156,35 @@ __global__ __launch_bounds__(Group<G>::kThreads) void layer_norm_forward_kernel(
 #pragma unroll
             for (int k = 0; k < V; ++k) v[i][k] = (v[i][k] - rest) * by;
             if (a.weight) {
-                unpack<T>(w[i], m);
+                unpack<T>(KEEP ? w[KEEP ? i : 0] : load_bits<T, WHOLE>(static_cast<const T*>(a.weight), c, a.n), m);
 #pragma unroll
                 for (int k = 0; k < V; ++k) v[i][k] *= m[k];
             }
             if (a.bias) {
-                unpack<T>(b[i], m);
+                unpack<T>(KEEP ? b[KEEP ? i : 0] : load_bits<T, WHOLE>(static_cast<const T*>(a.bias), c, a.n), m);
 #pragma unroll
                 for (int k = 0; k < V; ++k) v[i][k] += m[k];
             }
-            store_bits(static_cast<T*>(a.y) + row * a.n, c, a.n, pack<T>(v[i]));
+            store_bits<T, WHOLE>(static_cast<T*>(a.y) + row * a.n, c, a.n, pack<T>(v[i]));
         }
+    }
+}
+
+// A lane's sums of d h and d over its columns, in LDS: four at a time, the lanes side by
+// side.  `at` of `all` parts.
+template <int V>
+__device__ __forceinline__ void add_columns(float* lds, int at, int all, const float (&h)[V], const float (&d)[V]) {
+    fx4* sums = reinterpret_cast<fx4*>(lds);
+#pragma unroll
+    for (int q = 0; q < V / 4; ++q) {
+        fx4 &w = sums[q * all + at], &b = sums[(V / 4 + q) * all + at];
+        fx4 x = w, y = b;
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+            x[e] = fma_acc(d[4 * q + e], h[4 * q + e], x[e]);
+            y[e] += d[4 * q + e];
+        }
+        w = x, b = y;
     }
 }
 
@@ -193,56 +216,87 @@ __device__ __forceinline__ void add_groups(const float (&sum)[NV][V], float* to,
     }
 }
 
-template <typename T, int G, int NV>
+template <typename T, int G, int NV, bool WHOLE>
 __global__ __launch_bounds__(Group<G>::kThreads) void layer_norm_backward_kernel(LayerNormArgs a) {
     using Gr = Group<G>;
     constexpr int V = kVec<T>;
+    // 32 columns a lane: their sums are in LDS, and leave the next row its registers (3000
+    // x 16384 fp16: 104 us with the sums in registers and no row ahead, 85 so)
+    constexpr bool IN_LDS = NV * V == 32 && G > 64;
     __shared__ float lds[Gr::kGroups > 1 ? Gr::kThreads * NV * V : 4 * Gr::kWaves];
+    __shared__ __attribute__((aligned(16))) float sums[IN_LDS ? 2 * Gr::kThreads * NV * V : 1];
     Gr group{lds};
     const int lane = threadIdx.x % G, own = threadIdx.x / G;
     ux4 w[NV];
     float gw[NV][V], gb[NV][V];
 #pragma unroll
     for (int i = 0; i < NV; ++i) {
-        if (a.weight) w[i] = load_bits(static_cast<const T*>(a.weight), (i * G + lane) * V, a.n);
+        if (a.weight) w[i] = load_bits<T, WHOLE>(static_cast<const T*>(a.weight), (i * G + lane) * V, a.n);
 #pragma unroll
         for (int k = 0; k < V; ++k) gw[i][k] = gb[i][k] = 0.f;
+        if constexpr (IN_LDS) {
+#pragma unroll
+            for (int q = 0; q < V / 2; ++q) reinterpret_cast<fx4*>(sums)[q * NV * G + i * G + lane] = fx4{0.f, 0.f, 0.f, 0.f};
+        }
     }
-    for (int64_t r0 = static_cast<int64_t>(blockIdx.x) * Gr::kGroups; r0 < a.rows;
-         r0 += static_cast<int64_t>(a.blocks) * Gr::kGroups) {
-        const bool live = r0 + own < a.rows;
-        const int64_t row = live ? r0 + own : 0;
+    // A workgroup's registers leave one or two of them to a CU: the next row's loads are
+    // under way during this one's sums.
+    constexpr bool AHEAD = G >= 256;
+    struct Row {
+        ux4 x[NV], g[NV];
+        float mean, by;
+    };
+    const int64_t step = static_cast<int64_t>(a.blocks) * Gr::kGroups;
+    auto fetch = [&](int64_t r0, Row& f) {
+        const int64_t row = r0 + own < a.rows ? r0 + own : 0;
         const T* x = static_cast<const T*>(a.x) + row * a.x_stride;
         const T* g = static_cast<const T*>(a.grad_y) + row * a.gy_stride;
-        ux4 xs[NV], gs[NV], more[NV];
 #pragma unroll
         for (int i = 0; i < NV; ++i) {
-            xs[i] = load_bits(x, (i * G + lane) * V, a.n);
-            gs[i] = load_bits(g, (i * G + lane) * V, a.n);
+            f.x[i] = load_bits<T, WHOLE>(x, (i * G + lane) * V, a.n);
+            f.g[i] = load_bits<T, WHOLE>(g, (i * G + lane) * V, a.n);
         }
+        f.mean = a.stats[2 * row], f.by = a.stats[2 * row + 1];
+    };
+    Row cur, next;
+    int64_t r0 = static_cast<int64_t>(blockIdx.x) * Gr::kGroups;
+    if (AHEAD && r0 < a.rows) fetch(r0, cur);
+    for (; r0 < a.rows; r0 += step) {
+        const bool live = r0 + own < a.rows;
+        const int64_t row = live ? r0 + own : 0;
+        if constexpr (!AHEAD) fetch(r0, cur);
+        ux4 more[NV];
         if (a.grad_s) {
             const T* s = static_cast<const T*>(a.grad_s) + row * a.gs_stride;
 #pragma unroll
-            for (int i = 0; i < NV; ++i) more[i] = load_bits(s, (i * G + lane) * V, a.n);
+            for (int i = 0; i < NV; ++i) more[i] = load_bits<T, WHOLE>(s, (i * G + lane) * V, a.n);
         }
-        const float mean = a.stats[2 * row], by = a.stats[2 * row + 1];
+        if (AHEAD && r0 + step < a.rows) fetch(r0 + step, next);
+        const float mean = cur.mean, by = cur.by;
         float h[NV][V], d[NV][V], s1 = 0.f, s2 = 0.f;
 #pragma unroll
         for (int i = 0; i < NV; ++i) {
             const int c = (i * G + lane) * V;
             float m[V];
-            unpack<T>(xs[i], h[i]);
-            unpack<T>(gs[i], d[i]);
+            unpack<T>(cur.x[i], h[i]);
+            unpack<T>(cur.g[i], d[i]);
             if (a.weight) unpack<T>(w[i], m);
 #pragma unroll
-            for (int k = 0; k < V; ++k) {
+            for (int k = 0; k < V; ++k)
                 // past the row's end nothing: there x is 0, and less the mean no number
                 // that 0 would take away where the mean is none
-                h[i][k] = c + k < a.n ? (h[i][k] - mean) * by : 0.f;
-                if (live) {
+                h[i][k] = (WHOLE ? c : c + k) < a.n ? (h[i][k] - mean) * by : 0.f;
+            if constexpr (IN_LDS) {
+                add_columns<V>(sums, i * G + lane, NV * G, h[i], d[i]);
+            } else if (live) {
+#pragma unroll
+                for (int k = 0; k < V; ++k) {
                     gw[i][k] = fma_acc(d[i][k], h[i][k], gw[i][k]);
                     gb[i][k] += d[i][k];
                 }
+            }
+#pragma unroll
+            for (int k = 0; k < V; ++k) {
                 if (a.weight) d[i][k] *= m[k];
                 s1 += d[i][k];
                 s2 = fma_acc(d[i][k], h[i][k], s2);
@@ -250,21 +304,34 @@ __global__ __launch_bounds__(Group<G>::kThreads) void layer_norm_backward_kernel
         }
         group.sum(s1, s2);
         s1 *= a.inv_n, s2 *= a.inv_n;
-        if (!live || !a.gx) continue;
+        if (live && a.gx) {
 #pragma unroll
-        for (int i = 0; i < NV; ++i) {
-            float m[V];
-            if (a.grad_s) unpack<T>(more[i], m);
+            for (int i = 0; i < NV; ++i) {
+                float m[V];
+                if (a.grad_s) unpack<T>(more[i], m);
 #pragma unroll
-            for (int k = 0; k < V; ++k) {
-                d[i][k] = (d[i][k] - s1 - h[i][k] * s2) * by;
-                if (a.grad_s) d[i][k] += m[k];
+                for (int k = 0; k < V; ++k) {
+                    d[i][k] = (d[i][k] - s1 - h[i][k] * s2) * by;
+                    if (a.grad_s) d[i][k] += m[k];
+                }
+                store_bits<T, WHOLE>(static_cast<T*>(a.gx) + row * a.n, (i * G + lane) * V, a.n, pack<T>(d[i]));
             }
-            store_bits(static_cast<T*>(a.gx) + row * a.n, (i * G + lane) * V, a.n, pack<T>(d[i]));
         }
+        if constexpr (AHEAD) cur = next;
     }
     if (!a.partial) return;
     float* to = a.partial + static_cast<int64_t>(blockIdx.x) * 2 * a.n;
+    if constexpr (IN_LDS) {
+#pragma unroll
+        for (int i = 0; i < NV; ++i)
+#pragma unroll
+            for (int q = 0; q < V / 4; ++q) {
+                const fx4 x = reinterpret_cast<fx4*>(sums)[q * NV * G + i * G + lane];
+                const fx4 y = reinterpret_cast<fx4*>(sums)[(V / 4 + q) * NV * G + i * G + lane];
+#pragma unroll
+                for (int e = 0; e < 4; ++e) gw[i][4 * q + e] = x[e], gb[i][4 * q + e] = y[e];
+            }
+    }
     add_groups<G, NV, V>(gw, to, a.n, lds);
     add_groups<G, NV, V>(gb, to + a.n, a.n, lds);
 }
@@ -420,27 +487,33 @@ __global__ __launch_bounds__(1024) void layer_norm_weights_kernel(LayerNormArgs 
 
 // Workgroups that walk the rows: enough to fill the card; in the backward few
 // enough that their sums of the weights' gradients stay small next to the rows.
-static int norm_row_blocks(int64_t rows, int per, bool bwd) {
-    const int64_t most = static_cast<int64_t>(nsh_host::compute_units()) * (bwd ? 2 : 8);
-    return static_cast<int>(std::min(nsh_host::ceil_div(rows, per), most));
+static int norm_row_blocks(int64_t rows, int per, int64_t each) {
+    return static_cast<int>(std::min(nsh_host::ceil_div(rows, per), nsh_host::compute_units() * each));
 }
+constexpr int kMostNormBlocks = 2;  // of the backward, a CU
 
-template <typename T, int G, int NV>
-static int layer_norm_launch(LayerNormArgs a, bool bwd, hipStream_t st) {
+template <typename T, int G, int NV, bool WHOLE>
+static int layer_norm_rows(LayerNormArgs a, bool bwd, hipStream_t st) {
     using Gr = Group<G>;
-    a.blocks = norm_row_blocks(a.rows, Gr::kGroups, bwd);
+    // (rows of a workgroup: one each; the 512 lanes' registers leave one workgroup to a CU)
+    a.blocks = norm_row_blocks(a.rows, Gr::kGroups, bwd ? (G == 512 ? 1 : kMostNormBlocks) : G > 64 ? int64_t(1) << 20 : 8);
     if (!bwd) {
-        layer_norm_forward_kernel<T, G, NV><<<a.blocks, Gr::kThreads, 0, st>>>(a);
+        layer_norm_forward_kernel<T, G, NV, WHOLE><<<a.blocks, Gr::kThreads, 0, st>>>(a);
         return nsh_host::check_launch("layer_norm_forward");
     }
-    layer_norm_backward_kernel<T, G, NV><<<a.blocks, Gr::kThreads, 0, st>>>(a);
+    layer_norm_backward_kernel<T, G, NV, WHOLE><<<a.blocks, Gr::kThreads, 0, st>>>(a);
     if (a.partial) layer_norm_weights_kernel<T><<<dim3((a.n + 31) / 32, 2), 1024, 0, st>>>(a);
     return nsh_host::check_launch("layer_norm_backward");
 }
 
+template <typename T, int G, int NV>
+static int layer_norm_launch(const LayerNormArgs& a, bool bwd, hipStream_t st) {
+    return a.n % kVec<T> ? layer_norm_rows<T, G, NV, false>(a, bwd, st) : layer_norm_rows<T, G, NV, true>(a, bwd, st);
+}
+
 template <typename T>
 static int layer_norm_wide(LayerNormArgs a, bool bwd, hipStream_t st) {
-    a.blocks = norm_row_blocks(a.rows, 1, bwd);
+    a.blocks = norm_row_blocks(a.rows, 1, bwd ? kMostNormBlocks : 8);
     if (!bwd) {
         layer_norm_wide_forward_kernel<T><<<a.blocks, kWideThreads, 0, st>>>(a);
         return nsh_host::check_launch("layer_norm_forward");
@@ -468,7 +541,7 @@ static int layer_norm_dispatch(const LayerNormArgs& a, bool bwd, hipStream_t st)
     if (parts <= 128) return layer_norm_launch<T, 64, 2>(a, bwd, st);
     if (parts <= 256) return layer_norm_launch<T, 64, 4>(a, bwd, st);
     if (parts <= 512) return layer_norm_launch<T, 256, 2>(a, bwd, st);
-    if (parts <= 1024) return layer_norm_launch<T, 256, 4>(a, bwd, st);
+    if (parts <= 1024) return layer_norm_launch<T, 512, 2>(a, bwd, st);
     if (parts <= 2048) return layer_norm_launch<T, 512, 4>(a, bwd, st);
     return layer_norm_wide<T>(a, bwd, st);
 }
@@ -479,7 +552,7 @@ using nsh_host::fail;
 
 extern "C" int64_t nsh_layer_norm_workspace_bytes(const nsh_layer_norm_args* g) {
     if (!g || g->rows < 1 || g->n < 1) return -1;
-    return static_cast<int64_t>(nsh::norm_row_blocks(g->rows, 1, true)) * 2 * g->n * 4;
+    return static_cast<int64_t>(nsh::norm_row_blocks(g->rows, 1, nsh::kMostNormBlocks)) * 2 * g->n * 4;
 }
 
 static int layer_norm(const char* op, const nsh_layer_norm_args* g, bool bwd, void* stream) {

@@ -14,10 +14,14 @@ template <typename T> constexpr int kVec = 16 / sizeof(T);
 
 // Columns c .. c + kVec - 1 of a row of n, those past its end as zeros.  Rows need
 // no alignment beyond an element's: gfx950 splits a load that crosses a line.
-template <typename T>
+// WHOLE: n is a multiple of kVec (the path by elements costs a kernel up to a hundred
+// registers).
+template <typename T, bool WHOLE = false>
 __device__ __forceinline__ ux4 load_bits(const T* row, int c, int n) {
     ux4 r = {0, 0, 0, 0};
-    if (c + kVec<T> <= n) {
+    if constexpr (WHOLE) {
+        if (c < n) __builtin_memcpy(&r, row + c, 16);
+    } else if (c + kVec<T> <= n) {
         __builtin_memcpy(&r, row + c, 16);
     } else if (c < n) {
         T e[kVec<T>] = {};
@@ -53,9 +57,11 @@ __device__ __forceinline__ ux4 pack(const float (&v)[kVec<T>]) {
     }
 }
 
-template <typename T>
+template <typename T, bool WHOLE = false>
 __device__ __forceinline__ void store_bits(T* row, int c, int n, ux4 r) {
-    if (c + kVec<T> <= n) {
+    if constexpr (WHOLE) {
+        if (c < n) __builtin_memcpy(row + c, &r, 16);
+    } else if (c + kVec<T> <= n) {
         __builtin_memcpy(row + c, &r, 16);
     } else if (c < n) {
         T e[kVec<T>];
