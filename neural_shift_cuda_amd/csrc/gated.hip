@@ -8,9 +8,13 @@
 
 namespace nsh {
 
-NSH_GATED_ENTRIES(extern, f16)
-NSH_GATED_ENTRIES(extern, bf16)
-NSH_GATED_ENTRIES(extern, float)
+NSH_GATED_ENTRIES(extern, f16, false)
+NSH_GATED_ENTRIES(extern, bf16, false)
+NSH_GATED_ENTRIES(extern, float, false)
+NSH_GATED_ENTRIES(extern, float, true)
+NSH_GATED_FEW_ROWS(extern, f16)
+NSH_GATED_FEW_ROWS(extern, bf16)
+NSH_GATED_FEW_ROWS(extern, float)
 
 constexpr int kPassThreads = 256;
 
@@ -37,9 +41,34 @@ __global__ __launch_bounds__(kPassThreads) void gated_copy_kernel(CopyArgs a) {
     }
 }
 
+// The same into three planes of bf16.
+__global__ __launch_bounds__(kPassThreads) void gated_split_kernel(CopyArgs a) {
+    const CopyArgs::Side& s = a.side[blockIdx.y];
+    const int each = a.np / 8;
+    const int64_t all = s.rows * each, step = static_cast<int64_t>(gridDim.x) * kPassThreads, plane = s.rows * a.np;
+    for (int64_t i = static_cast<int64_t>(blockIdx.x) * kPassThreads + threadIdx.x; i < all; i += step) {
+        const int64_t row = i / each;
+        const int c = static_cast<int>(i - row * each) * 8;
+        const float* from = static_cast<const float*>(s.from) + row * s.stride;
+        float x[8], part[3][8];
+        unpack<float>(load_bits(from, c, a.n), *reinterpret_cast<float(*)[4]>(&x[0]));
+        unpack<float>(load_bits(from, c + 4, a.n), *reinterpret_cast<float(*)[4]>(&x[4]));
+#pragma unroll
+        for (int e = 0; e < 8; ++e) {
+            float p[3];
+            split(x[e], p);
+#pragma unroll
+            for (int k = 0; k < 3; ++k) part[k][e] = p[k];
+        }
+#pragma unroll
+        for (int k = 0; k < 3; ++k)
+            *reinterpret_cast<ux4*>(static_cast<bf16*>(s.to) + k * plane + row * a.np + c) = pack<bf16>(part[k]);
+    }
+}
+
 struct SlopeArgs {
     const void* gh;
-    int64_t gh_stride, rows, dgu_stride;  // elements
+    int64_t gh_stride, rows, dgu_stride, dgu_plane;  // elements
     char* kept;
     void* dgu;
     int F, Fp;
@@ -48,8 +77,9 @@ struct SlopeArgs {
 };
 
 // dg and du: a wave has 32 rows and 128 bytes of each, blocks of what was kept.
-template <typename T>
+template <typename T, bool PARTS>
 __global__ __launch_bounds__(kPassThreads) void gated_slope_kernel(SlopeArgs a) {
+    using E = typename Parts<T, PARTS>::E;
     constexpr int COLS = 128 / sizeof(T), BLOCKS = COLS / 32;
     using S = Stage<T, 32, COLS>;
     __shared__ __attribute__((aligned(256))) char stages[kPassThreads / 64][S::BYTES];
@@ -74,11 +104,25 @@ __global__ __launch_bounds__(kPassThreads) void gated_slope_kernel(SlopeArgs a) 
         // activation at 0, a number)
 #pragma unroll
         for (int b = 0; b < BLOCKS; ++b) x[b] = c0 + 32 * b < a.F ? d[b] * k[b].factor(side) : f32x16{};
-        wave_exchange();
+        using To = Stage<E, 32, COLS>;
+        E* to = static_cast<E*>(a.dgu) + m0 * a.dgu_stride + side * a.Fp + c0;
+        f32x16 parts[PARTS ? 3 : 1];
+        if constexpr (PARTS) {
 #pragma unroll
-        for (int b = 0; b < BLOCKS; ++b) S::put(stage, 0, b, x[b]);
-        wave_exchange();
-        S::store(stage, static_cast<T*>(a.dgu) + m0 * a.dgu_stride + side * a.Fp + c0, a.dgu_stride, rows, COLS);
+            for (int r = 0; r < 16; ++r) {
+                float p[3];
+                split(x[0][r], p);
+                parts[0][r] = p[0], parts[1][r] = p[1], parts[2][r] = p[2];
+            }
+        }
+#pragma unroll
+        for (int n = 0; n < (PARTS ? 3 : 1); ++n) {
+            wave_exchange();
+#pragma unroll
+            for (int b = 0; b < BLOCKS; ++b) To::put(stage, 0, b, PARTS ? parts[n] : x[b]);
+            wave_exchange();
+            To::store(stage, to + n * a.dgu_plane, a.dgu_stride, rows, COLS);
+        }
     }
 }
 
@@ -205,18 +249,35 @@ constexpr int64_t kWidest = int64_t(1) << 20;
 constexpr int64_t kStep = int64_t(1) << 23;  // bytes from a row to the next that a panel's 32-bit offsets take
 
 struct Plan {
-    int64_t esz, Kp, Fp;
-    bool copy[3];       // x, gate, up
-    int64_t copies[3];  // offsets in the workspace
+    bool few, parts;       // up to 64 rows; fp32 by bf16 products
+    int64_t esz, Kp, Fp;   // esz: bytes of the products' elements
+    bool copy[3];          // x, gate, up
+    int64_t copies[3];     // offsets in the workspace
+    int64_t planes;        // bytes of dgu's parts
     int64_t dgu, scale, most, part, bytes;
     nsh::Cut cut;
 };
 
 int64_t up(int64_t v, int64_t to) { return ceil_div(v, to) * to; }
 
+nsh::Cut cut_of(const nsh_gated_linear_args* g, bool bwd, nsh::Means by) {
+    return bwd ? nsh::gradient_cut(g->rows, g->K, g->F, by, g->grad_x != nullptr, g->grad_gate || g->grad_up)
+               : nsh::forward_cut(g->rows, g->F, g->K, by);
+}
+
 Plan plan_of(const nsh_gated_linear_args* g, bool bwd) {
     Plan p{};
-    p.esz = g->dtype == NSH_DTYPE_FLOAT32 ? 4 : 2;
+    const bool wide = g->dtype == NSH_DTYPE_FLOAT32;
+    p.few = !bwd && !g->kept && g->rows <= nsh::kFewRows;
+    if (!p.few) p.cut = cut_of(g, bwd, {wide, 1});
+    if (wide && !p.few) {
+        // against the time of taking the parts: 4 bytes read, 6 written and read once more
+        nsh::Cut parts = cut_of(g, bwd, {false, 6});
+        parts.time += 4 + static_cast<double>((g->rows + 2 * g->F) * g->K) * 10 / 3.5e6;
+        p.parts = parts.time < p.cut.time;
+        if (p.parts) p.cut = parts;
+    }
+    p.esz = wide && !p.parts ? 4 : 2;
     const int64_t vec = 16 / p.esz;
     p.Kp = up(g->K, vec), p.Fp = up(g->F, 64);
     const void* at[3] = {g->x, g->gate_weight, g->up_weight};
@@ -224,25 +285,23 @@ Plan plan_of(const nsh_gated_linear_args* g, bool bwd) {
     for (int i = 0; i < 3; ++i) {
         // (a single row has no step to the next)
         const bool steps = rows[i] == 1 || (stride[i] % vec == 0 && stride[i] >= g->K && stride[i] * p.esz <= kStep);
-        p.copy[i] = g->K % vec != 0 || !nsh_host::aligned(at[i], 16) || !steps;
+        p.copy[i] = p.parts || g->K % vec != 0 || !nsh_host::aligned(at[i], 16) || !steps;
         p.copies[i] = p.bytes;
-        if (p.copy[i]) p.bytes += up(rows[i] * p.Kp * p.esz, 256);
+        if (p.copy[i]) p.bytes += up(rows[i] * p.Kp * p.esz * (p.parts ? 3 : 1), 256);
     }
     if (!bwd) return p;
     p.dgu = p.bytes;
-    p.bytes += up(g->rows * (2 * p.Fp * p.esz + 128), 256);
+    p.planes = g->rows * (2 * p.Fp * p.esz + 128);
+    p.bytes += up(p.planes * (p.parts ? 3 : 1), 256);
     p.scale = p.bytes, p.bytes += 256;
     p.most = p.bytes, p.bytes += up(nsh::kMostBlocks * 4, 256);
     p.part = p.bytes;
-    p.cut = nsh::gradient_cut(g->rows, g->K, p.Fp, g->F, p.esz == 4, g->grad_x != nullptr, g->grad_gate || g->grad_up);
     if (p.cut.splits > 1) p.bytes += up(p.cut.splits * g->rows * up(g->K, 4) * 4, 256);
     return p;
 }
 
-int64_t forward_blocks(const nsh_gated_linear_args* g) {
-    const bool wide = g->dtype == NSH_DTYPE_FLOAT32;
-    return nsh::forward_cut(g->rows, g->F, up(g->K, wide ? 4 : 8), wide).tiles();
-}
+// (fp16: of the forward that keeps what the backward needs)
+int64_t forward_blocks(const nsh_gated_linear_args* g) { return cut_of(g, false, {false, 1}).tiles(); }
 
 int64_t kept_blocks(const nsh_gated_linear_args* g) {
     const int64_t each = g->dtype == NSH_DTYPE_FLOAT32    ? nsh::Kept<float>::BYTES
@@ -274,6 +333,7 @@ int copy_rows(const nsh_gated_linear_args* g, const Plan& p, nsh::GatedArgs& a, 
     int64_t most = 0;
     const void** at[3] = {&a.x, &a.wg, &a.wu};
     uint32_t* stride[3] = {&a.x_stride, &a.wg_stride, &a.wu_stride};
+    int64_t* plane[3] = {&a.x_plane, &a.wg_plane, &a.wu_plane};
     const int64_t steps[3] = {g->x_stride, g->gate_stride, g->up_stride}, rows[3] = {g->rows, g->F, g->F};
     for (int i = 0; i < 3; ++i) {
         *stride[i] = static_cast<uint32_t>(rows[i] == 1 ? p.Kp * p.esz : steps[i] * p.esz);
@@ -281,16 +341,21 @@ int copy_rows(const nsh_gated_linear_args* g, const Plan& p, nsh::GatedArgs& a, 
         c.side[n++] = {*at[i], ws + p.copies[i], rows[i], steps[i]};
         *at[i] = ws + p.copies[i];
         *stride[i] = static_cast<uint32_t>(p.Kp * p.esz);
+        *plane[i] = rows[i] * p.Kp * p.esz;
         most = std::max(most, rows[i] * (p.Kp * p.esz / 16));
     }
     if (!n) return NSH_OK;
     c.n = static_cast<int>(g->K), c.np = static_cast<int>(p.Kp);
     const int64_t blocks = std::min<int64_t>(ceil_div(most, nsh::kPassThreads), nsh_host::compute_units() * 16);
-    nsh::gated_copy_kernel<T><<<dim3(static_cast<unsigned>(blocks), n), nsh::kPassThreads, 0, st>>>(c);
+    const dim3 grid(static_cast<unsigned>(blocks), n);
+    if (p.parts)
+        nsh::gated_split_kernel<<<grid, nsh::kPassThreads, 0, st>>>(c);
+    else
+        nsh::gated_copy_kernel<T><<<grid, nsh::kPassThreads, 0, st>>>(c);
     return nsh_host::check_launch("gated_linear");
 }
 
-template <typename T>
+template <typename T, bool PARTS>
 int backward(const nsh_gated_linear_args* g, const Plan& p, nsh::GatedArgs a, char* ws, hipStream_t st) {
     float* scale = nullptr;
     if constexpr (__is_same(T, nsh::f16)) {
@@ -305,12 +370,13 @@ int backward(const nsh_gated_linear_args* g, const Plan& p, nsh::GatedArgs a, ch
         nsh::gated_scale_kernel<<<1, nsh::kPassThreads, 0, st>>>(most, static_cast<int>(n), reinterpret_cast<const float*>(a.kept + kept_blocks(g)), static_cast<int>(forward_blocks(g)), scale);
     }
     a.scale = scale, a.dgu = ws + p.dgu;
-    const uint32_t across = static_cast<uint32_t>(ceil_div(a.Fp, nsh::kPassThreads / 64 * 128 / p.esz));
-    const nsh::SlopeArgs s{g->grad_h, g->gh_stride, g->rows, 2 * p.Fp + 128 / p.esz, a.kept, a.dgu, a.F, a.Fp, across, scale};
-    nsh::gated_slope_kernel<T><<<static_cast<unsigned>(across * ceil_div(g->rows, 32)), nsh::kPassThreads, 0, st>>>(s);
+    a.dgu_plane = p.planes;
+    const uint32_t across = static_cast<uint32_t>(ceil_div(a.Fp, nsh::kPassThreads / 64 * 128 / sizeof(T)));
+    const nsh::SlopeArgs s{g->grad_h, g->gh_stride, g->rows, 2 * p.Fp + 128 / p.esz, p.planes / p.esz, a.kept, a.dgu, a.F, a.Fp, across, scale};
+    nsh::gated_slope_kernel<T, PARTS><<<static_cast<unsigned>(across * ceil_div(g->rows, 32)), nsh::kPassThreads, 0, st>>>(s);
     a.Kq = static_cast<int>(up(g->K, 4));
     a.part = p.cut.splits > 1 ? reinterpret_cast<float*>(ws + p.part) : nullptr;
-    const int rc = nsh::gated_gradients<T>(a, p.cut, st);
+    const int rc = nsh::gated_gradients<T, PARTS>(a, p.cut, st);
     if (rc != NSH_OK || !a.part) return rc;
     return nsh::gated_join<T>(a, p.cut.splits, st);
 }
@@ -327,9 +393,12 @@ int run(const nsh_gated_linear_args* g, const Plan& p, bool bwd, hipStream_t st)
     const int rc = copy_rows<T>(g, p, a, ws, st);
     if (rc != NSH_OK) return rc;
     a.kept = static_cast<char*>(g->kept);
-    if (bwd) return backward<T>(g, p, a, ws, st);
+    if constexpr (sizeof(T) == 4)
+        if (p.parts) return bwd ? backward<T, true>(g, p, a, ws, st) : nsh::gated_forward<T, true>(a, p.cut, st);
+    if (bwd) return backward<T, false>(g, p, a, ws, st);
+    if (p.few) return nsh::gated_few_rows<T>(a, st);
     if (__is_same(T, nsh::f16) && a.kept) a.most = reinterpret_cast<float*>(a.kept + kept_blocks(g));
-    return nsh::gated_forward<T>(a, st);
+    return nsh::gated_forward<T, false>(a, p.cut, st);
 }
 
 int gated_linear(const char* op, const nsh_gated_linear_args* g, bool bwd, void* stream) {

@@ -28,6 +28,7 @@ namespace nsh {
 struct GatedArgs {
     const void *x, *wg, *wu;
     uint32_t x_stride, wg_stride, wu_stride;  // bytes from row to row
+    int64_t x_plane, wg_plane, wu_plane, dgu_plane;  // bytes from a part to the next (struct Parts)
     int64_t rows;
     int K, F, Kp, Fp;     // Kp: columns of x and the weights as they lie; Fp: F in whole panels
     int activation;
@@ -230,16 +231,43 @@ __device__ __forceinline__ f32x16 gate_block(const GatedArgs& a, int64_t m, int 
     return h * u;
 }
 
-// Bytes of a row of dgu: not a power of two, which would have every row's same place in
-// one channel of the caches.
-template <typename T>
-__device__ __forceinline__ uint32_t dgu_stride(const GatedArgs& a) {
-    return 2 * a.Fp * static_cast<uint32_t>(sizeof(T)) + 128;
+// fp32 by bf16 products: a number is the sum of three of bf16, 24 bits in all, and the six
+// products of parts that are not below 2^-24 are summed, the smallest first, by the same
+// panels and six times as many.  A product of fp32 matrices takes 16 times as long as one
+// of bf16.  (2048 x 1024 -> 2816: forward 219 us by fp32 products, gradients 407.)
+template <typename T, bool PARTS>
+struct Parts {
+    using E = std::conditional_t<PARTS, bf16, T>;
+    static constexpr int N = PARTS ? 6 : 1;
+    // which parts (0: the largest) of the two sides the n-th product takes
+    static __device__ __forceinline__ int first(int n) { return PARTS ? 0x052 >> 2 * n & 3 : 0; }
+    static __device__ __forceinline__ int second(int n) { return PARTS ? 0x118 >> 2 * n & 3 : 0; }
+};
+
+// x as such a sum.  Each rounding is off by half a step of bf16 and leaves the rest exactly;
+// what is no number is in the last part alone, which meets the other side's largest only.
+__device__ __forceinline__ void split(float x, float (&part)[3]) {
+    constexpr float most = 3.3895313892515355e38f;  // bf16's largest: beyond it the rounding would be infinite
+    const bool number = fabsf(x) < INFINITY;
+    const float v = number ? x : 0.f;
+    part[0] = static_cast<float>(static_cast<__bf16>(fminf(fmaxf(v, -most), most)));
+    const float rest = v - part[0];
+    part[1] = static_cast<float>(static_cast<__bf16>(rest));
+    part[2] = number ? rest - part[1] : x;
 }
 
-template <typename T, int BM, int BN, int WAVES_M, int WAVES_N, int KB>
+// Bytes of a row of dgu: not a power of two, which would have every row's same place in
+// one channel of the caches.
+template <typename E>
+__device__ __forceinline__ uint32_t dgu_stride(const GatedArgs& a) {
+    return 2 * a.Fp * static_cast<uint32_t>(sizeof(E)) + 128;
+}
+
+template <typename T, bool PARTS, int BM, int BN, int WAVES_M, int WAVES_N, int KB>
 __global__ __launch_bounds__(64 * WAVES_M * WAVES_N, 2) void gated_forward_kernel(GatedArgs a) {
-    using P = Product<T, BM, BN, WAVES_M, WAVES_N, KB, kAlong, kAlong, true>;
+    using Of = Parts<T, PARTS>;
+    using E = typename Of::E;
+    using P = Product<E, BM, BN, WAVES_M, WAVES_N, KB, kAlong, kAlong, true>;
     __shared__ __attribute__((aligned(1024))) char f0[P::FIRST_BYTES], s0[P::SECOND_BYTES];
     __shared__ __attribute__((aligned(1024))) char f1[P::FIRST_BYTES], s1[P::SECOND_BYTES];
     const TileOrder t(blockIdx.x, gridDim.x, a.tiles_m, a.tiles_n, 8);
@@ -253,17 +281,16 @@ __global__ __launch_bounds__(64 * WAVES_M * WAVES_N, 2) void gated_forward_kerne
     const char* x = static_cast<const char*>(a.x) + m0 * a.x_stride;
     const char* wg = static_cast<const char*>(a.wg) + static_cast<int64_t>(c0) * a.wg_stride;
     const char* wu = static_cast<const char*>(a.wu) + static_cast<int64_t>(c0) * a.wu_stride;
-    const int64_t wide = static_cast<int64_t>(a.Kp) * sizeof(T);
+    const int64_t wide = static_cast<int64_t>(a.Kp) * sizeof(E);
     const int left_m = static_cast<int>(min(a.rows - m0, int64_t(BM)));
     P p;
     p.init();
-    const int n = (a.Kp + P::BK - 1) / P::BK;
-    p.run(n, f0, s0, f1, s1, [&](int i, char* f, char* s) {
-        const int64_t at = static_cast<int64_t>(i) * KB;
-        const int left_f = i < n ? a.F - c0 : 0;
-        gate.load(f, wg + at, a.wg_stride, left_f, wide - at, wave);
-        up.load(f + P::FIRST_BYTES / 2, wu + at, a.wu_stride, left_f, wide - at, wave);
-        rows.load(s, x + at, a.x_stride, i < n ? left_m : 0, wide - at, wave);
+    p.run((a.Kp + P::BK - 1) / P::BK * Of::N, f0, s0, f1, s1, [&](int i, char* f, char* s) {
+        const int block = i / Of::N, term = i % Of::N;
+        const int64_t at = static_cast<int64_t>(block) * KB;
+        gate.load(f, wg + Of::first(term) * a.wg_plane + at, a.wg_stride, a.F - c0, wide - at, wave);
+        up.load(f + P::FIRST_BYTES / 2, wu + Of::first(term) * a.wu_plane + at, a.wu_stride, a.F - c0, wide - at, wave);
+        rows.load(s, x + Of::second(term) * a.x_plane + at, a.x_stride, left_m, wide - at, wave);
     });
     float most = 0.f;
     const int64_t m = m0 + P::wave_m() * P::WM;
@@ -289,10 +316,10 @@ __global__ __launch_bounds__(64 * WAVES_M * WAVES_N, 2) void gated_forward_kerne
 }
 
 // dx: over the hidden columns of dg, then of du.
-template <typename P>
+template <typename T, typename Of, typename P>
 __device__ __forceinline__ void input_gradient(const GatedArgs& a, uint32_t id, char (&f0)[P::FIRST_BYTES], char (&s0)[P::SECOND_BYTES],
                                                char (&f1)[P::FIRST_BYTES], char (&s1)[P::SECOND_BYTES]) {
-    using T = typename P::T;
+    using E = typename P::T;
     const uint32_t tiles = static_cast<uint32_t>(a.tiles_m) * a.tiles_n;
     const int split = TileOrder::uniform(id / tiles);
     const TileOrder t(id - split * tiles, tiles, a.tiles_m, a.tiles_n, 8);
@@ -303,25 +330,26 @@ __device__ __forceinline__ void input_gradient(const GatedArgs& a, uint32_t id, 
     typename P::SecondPanel rows;
     gate.init(a.wg_stride);
     up.init(a.wu_stride);
-    const uint32_t stride = dgu_stride<T>(a);
+    const uint32_t stride = dgu_stride<E>(a);
     rows.init(stride);
     const char* d = static_cast<const char*>(a.dgu) + m0 * stride;
-    const char* wg = static_cast<const char*>(a.wg) + c0 * static_cast<int64_t>(sizeof(T));
-    const char* wu = static_cast<const char*>(a.wu) + c0 * static_cast<int64_t>(sizeof(T));
+    const char* wg = static_cast<const char*>(a.wg) + c0 * static_cast<int64_t>(sizeof(E));
+    const char* wu = static_cast<const char*>(a.wu) + c0 * static_cast<int64_t>(sizeof(E));
     const int left_m = static_cast<int>(min(a.rows - m0, int64_t(P::BM)));
-    const int64_t left_c = (a.Kp - c0) * static_cast<int64_t>(sizeof(T));
-    const int half = a.Fp / P::BK, all = 2 * half;
+    const int64_t left_c = (a.Kp - c0) * static_cast<int64_t>(sizeof(E));
+    const int half = a.Fp / P::BK, all = 2 * half * Of::N;
     const int begin = TileOrder::uniform(all * static_cast<uint32_t>(split) / a.splits);
     const int end = TileOrder::uniform(all * static_cast<uint32_t>(split + 1) / a.splits);
     P p;
     p.init();
     p.run(end - begin, f0, s0, f1, s1, [&](int i, char* f, char* s) {
-        const int at = begin + i, in = at < half ? at : at - half;
-        const bool one = at < half;
+        const int block = (begin + i) / Of::N, term = (begin + i) % Of::N;
+        const bool one = block < half;
+        const int64_t row = static_cast<int64_t>(one ? block : block - half) * P::BK;
         const uint32_t step = one ? a.wg_stride : a.wu_stride;
-        P::FirstPanel::either(one, gate, up).load(f, (one ? wg : wu) + static_cast<int64_t>(in) * P::BK * step, step,
-                                                  at < end ? a.F - in * P::BK : 0, left_c, wave);
-        rows.load(s, d + static_cast<int64_t>(at) * P::KB, stride, at < end ? left_m : 0, P::KB, wave);
+        const int64_t plane = Of::first(term) * (one ? a.wg_plane : a.wu_plane);
+        P::FirstPanel::either(one, gate, up).load(f, (one ? wg : wu) + plane + row * step, step, a.F - static_cast<int>(row), left_c, wave);
+        rows.load(s, d + Of::second(term) * a.dgu_plane + static_cast<int64_t>(block) * P::KB, stride, left_m, P::KB, wave);
     });
     const float by = __is_same(T, f16) && a.scale ? a.scale[1] : 1.f;
     const int64_t m = m0 + P::wave_m() * P::WM, c = c0 + P::column(0);
@@ -335,10 +363,10 @@ __device__ __forceinline__ void input_gradient(const GatedArgs& a, uint32_t id, 
 }
 
 // Both weights' gradients: tiles of hidden rows of the one, then of the other.
-template <typename P>
+template <typename T, typename Of, typename P>
 __device__ __forceinline__ void weight_gradient(const GatedArgs& a, uint32_t id, char (&f0)[P::FIRST_BYTES], char (&s0)[P::SECOND_BYTES],
                                                 char (&f1)[P::FIRST_BYTES], char (&s1)[P::SECOND_BYTES]) {
-    using T = typename P::T;
+    using E = typename P::T;
     const int each = a.weight_m / 2;
     const TileOrder t(id, static_cast<uint32_t>(a.weight_m) * a.weight_n, a.weight_m, a.weight_n, 8);
     const int side = t.m >= each;
@@ -350,19 +378,19 @@ __device__ __forceinline__ void weight_gradient(const GatedArgs& a, uint32_t id,
     typename P::FirstPanel in;
     typename P::SecondPanel d;
     in.init(a.x_stride);
-    const uint32_t stride = dgu_stride<T>(a);
+    const uint32_t stride = dgu_stride<E>(a);
     d.init(stride);
-    const char* x = static_cast<const char*>(a.x) + c0 * static_cast<int64_t>(sizeof(T));
-    const char* dgu = static_cast<const char*>(a.dgu) + (static_cast<int64_t>(side) * a.Fp + f_first) * static_cast<int64_t>(sizeof(T));
-    const int64_t left_c = (a.Kp - c0) * static_cast<int64_t>(sizeof(T));
-    const int64_t left_f = (static_cast<int64_t>(a.Fp) - f_first) * static_cast<int64_t>(sizeof(T));
+    const char* x = static_cast<const char*>(a.x) + c0 * static_cast<int64_t>(sizeof(E));
+    const char* dgu = static_cast<const char*>(a.dgu) + (static_cast<int64_t>(side) * a.Fp + f_first) * static_cast<int64_t>(sizeof(E));
+    const int64_t left_c = (a.Kp - c0) * static_cast<int64_t>(sizeof(E));
+    const int64_t left_f = (static_cast<int64_t>(a.Fp) - f_first) * static_cast<int64_t>(sizeof(E));
     P p;
     p.init();
-    p.run(static_cast<int>((a.rows + P::BK - 1) / P::BK), f0, s0, f1, s1, [&](int i, char* f, char* s) {
-        const int64_t at = static_cast<int64_t>(i) * P::BK;
-        const int left = static_cast<int>(max(min(a.rows - at, int64_t(P::BK)), int64_t(0)));
-        in.load(f, x + at * a.x_stride, a.x_stride, left, left_c, wave);
-        d.load(s, dgu + at * stride, stride, left, left_f, wave);
+    p.run(static_cast<int>((a.rows + P::BK - 1) / P::BK) * Of::N, f0, s0, f1, s1, [&](int i, char* f, char* s) {
+        const int64_t at = static_cast<int64_t>(i / Of::N) * P::BK;
+        const int term = i % Of::N, left = static_cast<int>(min(a.rows - at, int64_t(P::BK)));
+        in.load(f, x + Of::first(term) * a.x_plane + at * a.x_stride, a.x_stride, left, left_c, wave);
+        d.load(s, dgu + Of::second(term) * a.dgu_plane + at * stride, stride, left, left_f, wave);
     });
     const float by = __is_same(T, f16) && a.scale ? a.scale[1] : 1.f;
     const int64_t f = f_first + P::wave_m() * P::WM, c = c0 + P::column(0);
@@ -373,19 +401,21 @@ __device__ __forceinline__ void weight_gradient(const GatedArgs& a, uint32_t id,
 
 // Both, in one launch: neither alone fills the card but for large calls.  Whichever has the
 // longer workgroups comes first.
-template <typename T, int BM, int BN, int WAVES_M, int WAVES_N, int KB>
+template <typename T, bool PARTS, int BM, int BN, int WAVES_M, int WAVES_N, int KB>
 __global__ __launch_bounds__(64 * WAVES_M * WAVES_N, 2) void gated_gradients_kernel(GatedArgs a) {
-    using In = Product<T, BM, BN, WAVES_M, WAVES_N, KB, kAcross, kAlong, false>;
-    using Weights = Product<T, BM, BN, WAVES_M, WAVES_N, KB, kAcross, kAcross, false>;
+    using Of = Parts<T, PARTS>;
+    using E = typename Of::E;
+    using In = Product<E, BM, BN, WAVES_M, WAVES_N, KB, kAcross, kAlong, false>;
+    using Weights = Product<E, BM, BN, WAVES_M, WAVES_N, KB, kAcross, kAcross, false>;
     __shared__ __attribute__((aligned(1024))) char f0[In::FIRST_BYTES], s0[In::SECOND_BYTES];
     __shared__ __attribute__((aligned(1024))) char f1[In::FIRST_BYTES], s1[In::SECOND_BYTES];
     const uint32_t first = a.first;
     const bool second = blockIdx.x >= first;
     const uint32_t id = second ? blockIdx.x - first : blockIdx.x;
     if (second == a.weights_first)
-        input_gradient<In>(a, id, f0, s0, f1, s1);
+        input_gradient<T, Of, In>(a, id, f0, s0, f1, s1);
     else
-        weight_gradient<Weights>(a, id, f0, s0, f1, s1);
+        weight_gradient<T, Of, Weights>(a, id, f0, s0, f1, s1);
 }
 
 // ---------------------------------------------------------------------------
@@ -548,8 +578,16 @@ inline double panels_until_done(Part a, Part b, double setup, int64_t slots) {
 
 struct Cut {
     int shape, tiles_m, tiles_n, splits, weight_m, weight_n;
+    double time;
     int64_t tiles() const { return static_cast<int64_t>(tiles_m) * tiles_n; }
     int64_t weights() const { return static_cast<int64_t>(weight_m) * weight_n; }
+};
+
+// How a call's products are formed: of fp32 numbers, or of `terms` products of 16 bits.
+struct Means {
+    bool wide;
+    int terms;
+    int64_t panels(int64_t length) const { return nsh_host::ceil_div(length, wide ? 32 : 64) * terms; }
 };
 
 inline double time_of(const Shape& s, const float (&rate)[3], Part a, Part b) {
@@ -558,14 +596,13 @@ inline double time_of(const Shape& s, const float (&rate)[3], Part a, Part b) {
     return panels_until_done(a, b, s.setup, cus * share) * rate[share - 1];
 }
 
-inline Cut forward_cut(int64_t rows, int64_t F, int64_t Kp, bool wide) {
+inline Cut forward_cut(int64_t rows, int64_t F, int64_t K, Means by) {
     Cut best{};
-    double least = 0;
-    for (int i = wide ? 1 : 0; i < 3; ++i) {
+    for (int i = by.wide ? 1 : 0; i < 3; ++i) {
         const Shape& s = kShapes[i];
-        Cut c{i, static_cast<int>(nsh_host::ceil_div(rows, s.bm)), static_cast<int>(nsh_host::ceil_div(F, s.bn / 2)), 1, 0, 0};
-        const double t = time_of(s, wide ? s.wide : s.along, {c.tiles(), nsh_host::ceil_div(Kp, wide ? 32 : 64)}, {0, 0});
-        if (least == 0 || t < least) least = t, best = c;
+        Cut c{i, static_cast<int>(nsh_host::ceil_div(rows, s.bm)), static_cast<int>(nsh_host::ceil_div(F, s.bn / 2)), 1, 0, 0, 0};
+        c.time = time_of(s, by.wide ? s.wide : s.along, {c.tiles(), by.panels(K)}, {0, 0});
+        if (best.time == 0 || c.time < best.time) best = c;
     }
     return best;
 }
@@ -573,79 +610,79 @@ inline Cut forward_cut(int64_t rows, int64_t F, int64_t Kp, bool wide) {
 // Of dx, of the weights' gradients, or of both in one launch: with few tiles of dx,
 // workgroups share a tile's sum over the hidden columns, and another launch joins them
 // (4 us, and their sums' bytes at 3.5 TB/s).
-inline Cut gradient_cut(int64_t rows, int64_t K, int64_t Fp, int64_t F, bool wide, bool input, bool weights) {
+inline Cut gradient_cut(int64_t rows, int64_t K, int64_t F, Means by, bool input, bool weights) {
     Cut best{};
-    double least = 0;
-    const int64_t bk = wide ? 32 : 64;
-    for (int i = wide ? 1 : 0; i < 3; ++i) {
+    for (int i = by.wide ? 1 : 0; i < 3; ++i) {
         const Shape& s = kShapes[i];
-        Cut c{i, 0, 0, 1, 0, 0};
+        Cut c{i, 0, 0, 1, 0, 0, 0};
         if (input) c.tiles_m = static_cast<int>(nsh_host::ceil_div(rows, s.bm)), c.tiles_n = static_cast<int>(nsh_host::ceil_div(K, s.bn));
         if (weights) c.weight_m = 2 * static_cast<int>(nsh_host::ceil_div(F, s.bm)), c.weight_n = static_cast<int>(nsh_host::ceil_div(K, s.bn));
-        const int64_t panels = 2 * Fp / bk;
+        const int64_t panels = 2 * by.panels(F);
         for (const int splits : {1, 2, 3, 4, 6, 8, 12, 16}) {  // (those that the join knows)
             if (splits > 1 && (!input || panels / splits < 4)) break;
             c.splits = splits;
-            double t = time_of(s, wide ? s.wide : s.across, {c.tiles() * splits, nsh_host::ceil_div(panels, splits)},
-                               {c.weights(), nsh_host::ceil_div(rows, bk)});
-            if (splits > 1) t += 4 + static_cast<double>(splits * rows * K) * 4 / 3.5e6;
-            if (least == 0 || t < least) least = t, best = c;
+            c.time = time_of(s, by.wide ? s.wide : s.across, {c.tiles() * splits, nsh_host::ceil_div(panels, splits)},
+                             {c.weights(), by.panels(rows)});
+            if (splits > 1) c.time += 4 + static_cast<double>(splits * rows * K) * 4 / 3.5e6;
+            if (best.time == 0 || c.time < best.time) best = c;
         }
     }
     return best;
 }
 
 template <typename T>
-int gated_forward(GatedArgs a, hipStream_t st) {
-    if (a.rows <= kFewRows && !a.kept) {
-        // twice the waves a workgroup where there are too few for two on every CU
-        const unsigned grid = (a.F + 15) / 16;
-        const bool more = grid < 2u * nsh_host::compute_units();
-        auto go = [&](auto groups) {
-            // (45 rows, 4096 -> 11000: 58 us by 64 bytes, 44 by 128; eight waves' panels of
-            // those fit the LDS up to 32 rows)
-            constexpr int MG = decltype(groups)::value;
-            if (more)
-                gated_rows_kernel<T, MG, 8, MG < 3 ? 128 : 64><<<grid, 512, 0, st>>>(a);
-            else
-                gated_rows_kernel<T, MG, 4, 128><<<grid, 256, 0, st>>>(a);
-        };
-        if (a.rows <= 16)
-            go(std::integral_constant<int, 1>{});
-        else if (a.rows <= 32)
-            go(std::integral_constant<int, 2>{});
-        else if (a.rows <= 48)
-            go(std::integral_constant<int, 3>{});
+int gated_few_rows(GatedArgs a, hipStream_t st) {
+    // twice the waves a workgroup where there are too few for two on every CU
+    const unsigned grid = (a.F + 15) / 16;
+    const bool more = grid < 2u * nsh_host::compute_units();
+    auto go = [&](auto groups) {
+        // (45 rows, 4096 -> 11000: 58 us by 64 bytes, 44 by 128; eight waves' panels of
+        // those fit the LDS up to 32 rows)
+        constexpr int MG = decltype(groups)::value;
+        if (more)
+            gated_rows_kernel<T, MG, 8, MG < 3 ? 128 : 64><<<grid, 512, 0, st>>>(a);
         else
-            go(std::integral_constant<int, 4>{});
-        return nsh_host::check_launch("gated_linear_forward");
-    }
-    const Cut c = forward_cut(a.rows, a.F, a.Kp, sizeof(T) == 4);
-    a.tiles_m = c.tiles_m, a.tiles_n = c.tiles_n;
-    const unsigned grid = static_cast<unsigned>(c.tiles());
-    if constexpr (sizeof(T) == 2)
-        if (c.shape == 0) gated_forward_kernel<T, 256, 256, 4, 2, 128><<<grid, 512, 0, st>>>(a);
-    if (c.shape == 1) gated_forward_kernel<T, 128, 128, 2, 2, 128><<<grid, 256, 0, st>>>(a);
-    if (c.shape == 2) gated_forward_kernel<T, 64, 128, 2, 2, 128><<<grid, 256, 0, st>>>(a);
+            gated_rows_kernel<T, MG, 4, 128><<<grid, 256, 0, st>>>(a);
+    };
+    if (a.rows <= 16)
+        go(std::integral_constant<int, 1>{});
+    else if (a.rows <= 32)
+        go(std::integral_constant<int, 2>{});
+    else if (a.rows <= 48)
+        go(std::integral_constant<int, 3>{});
+    else
+        go(std::integral_constant<int, 4>{});
     return nsh_host::check_launch("gated_linear_forward");
 }
 
-template <typename T>
+template <typename T, bool PARTS>
+int gated_forward(GatedArgs a, const Cut& c, hipStream_t st) {
+    a.tiles_m = c.tiles_m, a.tiles_n = c.tiles_n;
+    const unsigned grid = static_cast<unsigned>(c.tiles());
+    if constexpr (sizeof(T) == 2 || PARTS)
+        if (c.shape == 0) gated_forward_kernel<T, PARTS, 256, 256, 4, 2, 128><<<grid, 512, 0, st>>>(a);
+    if (c.shape == 1) gated_forward_kernel<T, PARTS, 128, 128, 2, 2, 128><<<grid, 256, 0, st>>>(a);
+    if (c.shape == 2) gated_forward_kernel<T, PARTS, 64, 128, 2, 2, 128><<<grid, 256, 0, st>>>(a);
+    return nsh_host::check_launch("gated_linear_forward");
+}
+
+template <typename T, bool PARTS>
 int gated_gradients(GatedArgs a, const Cut& c, hipStream_t st) {
     a.tiles_m = c.tiles_m, a.tiles_n = c.tiles_n, a.splits = c.splits, a.weight_m = c.weight_m, a.weight_n = c.weight_n;
     const int64_t in = c.tiles() * c.splits, all = in + c.weights();
     a.weights_first = 2 * a.Fp / c.splits < a.rows;
     a.first = static_cast<int>(a.weights_first ? c.weights() : in);
     const unsigned grid = static_cast<unsigned>(all);
-    if constexpr (sizeof(T) == 2)
-        if (c.shape == 0) gated_gradients_kernel<T, 256, 256, 4, 2, 128><<<grid, 512, 0, st>>>(a);
-    if (c.shape == 1) gated_gradients_kernel<T, 128, 128, 2, 2, 128><<<grid, 256, 0, st>>>(a);
-    if (c.shape == 2) gated_gradients_kernel<T, 64, 128, 2, 2, 128><<<grid, 256, 0, st>>>(a);
+    if constexpr (sizeof(T) == 2 || PARTS)
+        if (c.shape == 0) gated_gradients_kernel<T, PARTS, 256, 256, 4, 2, 128><<<grid, 512, 0, st>>>(a);
+    if (c.shape == 1) gated_gradients_kernel<T, PARTS, 128, 128, 2, 2, 128><<<grid, 256, 0, st>>>(a);
+    if (c.shape == 2) gated_gradients_kernel<T, PARTS, 64, 128, 2, 2, 128><<<grid, 256, 0, st>>>(a);
     return nsh_host::check_launch("gated_linear_backward");
 }
 
-#define NSH_GATED_ENTRIES(EXTERN, T)                               \
-    EXTERN template int gated_forward<T>(GatedArgs, hipStream_t); \
-    EXTERN template int gated_gradients<T>(GatedArgs, const Cut&, hipStream_t);
+#define NSH_GATED_ENTRIES(EXTERN, T, PARTS)                                        \
+    EXTERN template int gated_forward<T, PARTS>(GatedArgs, const Cut&, hipStream_t); \
+    EXTERN template int gated_gradients<T, PARTS>(GatedArgs, const Cut&, hipStream_t);
+#define NSH_GATED_FEW_ROWS(EXTERN, T) EXTERN template int gated_few_rows<T>(GatedArgs, hipStream_t);
 
 }  // namespace nsh
