@@ -268,8 +268,10 @@ __global__ __launch_bounds__(64 * WAVES_M * WAVES_N, 2) void gated_forward_kerne
     using Of = Parts<T, PARTS>;
     using E = typename Of::E;
     using P = Product<E, BM, BN, WAVES_M, WAVES_N, KB, kAlong, kAlong, true>;
-    __shared__ __attribute__((aligned(1024))) char f0[P::FIRST_BYTES], s0[P::SECOND_BYTES];
-    __shared__ __attribute__((aligned(1024))) char f1[P::FIRST_BYTES], s1[P::SECOND_BYTES];
+    // (panels of 24 KB: a third leaves room for two workgroups a CU; 100 rows, 2048 -> 5504: 30
+    // us with two, 23 with three)
+    constexpr bool THREE = BM < 128;
+    __shared__ __attribute__((aligned(1024))) char b0[P::BYTES], b1[P::BYTES], b2[THREE ? P::BYTES : 1];
     const TileOrder t(blockIdx.x, gridDim.x, a.tiles_m, a.tiles_n, 8);
     const int64_t m0 = static_cast<int64_t>(t.m) * BM;
     const int c0 = t.n * (BN / 2), wave = wave_id();
@@ -285,25 +287,31 @@ __global__ __launch_bounds__(64 * WAVES_M * WAVES_N, 2) void gated_forward_kerne
     const int left_m = static_cast<int>(min(a.rows - m0, int64_t(BM)));
     P p;
     p.init();
-    p.run((a.Kp + P::BK - 1) / P::BK * Of::N, f0, s0, f1, s1, [&](int i, char* f, char* s) {
+    const int n = (a.Kp + P::BK - 1) / P::BK * Of::N;
+    const auto load = [&](int i, char* f, char* s) {
         const int block = i / Of::N, term = i % Of::N;
         const int64_t at = static_cast<int64_t>(block) * KB;
-        gate.load(f, wg + Of::first(term) * a.wg_plane + at, a.wg_stride, a.F - c0, wide - at, wave);
-        up.load(f + P::FIRST_BYTES / 2, wu + Of::first(term) * a.wu_plane + at, a.wu_stride, a.F - c0, wide - at, wave);
-        rows.load(s, x + Of::second(term) * a.x_plane + at, a.x_stride, left_m, wide - at, wave);
-    });
+        const int left_f = i < n ? a.F - c0 : 0;
+        gate.load(f, wg + Of::first(term) * a.wg_plane + at, a.wg_stride, left_f, wide - at, wave);
+        up.load(f + P::FIRST_BYTES / 2, wu + Of::first(term) * a.wu_plane + at, a.wu_stride, left_f, wide - at, wave);
+        rows.load(s, x + Of::second(term) * a.x_plane + at, a.x_stride, i < n ? left_m : 0, wide - at, wave);
+    };
+    if constexpr (THREE)
+        p.run(n, b0, b1, b2, load);
+    else
+        p.run(n, b0, b1, load);
     float most = 0.f;
     const int64_t m = m0 + P::wave_m() * P::WM;
     const int c = c0 + P::column(0);
     __syncthreads();  // the panels' place is free
-    store_tile<T, P::WM, P::WN / 2>(P::stage(f0, s0, f1, s1), static_cast<T*>(a.h) + m * a.F + c, a.F, a.rows - m, a.F - c,
+    store_tile<T, P::WM, P::WN / 2>(P::stage(b0, b1), static_cast<T*>(a.h) + m * a.F + c, a.F, a.rows - m, a.F - c,
                                     [&](int i, int b) {
                                         return gate_block<T>(a, m0 + P::row(i), c0 + P::column(b), p.acc[i][b],
                                                              p.acc[i][b + P::NB / 2], most);
                                     });
     if constexpr (__is_same(T, f16)) {
         if (!a.most) return;
-        float* meet = reinterpret_cast<float*>(f0);
+        float* meet = reinterpret_cast<float*>(b0);
         __syncthreads();
         meet[threadIdx.x] = most;
         __syncthreads();
@@ -317,8 +325,7 @@ __global__ __launch_bounds__(64 * WAVES_M * WAVES_N, 2) void gated_forward_kerne
 
 // dx: over the hidden columns of dg, then of du.
 template <typename T, typename Of, typename P>
-__device__ __forceinline__ void input_gradient(const GatedArgs& a, uint32_t id, char (&f0)[P::FIRST_BYTES], char (&s0)[P::SECOND_BYTES],
-                                               char (&f1)[P::FIRST_BYTES], char (&s1)[P::SECOND_BYTES]) {
+__device__ __forceinline__ void input_gradient(const GatedArgs& a, uint32_t id, char (&b0)[P::BYTES], char (&b1)[P::BYTES]) {
     using E = typename P::T;
     const uint32_t tiles = static_cast<uint32_t>(a.tiles_m) * a.tiles_n;
     const int split = TileOrder::uniform(id / tiles);
@@ -342,7 +349,7 @@ __device__ __forceinline__ void input_gradient(const GatedArgs& a, uint32_t id, 
     const int end = TileOrder::uniform(all * static_cast<uint32_t>(split + 1) / a.splits);
     P p;
     p.init();
-    p.run(end - begin, f0, s0, f1, s1, [&](int i, char* f, char* s) {
+    p.run(end - begin, b0, b1, [&](int i, char* f, char* s) {
         const int block = (begin + i) / Of::N, term = (begin + i) % Of::N;
         const bool one = block < half;
         const int64_t row = static_cast<int64_t>(one ? block : block - half) * P::BK;
@@ -354,7 +361,7 @@ __device__ __forceinline__ void input_gradient(const GatedArgs& a, uint32_t id, 
     const float by = __is_same(T, f16) && a.scale ? a.scale[1] : 1.f;
     const int64_t m = m0 + P::wave_m() * P::WM, c = c0 + P::column(0);
     __syncthreads();  // the panels' place is free
-    char* stage = P::stage(f0, s0, f1, s1);
+    char* stage = P::stage(b0, b1);
     const auto value = [&](int i, int b) { return p.acc[i][b] * by; };
     if (a.part)
         store_tile<float, P::WM, P::WN>(stage, a.part + (split * a.rows + m) * a.Kq + c, a.Kq, a.rows - m, a.K - c, value);
@@ -364,8 +371,7 @@ __device__ __forceinline__ void input_gradient(const GatedArgs& a, uint32_t id, 
 
 // Both weights' gradients: tiles of hidden rows of the one, then of the other.
 template <typename T, typename Of, typename P>
-__device__ __forceinline__ void weight_gradient(const GatedArgs& a, uint32_t id, char (&f0)[P::FIRST_BYTES], char (&s0)[P::SECOND_BYTES],
-                                                char (&f1)[P::FIRST_BYTES], char (&s1)[P::SECOND_BYTES]) {
+__device__ __forceinline__ void weight_gradient(const GatedArgs& a, uint32_t id, char (&b0)[P::BYTES], char (&b1)[P::BYTES]) {
     using E = typename P::T;
     const int each = a.weight_m / 2;
     const TileOrder t(id, static_cast<uint32_t>(a.weight_m) * a.weight_n, a.weight_m, a.weight_n, 8);
@@ -386,7 +392,7 @@ __device__ __forceinline__ void weight_gradient(const GatedArgs& a, uint32_t id,
     const int64_t left_f = (static_cast<int64_t>(a.Fp) - f_first) * static_cast<int64_t>(sizeof(E));
     P p;
     p.init();
-    p.run(static_cast<int>((a.rows + P::BK - 1) / P::BK) * Of::N, f0, s0, f1, s1, [&](int i, char* f, char* s) {
+    p.run(static_cast<int>((a.rows + P::BK - 1) / P::BK) * Of::N, b0, b1, [&](int i, char* f, char* s) {
         const int64_t at = static_cast<int64_t>(i / Of::N) * P::BK;
         const int term = i % Of::N, left = static_cast<int>(min(a.rows - at, int64_t(P::BK)));
         in.load(f, x + Of::first(term) * a.x_plane + at * a.x_stride, a.x_stride, left, left_c, wave);
@@ -395,7 +401,7 @@ __device__ __forceinline__ void weight_gradient(const GatedArgs& a, uint32_t id,
     const float by = __is_same(T, f16) && a.scale ? a.scale[1] : 1.f;
     const int64_t f = f_first + P::wave_m() * P::WM, c = c0 + P::column(0);
     __syncthreads();  // the panels' place is free
-    store_tile<T, P::WM, P::WN>(P::stage(f0, s0, f1, s1), out + f * a.K + c, a.K, a.F - f, a.K - c,
+    store_tile<T, P::WM, P::WN>(P::stage(b0, b1), out + f * a.K + c, a.K, a.F - f, a.K - c,
                                 [&](int i, int b) { return p.acc[i][b] * by; });
 }
 
@@ -407,15 +413,14 @@ __global__ __launch_bounds__(64 * WAVES_M * WAVES_N, 2) void gated_gradients_ker
     using E = typename Of::E;
     using In = Product<E, BM, BN, WAVES_M, WAVES_N, KB, kAcross, kAlong, false>;
     using Weights = Product<E, BM, BN, WAVES_M, WAVES_N, KB, kAcross, kAcross, false>;
-    __shared__ __attribute__((aligned(1024))) char f0[In::FIRST_BYTES], s0[In::SECOND_BYTES];
-    __shared__ __attribute__((aligned(1024))) char f1[In::FIRST_BYTES], s1[In::SECOND_BYTES];
+    __shared__ __attribute__((aligned(1024))) char b0[In::BYTES], b1[In::BYTES];
     const uint32_t first = a.first;
     const bool second = blockIdx.x >= first;
     const uint32_t id = second ? blockIdx.x - first : blockIdx.x;
     if (second == a.weights_first)
-        input_gradient<T, Of, In>(a, id, f0, s0, f1, s1);
+        input_gradient<T, Of, In>(a, id, b0, b1);
     else
-        weight_gradient<T, Of, Weights>(a, id, f0, s0, f1, s1);
+        weight_gradient<T, Of, Weights>(a, id, b0, b1);
 }
 
 // ---------------------------------------------------------------------------
@@ -543,16 +548,16 @@ __global__ __launch_bounds__(64 * WAVES) void gated_rows_kernel(GatedArgs a) {
 constexpr int kFewRows = 64;
 
 // Workgroup tiles, and the microseconds that a panel takes where one, two or three of
-// them share a CU (measured at sizes that leave the clock alone; `setup`: what a workgroup
-// takes besides, in panels).
+// them share a CU (measured at sizes that leave the clock alone; 0: they do not fit);
+// `setup`: what a workgroup takes besides, in panels.
 struct Shape {
-    int bm, bn, most;
+    int bm, bn;
     float along[3], across[3], wide[3];
     float setup;
 };
-constexpr Shape kShapes[3] = {{256, 256, 1, {1.42f}, {1.5f}, {0.f}, 5.f},
-                              {128, 128, 2, {0.72f, 1.12f}, {0.73f, 1.15f}, {1.9f, 3.5f}, 5.f},
-                              {64, 128, 3, {0.55f, 0.65f, 0.85f}, {0.57f, 0.9f, 1.25f}, {0.98f, 1.8f, 2.65f}, 5.f}};
+constexpr Shape kShapes[3] = {{256, 256, {1.42f}, {1.5f}, {}, 5.f},
+                              {128, 128, {0.72f, 1.12f}, {0.73f, 1.15f}, {1.9f, 3.5f}, 5.f},
+                              {64, 128, {0.5f, 0.6f}, {0.57f, 0.9f, 1.25f}, {0.98f, 1.8f}, 5.f}};
 
 // n workgroups of `length` panels, on as many CUs as there are.
 struct Part {
@@ -592,7 +597,8 @@ struct Means {
 
 inline double time_of(const Shape& s, const float (&rate)[3], Part a, Part b) {
     const int64_t cus = nsh_host::compute_units();
-    const int share = static_cast<int>(std::min<int64_t>(s.most, nsh_host::ceil_div(a.n + b.n, cus)));
+    int share = 1;
+    while (share < 3 && rate[share] > 0 && share * cus < a.n + b.n) ++share;
     return panels_until_done(a, b, s.setup, cus * share) * rate[share - 1];
 }
 

@@ -118,7 +118,7 @@ struct Product {
     using Second = Operand<T, SECOND == kAlong ? BK : BM, SECOND>;
     using FirstPanel = Panel<T, FIRST == kAlong ? (PAIRED ? BN / 2 : BN) : BK, FIRST == kAlong ? BK : BN, NT, FIRST>;
     using SecondPanel = Panel<T, SECOND == kAlong ? BM : BK, SECOND == kAlong ? BK : BM, NT, SECOND>;
-    static constexpr int FIRST_BYTES = BN * KB, SECOND_BYTES = BM * KB;
+    static constexpr int FIRST_BYTES = BN * KB, SECOND_BYTES = BM * KB, BYTES = FIRST_BYTES + SECOND_BYTES;
     static_assert(STEPS % 2 == 0 && (!PAIRED || (FIRST == kAlong && NB % 2 == 0)), "");
 
     f32x16 acc[MT][NB];
@@ -143,12 +143,12 @@ struct Product {
 #pragma unroll
             for (int b = 0; b < NB; ++b) acc[i][b] = f32x16{};
     }
-    __device__ __forceinline__ void read(Step& x, const char* first, const char* second, int s) const {
+    __device__ __forceinline__ void read(Step& x, const char* panel, int s) const {
 #pragma unroll
         for (int b = 0; b < NB; ++b)
-            x.f[b] = First::read(first, by_first, PAIRED && b >= NB / 2 ? BN / 2 + (b - NB / 2) * 32 : b * 32, s);
+            x.f[b] = First::read(panel, by_first, PAIRED && b >= NB / 2 ? BN / 2 + (b - NB / 2) * 32 : b * 32, s);
 #pragma unroll
-        for (int i = 0; i < MT; ++i) x.s[i] = Second::read(second, by_second, i * 32, s);
+        for (int i = 0; i < MT; ++i) x.s[i] = Second::read(panel + FIRST_BYTES, by_second, i * 32, s);
     }
     template <int FROM, int TO>
     __device__ __forceinline__ void multiply(const Step& x) {
@@ -157,6 +157,10 @@ struct Product {
 #pragma unroll
             for (int b = 0; b < NB; ++b) acc[i][b] = Eight<T>::mma(x.f[b], x.s[i], acc[i][b]);
     }
+
+    static constexpr int LOADS = BYTES / (NT * 16);  // of a panel, a lane
+    static constexpr int READS = NB * First::READS + MT * Second::READS;    // of a step
+    static constexpr int ROW = NB * (sizeof(T) == 4 ? 8 : 1);               // products of 32 rows
 
     // The region's products with reads between them: a product issues in 4 cycles and
     // takes 32, and what stands in front of a run of them keeps it waiting.
@@ -171,58 +175,96 @@ struct Product {
         order();
     }
 
+    // A panel's products but the last step's, which is read.
+    __device__ __forceinline__ void steps(Step& x, Step& y, const char* b) {
+#pragma unroll
+        for (int st = 0; st + 1 < STEPS; ++st) {
+            read(st % 2 ? x : y, b, st + 1);
+            multiply<0, MT>(st % 2 ? y : x);
+            mix<MT * ROW, READS>();
+        }
+    }
+    // The panels change hands: the next one is there (but the loads of LATER others may be
+    // under way) and everyone past this one's reads; its first step is read, and `ahead` asks
+    // for the one that takes this one's place, during the last step's products.
+    template <int LATER, typename Ahead>
+    __device__ __forceinline__ void turn(Step& x, Step& y, const char* next, const Ahead& ahead) {
+        landed<LATER>();
+        read(x, next, 0);  // (behind the last panel nothing that is used)
+        multiply<0, (MT + 1) / 2>(y);
+        mix<(MT + 1) / 2 * ROW, READS>();
+        ahead();
+        order();
+        multiply<(MT + 1) / 2, MT>(y);
+        order();
+    }
+
     // All n panels (n >= 1); load(i, first, second) asks for panel i.
     template <typename Load>
-    __device__ __forceinline__ void run(int n, char (&f0)[FIRST_BYTES], char (&s0)[SECOND_BYTES], char (&f1)[FIRST_BYTES],
-                                        char (&s1)[SECOND_BYTES], const Load& load) {
-        constexpr int READS = NB * First::READS + MT * Second::READS;
-        constexpr int ROW = NB * (sizeof(T) == 4 ? 8 : 1);  // products of 32 rows
+    __device__ __forceinline__ void run(int n, char (&b0)[BYTES], char (&b1)[BYTES], const Load& load) {
         Step x, y;
-        load(0, f0, s0);
-        landed();
-        if (n > 1) load(1, f1, s1);
-        read(x, f0, s0, 0);
+        load(0, b0, b0 + FIRST_BYTES);
+        landed<0>();
+        if (n > 1) load(1, b1, b1 + FIRST_BYTES);
+        read(x, b0, 0);
         order();
-        auto panel = [&](int i, char (&f)[FIRST_BYTES], char (&s)[SECOND_BYTES], char (&fn)[FIRST_BYTES], char (&sn)[SECOND_BYTES]) {
-#pragma unroll
-            for (int st = 0; st + 1 < STEPS; ++st) {
-                read(st % 2 ? x : y, f, s, st + 1);
-                multiply<0, MT>(st % 2 ? y : x);
-                mix<MT * ROW, READS>();
-            }
-            landed();
-            order();
-            read(x, fn, sn, 0);  // (behind the last panel nothing that is used)
-            multiply<0, (MT + 1) / 2>(y);
-            mix<(MT + 1) / 2 * ROW, READS>();
-            if (i + 2 < n) load(i + 2, f, s);
-            order();
-            multiply<(MT + 1) / 2, MT>(y);
-            order();
-        };
         for (int i = 0; i < n; i += 2) {
-            panel(i, f0, s0, f1, s1);
-            if (i + 1 < n) panel(i + 1, f1, s1, f0, s0);
+            steps(x, y, b0);
+            turn<0>(x, y, b1, [&] { if (i + 2 < n) load(i + 2, b0, b0 + FIRST_BYTES); });
+            if (i + 1 < n) {
+                steps(x, y, b1);
+                turn<0>(x, y, b0, [&] { if (i + 3 < n) load(i + 3, b1, b1 + FIRST_BYTES); });
+            }
         }
         settle<T>();
     }
 
-    // A place of the wave's own in the panels, for 32 x 64 in fp32.
-    static __device__ __forceinline__ char* stage(char (&f0)[FIRST_BYTES], char (&s0)[SECOND_BYTES], char (&f1)[FIRST_BYTES],
-                                                  char (&s1)[SECOND_BYTES]) {
-        constexpr int BYTES = 32 * 64 * 4, IN_F = FIRST_BYTES / BYTES, IN_S = SECOND_BYTES / BYTES;
-        static_assert(2 * (IN_F + IN_S) >= NT / 64, "a place for every wave");
-        const int w = wave_id();
-        return w < IN_F ? f0 + w * BYTES
-               : w < 2 * IN_F ? f1 + (w - IN_F) * BYTES
-               : w < 2 * IN_F + IN_S ? s0 + (w - 2 * IN_F) * BYTES : s1 + (w - 2 * IN_F - IN_S) * BYTES;
+    // The same with two panels ahead.  From n on load() asks for nothing (a buffer of no
+    // bytes): the compiler tells loads under way apart by their number, and a load that may
+    // not be there would have it wait for all of them (as it does at the loop's head).
+    template <typename Load>
+    __device__ __forceinline__ void run(int n, char (&b0)[BYTES], char (&b1)[BYTES], char (&b2)[BYTES], const Load& load) {
+        Step x, y;
+        load(0, b0, b0 + FIRST_BYTES);
+        load(1, b1, b1 + FIRST_BYTES);
+        load(2, b2, b2 + FIRST_BYTES);
+        landed<2 * LOADS>();
+        read(x, b0, 0);
+        order();
+        for (int i = 0;; i += 3) {
+            steps(x, y, b0);
+            turn<LOADS>(x, y, b1, [&] { load(i + 3, b0, b0 + FIRST_BYTES); });
+            if (i + 1 >= n) break;
+            steps(x, y, b1);
+            turn<LOADS>(x, y, b2, [&] { load(i + 4, b1, b1 + FIRST_BYTES); });
+            if (i + 2 >= n) break;
+            steps(x, y, b2);
+            turn<LOADS>(x, y, b0, [&] { load(i + 5, b2, b2 + FIRST_BYTES); });
+            if (i + 3 >= n) break;
+        }
+        settle<T>();
+        landed<0>();  // what was asked for past the end has no place in what follows
     }
 
-    // Every wave's loads have landed, and every wave has read what it needs of the
-    // panel before.
+    // A place of the wave's own in the panels, for 32 x 64 in fp32.
+    static __device__ __forceinline__ char* stage(char (&b0)[BYTES], char (&b1)[BYTES]) {
+        constexpr int SIZE = 32 * 64 * 4, EACH = BYTES / SIZE;
+        static_assert(2 * EACH >= NT / 64, "a place for every wave");
+        const int w = wave_id();
+        return w < EACH ? b0 + w * SIZE : b1 + (w - EACH) * SIZE;
+    }
+
+    // Every wave's loads but its last LATER ones have landed, and every wave has read what
+    // it needs of the panel before.
+    template <int LATER>
     static __device__ __forceinline__ void landed() {
-        __builtin_amdgcn_s_waitcnt(0x0070);  // vmcnt(0), lgkmcnt(0)
-        __syncthreads();
+        static_assert(LATER < 16, "");
+        __builtin_amdgcn_s_waitcnt(0x0070 | LATER);  // vmcnt, lgkmcnt(0)
+        if constexpr (LATER == 0)
+            __syncthreads();
+        else
+            __builtin_amdgcn_s_barrier();
+        order();
     }
 };
 
