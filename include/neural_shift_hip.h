@@ -590,7 +590,8 @@ NSH_API int64_t nsh_attention_workspace_bytes(const nsh_attention_args* args, in
  *   h = (s - mean(s)) * (var(s) + eps)^(-1/2);  y = h * weight + bias
  *   grad_x = grad_s + d(y), of x and of the residual alike
  * A NULL weight is 1, a NULL bias 0.  Inputs have a unit last stride, the given
- * strides from row to row (elements) and any alignment; outputs are contiguous. */
+ * strides from row to row (elements) and any alignment; outputs are contiguous.
+ * n <= 2^26, rows <= 2^40. */
 typedef struct nsh_layer_norm_args {
     const void *x, *residual, *weight, *bias; /* backward: x is what was normed, s with a residual */
     int64_t rows, n, x_stride, residual_stride;
@@ -614,8 +615,10 @@ NSH_API int64_t nsh_layer_norm_workspace_bytes(const nsh_layer_norm_args* args);
  *   g = x gate^T,  u = x up^T,  h = act(g) * u
  * x (rows, K), gate and up (F, K) with a unit last stride and the given strides from row
  * to row (elements), any alignment (rows that do not start on 16 bytes, or whose width is
- * no multiple of 16 bytes, are copied into the workspace first).  K, F <= 2^20.  Products,
- * the activation and all sums are float; dg and du are rounded to `dtype` (fp16: times a
+ * no multiple of 16 bytes, are copied into the workspace first).  K, F <= 2^20, rows <=
+ * 2^28.  Products, the activation and all sums are float (of fp32 matrices, where it is
+ * faster, each product from six of bf16 parts, copied into the workspace: what is finite
+ * keeps fp32's bits, infinity times infinity is NaN); dg and du are rounded to `dtype` (fp16: times a
  * power of two that the call chooses) as operands of the gradients' products. */
 #define NSH_ACTIVATION_SILU 1
 #define NSH_ACTIVATION_GELU 2      /* g * Phi(g) */
@@ -628,12 +631,12 @@ typedef struct nsh_gated_linear_args {
     int32_t dtype, activation;
     void* h; /* forward: (rows, F), contiguous */
     /* nsh_gated_linear_kept_bytes, 16-byte aligned, or NULL.  Forward: written, what
-     * the backward needs.  Backward: read, with the forward's rows, F and dtype. */
+     * the backward needs.  Backward: read, with the forward's rows, K, F and dtype. */
     void* kept;
     const void* grad_h; /* backward, with its stride; gradients contiguous, NULL = not wanted */
     int64_t gh_stride;
     void *grad_x, *grad_gate, *grad_up;
-    void* workspace; /* nsh_gated_linear_workspace_bytes, 16-byte aligned */
+    void* workspace; /* nsh_gated_linear_workspace_bytes of these arguments, 16-byte aligned */
     int64_t workspace_bytes;
 } nsh_gated_linear_args;
 NSH_API int nsh_gated_linear_forward(const nsh_gated_linear_args* args, void* stream);

@@ -315,8 +315,8 @@ int check(const char* op, const nsh_gated_linear_args* g, bool bwd) {
     if (g->dtype < NSH_DTYPE_FLOAT16 || g->dtype > NSH_DTYPE_FLOAT32)
         return fail(NSH_ERR_INVALID, "%s: unsupported dtype code %d", op, g->dtype);
     if (g->rows < 1 || g->K < 1 || g->F < 1) return fail(NSH_ERR_INVALID, "%s: empty tensor", op);
-    if (g->K > kWidest || g->F > kWidest || g->rows > (int64_t(1) << 30))
-        return fail(NSH_ERR_INVALID, "%s: width or hidden size above 2^20, or more than 2^30 rows", op);
+    if (g->K > kWidest || g->F > kWidest || g->rows > (int64_t(1) << 28))
+        return fail(NSH_ERR_INVALID, "%s: width or hidden size above 2^20, or more than 2^28 rows", op);
     if (g->activation < NSH_ACTIVATION_SILU || g->activation > NSH_ACTIVATION_SIGMOID)
         return fail(NSH_ERR_INVALID, "%s: unknown activation code %d", op, g->activation);
     if (!g->x || !g->gate_weight || !g->up_weight ||

@@ -165,7 +165,8 @@ struct Kept {
             } else {
                 uint32_t b[16];
 #pragma unroll
-                for (int r = 0; r < 16; ++r) b[r] = __float_as_uint(v[r]) + 0x80u;
+                for (int r = 0; r < 16; ++r)  // (no carry out of what is no number)
+                    b[r] = v[r] == v[r] ? __float_as_uint(v[r]) + 0x80u : 0x7fc00000u;
 #pragma unroll
                 for (int q = 0; q < 2; ++q) {
                     ux4 x;  // upper halves of two

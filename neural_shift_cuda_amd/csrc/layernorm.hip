@@ -495,8 +495,9 @@ constexpr int kMostNormBlocks = 2;  // of the backward, a CU
 template <typename T, int G, int NV, bool WHOLE>
 static int layer_norm_rows(LayerNormArgs a, bool bwd, hipStream_t st) {
     using Gr = Group<G>;
-    // (rows of a workgroup: one each; the 512 lanes' registers leave one workgroup to a CU)
-    a.blocks = norm_row_blocks(a.rows, Gr::kGroups, bwd ? (G == 512 ? 1 : kMostNormBlocks) : G > 64 ? int64_t(1) << 20 : 8);
+    // (rows of a workgroup: one each, as far as a launch's 2^32 threads go; backward, the 512
+    // lanes' registers leave one workgroup to a CU)
+    a.blocks = norm_row_blocks(a.rows, Gr::kGroups, bwd ? (G == 512 ? 1 : kMostNormBlocks) : G > 64 ? 1 << 13 : 8);
     if (!bwd) {
         layer_norm_forward_kernel<T, G, NV, WHOLE><<<a.blocks, Gr::kThreads, 0, st>>>(a);
         return nsh_host::check_launch("layer_norm_forward");
@@ -560,8 +561,8 @@ static int layer_norm(const char* op, const nsh_layer_norm_args* g, bool bwd, vo
     if (g->dtype < NSH_DTYPE_FLOAT16 || g->dtype > NSH_DTYPE_FLOAT32)
         return fail(NSH_ERR_INVALID, "%s: unsupported dtype code %d", op, g->dtype);
     if (g->rows < 1 || g->n < 1) return fail(NSH_ERR_INVALID, "%s: empty tensor", op);
-    if (g->n > (int64_t(1) << 30) || g->rows > (int64_t(1) << 40))
-        return fail(NSH_ERR_INVALID, "%s: rows wider than 2^30 or more than 2^40", op);
+    if (g->n > (int64_t(1) << 26) || g->rows > (int64_t(1) << 40))
+        return fail(NSH_ERR_INVALID, "%s: rows wider than 2^26 or more than 2^40", op);
     if (!(g->eps >= 0) || std::isinf(g->eps)) return fail(NSH_ERR_INVALID, "%s: eps must be finite and not negative", op);
     if (bwd ? !g->x || !g->grad_y || !g->stats || (!g->grad_x && !g->grad_weight && !g->grad_bias)
             : !g->x || !g->y || !g->residual != !g->s)

@@ -120,7 +120,7 @@ def layer_norm(x: torch.Tensor, weight: Optional[torch.Tensor] = None,
 
     Returns y, or (y, s) with a residual, contiguous.  Differentiable in all of
     them (x and residual have the same gradient); the weights' gradients are
-    summed in fp32 in a fixed order."""
+    summed in fp32 in a fixed order.  The GPU serves widths up to 2^26."""
     if not x.is_cuda:
         return layer_norm_reference(x, weight, bias, residual=residual, eps=eps)
     done = _C and _C.layer_norm_as_is(x, weight, bias, residual, eps)
@@ -149,9 +149,11 @@ def gated_linear(x: torch.Tensor, gate_weight: torch.Tensor, up_weight: torch.Te
     "sigmoid".
 
     Returns h (..., hidden), contiguous: products, activation and their product
-    in fp32, rounded once.  Differentiable in all three; training keeps two fp32 values
-    for each of h.  The GPU serves width and hidden up to 2^20; rows that do not start
-    on 16 bytes are copied first."""
+    in fp32, rounded once.  Differentiable in all three; training keeps two factors for each
+    of h (4.1 bytes in bf16, 6 in fp16, 8 in fp32).  The GPU serves width and hidden up
+    to 2^20; rows that do not start on 16 bytes are copied first.  In fp32 large products
+    are summed from bf16 products of three parts, with fp32's bits; infinity times infinity
+    is then no number."""
     if not x.is_cuda:
         return gated_linear_reference(x, gate_weight, up_weight, activation=activation)
     code = _CODES.get(activation)

@@ -443,3 +443,30 @@ def test_a_blocks_second_half(dtype, M, K, F):
         graph.replay()
         torch.cuda.synchronize()
         assert same(res, want), f"replay {r}"
+
+
+def test_more_rows_than_workgroups():
+    """A workgroup a row, as far as a launch's threads go: the last rows are those of a
+    workgroup's second turn."""
+    M, n = (1 << 21) + 300, 2056
+    xs, w = tensors((300, n), (n,), dtype=torch.bfloat16)
+    x = torch.ones(M, n, device=DEV, dtype=torch.bfloat16)
+    x[-300:] = xs
+    y = layer_norm(x, w)
+    vals, tols = oracle.layer_norm(xs.cpu(), w.cpu(), None, None, 1e-5)
+    oracle.close(y[-300:], vals["y"], tols["y"], "y")
+    assert not y[:-300].any()
+
+
+@pytest.mark.parametrize("dtype", [torch.float16, torch.bfloat16, torch.float32])
+@pytest.mark.parametrize("bad", [float("nan"), float("inf")])
+def test_gradients_of_a_row_without_numbers(dtype, bad):
+    x, gate, up = gated_leaves(70, 64, 96, dtype)
+    gh = tensors((70, 96), dtype=dtype, seed=8)[0]
+    vals, tols = oracle.gated(x.cpu(), gate.cpu(), up.cpu(), "silu", gh.cpu())
+    x[33, 5] = bad
+    leaf = [t.requires_grad_() for t in (x, gate, up)]
+    gx, gg, gu = torch.autograd.grad(gated_linear(*leaf), leaf, gh)
+    assert gx[33].isnan().all() and gg[:, 5].isnan().all() and not gu[:, 5].isfinite().any()
+    rest = [m for m in range(70) if m != 33]
+    oracle.close(gx[rest], vals["gx"][rest], tols["gx"][rest], "gx")
