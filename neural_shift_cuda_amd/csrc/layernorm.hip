@@ -241,7 +241,11 @@ __global__ __launch_bounds__(Group<G>::kThreads) void layer_norm_backward_kernel
     }
     // A workgroup's registers leave one or two of them to a CU: the next row's loads are
     // under way during this one's sums.
-    constexpr bool AHEAD = G >= 256;
+    // (32 columns a lane and the path by elements would spill)
+    constexpr bool AHEAD = G >= 256 && (WHOLE || NV * V < 32);
+    // Every lane loads then, those past the row's end its start: a load that may not be there
+    // has the compiler wait for all that are under way.
+    constexpr bool EVERY = AHEAD && WHOLE;
     struct Row {
         ux4 x[NV], g[NV];
         float mean, by;
@@ -253,15 +257,18 @@ __global__ __launch_bounds__(Group<G>::kThreads) void layer_norm_backward_kernel
         const T* g = static_cast<const T*>(a.grad_y) + row * a.gy_stride;
 #pragma unroll
         for (int i = 0; i < NV; ++i) {
-            f.x[i] = load_bits<T, WHOLE>(x, (i * G + lane) * V, a.n);
-            f.g[i] = load_bits<T, WHOLE>(g, (i * G + lane) * V, a.n);
+            const int c = (i * G + lane) * V;
+            if constexpr (EVERY) {
+                __builtin_memcpy(&f.x[i], x + (c < a.n ? c : 0), 16);
+                __builtin_memcpy(&f.g[i], g + (c < a.n ? c : 0), 16);
+            } else {
+                f.x[i] = load_bits<T, WHOLE>(x, c, a.n);
+                f.g[i] = load_bits<T, WHOLE>(g, c, a.n);
+            }
         }
         f.mean = a.stats[2 * row], f.by = a.stats[2 * row + 1];
     };
-    Row cur, next;
-    int64_t r0 = static_cast<int64_t>(blockIdx.x) * Gr::kGroups;
-    if (AHEAD && r0 < a.rows) fetch(r0, cur);
-    for (; r0 < a.rows; r0 += step) {
+    auto gradients = [&](int64_t r0, Row& cur, Row& next) {
         const bool live = r0 + own < a.rows;
         const int64_t row = live ? r0 + own : 0;
         if constexpr (!AHEAD) fetch(r0, cur);
@@ -271,13 +278,15 @@ __global__ __launch_bounds__(Group<G>::kThreads) void layer_norm_backward_kernel
 #pragma unroll
             for (int i = 0; i < NV; ++i) more[i] = load_bits<T, WHOLE>(s, (i * G + lane) * V, a.n);
         }
-        if (AHEAD && r0 + step < a.rows) fetch(r0 + step, next);
+        // (behind the last row this one once more)
+        if constexpr (AHEAD) fetch(r0 + step < a.rows ? r0 + step : r0, next);
         const float mean = cur.mean, by = cur.by;
         float h[NV][V], d[NV][V], s1 = 0.f, s2 = 0.f;
 #pragma unroll
         for (int i = 0; i < NV; ++i) {
             const int c = (i * G + lane) * V;
             float m[V];
+            if (EVERY && c >= a.n) cur.g[i] = ux4{0, 0, 0, 0};
             unpack<T>(cur.x[i], h[i]);
             unpack<T>(cur.g[i], d[i]);
             if (a.weight) unpack<T>(w[i], m);
@@ -317,7 +326,19 @@ __global__ __launch_bounds__(Group<G>::kThreads) void layer_norm_backward_kernel
                 store_bits<T, WHOLE>(static_cast<T*>(a.gx) + row * a.n, (i * G + lane) * V, a.n, pack<T>(d[i]));
             }
         }
-        if constexpr (AHEAD) cur = next;
+    };
+    int64_t r0 = static_cast<int64_t>(blockIdx.x) * Gr::kGroups;
+    Row even, odd;
+    if constexpr (AHEAD) {  // (r0 < a.rows: there are no more workgroups than rows)
+        fetch(r0, even);
+        for (;;) {
+            gradients(r0, even, odd);
+            if ((r0 += step) >= a.rows) break;
+            gradients(r0, odd, even);
+            if ((r0 += step) >= a.rows) break;
+        }
+    } else {
+        for (; r0 < a.rows; r0 += step) gradients(r0, even, even);
     }
     if (!a.partial) return;
     float* to = a.partial + static_cast<int64_t>(blockIdx.x) * 2 * a.n;
