@@ -34,6 +34,33 @@ struct LayerNormArgs {
     float eps, inv_n;
 };
 
+// Columns c .. c + kVec - 1 of a row of n >= kVec, and of one with fewer left its last
+// kVec, which in_place() brings to where they belong, zeros behind them.  Every lane loads:
+// a load that may not be there has the compiler wait for all that are under way.  NEAR false:
+// load_bits(), for n < kVec, and where nothing is under way and registers are short.
+template <typename T, bool NEAR, bool WHOLE>
+__device__ __forceinline__ ux4 load_near(const T* row, int c, int n) {
+    if constexpr (!NEAR) return load_bits<T, WHOLE>(row, c, n);
+    ux4 r;
+    __builtin_memcpy(&r, row + min(c, n - kVec<T>), 16);
+    return r;
+}
+template <typename T, bool NEAR, bool WHOLE>
+__device__ __forceinline__ void in_place(ux4& r, int c, int n) {
+    if constexpr (!NEAR) return;
+    const int past = c + kVec<T> - n;
+    if (WHOLE ? past > 0 : past >= kVec<T>)
+        r = ux4{0, 0, 0, 0};
+    else if (!WHOLE && past > 0)
+        r = __builtin_bit_cast(ux4, __builtin_bit_cast(unsigned __int128, r) >> (past * 8 * static_cast<int>(sizeof(T))));
+}
+template <typename T, bool NEAR, bool WHOLE>
+__device__ __forceinline__ ux4 load_row(const T* row, int c, int n) {
+    ux4 r = load_near<T, NEAR, WHOLE>(row, c, n);
+    in_place<T, NEAR, WHOLE>(r, c, n);
+    return r;
+}
+
 // Groups of G lanes; several waves meet through LDS, `turn` telling two sums in a
 // row apart.
 template <int G>
@@ -89,46 +116,66 @@ __global__ __launch_bounds__(Group<G>::kThreads) void layer_norm_forward_kernel(
     constexpr int V = kVec<T>;
     __shared__ float meet[Gr::kWaves > 1 ? 4 * Gr::kWaves : 1];
     Gr group{meet};
-    // Groups of a wave keep the weights for all their rows; a workgroup has one row, and
-    // reads them at its end: registers for more workgroups at once instead.
-    constexpr bool KEEP = G <= 64;
+    // Groups of a wave keep the weights for all their rows; a workgroup of 256 has one row, and
+    // reads them at its end: registers for more workgroups at once instead.  One of 512 walks
+    // rows, and has the next one's loads under way (3000 x 16384 fp16: 48 us with a row each, 38
+    // so).
+    constexpr bool AHEAD = G == 512, KEEP = G <= 64 || AHEAD;
+    constexpr bool NEAR = G > 8 && (AHEAD || !WHOLE);
     const int lane = threadIdx.x % G, own = threadIdx.x / G;
     ux4 w[KEEP ? NV : 1], b[KEEP ? NV : 1];
     if constexpr (KEEP) {
 #pragma unroll
         for (int i = 0; i < NV; ++i) {
             const int c = (i * G + lane) * V;
-            if (a.weight) w[i] = load_bits<T, WHOLE>(static_cast<const T*>(a.weight), c, a.n);
-            if (a.bias) b[i] = load_bits<T, WHOLE>(static_cast<const T*>(a.bias), c, a.n);
+            if (a.weight) w[i] = load_near<T, NEAR, WHOLE>(static_cast<const T*>(a.weight), c, a.n);
+            if (a.bias) b[i] = load_near<T, NEAR, WHOLE>(static_cast<const T*>(a.bias), c, a.n);
+        }
+#pragma unroll
+        for (int i = 0; i < NV; ++i) {
+            const int c = (i * G + lane) * V;
+            if (a.weight) in_place<T, NEAR, WHOLE>(w[i], c, a.n);
+            if (a.bias) in_place<T, NEAR, WHOLE>(b[i], c, a.n);
         }
     }
-    // every lane of the workgroup takes every turn: the groups meet in lane exchanges
-    for (int64_t r0 = static_cast<int64_t>(blockIdx.x) * Gr::kGroups; r0 < a.rows;
-         r0 += static_cast<int64_t>(a.blocks) * Gr::kGroups) {
-        const bool live = r0 + own < a.rows;
-        const int64_t row = live ? r0 + own : 0;
+    struct Row {
+        ux4 x[NV], more[NV];
+    };
+    const int64_t step = static_cast<int64_t>(a.blocks) * Gr::kGroups;
+    auto fetch = [&](int64_t r0, Row& f) {
+        const int64_t row = r0 + own < a.rows ? r0 + own : 0;
         const T* x = static_cast<const T*>(a.x) + row * a.x_stride;
-        ux4 bits[NV], more[NV];
 #pragma unroll
-        for (int i = 0; i < NV; ++i) bits[i] = load_bits<T, WHOLE>(x, (i * G + lane) * V, a.n);
+        for (int i = 0; i < NV; ++i) f.x[i] = load_near<T, NEAR, WHOLE>(x, (i * G + lane) * V, a.n);
         if (a.residual) {
             const T* r = static_cast<const T*>(a.residual) + row * a.residual_stride;
 #pragma unroll
-            for (int i = 0; i < NV; ++i) more[i] = load_bits<T, WHOLE>(r, (i * G + lane) * V, a.n);
+            for (int i = 0; i < NV; ++i) f.more[i] = load_near<T, NEAR, WHOLE>(r, (i * G + lane) * V, a.n);
         }
+    };
+    // every lane of the workgroup takes every turn: the groups meet in lane exchanges
+    auto norm = [&](int64_t r0, Row& cur, Row& next) {
+        const bool live = r0 + own < a.rows;
+        const int64_t row = live ? r0 + own : 0;
+        if constexpr (AHEAD)
+            fetch(r0 + step < a.rows ? r0 + step : r0, next);
+        else
+            fetch(r0, cur);
         float v[NV][V], total = 0.f;
 #pragma unroll
         for (int i = 0; i < NV; ++i) {
             const int c = (i * G + lane) * V;
-            unpack<T>(bits[i], v[i]);
+            in_place<T, NEAR, WHOLE>(cur.x[i], c, a.n);
+            unpack<T>(cur.x[i], v[i]);
             if (a.residual) {
                 float m[V];
-                unpack<T>(more[i], m);
+                in_place<T, NEAR, WHOLE>(cur.more[i], c, a.n);
+                unpack<T>(cur.more[i], m);
 #pragma unroll
                 for (int k = 0; k < V; ++k) v[i][k] += m[k];
-                bits[i] = pack<T>(v[i]);
-                unpack<T>(bits[i], v[i]);
-                if (live) store_bits<T, WHOLE>(static_cast<T*>(a.s) + row * a.n, c, a.n, bits[i]);
+                cur.x[i] = pack<T>(v[i]);
+                unpack<T>(cur.x[i], v[i]);
+                if (live) store_bits<T, WHOLE>(static_cast<T*>(a.s) + row * a.n, c, a.n, cur.x[i]);
             }
 #pragma unroll
             for (int k = 0; k < V; ++k) total += v[i][k];
@@ -147,7 +194,7 @@ __global__ __launch_bounds__(Group<G>::kThreads) void layer_norm_forward_kernel(
         }
         float by;
         const float rest = variance(group, square, off, a, by);
-        if (!live) continue;
+        if (!live) return;
         if (a.stats && lane == 0) a.stats[2 * row] = mean + rest, a.stats[2 * row + 1] = by;
 #pragma unroll
         for (int i = 0; i < NV; ++i) {
@@ -156,17 +203,30 @@ __global__ __launch_bounds__(Group<G>::kThreads) void layer_norm_forward_kernel(
 #pragma unroll
             for (int k = 0; k < V; ++k) v[i][k] = (v[i][k] - rest) * by;
             if (a.weight) {
-                unpack<T>(KEEP ? w[KEEP ? i : 0] : load_bits<T, WHOLE>(static_cast<const T*>(a.weight), c, a.n), m);
+                unpack<T>(KEEP ? w[KEEP ? i : 0] : load_row<T, NEAR, WHOLE>(static_cast<const T*>(a.weight), c, a.n), m);
 #pragma unroll
                 for (int k = 0; k < V; ++k) v[i][k] *= m[k];
             }
             if (a.bias) {
-                unpack<T>(KEEP ? b[KEEP ? i : 0] : load_bits<T, WHOLE>(static_cast<const T*>(a.bias), c, a.n), m);
+                unpack<T>(KEEP ? b[KEEP ? i : 0] : load_row<T, NEAR, WHOLE>(static_cast<const T*>(a.bias), c, a.n), m);
 #pragma unroll
                 for (int k = 0; k < V; ++k) v[i][k] += m[k];
             }
             store_bits<T, WHOLE>(static_cast<T*>(a.y) + row * a.n, c, a.n, pack<T>(v[i]));
         }
+    };
+    int64_t r0 = static_cast<int64_t>(blockIdx.x) * Gr::kGroups;
+    Row even, odd;
+    if constexpr (AHEAD) {
+        fetch(r0, even);
+        for (;;) {
+            norm(r0, even, odd);
+            if ((r0 += step) >= a.rows) break;
+            norm(r0, odd, even);
+            if ((r0 += step) >= a.rows) break;
+        }
+    } else {
+        for (; r0 < a.rows; r0 += step) norm(r0, even, even);
     }
 }
 
@@ -220,6 +280,10 @@ template <typename T, int G, int NV, bool WHOLE>
 __global__ __launch_bounds__(Group<G>::kThreads) void layer_norm_backward_kernel(LayerNormArgs a) {
     using Gr = Group<G>;
     constexpr int V = kVec<T>;
+    // A workgroup's registers leave one or two of them to a CU: the next row's loads are
+    // under way during this one's sums.  (Where its columns past a whole vector let it: 32 a
+    // lane would spill.)
+    constexpr bool AHEAD = G >= 256 && (WHOLE || NV * V < 32), NEAR = AHEAD;
     // 32 columns a lane: their sums are in LDS, and leave the next row its registers (3000
     // x 16384 fp16: 104 us with the sums in registers and no row ahead, 85 so)
     constexpr bool IN_LDS = NV * V == 32 && G > 64;
@@ -231,7 +295,7 @@ __global__ __launch_bounds__(Group<G>::kThreads) void layer_norm_backward_kernel
     float gw[NV][V], gb[NV][V];
 #pragma unroll
     for (int i = 0; i < NV; ++i) {
-        if (a.weight) w[i] = load_bits<T, WHOLE>(static_cast<const T*>(a.weight), (i * G + lane) * V, a.n);
+        if (a.weight) w[i] = load_near<T, NEAR, WHOLE>(static_cast<const T*>(a.weight), (i * G + lane) * V, a.n);
 #pragma unroll
         for (int k = 0; k < V; ++k) gw[i][k] = gb[i][k] = 0.f;
         if constexpr (IN_LDS) {
@@ -239,13 +303,9 @@ __global__ __launch_bounds__(Group<G>::kThreads) void layer_norm_backward_kernel
             for (int q = 0; q < V / 2; ++q) reinterpret_cast<fx4*>(sums)[q * NV * G + i * G + lane] = fx4{0.f, 0.f, 0.f, 0.f};
         }
     }
-    // A workgroup's registers leave one or two of them to a CU: the next row's loads are
-    // under way during this one's sums.
-    // (32 columns a lane and the path by elements would spill)
-    constexpr bool AHEAD = G >= 256 && (WHOLE || NV * V < 32);
-    // Every lane loads then, those past the row's end its start: a load that may not be there
-    // has the compiler wait for all that are under way.
-    constexpr bool EVERY = AHEAD && WHOLE;
+#pragma unroll
+    for (int i = 0; i < NV; ++i)
+        if (a.weight) in_place<T, NEAR, WHOLE>(w[i], (i * G + lane) * V, a.n);
     struct Row {
         ux4 x[NV], g[NV];
         float mean, by;
@@ -257,14 +317,8 @@ __global__ __launch_bounds__(Group<G>::kThreads) void layer_norm_backward_kernel
         const T* g = static_cast<const T*>(a.grad_y) + row * a.gy_stride;
 #pragma unroll
         for (int i = 0; i < NV; ++i) {
-            const int c = (i * G + lane) * V;
-            if constexpr (EVERY) {
-                __builtin_memcpy(&f.x[i], x + (c < a.n ? c : 0), 16);
-                __builtin_memcpy(&f.g[i], g + (c < a.n ? c : 0), 16);
-            } else {
-                f.x[i] = load_bits<T, WHOLE>(x, c, a.n);
-                f.g[i] = load_bits<T, WHOLE>(g, c, a.n);
-            }
+            f.x[i] = load_near<T, NEAR, WHOLE>(x, (i * G + lane) * V, a.n);
+            f.g[i] = load_near<T, NEAR, WHOLE>(g, (i * G + lane) * V, a.n);
         }
         f.mean = a.stats[2 * row], f.by = a.stats[2 * row + 1];
     };
@@ -276,7 +330,7 @@ __global__ __launch_bounds__(Group<G>::kThreads) void layer_norm_backward_kernel
         if (a.grad_s) {
             const T* s = static_cast<const T*>(a.grad_s) + row * a.gs_stride;
 #pragma unroll
-            for (int i = 0; i < NV; ++i) more[i] = load_bits<T, WHOLE>(s, (i * G + lane) * V, a.n);
+            for (int i = 0; i < NV; ++i) more[i] = load_near<T, NEAR, WHOLE>(s, (i * G + lane) * V, a.n);
         }
         // (behind the last row this one once more)
         if constexpr (AHEAD) fetch(r0 + step < a.rows ? r0 + step : r0, next);
@@ -286,7 +340,8 @@ __global__ __launch_bounds__(Group<G>::kThreads) void layer_norm_backward_kernel
         for (int i = 0; i < NV; ++i) {
             const int c = (i * G + lane) * V;
             float m[V];
-            if (EVERY && c >= a.n) cur.g[i] = ux4{0, 0, 0, 0};
+            in_place<T, NEAR, WHOLE>(cur.x[i], c, a.n);
+            in_place<T, NEAR, WHOLE>(cur.g[i], c, a.n);
             unpack<T>(cur.x[i], h[i]);
             unpack<T>(cur.g[i], d[i]);
             if (a.weight) unpack<T>(w[i], m);
@@ -317,7 +372,10 @@ __global__ __launch_bounds__(Group<G>::kThreads) void layer_norm_backward_kernel
 #pragma unroll
             for (int i = 0; i < NV; ++i) {
                 float m[V];
-                if (a.grad_s) unpack<T>(more[i], m);
+                if (a.grad_s) {
+                    in_place<T, NEAR, WHOLE>(more[i], (i * G + lane) * V, a.n);
+                    unpack<T>(more[i], m);
+                }
 #pragma unroll
                 for (int k = 0; k < V; ++k) {
                     d[i][k] = (d[i][k] - s1 - h[i][k] * s2) * by;
@@ -518,7 +576,7 @@ static int layer_norm_rows(LayerNormArgs a, bool bwd, hipStream_t st) {
     using Gr = Group<G>;
     // (rows of a workgroup: one each, as far as a launch's 2^32 threads go; backward, the 512
     // lanes' registers leave one workgroup to a CU)
-    a.blocks = norm_row_blocks(a.rows, Gr::kGroups, bwd ? (G == 512 ? 1 : kMostNormBlocks) : G > 64 ? 1 << 13 : 8);
+    a.blocks = norm_row_blocks(a.rows, Gr::kGroups, bwd ? (G == 512 ? 1 : kMostNormBlocks) : G == 512 ? 2 : G > 64 ? 1 << 13 : 8);
     if (!bwd) {
         layer_norm_forward_kernel<T, G, NV, WHOLE><<<a.blocks, Gr::kThreads, 0, st>>>(a);
         return nsh_host::check_launch("layer_norm_forward");
