@@ -36,7 +36,7 @@ __global__ __launch_bounds__(kPassThreads) void gated_copy_kernel(CopyArgs a) {
     for (int64_t i = static_cast<int64_t>(blockIdx.x) * kPassThreads + threadIdx.x; i < all; i += step) {
         const int64_t row = i / each;
         const int c = static_cast<int>(i - row * each) * kVec<T>;
-        const ux4 v = load_bits(static_cast<const T*>(s.from) + row * s.stride, c, a.n);
+        const ux4 v = load_any(static_cast<const T*>(s.from) + row * s.stride, c, a.n);
         *reinterpret_cast<ux4*>(static_cast<T*>(s.to) + row * a.np + c) = v;
     }
 }
@@ -51,8 +51,8 @@ __global__ __launch_bounds__(kPassThreads) void gated_split_kernel(CopyArgs a) {
         const int c = static_cast<int>(i - row * each) * 8;
         const float* from = static_cast<const float*>(s.from) + row * s.stride;
         float x[8], part[3][8];
-        unpack<float>(load_bits(from, c, a.n), *reinterpret_cast<float(*)[4]>(&x[0]));
-        unpack<float>(load_bits(from, c + 4, a.n), *reinterpret_cast<float(*)[4]>(&x[4]));
+        unpack<float>(load_any(from, c, a.n), *reinterpret_cast<float(*)[4]>(&x[0]));
+        unpack<float>(load_any(from, c + 4, a.n), *reinterpret_cast<float(*)[4]>(&x[4]));
 #pragma unroll
         for (int e = 0; e < 8; ++e) {
             float p[3];
@@ -154,10 +154,14 @@ __global__ __launch_bounds__(kPassThreads) void gated_most_kernel(const f16* gh,
         for (int64_t c = static_cast<int64_t>(blockIdx.x) * (kPassThreads * 8 * kParts) + threadIdx.x * 8; c < n;
              c += static_cast<int64_t>(gridDim.x) * (kPassThreads * 8 * kParts)) {
             ux4 v[kParts];
+            // (past the end the last numbers once more)
 #pragma unroll
             for (int i = 0; i < kParts; ++i) {
                 const int64_t at = c + i * kPassThreads * 8;
-                v[i] = load_bits(gh + row * stride + (at < n ? at : 0), 0, static_cast<int>(max(min(n - at, int64_t(8)), int64_t(0))));
+                if (n < 8)
+                    v[i] = load_bits(gh + row * stride, 0, static_cast<int>(n));
+                else
+                    __builtin_memcpy(&v[i], gh + row * stride + min(at, n - 8), 16);
             }
 #pragma unroll
             for (int i = 0; i < kParts; ++i) {

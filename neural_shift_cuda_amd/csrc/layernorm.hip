@@ -34,33 +34,6 @@ struct LayerNormArgs {
     float eps, inv_n;
 };
 
-// Columns c .. c + kVec - 1 of a row of n >= kVec, and of one with fewer left its last
-// kVec, which in_place() brings to where they belong, zeros behind them.  Every lane loads:
-// a load that may not be there has the compiler wait for all that are under way.  NEAR false:
-// load_bits(), for n < kVec, and where nothing is under way and registers are short.
-template <typename T, bool NEAR, bool WHOLE>
-__device__ __forceinline__ ux4 load_near(const T* row, int c, int n) {
-    if constexpr (!NEAR) return load_bits<T, WHOLE>(row, c, n);
-    ux4 r;
-    __builtin_memcpy(&r, row + min(c, n - kVec<T>), 16);
-    return r;
-}
-template <typename T, bool NEAR, bool WHOLE>
-__device__ __forceinline__ void in_place(ux4& r, int c, int n) {
-    if constexpr (!NEAR) return;
-    const int past = c + kVec<T> - n;
-    if (WHOLE ? past > 0 : past >= kVec<T>)
-        r = ux4{0, 0, 0, 0};
-    else if (!WHOLE && past > 0)
-        r = __builtin_bit_cast(ux4, __builtin_bit_cast(unsigned __int128, r) >> (past * 8 * static_cast<int>(sizeof(T))));
-}
-template <typename T, bool NEAR, bool WHOLE>
-__device__ __forceinline__ ux4 load_row(const T* row, int c, int n) {
-    ux4 r = load_near<T, NEAR, WHOLE>(row, c, n);
-    in_place<T, NEAR, WHOLE>(r, c, n);
-    return r;
-}
-
 // Groups of G lanes; several waves meet through LDS, `turn` telling two sums in a
 // row apart.
 template <int G>
