@@ -591,7 +591,7 @@ NSH_API int64_t nsh_attention_workspace_bytes(const nsh_attention_args* args, in
  *   grad_x = grad_s + d(y), of x and of the residual alike
  * A NULL weight is 1, a NULL bias 0.  Inputs have a unit last stride, the given
  * strides from row to row (elements) and any alignment; outputs are contiguous.
- * n <= 2^26, rows <= 2^40. */
+ * n <= 2^30, rows <= 2^40. */
 typedef struct nsh_layer_norm_args {
     const void *x, *residual, *weight, *bias; /* backward: x is what was normed, s with a residual */
     int64_t rows, n, x_stride, residual_stride;
@@ -616,7 +616,7 @@ NSH_API int64_t nsh_layer_norm_workspace_bytes(const nsh_layer_norm_args* args);
  * x (rows, K), gate and up (F, K) with a unit last stride and the given strides from row
  * to row (elements), any alignment (rows that do not start on 16 bytes, or whose width is
  * no multiple of 16 bytes, are copied into the workspace first).  K, F <= 2^20, rows <=
- * 2^28.  Products, the activation and all sums are float (of fp32 matrices, where it is
+ * 2^30.  Products, the activation and all sums are float (of fp32 matrices, where it is
  * faster, each product from six of bf16 parts, copied into the workspace: what is finite
  * keeps fp32's bits, infinity times infinity is NaN); dg and du are rounded to `dtype` (fp16: times a
  * power of two that the call chooses) as operands of the gradients' products. */

@@ -68,7 +68,7 @@ __global__ __launch_bounds__(kPassThreads) void gated_split_kernel(CopyArgs a) {
 
 struct SlopeArgs {
     const void* gh;
-    int64_t gh_stride, rows, dgu_stride, dgu_plane;  // elements
+    int64_t gh_stride, first, rows, dgu_stride, dgu_plane;  // elements; rows from the first on
     char* kept;
     void* dgu;
     int F, Fp;
@@ -87,8 +87,8 @@ __global__ __launch_bounds__(kPassThreads) void gated_slope_kernel(SlopeArgs a) 
     const uint32_t down = blockIdx.x / a.across, across = blockIdx.x - down * a.across;
     const int c0 = (across * (kPassThreads / 64) + wave_id()) * COLS;
     if (c0 >= a.Fp) return;
-    const int64_t m0 = static_cast<int64_t>(down) * 32, rows = a.rows - m0;
     const float by = __is_same(T, f16) && a.scale ? a.scale[0] : 1.f;
+    const int64_t m0 = a.first + static_cast<int64_t>(down) * 32, rows = a.rows - m0;
     Kept<T> k[BLOCKS];
 #pragma unroll
     for (int b = 0; b < BLOCKS; ++b)
@@ -277,8 +277,8 @@ Plan plan_of(const nsh_gated_linear_args* g, bool bwd) {
     if (wide && !p.few) {
         // against the time of taking the parts: 4 bytes read, 6 written and read once more
         nsh::Cut parts = cut_of(g, bwd, {false, 6});
-        parts.time += 4 + static_cast<double>((g->rows + 2 * g->F) * g->K) * 10 / 3.5e6;
-        p.parts = parts.time < p.cut.time;
+        const double taken = parts.time + 4 + static_cast<double>((g->rows + 2 * g->F) * g->K) * 10 / 3.5e6;
+        p.parts = parts.time > 0 && (p.cut.time == 0 || taken < p.cut.time);
         if (p.parts) p.cut = parts;
     }
     p.esz = wide && !p.parts ? 4 : 2;
@@ -319,8 +319,8 @@ int check(const char* op, const nsh_gated_linear_args* g, bool bwd) {
     if (g->dtype < NSH_DTYPE_FLOAT16 || g->dtype > NSH_DTYPE_FLOAT32)
         return fail(NSH_ERR_INVALID, "%s: unsupported dtype code %d", op, g->dtype);
     if (g->rows < 1 || g->K < 1 || g->F < 1) return fail(NSH_ERR_INVALID, "%s: empty tensor", op);
-    if (g->K > kWidest || g->F > kWidest || g->rows > (int64_t(1) << 28))
-        return fail(NSH_ERR_INVALID, "%s: width or hidden size above 2^20, or more than 2^28 rows", op);
+    if (g->K > kWidest || g->F > kWidest || g->rows > (int64_t(1) << 30))
+        return fail(NSH_ERR_INVALID, "%s: width or hidden size above 2^20, or more than 2^30 rows", op);
     if (g->activation < NSH_ACTIVATION_SILU || g->activation > NSH_ACTIVATION_SIGMOID)
         return fail(NSH_ERR_INVALID, "%s: unknown activation code %d", op, g->activation);
     if (!g->x || !g->gate_weight || !g->up_weight ||
@@ -376,8 +376,12 @@ int backward(const nsh_gated_linear_args* g, const Plan& p, nsh::GatedArgs a, ch
     a.scale = scale, a.dgu = ws + p.dgu;
     a.dgu_plane = p.planes;
     const uint32_t across = static_cast<uint32_t>(ceil_div(a.Fp, nsh::kPassThreads / 64 * 128 / sizeof(T)));
-    const nsh::SlopeArgs s{g->grad_h, g->gh_stride, g->rows, 2 * p.Fp + 128 / p.esz, p.planes / p.esz, a.kept, a.dgu, a.F, a.Fp, across, scale};
-    nsh::gated_slope_kernel<T, PARTS><<<static_cast<unsigned>(across * ceil_div(g->rows, 32)), nsh::kPassThreads, 0, st>>>(s);
+    nsh::SlopeArgs s{g->grad_h, g->gh_stride, 0, g->rows, 2 * p.Fp + 128 / p.esz, p.planes / p.esz, a.kept, a.dgu, a.F, a.Fp, across, scale};
+    const int64_t most = std::max((1 << 20) / across, 1u);  // rows of blocks a launch
+    for (; s.first < g->rows; s.first += most * 32) {
+        const int64_t downs = std::min(ceil_div(g->rows - s.first, 32), most);
+        nsh::gated_slope_kernel<T, PARTS><<<static_cast<unsigned>(across * downs), nsh::kPassThreads, 0, st>>>(s);
+    }
     a.Kq = static_cast<int>(up(g->K, 4));
     a.part = p.cut.splits > 1 ? reinterpret_cast<float*>(ws + p.part) : nullptr;
     const int rc = nsh::gated_gradients<T, PARTS>(a, p.cut, st);
@@ -409,6 +413,7 @@ int gated_linear(const char* op, const nsh_gated_linear_args* g, bool bwd, void*
     const int rc = check(op, g, bwd);
     if (rc != NSH_OK) return rc;
     const Plan p = plan_of(g, bwd);
+    if (!p.few && p.cut.time == 0) return fail(NSH_ERR_INVALID, "%s: more tiles than one launch takes", op);
     if (p.bytes > 0 && (!g->workspace || g->workspace_bytes < p.bytes))
         return fail(NSH_ERR_INVALID, "%s: workspace smaller than nsh_gated_linear_workspace_bytes", op);
     if (p.bytes > 0 && !nsh_host::aligned(g->workspace, 16)) return fail(NSH_ERR_INVALID, "%s: misaligned workspace", op);

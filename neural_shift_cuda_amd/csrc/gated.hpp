@@ -596,7 +596,9 @@ struct Means {
     int64_t panels(int64_t length) const { return nsh_host::ceil_div(length, wide ? 32 : 64) * terms; }
 };
 
+// (0: no launch takes as many)
 inline double time_of(const Shape& s, const float (&rate)[3], Part a, Part b) {
+    if ((a.n + b.n) * (s.bm == 256 ? 512 : 256) >> 32) return 0;
     const int64_t cus = nsh_host::compute_units();
     int share = 1;
     while (share < 3 && rate[share] > 0 && share * cus < a.n + b.n) ++share;
@@ -609,7 +611,7 @@ inline Cut forward_cut(int64_t rows, int64_t F, int64_t K, Means by) {
         const Shape& s = kShapes[i];
         Cut c{i, static_cast<int>(nsh_host::ceil_div(rows, s.bm)), static_cast<int>(nsh_host::ceil_div(F, s.bn / 2)), 1, 0, 0, 0};
         c.time = time_of(s, by.wide ? s.wide : s.along, {c.tiles(), by.panels(K)}, {0, 0});
-        if (best.time == 0 || c.time < best.time) best = c;
+        if (c.time > 0 && (best.time == 0 || c.time < best.time)) best = c;
     }
     return best;
 }
@@ -630,6 +632,7 @@ inline Cut gradient_cut(int64_t rows, int64_t K, int64_t F, Means by, bool input
             c.splits = splits;
             c.time = time_of(s, by.wide ? s.wide : s.across, {c.tiles() * splits, nsh_host::ceil_div(panels, splits)},
                              {c.weights(), by.panels(rows)});
+            if (c.time == 0) break;
             if (splits > 1) c.time += 4 + static_cast<double>(splits * rows * K) * 4 / 3.5e6;
             if (best.time == 0 || c.time < best.time) best = c;
         }

@@ -521,19 +521,21 @@ __global__ __launch_bounds__(1024) void layer_norm_weights_kernel(LayerNormArgs 
     void* out = blockIdx.y ? a.gb : a.gw;
     if (!out) return;
     const int col = threadIdx.x % 32, run = threadIdx.x / 32;
-    const int64_t c = static_cast<int64_t>(blockIdx.x) * 32 + col;
     const float* at = a.partial + (blockIdx.y ? a.n : 0);
     const int len = (a.blocks + 31) / 32, end = min(a.blocks, (run + 1) * len);
-    float s = 0.f;
-    if (c < a.n) {
+    for (int64_t c = static_cast<int64_t>(blockIdx.x) * 32 + col; c - col < a.n; c += static_cast<int64_t>(gridDim.x) * 32) {
+        float s = 0.f;
+        if (c < a.n) {
 #pragma unroll 8
-        for (int i = run * len; i < end; ++i) s += at[static_cast<int64_t>(i) * 2 * a.n + c];
-    }
-    part[run][col] = s;
-    __syncthreads();
-    if (run == 0 && c < a.n) {
-        for (int i = 1; i < 32; ++i) s += part[i][col];
-        static_cast<T*>(out)[c] = from_acc<T>(s);
+            for (int i = run * len; i < end; ++i) s += at[static_cast<int64_t>(i) * 2 * a.n + c];
+        }
+        part[run][col] = s;
+        __syncthreads();
+        if (run == 0 && c < a.n) {
+            for (int i = 1; i < 32; ++i) s += part[i][col];
+            static_cast<T*>(out)[c] = from_acc<T>(s);
+        }
+        __syncthreads();
     }
 }
 
@@ -543,6 +545,13 @@ static int norm_row_blocks(int64_t rows, int per, int64_t each) {
     return static_cast<int>(std::min(nsh_host::ceil_div(rows, per), nsh_host::compute_units() * each));
 }
 constexpr int kMostNormBlocks = 2;  // of the backward, a CU
+
+// (a launch takes less than 2^32 threads)
+template <typename T>
+static void layer_norm_weights(const LayerNormArgs& a, hipStream_t st) {
+    const int blocks = std::min((a.n + 31) / 32, 1 << 20);
+    layer_norm_weights_kernel<T><<<dim3(blocks, 2), 1024, 0, st>>>(a);
+}
 
 template <typename T, int G, int NV, bool WHOLE>
 static int layer_norm_rows(LayerNormArgs a, bool bwd, hipStream_t st) {
@@ -555,7 +564,7 @@ static int layer_norm_rows(LayerNormArgs a, bool bwd, hipStream_t st) {
         return nsh_host::check_launch("layer_norm_forward");
     }
     layer_norm_backward_kernel<T, G, NV, WHOLE><<<a.blocks, Gr::kThreads, 0, st>>>(a);
-    if (a.partial) layer_norm_weights_kernel<T><<<dim3((a.n + 31) / 32, 2), 1024, 0, st>>>(a);
+    if (a.partial) layer_norm_weights<T>(a, st);
     return nsh_host::check_launch("layer_norm_backward");
 }
 
@@ -575,7 +584,7 @@ static int layer_norm_wide(LayerNormArgs a, bool bwd, hipStream_t st) {
     if (a.partial) {
         constexpr int kCols = 64 * kVec<T>;
         layer_norm_columns_kernel<T><<<dim3((a.n + kCols - 1) / kCols, a.blocks), 64, 0, st>>>(a);
-        layer_norm_weights_kernel<T><<<dim3((a.n + 31) / 32, 2), 1024, 0, st>>>(a);
+        layer_norm_weights<T>(a, st);
     }
     return nsh_host::check_launch("layer_norm_backward");
 }
@@ -613,8 +622,8 @@ static int layer_norm(const char* op, const nsh_layer_norm_args* g, bool bwd, vo
     if (g->dtype < NSH_DTYPE_FLOAT16 || g->dtype > NSH_DTYPE_FLOAT32)
         return fail(NSH_ERR_INVALID, "%s: unsupported dtype code %d", op, g->dtype);
     if (g->rows < 1 || g->n < 1) return fail(NSH_ERR_INVALID, "%s: empty tensor", op);
-    if (g->n > (int64_t(1) << 26) || g->rows > (int64_t(1) << 40))
-        return fail(NSH_ERR_INVALID, "%s: rows wider than 2^26 or more than 2^40", op);
+    if (g->n > (int64_t(1) << 30) || g->rows > (int64_t(1) << 40))
+        return fail(NSH_ERR_INVALID, "%s: rows wider than 2^30 or more than 2^40", op);
     if (!(g->eps >= 0) || std::isinf(g->eps)) return fail(NSH_ERR_INVALID, "%s: eps must be finite and not negative", op);
     if (bwd ? !g->x || !g->grad_y || !g->stats || (!g->grad_x && !g->grad_weight && !g->grad_bias)
             : !g->x || !g->y || !g->residual != !g->s)

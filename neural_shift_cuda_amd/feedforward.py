@@ -120,7 +120,7 @@ def layer_norm(x: torch.Tensor, weight: Optional[torch.Tensor] = None,
 
     Returns y, or (y, s) with a residual, contiguous.  Differentiable in all of
     them (x and residual have the same gradient); the weights' gradients are
-    summed in fp32 in a fixed order.  The GPU serves widths up to 2^26."""
+    summed in fp32 in a fixed order.  The GPU serves widths up to 2^30."""
     if not x.is_cuda:
         return layer_norm_reference(x, weight, bias, residual=residual, eps=eps)
     done = _C and _C.layer_norm_as_is(x, weight, bias, residual, eps)

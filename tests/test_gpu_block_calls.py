@@ -458,6 +458,23 @@ def test_more_rows_than_workgroups():
     assert not y[:-300].any()
 
 
+def test_rows_wider_than_a_launch_of_their_columns():
+    """The weights' sums are taken 32 columns a workgroup, and again behind 2^25 of them."""
+    n = (1 << 25) + 70
+    x, gy = torch.zeros(2, n, device=DEV, dtype=torch.float16), torch.zeros(2, n, device=DEV, dtype=torch.float16)
+    x[0, :n // 2], x[0, n // 2:] = 1.0, -1.0  # mean 0, variance 1
+    gy[:, -100:] = tensors((2, 100), dtype=torch.float16)[0]
+    b = torch.zeros(n, device=DEV, dtype=torch.float16).requires_grad_()
+    w = torch.ones(n, device=DEV, dtype=torch.float16).requires_grad_()
+    y = layer_norm(x, w, b, eps=0.0625)
+    assert (y[0, n // 2:] == y[0, -1]).all() and abs(float(y[0, -1]) + 1.0625 ** -0.5) < 1e-3 and not y[1].any()
+    gw, gb = torch.autograd.grad(y, [w, b], gy)
+    want = gy[0, -100:].double() * -1.0625 ** -0.5
+    assert (gw[-100:].double() - want).abs().max() <= 2.0 ** -9 * want.abs().max() and not gw[:-100].any()
+    total = gy[:, -100:].double().sum(0)
+    assert ((gb[-100:].double() - total).abs() <= 2.0 ** -11 * total.abs() + 2.0 ** -24).all() and not gb[:-100].any()
+
+
 @pytest.mark.parametrize("dtype", [torch.float16, torch.bfloat16, torch.float32])
 @pytest.mark.parametrize("bad", [float("nan"), float("inf")])
 def test_gradients_of_a_row_without_numbers(dtype, bad):
@@ -470,3 +487,34 @@ def test_gradients_of_a_row_without_numbers(dtype, bad):
     assert gx[33].isnan().all() and gg[:, 5].isnan().all() and not gu[:, 5].isfinite().any()
     rest = [m for m in range(70) if m != 33]
     oracle.close(gx[rest], vals["gx"][rest], tols["gx"][rest], "gx")
+
+
+def test_more_rows_than_a_launch_has_threads():
+    """2^30 rows: 64 of them a workgroup would be a launch of 2^32 threads."""
+    M, K, F = 1 << 30, 8, 1
+    xs, gate, up = gated_leaves(100, K, F, torch.bfloat16)
+    x = torch.zeros(M, K, device=DEV, dtype=torch.bfloat16)
+    x[-100:] = xs
+    h = gated_linear(x, gate, up)
+    vals, tols = oracle.gated(xs.cpu(), gate.cpu(), up.cpu(), "silu")
+    oracle.close(h[-100:], vals["h"], tols["h"], "h")
+    assert not h[:-100].any()
+    with pytest.raises(RuntimeError, match="2\\^30"):
+        gated_linear(torch.zeros(1, K, device=DEV, dtype=torch.bfloat16).expand(M + 1, K), gate, up)
+
+
+def test_gradients_of_more_blocks_than_workgroups():
+    """dg and du of 2^25 rows and some: workgroups take turns."""
+    M, K, F = (1 << 25) + 100, 8, 16
+    xs, gate, up = gated_leaves(100, K, F, torch.bfloat16)
+    x = torch.zeros(M, K, device=DEV, dtype=torch.bfloat16)
+    x[-100:] = xs
+    leaf = [t.requires_grad_() for t in (x, gate, up)]
+    h = gated_linear(*leaf)
+    gh = torch.zeros_like(h)
+    gh[-100:] = tensors((100, F), dtype=torch.bfloat16, seed=4)[0]
+    got = torch.autograd.grad(h, leaf, gh)
+    vals, tols = oracle.gated(xs.cpu(), gate.detach().cpu(), up.detach().cpu(), "silu", gh[-100:].cpu())
+    for v, n in zip((h, *got), ("h", "gx", "ggate", "gup")):
+        oracle.close(v[-100:], vals[n], tols[n], n)
+    assert not got[0][:-100].any()
