@@ -36,7 +36,7 @@ __global__ __launch_bounds__(kPassThreads) void gated_copy_kernel(CopyArgs a) {
     for (int64_t i = static_cast<int64_t>(blockIdx.x) * kPassThreads + threadIdx.x; i < all; i += step) {
         const int64_t row = i / each;
         const int c = static_cast<int>(i - row * each) * kVec<T>;
-        const ux4 v = load_any(static_cast<const T*>(s.from) + row * s.stride, c, a.n);
+        const ux4 v = load_row<T, kShort>(static_cast<const T*>(s.from) + row * s.stride, c, a.n);
         *reinterpret_cast<ux4*>(static_cast<T*>(s.to) + row * a.np + c) = v;
     }
 }
@@ -51,8 +51,8 @@ __global__ __launch_bounds__(kPassThreads) void gated_split_kernel(CopyArgs a) {
         const int c = static_cast<int>(i - row * each) * 8;
         const float* from = static_cast<const float*>(s.from) + row * s.stride;
         float x[8], part[3][8];
-        unpack<float>(load_any(from, c, a.n), *reinterpret_cast<float(*)[4]>(&x[0]));
-        unpack<float>(load_any(from, c + 4, a.n), *reinterpret_cast<float(*)[4]>(&x[4]));
+        unpack<float>(load_row<float, kShort>(from, c, a.n), *reinterpret_cast<float(*)[4]>(&x[0]));
+        unpack<float>(load_row<float, kShort>(from, c + 4, a.n), *reinterpret_cast<float(*)[4]>(&x[4]));
 #pragma unroll
         for (int e = 0; e < 8; ++e) {
             float p[3];

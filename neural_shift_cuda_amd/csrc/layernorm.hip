@@ -83,6 +83,13 @@ __device__ __forceinline__ float variance(Gr& group, float square, float off, co
     return rest;
 }
 
+// Whole vectors need nothing but a mask, which keeps registers free where no row is loaded
+// ahead (16384 x 2048 bf16, forward: 46 us, 52 by kNear); others (backward, by elements and
+// by kNear: 16384 x 2047 bf16 65 and 42 us, 16384 x 333 25 and 13).
+constexpr Reach reach_of(int lanes, bool ahead, bool whole) {
+    return whole && !ahead ? kMasked : lanes == 8 ? kShort : kNear;
+}
+
 template <typename T, int G, int NV, bool WHOLE>
 __global__ __launch_bounds__(Group<G>::kThreads) void layer_norm_forward_kernel(LayerNormArgs a) {
     using Gr = Group<G>;
@@ -94,21 +101,21 @@ __global__ __launch_bounds__(Group<G>::kThreads) void layer_norm_forward_kernel(
     // rows, and has the next one's loads under way (3000 x 16384 fp16: 48 us with a row each, 38
     // so).
     constexpr bool AHEAD = G == 512, KEEP = G <= 64 || AHEAD;
-    constexpr bool NEAR = G > 8 && (AHEAD || !WHOLE);
+    constexpr Reach REACH = reach_of(G, AHEAD, WHOLE);
     const int lane = threadIdx.x % G, own = threadIdx.x / G;
     ux4 w[KEEP ? NV : 1], b[KEEP ? NV : 1];
     if constexpr (KEEP) {
 #pragma unroll
         for (int i = 0; i < NV; ++i) {
             const int c = (i * G + lane) * V;
-            if (a.weight) w[i] = load_near<T, NEAR, WHOLE>(static_cast<const T*>(a.weight), c, a.n);
-            if (a.bias) b[i] = load_near<T, NEAR, WHOLE>(static_cast<const T*>(a.bias), c, a.n);
+            if (a.weight) w[i] = load_near<T, REACH>(static_cast<const T*>(a.weight), c, a.n);
+            if (a.bias) b[i] = load_near<T, REACH>(static_cast<const T*>(a.bias), c, a.n);
         }
 #pragma unroll
         for (int i = 0; i < NV; ++i) {
             const int c = (i * G + lane) * V;
-            if (a.weight) in_place<T, NEAR, WHOLE>(w[i], c, a.n);
-            if (a.bias) in_place<T, NEAR, WHOLE>(b[i], c, a.n);
+            if (a.weight) in_place<T, REACH, WHOLE>(w[i], c, a.n);
+            if (a.bias) in_place<T, REACH, WHOLE>(b[i], c, a.n);
         }
     }
     struct Row {
@@ -119,11 +126,11 @@ __global__ __launch_bounds__(Group<G>::kThreads) void layer_norm_forward_kernel(
         const int64_t row = r0 + own < a.rows ? r0 + own : 0;
         const T* x = static_cast<const T*>(a.x) + row * a.x_stride;
 #pragma unroll
-        for (int i = 0; i < NV; ++i) f.x[i] = load_near<T, NEAR, WHOLE>(x, (i * G + lane) * V, a.n);
+        for (int i = 0; i < NV; ++i) f.x[i] = load_near<T, REACH>(x, (i * G + lane) * V, a.n);
         if (a.residual) {
             const T* r = static_cast<const T*>(a.residual) + row * a.residual_stride;
 #pragma unroll
-            for (int i = 0; i < NV; ++i) f.more[i] = load_near<T, NEAR, WHOLE>(r, (i * G + lane) * V, a.n);
+            for (int i = 0; i < NV; ++i) f.more[i] = load_near<T, REACH>(r, (i * G + lane) * V, a.n);
         }
     };
     // every lane of the workgroup takes every turn: the groups meet in lane exchanges
@@ -138,11 +145,11 @@ __global__ __launch_bounds__(Group<G>::kThreads) void layer_norm_forward_kernel(
 #pragma unroll
         for (int i = 0; i < NV; ++i) {
             const int c = (i * G + lane) * V;
-            in_place<T, NEAR, WHOLE>(cur.x[i], c, a.n);
+            in_place<T, REACH, WHOLE>(cur.x[i], c, a.n);
             unpack<T>(cur.x[i], v[i]);
             if (a.residual) {
                 float m[V];
-                in_place<T, NEAR, WHOLE>(cur.more[i], c, a.n);
+                in_place<T, REACH, WHOLE>(cur.more[i], c, a.n);
                 unpack<T>(cur.more[i], m);
 #pragma unroll
                 for (int k = 0; k < V; ++k) v[i][k] += m[k];
@@ -176,12 +183,12 @@ __global__ __launch_bounds__(Group<G>::kThreads) void layer_norm_forward_kernel(
 #pragma unroll
             for (int k = 0; k < V; ++k) v[i][k] = (v[i][k] - rest) * by;
             if (a.weight) {
-                unpack<T>(KEEP ? w[KEEP ? i : 0] : load_row<T, NEAR, WHOLE>(static_cast<const T*>(a.weight), c, a.n), m);
+                unpack<T>(KEEP ? w[KEEP ? i : 0] : load_row<T, REACH, WHOLE>(static_cast<const T*>(a.weight), c, a.n), m);
 #pragma unroll
                 for (int k = 0; k < V; ++k) v[i][k] *= m[k];
             }
             if (a.bias) {
-                unpack<T>(KEEP ? b[KEEP ? i : 0] : load_row<T, NEAR, WHOLE>(static_cast<const T*>(a.bias), c, a.n), m);
+                unpack<T>(KEEP ? b[KEEP ? i : 0] : load_row<T, REACH, WHOLE>(static_cast<const T*>(a.bias), c, a.n), m);
 #pragma unroll
                 for (int k = 0; k < V; ++k) v[i][k] += m[k];
             }
@@ -256,7 +263,8 @@ __global__ __launch_bounds__(Group<G>::kThreads) void layer_norm_backward_kernel
     // A workgroup's registers leave one or two of them to a CU: the next row's loads are
     // under way during this one's sums.  (Where its columns past a whole vector let it: 32 a
     // lane would spill.)
-    constexpr bool AHEAD = G >= 256 && (WHOLE || NV * V < 32), NEAR = AHEAD;
+    constexpr bool AHEAD = G >= 256 && (WHOLE || NV * V < 32);
+    constexpr Reach REACH = reach_of(G, AHEAD, WHOLE);
     // 32 columns a lane: their sums are in LDS, and leave the next row its registers (3000
     // x 16384 fp16: 104 us with the sums in registers and no row ahead, 85 so)
     constexpr bool IN_LDS = NV * V == 32 && G > 64;
@@ -268,7 +276,7 @@ __global__ __launch_bounds__(Group<G>::kThreads) void layer_norm_backward_kernel
     float gw[NV][V], gb[NV][V];
 #pragma unroll
     for (int i = 0; i < NV; ++i) {
-        if (a.weight) w[i] = load_near<T, NEAR, WHOLE>(static_cast<const T*>(a.weight), (i * G + lane) * V, a.n);
+        if (a.weight) w[i] = load_near<T, REACH>(static_cast<const T*>(a.weight), (i * G + lane) * V, a.n);
 #pragma unroll
         for (int k = 0; k < V; ++k) gw[i][k] = gb[i][k] = 0.f;
         if constexpr (IN_LDS) {
@@ -278,7 +286,7 @@ __global__ __launch_bounds__(Group<G>::kThreads) void layer_norm_backward_kernel
     }
 #pragma unroll
     for (int i = 0; i < NV; ++i)
-        if (a.weight) in_place<T, NEAR, WHOLE>(w[i], (i * G + lane) * V, a.n);
+        if (a.weight) in_place<T, REACH, WHOLE>(w[i], (i * G + lane) * V, a.n);
     struct Row {
         ux4 x[NV], g[NV];
         float mean, by;
@@ -290,8 +298,8 @@ __global__ __launch_bounds__(Group<G>::kThreads) void layer_norm_backward_kernel
         const T* g = static_cast<const T*>(a.grad_y) + row * a.gy_stride;
 #pragma unroll
         for (int i = 0; i < NV; ++i) {
-            f.x[i] = load_near<T, NEAR, WHOLE>(x, (i * G + lane) * V, a.n);
-            f.g[i] = load_near<T, NEAR, WHOLE>(g, (i * G + lane) * V, a.n);
+            f.x[i] = load_near<T, REACH>(x, (i * G + lane) * V, a.n);
+            f.g[i] = load_near<T, REACH>(g, (i * G + lane) * V, a.n);
         }
         f.mean = a.stats[2 * row], f.by = a.stats[2 * row + 1];
     };
@@ -303,7 +311,7 @@ __global__ __launch_bounds__(Group<G>::kThreads) void layer_norm_backward_kernel
         if (a.grad_s) {
             const T* s = static_cast<const T*>(a.grad_s) + row * a.gs_stride;
 #pragma unroll
-            for (int i = 0; i < NV; ++i) more[i] = load_near<T, NEAR, WHOLE>(s, (i * G + lane) * V, a.n);
+            for (int i = 0; i < NV; ++i) more[i] = load_near<T, REACH>(s, (i * G + lane) * V, a.n);
         }
         // (behind the last row this one once more)
         if constexpr (AHEAD) fetch(r0 + step < a.rows ? r0 + step : r0, next);
@@ -313,8 +321,8 @@ __global__ __launch_bounds__(Group<G>::kThreads) void layer_norm_backward_kernel
         for (int i = 0; i < NV; ++i) {
             const int c = (i * G + lane) * V;
             float m[V];
-            in_place<T, NEAR, WHOLE>(cur.x[i], c, a.n);
-            in_place<T, NEAR, WHOLE>(cur.g[i], c, a.n);
+            in_place<T, REACH, WHOLE>(cur.x[i], c, a.n);
+            in_place<T, REACH, WHOLE>(cur.g[i], c, a.n);
             unpack<T>(cur.x[i], h[i]);
             unpack<T>(cur.g[i], d[i]);
             if (a.weight) unpack<T>(w[i], m);
@@ -346,7 +354,7 @@ __global__ __launch_bounds__(Group<G>::kThreads) void layer_norm_backward_kernel
             for (int i = 0; i < NV; ++i) {
                 float m[V];
                 if (a.grad_s) {
-                    in_place<T, NEAR, WHOLE>(more[i], (i * G + lane) * V, a.n);
+                    in_place<T, REACH, WHOLE>(more[i], (i * G + lane) * V, a.n);
                     unpack<T>(more[i], m);
                 }
 #pragma unroll
@@ -397,10 +405,10 @@ using WideGroup = Group<kWideThreads>;
 
 template <typename T>
 __device__ __forceinline__ void wide_values(const LayerNormArgs& a, int64_t row, int c, bool summed, float (&v)[kVec<T>]) {
-    unpack<T>(load_bits(static_cast<const T*>(a.x) + row * a.x_stride, c, a.n), v);
+    unpack<T>(load_row<T, kNear>(static_cast<const T*>(a.x) + row * a.x_stride, c, a.n), v);
     if (summed && a.residual) {
         float m[kVec<T>];
-        unpack<T>(load_bits(static_cast<const T*>(a.residual) + row * a.residual_stride, c, a.n), m);
+        unpack<T>(load_row<T, kNear>(static_cast<const T*>(a.residual) + row * a.residual_stride, c, a.n), m);
 #pragma unroll
         for (int k = 0; k < kVec<T>; ++k) v[k] += m[k];
         unpack<T>(pack<T>(v), v);
@@ -435,12 +443,12 @@ __global__ __launch_bounds__(kWideThreads) void layer_norm_wide_forward_kernel(L
 #pragma unroll
             for (int k = 0; k < V; ++k) v[k] = (v[k] - mean - rest) * by;
             if (a.weight) {
-                unpack<T>(load_bits(static_cast<const T*>(a.weight), c, a.n), m);
+                unpack<T>(load_row<T, kNear>(static_cast<const T*>(a.weight), c, a.n), m);
 #pragma unroll
                 for (int k = 0; k < V; ++k) v[k] *= m[k];
             }
             if (a.bias) {
-                unpack<T>(load_bits(static_cast<const T*>(a.bias), c, a.n), m);
+                unpack<T>(load_row<T, kNear>(static_cast<const T*>(a.bias), c, a.n), m);
 #pragma unroll
                 for (int k = 0; k < V; ++k) v[k] += m[k];
             }
@@ -461,9 +469,9 @@ __global__ __launch_bounds__(kWideThreads) void layer_norm_wide_backward_kernel(
         for (int turn = 0; turn < 2; ++turn) {
             for (int c = threadIdx.x * V; c < a.n; c += kStep) {
                 wide_values<T>(a, row, c, false, h);
-                unpack<T>(load_bits(g, c, a.n), d);
+                unpack<T>(load_row<T, kNear>(g, c, a.n), d);
                 if (a.weight) {
-                    unpack<T>(load_bits(static_cast<const T*>(a.weight), c, a.n), m);
+                    unpack<T>(load_row<T, kNear>(static_cast<const T*>(a.weight), c, a.n), m);
 #pragma unroll
                     for (int k = 0; k < V; ++k) d[k] *= m[k];
                 }
@@ -477,7 +485,7 @@ __global__ __launch_bounds__(kWideThreads) void layer_norm_wide_backward_kernel(
 #pragma unroll
                 for (int k = 0; k < V; ++k) d[k] = (d[k] - s1 - h[k] * s2) * by;
                 if (a.grad_s) {
-                    unpack<T>(load_bits(static_cast<const T*>(a.grad_s) + row * a.gs_stride, c, a.n), m);
+                    unpack<T>(load_row<T, kNear>(static_cast<const T*>(a.grad_s) + row * a.gs_stride, c, a.n), m);
 #pragma unroll
                     for (int k = 0; k < V; ++k) d[k] += m[k];
                 }
@@ -501,7 +509,7 @@ __global__ __launch_bounds__(64) void layer_norm_columns_kernel(LayerNormArgs a)
         const float mean = a.stats[2 * row], by = a.stats[2 * row + 1];
         float h[V], d[V];
         wide_values<T>(a, row, c, false, h);
-        unpack<T>(load_bits(static_cast<const T*>(a.grad_y) + row * a.gy_stride, c, a.n), d);
+        unpack<T>(load_row<T, kNear>(static_cast<const T*>(a.grad_y) + row * a.gy_stride, c, a.n), d);
 #pragma unroll
         for (int k = 0; k < V; ++k) {
             gw[k] = fma_acc(d[k], (h[k] - mean) * by, gw[k]);

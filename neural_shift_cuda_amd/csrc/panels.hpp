@@ -347,17 +347,16 @@ struct Stage {
     static __device__ __forceinline__ void load(char* lds, const T* from, int64_t stride, int64_t rows, int64_t cols) {
         const int l = threadIdx.x & 63, n = static_cast<int>(min(cols, int64_t(COLS)));
         ux4 v[TURNS];
-        const bool near = n >= kVec<T>;
 #pragma unroll
         for (int t = 0; t < TURNS; ++t) {
             const int x = t * 64 + l, row = x / CHUNKS, c = x % CHUNKS * kVec<T>;
             v[t] = ux4{0, 0, 0, 0};
-            if (row < rows) v[t] = near ? load_near<T, true, false>(from + row * stride, c, n) : load_bits(from + row * stride, c, n);
+            if (row < rows) v[t] = load_near<T, kShort>(from + row * stride, c, n);
         }
 #pragma unroll
         for (int t = 0; t < TURNS; ++t) {
             const int x = t * 64 + l;
-            if (near) in_place<T, true, false>(v[t], x % CHUNKS * kVec<T>, n);
+            in_place<T, kShort>(v[t], x % CHUNKS * kVec<T>, n);
             *reinterpret_cast<ux4*>(lds + at(x / CHUNKS, x % CHUNKS)) = v[t];
         }
     }

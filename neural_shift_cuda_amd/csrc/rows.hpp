@@ -72,38 +72,37 @@ __device__ __forceinline__ void store_bits(T* row, int c, int n, ux4 r) {
     }
 }
 
-// Columns c .. c + kVec - 1 of a row of n >= kVec, and of one with fewer left its last
-// kVec, which in_place() brings to where they belong, zeros behind them.  Every lane loads:
-// a load that may not be there has the compiler wait for all that are under way.  NEAR false:
-// load_bits(), for n < kVec, and where nothing is under way and registers are short (a row's
-// last elements take it a load each, one after the other).
-template <typename T, bool NEAR, bool WHOLE>
+// How a lane past a row's end, or with less than kVec columns left, loads.
+//   kMasked: not at all (rows of whole vectors)
+//   kNear: the row's last kVec, which in_place() brings to where they belong, zeros behind
+//     them.  Every lane loads: a load that may not be there has the compiler wait for all that
+//     are under way, and single elements would be loads of their own, one after the other.
+//   kShort: so, and by elements where the row has less than kVec.
+enum Reach { kMasked, kNear, kShort };
+
+template <typename T, Reach REACH>
 __device__ __forceinline__ ux4 load_near(const T* row, int c, int n) {
-    if constexpr (!NEAR) return load_bits<T, WHOLE>(row, c, n);
+    if constexpr (REACH == kMasked) return load_bits<T, true>(row, c, n);
+    if (REACH == kShort && n < kVec<T>) return load_bits(row, c, n);
     ux4 r;
     __builtin_memcpy(&r, row + min(c, n - kVec<T>), 16);
     return r;
 }
-template <typename T, bool NEAR, bool WHOLE>
+template <typename T, Reach REACH, bool WHOLE = false>
 __device__ __forceinline__ void in_place(ux4& r, int c, int n) {
-    if constexpr (!NEAR) return;
+    if constexpr (REACH == kMasked) return;
     const int past = c + kVec<T> - n;
+    if (REACH == kShort && n < kVec<T>) return;
     if (WHOLE ? past > 0 : past >= kVec<T>)
         r = ux4{0, 0, 0, 0};
     else if (!WHOLE && past > 0)
         r = __builtin_bit_cast(ux4, __builtin_bit_cast(unsigned __int128, r) >> (past * 8 * static_cast<int>(sizeof(T))));
 }
-template <typename T, bool NEAR, bool WHOLE>
+template <typename T, Reach REACH, bool WHOLE = false>
 __device__ __forceinline__ ux4 load_row(const T* row, int c, int n) {
-    ux4 r = load_near<T, NEAR, WHOLE>(row, c, n);
-    in_place<T, NEAR, WHOLE>(r, c, n);
+    ux4 r = load_near<T, REACH>(row, c, n);
+    in_place<T, REACH, WHOLE>(r, c, n);
     return r;
-}
-
-// Rows of any length.
-template <typename T>
-__device__ __forceinline__ ux4 load_any(const T* row, int c, int n) {
-    return n < kVec<T> ? load_bits(row, c, n) : load_row<T, true, false>(row, c, n);
 }
 
 template <int CTRL>
