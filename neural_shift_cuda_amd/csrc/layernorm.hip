@@ -505,6 +505,7 @@ __global__ __launch_bounds__(64) void layer_norm_columns_kernel(LayerNormArgs a)
     constexpr int V = kVec<T>;
     const int c = (blockIdx.x * 64 + threadIdx.x) * V;
     float gw[V] = {}, gb[V] = {};
+#pragma unroll 4
     for (int64_t row = blockIdx.y; row < a.rows; row += gridDim.y) {
         const float mean = a.stats[2 * row], by = a.stats[2 * row + 1];
         float h[V], d[V];
@@ -590,8 +591,12 @@ static int layer_norm_wide(LayerNormArgs a, bool bwd, hipStream_t st) {
     }
     if (a.gx) layer_norm_wide_backward_kernel<T><<<a.blocks, kWideThreads, 0, st>>>(a);
     if (a.partial) {
+        // 16 waves a CU, no more than there is room for (600 x 40000 bf16: 25 us, and 108 with
+        // 512 of them down the rows, whose sums are more than the rows)
         constexpr int kCols = 64 * kVec<T>;
-        layer_norm_columns_kernel<T><<<dim3((a.n + kCols - 1) / kCols, a.blocks), 64, 0, st>>>(a);
+        const int across = (a.n + kCols - 1) / kCols;
+        a.blocks = std::min<int64_t>(a.blocks, nsh_host::ceil_div(16 * nsh_host::compute_units(), across));
+        layer_norm_columns_kernel<T><<<dim3(across, a.blocks), 64, 0, st>>>(a);
         layer_norm_weights<T>(a, st);
     }
     return nsh_host::check_launch("layer_norm_backward");
