@@ -546,6 +546,9 @@ __global__ __launch_bounds__(64 * WAVES) void gated_rows_kernel(GatedArgs a) {
 // Which workgroups a call takes
 // ---------------------------------------------------------------------------
 
+// Up to here the weights are read past the tiles (48 rows, 2048 -> 8192 bf16: 15.5 us, 22.8 by
+// tiles; 64 rows: 18.7 and 23.0; 64 rows, 4096 -> 11000 fp16: 52.1 and 52.5; one group of 16 rows
+// more would not fit the LDS twice).
 constexpr int kFewRows = 64;
 
 // Workgroup tiles, and the microseconds that a panel takes where one, two or three of
@@ -642,26 +645,21 @@ inline Cut gradient_cut(int64_t rows, int64_t K, int64_t F, Means by, bool input
 
 template <typename T>
 int gated_few_rows(GatedArgs a, hipStream_t st) {
-    // twice the waves a workgroup where there are too few for two on every CU
     const unsigned grid = (a.F + 15) / 16;
-    const bool more = grid < 2u * nsh_host::compute_units();
-    auto go = [&](auto groups) {
-        // (45 rows, 4096 -> 11000: 58 us by 64 bytes, 44 by 128; eight waves' panels of
-        // those fit the LDS up to 32 rows)
-        constexpr int MG = decltype(groups)::value;
-        if (more)
-            gated_rows_kernel<T, MG, 8, MG < 3 ? 128 : 64><<<grid, 512, 0, st>>>(a);
-        else
-            gated_rows_kernel<T, MG, 4, 128><<<grid, 256, 0, st>>>(a);
-    };
-    if (a.rows <= 16)
-        go(std::integral_constant<int, 1>{});
+    // One group of rows and workgroups for a part of the CUs: twice the waves (4 rows, 8192 -> 1024
+    // bf16: 10.5 us, 11.9 with four; with a workgroup on every CU, 16 rows, 2048 -> 5504: 13.0
+    // and 12.3).  More groups leave eight waves panels of 64 bytes a row (40 rows, 4096 -> 2048
+    // fp16: 12.4 and 10.9; 45 rows, 4096 -> 11000: 58 us by 64 bytes, 43 by 128).
+    if (a.rows <= 16 && grid < static_cast<unsigned>(nsh_host::compute_units()))
+        gated_rows_kernel<T, 1, 8, 128><<<grid, 512, 0, st>>>(a);
+    else if (a.rows <= 16)
+        gated_rows_kernel<T, 1, 4, 128><<<grid, 256, 0, st>>>(a);
     else if (a.rows <= 32)
-        go(std::integral_constant<int, 2>{});
+        gated_rows_kernel<T, 2, 4, 128><<<grid, 256, 0, st>>>(a);
     else if (a.rows <= 48)
-        go(std::integral_constant<int, 3>{});
+        gated_rows_kernel<T, 3, 4, 128><<<grid, 256, 0, st>>>(a);
     else
-        go(std::integral_constant<int, 4>{});
+        gated_rows_kernel<T, 4, 4, 128><<<grid, 256, 0, st>>>(a);
     return nsh_host::check_launch("gated_linear_forward");
 }
 
