@@ -235,7 +235,8 @@ __device__ __forceinline__ f32x16 gate_block(const GatedArgs& a, int64_t m, int 
 // fp32 by bf16 products: a number is the sum of three of bf16, 24 bits in all, and the six
 // products of parts that are not below 2^-24 are summed, the smallest first, by the same
 // panels and six times as many.  A product of fp32 matrices takes 16 times as long as one
-// of bf16.  (2048 x 1024 -> 2816: forward 219 us by fp32 products, gradients 407.)
+// of bf16.  (2048 x 1024 -> 2816: forward 138 us, 219 by fp32 products, gradients 266, 407; the
+// matrix units are busy for 46 and 49%, with 176 and 216 tiles for 256 CUs.)
 template <typename T, bool PARTS>
 struct Parts {
     using E = std::conditional_t<PARTS, bf16, T>;
@@ -446,7 +447,8 @@ __device__ __forceinline__ f32x4 multiply16(ux4 first, ux4 second, f32x4 c) {
 // 16 hidden columns and MG groups of 16 rows a workgroup, whose waves take turns in KB
 // bytes of the contraction, each with panels of its own in LDS and no barrier.  (Straight to
 // registers a lane would load 16 bytes of its own row, and lanes side by side other
-// rows: 45 rows, 4096 -> 11000, took 65 us, four times the caches' requests.)
+// rows: 45 rows, 4096 -> 11000, took 65 us, four times the caches' requests.)  Bound by the
+// weights' stream: that call 43 us, 4.2 TB/s, and 1 row, 2048 -> 8192 bf16 11.7 us, 5.7.
 template <typename T, int MG, int WAVES, int KB>
 __global__ __launch_bounds__(64 * WAVES) void gated_rows_kernel(GatedArgs a) {
     using L = Tile<T, KB / sizeof(T)>;
@@ -547,8 +549,8 @@ __global__ __launch_bounds__(64 * WAVES) void gated_rows_kernel(GatedArgs a) {
 // ---------------------------------------------------------------------------
 
 // Up to here the weights are read past the tiles (48 rows, 2048 -> 8192 bf16: 15.5 us, 22.8 by
-// tiles; 64 rows: 18.7 and 23.0; 64 rows, 4096 -> 11000 fp16: 52.1 and 52.5; one group of 16 rows
-// more would not fit the LDS twice).
+// tiles; 64 rows: 18.7 and 23.0; 64 rows, 4096 -> 11000 fp16: 52.1 and 52.5, where the panels leave
+// one workgroup to a CU).
 constexpr int kFewRows = 64;
 
 // Workgroup tiles, and the microseconds that a panel takes where one, two or three of

@@ -11,11 +11,14 @@
 // up to 64 lanes of a wave, then a workgroup of 256 or 512.  So mean and variance
 // are two sums over the same registers, the variance about the mean (as a
 // difference of squares it would lose what the mean is larger than the deviations).
-// Rows wider than a workgroup holds are read again for each sum.
+// Rows wider than a workgroup holds are read again for each sum.  Bound by memory: 16384 x
+// 2048 bf16 with a residual, forward 268 MB in 45.5 us (5.9 TB/s), backward as much in 44.5;
+// 3000 x 16384 fp16 forward 197 MB in 39 (5.0), backward 295 in 77 (3.8: a row's loads and the
+// sums over it take turns in the one workgroup that a CU's registers hold).
 //
 // gw and gb: a lane adds up its own columns over the rows that its group walks, the
 // groups of a workgroup add in order, and a second launch adds the workgroups'
-// sums in order.
+// sums in order (256 of them, 2048 columns: 4 us; 16384: 7.5).
 #include <algorithm>
 #include <cmath>
 
@@ -549,7 +552,8 @@ __global__ __launch_bounds__(1024) void layer_norm_weights_kernel(LayerNormArgs 
 }
 
 // Workgroups that walk the rows: enough to fill the card; in the backward few
-// enough that their sums of the weights' gradients stay small next to the rows.
+// enough that their sums of the weights' gradients stay small next to the rows (two a CU:
+// 16384 x 2048 bf16 44.5 us and 4.0 for the sums, four: 49 and 4.6).
 static int norm_row_blocks(int64_t rows, int per, int64_t each) {
     return static_cast<int>(std::min(nsh_host::ceil_div(rows, per), nsh_host::compute_units() * each));
 }
@@ -603,8 +607,9 @@ static int layer_norm_wide(LayerNormArgs a, bool bwd, hipStream_t st) {
 }
 
 // Lanes a row: as few as hold it in one part of 16 bytes each, up to a wave with four
-// parts; then a workgroup.  Where that leaves most CUs without a row, the workgroup
-// takes rows that a wave would hold.
+// parts; then a workgroup (16384 x 2048 bf16 by waves 46 us forward and 45 backward, by workgroups
+// 47 and 55; 16384 x 1040 18 and 27, 23 and 35).  Up to a row for each CU, the workgroup takes
+// rows that a wave would hold (64 x 2000 fp16: 3.4 and 5.4 us, by waves 4.0 and 6.2).
 template <typename T>
 static int layer_norm_dispatch(const LayerNormArgs& a, bool bwd, hipStream_t st) {
     const int64_t parts = nsh_host::ceil_div(a.n, kVec<T>);

@@ -4,8 +4,8 @@
 //   out[m][n] = sum_k second[m][k] first[n][k]
 //
 // A workgroup owns BM x BN of the result.  Of both matrices it takes KB bytes of the
-// contraction at a time (BK elements) straight from memory to LDS, two panels ahead
-// of each other: with the contraction running along the rows (`kAlong`, one LDS row
+// contraction at a time (BK elements) straight from memory to LDS, one panel ahead of the
+// products (two in the smallest tiles): with the contraction running along the rows (`kAlong`, one LDS row
 // for each row of the result) or across them (`kAcross`, one LDS row for each
 // contraction step, read by columns).  The chunk order within an LDS row is
 // attention_tiles.hpp's, free of bank conflicts both ways.

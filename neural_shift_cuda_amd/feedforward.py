@@ -150,7 +150,7 @@ def gated_linear(x: torch.Tensor, gate_weight: torch.Tensor, up_weight: torch.Te
 
     Returns h (..., hidden), contiguous: products, activation and their product
     in fp32, rounded once.  Differentiable in all three; training keeps two factors for each
-    of h (4.1 bytes in bf16, 6 in fp16, 8 in fp32).  The GPU serves width and hidden up
+    of h (4.25 bytes in bf16, 6 in fp16, 8 in fp32).  The GPU serves width and hidden up
     to 2^20; rows that do not start on 16 bytes are copied first.  In fp32 large products
     are summed from bf16 products of three parts, with fp32's bits; infinity times infinity
     is then no number."""
