@@ -579,11 +579,11 @@ inline double panels_until_done(Part a, Part b, double setup, int64_t slots) {
     double done = over ? late : early;
     if (!b.n) return done;
     auto room = [&](double t) {
-        return static_cast<double>(over) * std::max(0.0, std::floor((t - late) / lb)) +
-               static_cast<double>(slots - over) * std::max(0.0, std::floor((t - early) / lb));
+        return (t > late ? over * static_cast<int64_t>((t - late) / lb) : 0) +
+               (t > early ? (slots - over) * static_cast<int64_t>((t - early) / lb) : 0);
     };
     double t = (static_cast<double>(a.n) * la + static_cast<double>(b.n) * lb) / static_cast<double>(slots);
-    while (room(t) < static_cast<double>(b.n)) t += lb / 8;
+    while (room(t) < b.n) t += lb / 8;
     return std::max(done, t);
 }
 
@@ -602,20 +602,20 @@ struct Means {
 };
 
 // (0: no launch takes as many)
-inline double time_of(const Shape& s, const float (&rate)[3], Part a, Part b) {
+inline double time_of(const Shape& s, const float (&rate)[3], Part a, Part b, int64_t cus) {
     if ((a.n + b.n) * (s.bm == 256 ? 512 : 256) >> 32) return 0;
-    const int64_t cus = nsh_host::compute_units();
     int share = 1;
     while (share < 3 && rate[share] > 0 && share * cus < a.n + b.n) ++share;
     return panels_until_done(a, b, s.setup, cus * share) * rate[share - 1];
 }
 
 inline Cut forward_cut(int64_t rows, int64_t F, int64_t K, Means by) {
+    const int64_t cus = nsh_host::compute_units();
     Cut best{};
     for (int i = by.wide ? 1 : 0; i < 3; ++i) {
         const Shape& s = kShapes[i];
         Cut c{i, static_cast<int>(nsh_host::ceil_div(rows, s.bm)), static_cast<int>(nsh_host::ceil_div(F, s.bn / 2)), 1, 0, 0, 0};
-        c.time = time_of(s, by.wide ? s.wide : s.along, {c.tiles(), by.panels(K)}, {0, 0});
+        c.time = time_of(s, by.wide ? s.wide : s.along, {c.tiles(), by.panels(K)}, {0, 0}, cus);
         if (c.time > 0 && (best.time == 0 || c.time < best.time)) best = c;
     }
     return best;
@@ -625,6 +625,7 @@ inline Cut forward_cut(int64_t rows, int64_t F, int64_t K, Means by) {
 // workgroups share a tile's sum over the hidden columns, and another launch joins them
 // (4 us, and their sums' bytes at 3.5 TB/s).
 inline Cut gradient_cut(int64_t rows, int64_t K, int64_t F, Means by, bool input, bool weights) {
+    const int64_t cus = nsh_host::compute_units();
     Cut best{};
     for (int i = by.wide ? 1 : 0; i < 3; ++i) {
         const Shape& s = kShapes[i];
@@ -636,7 +637,7 @@ inline Cut gradient_cut(int64_t rows, int64_t K, int64_t F, Means by, bool input
             if (splits > 1 && (!input || panels / splits < 4)) break;
             c.splits = splits;
             c.time = time_of(s, by.wide ? s.wide : s.across, {c.tiles() * splits, nsh_host::ceil_div(panels, splits)},
-                             {c.weights(), by.panels(rows)});
+                             {c.weights(), by.panels(rows)}, cus);
             if (c.time == 0) break;
             if (splits > 1) c.time += 4 + static_cast<double>(splits * rows * K) * 4 / 3.5e6;
             if (best.time == 0 || c.time < best.time) best = c;

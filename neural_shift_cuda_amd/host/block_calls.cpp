@@ -10,7 +10,8 @@ using namespace nsh_calls;
 
 // Rows with a unit last stride and one step from each to the next, where the tensor
 // lies so; a copy otherwise.
-Tensor rows_of(const Tensor& t) {
+Tensor rows_of(const Tensor& t0) {
+    const Tensor t = t0.resolve_neg();  // (a conjugate's imaginary part)
     const int64_t dim = t.dim(), n = t.size(dim - 1);
     if (dim == 2 && (t.stride(1) == 1 || n == 1)) return t;
     bool whole = t.stride(dim - 1) == 1 || n == 1;

@@ -8,6 +8,7 @@ import torch.autograd.forward_ad as forward_ad
 
 import block_oracle as oracle
 from neural_shift_cuda import gated_linear, layer_norm
+from test_gpu_layer_norm import check as check_norm, inputs as norm_inputs
 
 pytestmark = [
     pytest.mark.gpu,
@@ -518,3 +519,22 @@ def test_gradients_of_more_blocks_than_workgroups():
     for v, n in zip((h, *got), ("h", "gx", "ggate", "gup")):
         oracle.close(v[-100:], vals[n], tols[n], n)
     assert not got[0][:-100].any()
+
+
+def test_a_conjugates_imaginary_part():
+    """A real tensor whose numbers lie in memory with the other sign."""
+    a = tensors((40, 1))[0]
+    x = torch.complex(a, a).conj().imag
+    assert x.is_neg()
+    w = tensors((8, 1), seed=4)[0]
+    assert torch.equal(gated_linear(x, w, w), gated_linear(-a, w, w))
+    y, s = layer_norm(x, residual=x)
+    assert torch.equal(s, -2 * a) and not y.any()
+
+
+@pytest.mark.parametrize("dtype,n", [("bf16", 4104), ("bf16", 4099), ("fp16", 16001), ("fp16", 12000), ("fp32", 2051),
+                                     ("fp32", 8188), ("bf16", 17003)])
+def test_rows_that_workgroups_walk(dtype, n):
+    """Three rows and more a workgroup of 512, forward and backward, with the loads of the
+    next ones under way, and rows that are read again."""
+    check_norm(norm_inputs(1700, n, dtype, residual=n % 2 == 0))
