@@ -13,8 +13,8 @@
 // difference of squares it would lose what the mean is larger than the deviations).
 // Rows wider than a workgroup holds are read again for each sum.  Bound by memory: 16384 x
 // 2048 bf16 with a residual, forward 268 MB in 45.5 us (5.9 TB/s), backward as much in 44.5;
-// 3000 x 16384 fp16 forward 197 MB in 39 (5.0), backward 295 in 77 (3.8: a row's loads and the
-// sums over it take turns in the one workgroup that a CU's registers hold).
+// 3000 x 16384 fp16 forward 197 MB in 39 (5.0), backward 295 in 64 (4.6: a CU's registers hold
+// one workgroup, whose loads and sums overlap by one row).
 //
 // gw and gb: a lane adds up its own columns over the rows that its group walks, the
 // groups of a workgroup add in order, and a second launch adds the workgroups'
@@ -231,18 +231,26 @@ __device__ __forceinline__ void add_columns(float* lds, int at, int all, const f
     }
 }
 
+// A lane's columns side by side (by elements, each a store 32 bytes off the next lane's:
+// 3000 x 16384 fp16 77 us instead of 64).
+template <int V>
+__device__ __forceinline__ void store_sums(const float (&sum)[V], float* to, int c, int n) {
+    if (c + V <= n) {
+        __builtin_memcpy(to + c, sum, sizeof(sum));
+        return;
+    }
+#pragma unroll
+    for (int k = 0; k < V; ++k)
+        if (c + k < n) to[c + k] = sum[k];
+}
+
 // Sums over the rows of a workgroup's groups, in their order, to its partial sums.
 template <int G, int NV, int V>
 __device__ __forceinline__ void add_groups(const float (&sum)[NV][V], float* to, int n, float* lds) {
     using Gr = Group<G>;
     if constexpr (Gr::kGroups == 1) {
 #pragma unroll
-        for (int i = 0; i < NV; ++i)
-#pragma unroll
-            for (int k = 0; k < V; ++k) {
-                const int c = (i * G + threadIdx.x) * V + k;
-                if (c < n) to[c] = sum[i][k];
-            }
+        for (int i = 0; i < NV; ++i) store_sums(sum[i], to, (i * G + static_cast<int>(threadIdx.x)) * V, n);
     } else {
         const int lane = threadIdx.x % G, own = threadIdx.x / G;
         __syncthreads();
@@ -269,7 +277,8 @@ __global__ __launch_bounds__(Group<G>::kThreads) void layer_norm_backward_kernel
     constexpr bool AHEAD = G >= 256 && (WHOLE || NV * V < 32);
     constexpr Reach REACH = reach_of(G, AHEAD, WHOLE);
     // 32 columns a lane: their sums are in LDS, and leave the next row its registers (3000
-    // x 16384 fp16: 104 us with the sums in registers and no row ahead, 85 so)
+    // x 16384 fp16: 104 us with the sums in registers and no row ahead, 85 so, before the
+// loads were unconditional and the sums stored side by side: 64)
     constexpr bool IN_LDS = NV * V == 32 && G > 64;
     __shared__ float lds[Gr::kGroups > 1 ? Gr::kThreads * NV * V : 4 * Gr::kWaves];
     __shared__ __attribute__((aligned(16))) float sums[IN_LDS ? 2 * Gr::kThreads * NV * V : 1];
@@ -521,9 +530,8 @@ __global__ __launch_bounds__(64) void layer_norm_columns_kernel(LayerNormArgs a)
         }
     }
     float* to = a.partial + static_cast<int64_t>(blockIdx.y) * 2 * a.n;
-#pragma unroll
-    for (int k = 0; k < V; ++k)
-        if (c + k < a.n) to[c + k] = gw[k], to[a.n + c + k] = gb[k];
+    store_sums(gw, to, c, a.n);
+    store_sums(gb, to + a.n, c, a.n);
 }
 
 // 32 columns per workgroup, 32 runs of blocks each: gw (blockIdx.y 0) or gb.
@@ -595,7 +603,7 @@ static int layer_norm_wide(LayerNormArgs a, bool bwd, hipStream_t st) {
     }
     if (a.gx) layer_norm_wide_backward_kernel<T><<<a.blocks, kWideThreads, 0, st>>>(a);
     if (a.partial) {
-        // 16 waves a CU, no more than there is room for (600 x 40000 bf16: 25 us, and 108 with
+        // 16 waves a CU, no more than there is room for (600 x 40000 bf16: 18 us, and 108 with
         // 512 of them down the rows, whose sums are more than the rows)
         constexpr int kCols = 64 * kVec<T>;
         const int across = (a.n + kCols - 1) / kCols;
@@ -609,7 +617,7 @@ static int layer_norm_wide(LayerNormArgs a, bool bwd, hipStream_t st) {
 // Lanes a row: as few as hold it in one part of 16 bytes each, up to a wave with four
 // parts; then a workgroup (16384 x 2048 bf16 by waves 46 us forward and 45 backward, by workgroups
 // 47 and 55; 16384 x 1040 18 and 27, 23 and 35).  Up to a row for each CU, the workgroup takes
-// rows that a wave would hold (64 x 2000 fp16: 3.4 and 5.4 us, by waves 4.0 and 6.2).
+// rows that a wave would hold (64 x 2000 fp16: 3.4 and 4.1 us, by waves 4.0 and 6.2).
 template <typename T>
 static int layer_norm_dispatch(const LayerNormArgs& a, bool bwd, hipStream_t st) {
     const int64_t parts = nsh_host::ceil_div(a.n, kVec<T>);
