@@ -313,15 +313,9 @@ __global__ __launch_bounds__(64 * WAVES_M * WAVES_N, 2) void gated_forward_kerne
                                     });
     if constexpr (__is_same(T, f16)) {
         if (!a.most) return;
-        float* meet = reinterpret_cast<float*>(b0);
         __syncthreads();
-        meet[threadIdx.x] = most;
-        __syncthreads();
-        for (int n = P::NT / 2; n >= 1; n /= 2) {
-            if (static_cast<int>(threadIdx.x) < n) meet[threadIdx.x] = fmaxf(meet[threadIdx.x], meet[threadIdx.x + n]);
-            __syncthreads();
-        }
-        if (threadIdx.x == 0) a.most[blockIdx.x] = meet[0];
+        most = workgroup_max<P::NT>(most, reinterpret_cast<float*>(b0));
+        if (threadIdx.x == 0) a.most[blockIdx.x] = most;
     }
 }
 

@@ -128,4 +128,23 @@ __device__ __forceinline__ float lanes_sum(float v) {
     return v;
 }
 
+// The largest of a workgroup's THREADS numbers, in all of them; lds: one for each wave.
+template <int THREADS>
+__device__ __forceinline__ float workgroup_max(float v, float* lds) {
+    v = fmaxf(v, lane_moved<0xB1>(v));
+    v = fmaxf(v, lane_moved<0x4E>(v));
+    v = fmaxf(v, lane_moved<0x141>(v));
+    v = fmaxf(v, lane_moved<0x140>(v));
+    const auto r = __builtin_amdgcn_permlane16_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+    v = fmaxf(__uint_as_float(r[0]), __uint_as_float(r[1]));
+    const auto s = __builtin_amdgcn_permlane32_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+    v = fmaxf(__uint_as_float(s[0]), __uint_as_float(s[1]));
+    if ((threadIdx.x & 63) == 0) lds[threadIdx.x / 64] = v;
+    __syncthreads();
+#pragma unroll
+    for (int w = 0; w < THREADS / 64; ++w) v = fmaxf(v, lds[w]);
+    __syncthreads();
+    return v;
+}
+
 }  // namespace nsh
