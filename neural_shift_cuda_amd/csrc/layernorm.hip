@@ -74,15 +74,24 @@ struct Group {
     }
 };
 
+// Divided by n, not times 1 / n, whose product the compiler would round only together with
+// what it is taken from: so the deviations of a row of one value are all the same, and whole
+// steps of the value's last place, their sums are exact, and what is left of them and of the
+// variance is 0.
+__device__ __forceinline__ float mean_of(float sum, const LayerNormArgs& a) { return sum / static_cast<float>(a.n); }
+
 // Of a row's deviations from its mean as first summed: 1 / sqrt(var + eps), and their own
 // mean, what that sum's rounding left (rows of one value would otherwise come out as its
 // last place over sqrt(eps)).
 template <typename Gr>
 __device__ __forceinline__ float variance(Gr& group, float square, float off, const LayerNormArgs& a, float& by) {
     group.sum(square, off);
-    const float rest = off * a.inv_n, var = square * a.inv_n;
+    const float rest = mean_of(off, a);
+    float var = mean_of(square, a);
     // (squares beyond fp32 leave infinity, and a row of zeros, as the formula does)
-    by = __builtin_amdgcn_rsqf(var - (var < INFINITY ? rest * rest : 0.f) + a.eps);
+    if (var < INFINITY) var -= rest * rest;
+    // (the difference may round below 0; what is no number stays so)
+    by = __builtin_amdgcn_rsqf((var < 0.f ? 0.f : var) + a.eps);
     return rest;
 }
 
@@ -163,7 +172,7 @@ __global__ __launch_bounds__(Group<G>::kThreads) void layer_norm_forward_kernel(
 #pragma unroll
             for (int k = 0; k < V; ++k) total += v[i][k];
         }
-        const float mean = group.sum(total) * a.inv_n;
+        const float mean = mean_of(group.sum(total), a);
         float square = 0.f, off = 0.f;
 #pragma unroll
         for (int i = 0; i < NV; ++i) {
@@ -440,7 +449,7 @@ __global__ __launch_bounds__(kWideThreads) void layer_norm_wide_forward_kernel(L
 #pragma unroll
             for (int k = 0; k < V; ++k) total += v[k];
         }
-        const float mean = group.sum(total) * a.inv_n;
+        const float mean = mean_of(group.sum(total), a);
         for (int c = threadIdx.x * V; c < a.n; c += kStep) {
             wide_values<T>(a, row, c, true, v);
 #pragma unroll

@@ -75,6 +75,7 @@ def layer_norm_reference(x, weight=None, bias=None, *, residual=None, eps: float
     y = s.to(_acc(x))
     if x.shape[-1]:
         y = y - y.mean(-1, keepdim=True)
+        y = y - y.mean(-1, keepdim=True)  # what the first sum's rounding left
         y = y * torch.rsqrt(y.square().mean(-1, keepdim=True) + eps)
     if weight is not None:
         y = y * weight.to(y.dtype)
