@@ -80,6 +80,13 @@ struct Group {
 // variance is 0.
 __device__ __forceinline__ float mean_of(float sum, const LayerNormArgs& a) { return sum / static_cast<float>(a.n); }
 
+// 1 / sqrt(v).  The instruction takes subnormal numbers for 0: rows of 1e-20 would be infinite.
+__device__ __forceinline__ float root_below(float v) {
+    const bool small = v < 0x1p-100f;
+    const float r = __builtin_amdgcn_rsqf(small ? v * 0x1p100f : v);
+    return small ? r * 0x1p50f : r;
+}
+
 // Of a row's deviations from its mean as first summed: 1 / sqrt(var + eps), and their own
 // mean, what that sum's rounding left (rows of one value would otherwise come out as its
 // last place over sqrt(eps)).
@@ -91,7 +98,7 @@ __device__ __forceinline__ float variance(Gr& group, float square, float off, co
     // (squares beyond fp32 leave infinity, and a row of zeros, as the formula does)
     if (var < INFINITY) var -= rest * rest;
     // (the difference may round below 0; what is no number stays so)
-    by = __builtin_amdgcn_rsqf((var < 0.f ? 0.f : var) + a.eps);
+    by = root_below((var < 0.f ? 0.f : var) + a.eps);
     return rest;
 }
 
