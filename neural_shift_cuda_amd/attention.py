@@ -390,6 +390,8 @@ class _TracedCall(torch.autograd.Function):
 
 
 def _traceable(call, tensors, **rules):
+    # (the kernels read memory, which holds a conjugate's imaginary part with the other sign)
+    tensors = [t.resolve_neg() if isinstance(t, torch.Tensor) and t.is_neg() else t for t in tensors]
     if not torch.jit.is_tracing():
         return call(*tensors, **rules)
     return _TracedCall.apply(functools.partial(call, **rules), *tensors)

@@ -81,16 +81,22 @@ inline bool graph(std::initializer_list<const Tensor*> tensors) {
 // What calls that need no conversion are looked over for
 // ---------------------------------------------------------------------------
 
+// In memory with its own sign (the imaginary part of a conjugate, say, is not).
+inline bool as_it_lies(const Tensor& t) { return !t.is_neg(); }
+
 inline bool served(const Tensor& t) {
     const auto type = t.scalar_type();
-    return type == at::kHalf || type == at::kBFloat16 || type == at::kFloat;
+    return (type == at::kHalf || type == at::kBFloat16 || type == at::kFloat) && as_it_lies(t);
 }
 
-inline bool alike(const Tensor& t, const Tensor& q) { return t.scalar_type() == q.scalar_type() && t.device() == q.device(); }
+inline bool alike(const Tensor& t, const Tensor& q) {
+    return t.scalar_type() == q.scalar_type() && t.device() == q.device() && as_it_lies(t);
+}
 
 // Not given, or contiguous in `type` and of this shape.
 inline bool plain(const Maybe& t, const Tensor& q, at::ScalarType type, at::IntArrayRef shape) {
-    return !t || (t->scalar_type() == type && t->device() == q.device() && t->sizes() == shape && t->is_contiguous());
+    return !t || (t->scalar_type() == type && t->device() == q.device() && t->sizes() == shape && t->is_contiguous() &&
+                  as_it_lies(*t));
 }
 
 }  // namespace nsh_calls

@@ -23,9 +23,14 @@ Tensor like(const Tensor& t) {
     return at::empty(t.sizes(), t.options());
 }
 
-// Rows with a unit last stride, in whole (`rows16`) 16-byte pieces.
-Tensor unit(const Tensor& t) { return t.stride(3) == 1 || t.size(3) == 1 ? t : t.contiguous(); }
-Tensor rows16(const Tensor& t) {
+// Rows with a unit last stride, in whole (`rows16`) 16-byte pieces.  (An upstream gradient may
+// come in memory with the other sign.)
+Tensor unit(const Tensor& t0) {
+    const Tensor t = t0.resolve_neg();
+    return t.stride(3) == 1 || t.size(3) == 1 ? t : t.contiguous();
+}
+Tensor rows16(const Tensor& t0) {
+    const Tensor t = t0.resolve_neg();
     const int64_t e = t.element_size(), all = t.stride(0) | t.stride(1) | t.stride(2);
     if (t.stride(3) == 1 && reinterpret_cast<uintptr_t>(t.data_ptr()) % 16 == 0 && all * e % 16 == 0 &&
         t.stride(2) * e <= int64_t(1) << 24)
@@ -156,7 +161,7 @@ struct BiasNode : torch::autograd::Function<BiasNode> {
         variable_list grads(4);
         {
             at::NoGradGuard none;
-            const Tensor g = upstream[0].contiguous();
+            const Tensor g = upstream[0].resolve_neg().contiguous();
             const int64_t rows = ctx->saved_data["rows"].toInt(), reach = (buckets.numel() - 1) / 2;
             grads[0] = at::empty({rows, g.size(0)}, g.options());
             if (!g.numel()) {
@@ -260,7 +265,7 @@ struct AttentionNode : torch::autograd::Function<AttentionNode> {
         {
             at::NoGradGuard none;
             const Tensor go = upstream[0].defined() ? rows16(upstream[0]) : at::zeros_like(out);
-            const Tensor gdegree = upstream.size() > 1 && upstream[1].defined() ? upstream[1].contiguous() : Tensor();
+            const Tensor gdegree = upstream.size() > 1 && upstream[1].defined() ? upstream[1].resolve_neg().contiguous() : Tensor();
             grads[0] = like(q), grads[1] = like(k), grads[2] = like(v);
             if (table.defined() && ctx->needs_input_grad(3)) grads[3] = at::empty_like(table);
             if (!q.numel() || !k.numel()) {
