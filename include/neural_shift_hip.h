@@ -617,9 +617,10 @@ NSH_API int64_t nsh_layer_norm_workspace_bytes(const nsh_layer_norm_args* args);
  * to row (elements), any alignment (rows that do not start on 16 bytes, or whose width is
  * no multiple of 16 bytes, are copied into the workspace first).  K, F <= 2^20, rows <=
  * 2^30.  Products, the activation and all sums are float (of fp32 matrices, where it is
- * faster, each product from six of bf16 parts, copied into the workspace: what is finite
- * keeps fp32's bits, infinity times infinity is NaN); dg and du are rounded to `dtype` (fp16: times a
- * power of two that the call chooses) as operands of the gradients' products. */
+ * faster, each product from six of bf16 parts, copied into the workspace: below 2^-21 of a
+ * product is left out, 4e-8 on average, and what is beyond fp32 or infinite is so with fp32's
+ * sign); dg and du are rounded to `dtype` (fp16: times a power of two that the call chooses) as
+ * operands of the gradients' products. */
 #define NSH_ACTIVATION_SILU 1
 #define NSH_ACTIVATION_GELU 2      /* g * Phi(g) */
 #define NSH_ACTIVATION_GELU_TANH 3 /* its form with a hyperbolic tangent */

@@ -151,10 +151,11 @@ def gated_linear(x: torch.Tensor, gate_weight: torch.Tensor, up_weight: torch.Te
 
     Returns h (..., hidden), contiguous: products, activation and their product
     in fp32, rounded once.  Differentiable in all three; training keeps two factors for each
-    of h (4.25 bytes in bf16, 6 in fp16, 8 in fp32).  The GPU serves width and hidden up
-    to 2^20; rows that do not start on 16 bytes are copied first.  In fp32 large products
-    are summed from bf16 products of three parts, with fp32's bits; infinity times infinity
-    is then no number."""
+    of h (4.25 bytes in bf16, 6 in fp16, 8 in fp32), and the gradients of the two projections
+    are rounded to the type, as operands of the products that give the inputs' gradients.  The
+    GPU serves width and hidden up to 2^20; rows that do not start on 16 bytes are copied
+    first.  In fp32 large products are summed from bf16 products of three parts, which leave
+    out 4e-8 of a product on average, and below 2^-21 of it."""
     if not x.is_cuda:
         return gated_linear_reference(x, gate_weight, up_weight, activation=activation)
     code = _CODES.get(activation)
