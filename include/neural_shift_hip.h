@@ -604,7 +604,8 @@ typedef struct nsh_layer_norm_args {
     const void *grad_y, *grad_s;
     int64_t gy_stride, gs_stride;
     void *grad_x, *grad_weight, *grad_bias;
-    void* workspace; /* nsh_layer_norm_workspace_bytes, 4-byte aligned; for the weights' gradients */
+    /* nsh_layer_norm_workspace_bytes (by rows, n and dtype), 4-byte aligned; for the weights' gradients */
+    void* workspace;
     int64_t workspace_bytes;
 } nsh_layer_norm_args;
 NSH_API int nsh_layer_norm_forward(const nsh_layer_norm_args* args, void* stream);

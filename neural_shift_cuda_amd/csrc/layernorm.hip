@@ -575,13 +575,46 @@ __global__ __launch_bounds__(1024) void layer_norm_weights_kernel(LayerNormArgs 
     }
 }
 
-// Workgroups that walk the rows: enough to fill the card; in the backward few
-// enough that their sums of the weights' gradients stay small next to the rows (two a CU:
-// 16384 x 2048 bf16 44.5 us and 4.0 for the sums, four: 49 and 4.6).
+// Lanes a row and parts of 16 bytes a lane; 0 lanes: rows that are read again for each sum.
+struct NormForm {
+    int lanes, parts;
+};
+
+// As few lanes as hold a row in one part each, up to a wave with four parts; then a workgroup
+// (16384 x 2048 bf16 by waves 46 us forward and 45 backward, by workgroups 47 and 55; 16384 x
+// 1040 18 and 27, 23 and 35).  Up to a row for each CU, the workgroup takes rows that a wave would
+// hold (64 x 2000 fp16: 3.4 and 4.1 us, by waves 4.0 and 6.2).
+static NormForm norm_form(int64_t rows, int64_t n, int vec) {
+    const int64_t parts = nsh_host::ceil_div(n, vec);
+    if (parts <= 64) return {parts <= 8 ? 8 : parts <= 16 ? 16 : parts <= 32 ? 32 : 64, 1};
+    if (parts <= 256 && rows <= nsh_host::compute_units()) return {256, 1};
+    if (parts <= 256) return {64, parts <= 128 ? 2 : 4};
+    if (parts <= 512) return {256, 2};
+    if (parts <= 2048) return {512, parts <= 1024 ? 2 : 4};
+    return {0, 0};
+}
+
+// Workgroups that walk the rows: enough to fill the card.
 static int norm_row_blocks(int64_t rows, int per, int64_t each) {
     return static_cast<int>(std::min(nsh_host::ceil_div(rows, per), nsh_host::compute_units() * each));
 }
-constexpr int kMostNormBlocks = 2;  // of the backward, a CU
+
+// In the backward few enough that their sums of the weights' gradients, one set a workgroup,
+// stay small next to the rows (two a CU: 16384 x 2048 bf16 44.5 us and 4.0 for the sums, four:
+// 49 and 4.6); 512 lanes' registers leave one workgroup to a CU.
+constexpr int kMostNormBlocks = 2;
+
+static int64_t wide_columns_across(int64_t n, int vec) { return nsh_host::ceil_div(n, 64 * vec); }
+
+// Sets of such sums, which the workspace holds and the launches write.
+static int norm_sums(int64_t rows, int64_t n, int vec) {
+    const NormForm f = norm_form(rows, n, vec);
+    if (f.lanes) return norm_row_blocks(rows, f.lanes < 256 ? 256 / f.lanes : 1, f.lanes == 512 ? 1 : kMostNormBlocks);
+    // 16 waves a CU, no more than there is room for (600 x 40000 bf16: 18 us, and 108 with
+    // 512 of them down the rows, whose sums are more than the rows)
+    return static_cast<int>(std::min<int64_t>(norm_row_blocks(rows, 1, kMostNormBlocks),
+                                              nsh_host::ceil_div(16 * nsh_host::compute_units(), wide_columns_across(n, vec))));
+}
 
 // (a launch takes less than 2^32 threads)
 template <typename T>
@@ -593,9 +626,8 @@ static void layer_norm_weights(const LayerNormArgs& a, hipStream_t st) {
 template <typename T, int G, int NV, bool WHOLE>
 static int layer_norm_rows(LayerNormArgs a, bool bwd, hipStream_t st) {
     using Gr = Group<G>;
-    // (rows of a workgroup: one each, as far as a launch's 2^32 threads go; backward, the 512
-    // lanes' registers leave one workgroup to a CU)
-    a.blocks = norm_row_blocks(a.rows, Gr::kGroups, bwd ? (G == 512 ? 1 : kMostNormBlocks) : G == 512 ? 2 : G > 64 ? 1 << 13 : 8);
+    // (forward, rows of a workgroup: one each, as far as a launch's 2^32 threads go)
+    a.blocks = bwd ? norm_sums(a.rows, a.n, kVec<T>) : norm_row_blocks(a.rows, Gr::kGroups, G == 512 ? 2 : G > 64 ? 1 << 13 : 8);
     if (!bwd) {
         layer_norm_forward_kernel<T, G, NV, WHOLE><<<a.blocks, Gr::kThreads, 0, st>>>(a);
         return nsh_host::check_launch("layer_norm_forward");
@@ -619,35 +651,28 @@ static int layer_norm_wide(LayerNormArgs a, bool bwd, hipStream_t st) {
     }
     if (a.gx) layer_norm_wide_backward_kernel<T><<<a.blocks, kWideThreads, 0, st>>>(a);
     if (a.partial) {
-        // 16 waves a CU, no more than there is room for (600 x 40000 bf16: 18 us, and 108 with
-        // 512 of them down the rows, whose sums are more than the rows)
-        constexpr int kCols = 64 * kVec<T>;
-        const int across = (a.n + kCols - 1) / kCols;
-        a.blocks = std::min<int64_t>(a.blocks, nsh_host::ceil_div(16 * nsh_host::compute_units(), across));
+        a.blocks = norm_sums(a.rows, a.n, kVec<T>);
+        const unsigned across = static_cast<unsigned>(wide_columns_across(a.n, kVec<T>));
         layer_norm_columns_kernel<T><<<dim3(across, a.blocks), 64, 0, st>>>(a);
         layer_norm_weights<T>(a, st);
     }
     return nsh_host::check_launch("layer_norm_backward");
 }
 
-// Lanes a row: as few as hold it in one part of 16 bytes each, up to a wave with four
-// parts; then a workgroup (16384 x 2048 bf16 by waves 46 us forward and 45 backward, by workgroups
-// 47 and 55; 16384 x 1040 18 and 27, 23 and 35).  Up to a row for each CU, the workgroup takes
-// rows that a wave would hold (64 x 2000 fp16: 3.4 and 4.1 us, by waves 4.0 and 6.2).
 template <typename T>
 static int layer_norm_dispatch(const LayerNormArgs& a, bool bwd, hipStream_t st) {
-    const int64_t parts = nsh_host::ceil_div(a.n, kVec<T>);
-    if (parts <= 8) return layer_norm_launch<T, 8, 1>(a, bwd, st);
-    if (parts <= 16) return layer_norm_launch<T, 16, 1>(a, bwd, st);
-    if (parts <= 32) return layer_norm_launch<T, 32, 1>(a, bwd, st);
-    if (parts <= 64) return layer_norm_launch<T, 64, 1>(a, bwd, st);
-    if (parts <= 256 && a.rows <= nsh_host::compute_units()) return layer_norm_launch<T, 256, 1>(a, bwd, st);
-    if (parts <= 128) return layer_norm_launch<T, 64, 2>(a, bwd, st);
-    if (parts <= 256) return layer_norm_launch<T, 64, 4>(a, bwd, st);
-    if (parts <= 512) return layer_norm_launch<T, 256, 2>(a, bwd, st);
-    if (parts <= 1024) return layer_norm_launch<T, 512, 2>(a, bwd, st);
-    if (parts <= 2048) return layer_norm_launch<T, 512, 4>(a, bwd, st);
-    return layer_norm_wide<T>(a, bwd, st);
+    const NormForm f = norm_form(a.rows, a.n, kVec<T>);
+    switch (f.lanes) {
+        case 8: return layer_norm_launch<T, 8, 1>(a, bwd, st);
+        case 16: return layer_norm_launch<T, 16, 1>(a, bwd, st);
+        case 32: return layer_norm_launch<T, 32, 1>(a, bwd, st);
+        case 64:
+            if (f.parts == 1) return layer_norm_launch<T, 64, 1>(a, bwd, st);
+            return f.parts == 2 ? layer_norm_launch<T, 64, 2>(a, bwd, st) : layer_norm_launch<T, 64, 4>(a, bwd, st);
+        case 256: return f.parts == 1 ? layer_norm_launch<T, 256, 1>(a, bwd, st) : layer_norm_launch<T, 256, 2>(a, bwd, st);
+        case 512: return f.parts == 2 ? layer_norm_launch<T, 512, 2>(a, bwd, st) : layer_norm_launch<T, 512, 4>(a, bwd, st);
+        default: return layer_norm_wide<T>(a, bwd, st);
+    }
 }
 
 }  // namespace nsh
@@ -655,8 +680,9 @@ static int layer_norm_dispatch(const LayerNormArgs& a, bool bwd, hipStream_t st)
 using nsh_host::fail;
 
 extern "C" int64_t nsh_layer_norm_workspace_bytes(const nsh_layer_norm_args* g) {
-    if (!g || g->rows < 1 || g->n < 1) return -1;
-    return static_cast<int64_t>(nsh::norm_row_blocks(g->rows, 1, nsh::kMostNormBlocks)) * 2 * g->n * 4;
+    if (!g || g->rows < 1 || g->n < 1 || g->dtype < NSH_DTYPE_FLOAT16 || g->dtype > NSH_DTYPE_FLOAT32) return -1;
+    const int vec = g->dtype == NSH_DTYPE_FLOAT32 ? 4 : 8;
+    return static_cast<int64_t>(nsh::norm_sums(g->rows, g->n, vec)) * 2 * g->n * 4;
 }
 
 static int layer_norm(const char* op, const nsh_layer_norm_args* g, bool bwd, void* stream) {
