@@ -145,7 +145,7 @@ std::tuple<Tensor, Tensor> gated_forward(const Tensor& x0, const Tensor& gate0, 
                                          bool keep) {
     const Tensor x = rows_of(x0), gate = rows_of(gate0), up = rows_of(up0);
     auto shape = x0.sizes().vec();
-    shape.back() = gate.size(0);
+    shape.back() = gate0.size(0);  // (a copy of weights without a width has lost its rows)
     const Tensor h = at::empty(shape, x0.options());
     nsh_gated_linear_args a = gated_args(x, gate, up, activation);
     Tensor kept;
