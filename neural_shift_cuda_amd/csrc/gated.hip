@@ -103,10 +103,18 @@ __global__ __launch_bounds__(kPassThreads) void gated_slope_kernel(SlopeArgs a) 
     for (int b = 0; b < BLOCKS; ++b) d[b] = S::get(stage, 0, b) * by;
 #pragma unroll
     for (int side = 0; side < 2; ++side) {
-        // (dh past F is 0, and what was kept of places past it in the last block is the
-        // activation at 0, a number)
 #pragma unroll
-        for (int b = 0; b < BLOCKS; ++b) x[b] = c0 + 32 * b < a.F ? d[b] * k[b].factor(side) : f32x16{};
+        for (int b = 0; b < BLOCKS; ++b) {
+            const int left = a.F - c0 - 32 * b;
+            x[b] = left > 0 ? d[b] * k[b].factor(side) : f32x16{};
+            // (dh past F is 0, but the factors kept there are those of a product of x with
+            // zeros, no numbers where x is infinite)
+            if (left > 0 && left < 32) {
+#pragma unroll
+                for (int r = 0; r < 16; ++r)
+                    if (8 * (r / 4) + 4 * static_cast<int>((threadIdx.x & 63) >> 5) + r % 4 >= left) x[b][r] = 0.f;
+            }
+        }
         using To = Stage<E, 32, COLS>;
         E* to = static_cast<E*>(a.dgu) + m0 * a.dgu_stride + side * a.Fp + c0;
         f32x16 parts[PARTS ? 3 : 1];

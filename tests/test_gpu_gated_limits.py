@@ -21,3 +21,22 @@ def test_weights_of_no_width_in_any_order():
         assert h.shape == (3, 5) and not h.any()
         for g, t in zip(torch.autograd.grad(h.sum(), (x, gate, up)), (x, gate, up)):
             assert g.shape == t.shape
+
+
+@pytest.mark.parametrize("dtype,M,F", [(torch.bfloat16, 70, 33), (torch.float16, 70, 33), (torch.float32, 70, 33),
+                                       (torch.bfloat16, 2000, 1100), (torch.float32, 2000, 1100)])
+def test_an_infinite_row_beside_a_ragged_end(dtype, M, F):
+    """Positive numbers all over: an infinity in x makes its row of h and dx infinite, and its
+    terms of the weights' gradients; the places past the last hidden column add nothing."""
+    K = 132
+    g = torch.Generator().manual_seed(F)
+    x, gate, up, gh = ((torch.rand(*s, generator=g) + 0.5).to(dtype) for s in ((M, K), (F, K), (F, K), (M, F)))
+    gate, up = gate / 128, up / 128
+    x[3, 7] = INF
+    leaves = [t.to(DEV).requires_grad_() for t in (x, gate, up)]
+    h = gated_linear(*leaves, activation="relu")
+    gx, gg, gu = torch.autograd.grad(h, leaves, gh.to(DEV))
+    assert (h[3] == INF).all() and (gx[3] == INF).all()
+    assert (gg == INF).all() and (gu == INF).all()
+    rest = [m for m in range(M) if m != 3]
+    assert h[rest].isfinite().all() and gx[rest].isfinite().all()
