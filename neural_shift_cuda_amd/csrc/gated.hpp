@@ -81,7 +81,10 @@ __device__ __forceinline__ float2 activate(float g) {
     } else if constexpr (KIND == kGeluTanh) {
         constexpr float a = 1.5957691216057308f, b = 0.044715f;  // 2 sqrt(2 / pi)
         const float s = sigmoid(a * g * fma_acc(b * g, g, 1.f));
-        return make_float2(g * s, fma_acc(g * s * (1.f - s), a * fma_acc(3.f * b * g, g, 1.f), s));
+        // (beyond 20 either way s is 1 or 0 to the last place; g's square would be infinite, and 0
+        // times it no number)
+        const float near = fminf(fmaxf(g, -20.f), 20.f);
+        return make_float2(g * s, fma_acc(near * s * (1.f - s), a * fma_acc(3.f * b * near, near, 1.f), s));
     } else if constexpr (KIND == kRelu) {
         return g > 0.f ? make_float2(g, 1.f) : make_float2(g == g ? 0.f : g, 0.f);
     } else {

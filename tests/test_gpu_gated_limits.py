@@ -40,3 +40,19 @@ def test_an_infinite_row_beside_a_ragged_end(dtype, M, F):
     assert (gg == INF).all() and (gu == INF).all()
     rest = [m for m in range(M) if m != 3]
     assert h[rest].isfinite().all() and gx[rest].isfinite().all()
+
+
+@pytest.mark.parametrize("dtype,M,F", [(torch.bfloat16, 70, 8), (torch.float32, 70, 8), (torch.float32, 2000, 1100)])
+def test_slopes_of_gelu_tanh_far_out(dtype, M, F):
+    """1 far above 0 and 0 far below it, where the cube is beyond fp32."""
+    K = 132
+    far = torch.tensor([1e13, 2e19, 1e20, 1e30, -1e13, -2e19, -1e20, -1e30])
+    x = torch.zeros(M, K, dtype=dtype)
+    x[:, 0], x[:, 1] = far.repeat(M // 8 + 1)[:M], 1.0
+    gate, up = torch.zeros(F, K, dtype=dtype), torch.zeros(F, K, dtype=dtype)
+    gate[:, 0], up[:, 1] = 1.0, 1.0
+    leaves = [t.to(DEV).requires_grad_() for t in (x, gate, up)]
+    h = gated_linear(*leaves, activation="gelu_tanh")
+    (gx,) = torch.autograd.grad(h, leaves[:1], torch.ones_like(h))
+    assert torch.equal(h, leaves[0][:, :1].clamp_min(0).expand(M, F))
+    assert torch.equal(gx[:, 0], F * (leaves[0][:, 0] > 0).to(dtype))
