@@ -74,11 +74,14 @@ struct Group {
     }
 };
 
-// Divided by n, not times 1 / n, whose product the compiler would round only together with
-// what it is taken from: so the deviations of a row of one value are all the same, and whole
-// steps of the value's last place, their sums are exact, and what is left of them and of the
-// variance is 0.
-__device__ __forceinline__ float mean_of(float sum, const LayerNormArgs& a) { return sum / static_cast<float>(a.n); }
+// sum / n: times 1 / n, and what that leaves.  (The product alone would be rounded only
+// together with what it is taken from, and be off by 1 / n's rounding.)  So the deviations of a
+// row of one value are all the same, and whole steps of the value's last place, their sums are
+// exact, and what is left of them and of the variance is 0.
+__device__ __forceinline__ float mean_of(float sum, const LayerNormArgs& a) {
+    const float mean = sum * a.inv_n;
+    return fma_acc(fma_acc(-mean, static_cast<float>(a.n), sum), a.inv_n, mean);
+}
 
 // 1 / sqrt(v).  The instruction takes subnormal numbers for 0: rows of 1e-20 would be infinite.
 __device__ __forceinline__ float root_below(float v) {
@@ -94,9 +97,9 @@ template <typename Gr>
 __device__ __forceinline__ float variance(Gr& group, float square, float off, const LayerNormArgs& a, float& by) {
     group.sum(square, off);
     const float rest = mean_of(off, a);
-    float var = mean_of(square, a);
+    float var = square * a.inv_n;
     // (squares beyond fp32 leave infinity, and a row of zeros, as the formula does)
-    if (var < INFINITY) var -= rest * rest;
+    if (var < INFINITY) var = mean_of(square, a) - rest * rest;
     // (the difference may round below 0; what is no number stays so)
     by = root_below((var < 0.f ? 0.f : var) + a.eps);
     return rest;
