@@ -88,8 +88,9 @@ __device__ __forceinline__ float2 activate(float g) {
     } else if constexpr (KIND == kRelu) {
         return g > 0.f ? make_float2(g, 1.f) : make_float2(g == g ? 0.f : g, 0.f);
     } else {
-        const float s = sigmoid(g);
-        return make_float2(s, s * (1.f - s));
+        // (by -|g|: 1 - s would be nothing but the last place of s where that is near 1)
+        const float e = __builtin_amdgcn_exp2f(-kLog2e * fabsf(g)), r = __builtin_amdgcn_rcpf(1.f + e);
+        return make_float2(g < 0.f ? e * r : r, e * r * r);
     }
 }
 

@@ -56,3 +56,25 @@ def test_slopes_of_gelu_tanh_far_out(dtype, M, F):
     (gx,) = torch.autograd.grad(h, leaves[:1], torch.ones_like(h))
     assert torch.equal(h, leaves[0][:, :1].clamp_min(0).expand(M, F))
     assert torch.equal(gx[:, 0], F * (leaves[0][:, 0] > 0).to(dtype))
+
+
+@pytest.mark.parametrize("M,F", [(70, 8), (2000, 1024)])
+def test_slopes_of_the_sigmoid_far_out(M, F):
+    """e^-|g| (1 + e^-|g|)^-2 with its own bits either way: the exponential's argument is rounded
+    (|g| / ln 2, and twice over: the product and its constant), and so are four more steps."""
+    K = 132
+    x = torch.zeros(M, K)
+    x[:, 0], x[:, 1] = torch.linspace(-60, 60, M), 1.0
+    gate, up = torch.zeros(F, K), torch.zeros(F, K)
+    gate[:, 0], up[:, 1] = 1.0, 1.0
+    leaves = [t.to(DEV).requires_grad_() for t in (x, gate, up)]
+    h = gated_linear(*leaves, activation="sigmoid")
+    gh = torch.zeros_like(h)
+    gh[:, 0] = 1.0  # one term a sum
+    (gx,) = torch.autograd.grad(h, leaves[:1], gh)
+    g = x[:, 0].double()
+    e = torch.exp(-g.abs())
+    want = e / (1 + e) ** 2
+    off = (gx[:, 0].double().cpu() - want).abs() / want
+    assert (off <= (2 * g.abs() + 16) * 2.0 ** -23).all(), float(off.max())
+    assert ((h[:, 0].double().cpu() - torch.sigmoid(g)).abs() <= (2 * g.abs() + 16) * 2.0 ** -23 * torch.sigmoid(g)).all()
