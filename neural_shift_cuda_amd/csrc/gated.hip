@@ -138,9 +138,10 @@ __global__ __launch_bounds__(kPassThreads) void gated_slope_kernel(SlopeArgs a) 
 }
 
 // fp16's numbers end at 2^-24 and lose bits from 2^-14 down, where the gradients of a
-// mean loss are.  dg and du are multiplied by a power of two, of the largest dh and the
-// largest factor, that brings them just under 2^15 and that the sums are divided by: what is
-// rounded off is then below 2^-39 of the largest wherever it is not half a step.
+// mean loss are.  dg and du are multiplied by a power of two that brings the largest dh times
+// the largest factor to 2^13 .. 2^15, and that the sums are divided by: what is rounded off,
+// where it is not half a step, is then at most 2^-38 of that product, which may be far above
+// the largest dg or du (a row of large factors whose dh is 0).
 constexpr int kMostBlocks = 2048;
 
 // Over rows of n, four parts of 16 bytes a lane at once (4096 x 4096: 10.4 us, 3.2 TB/s).

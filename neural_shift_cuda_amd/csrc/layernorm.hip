@@ -18,7 +18,7 @@
 //
 // gw and gb: a lane adds up its own columns over the rows that its group walks, the
 // groups of a workgroup add in order, and a second launch adds the workgroups'
-// sums in order (256 of them, 2048 columns: 4 us; 16384: 7.5).
+// sums in order (512 of them, 2048 columns: 4 us; 256, 16384 columns: 7.5).
 #include <algorithm>
 #include <cmath>
 
