@@ -121,7 +121,12 @@ struct Product {
     static constexpr int FIRST_BYTES = BN * KB, SECOND_BYTES = BM * KB, BYTES = FIRST_BYTES + SECOND_BYTES;
     static_assert(STEPS % 2 == 0 && (!PAIRED || (FIRST == kAlong && NB % 2 == 0)), "");
 
-    f32x16 acc[MT][NB];
+    // fp32: the sums of a chain of panels, 16 or 15, 512 of the contraction, are added to `whole`
+    // and start anew.  (In one chain of 4096 the roundings of h came to 1.7e-6 of it, twice a
+    // library's that shares a sum between workgroups.)
+    static constexpr bool FOLD = sizeof(T) == 4;
+    static constexpr int CHAIN2 = 16, CHAIN3 = 15;
+    f32x16 acc[MT][NB], whole[FOLD ? MT : 1][FOLD ? NB : 1];
     int by_first, by_second;
     struct Step {
         V f[NB], s[MT];
@@ -142,6 +147,27 @@ struct Product {
         for (int i = 0; i < MT; ++i)
 #pragma unroll
             for (int b = 0; b < NB; ++b) acc[i][b] = f32x16{};
+        if constexpr (FOLD) {
+#pragma unroll
+            for (int i = 0; i < MT; ++i)
+#pragma unroll
+                for (int b = 0; b < NB; ++b) whole[i][b] = f32x16{};
+        }
+    }
+    // acc added to `whole`, and started anew or, LAST, with all of it.
+    template <bool LAST>
+    __device__ __forceinline__ void fold() {
+        settle<T>();
+        if constexpr (FOLD) {
+#pragma unroll
+            for (int i = 0; i < MT; ++i)
+#pragma unroll
+                for (int b = 0; b < NB; ++b) {
+                    whole[i][b] += acc[i][b];
+                    acc[i][b] = LAST ? whole[i][b] : f32x16{};
+                }
+            order();
+        }
     }
     __device__ __forceinline__ void read(Step& x, const char* panel, int s) const {
 #pragma unroll
@@ -208,7 +234,19 @@ struct Product {
         if (n > 1) load(1, b1, b1 + FIRST_BYTES);
         read(x, b0, 0);
         order();
-        for (int i = 0; i < n; i += 2) {
+        int first = 0;
+        if constexpr (FOLD) {
+            for (; first + CHAIN2 < n; first += CHAIN2) {
+                for (int i = first; i < first + CHAIN2; i += 2) {
+                    steps(x, y, b0);
+                    turn<0>(x, y, b1, [&] { load(i + 2, b0, b0 + FIRST_BYTES); });
+                    steps(x, y, b1);
+                    turn<0>(x, y, b0, [&] { if (i + 3 < n) load(i + 3, b1, b1 + FIRST_BYTES); });
+                }
+                fold<false>();
+            }
+        }
+        for (int i = first; i < n; i += 2) {
             steps(x, y, b0);
             turn<0>(x, y, b1, [&] { if (i + 2 < n) load(i + 2, b0, b0 + FIRST_BYTES); });
             if (i + 1 < n) {
@@ -216,7 +254,7 @@ struct Product {
                 turn<0>(x, y, b0, [&] { if (i + 3 < n) load(i + 3, b1, b1 + FIRST_BYTES); });
             }
         }
-        settle<T>();
+        fold<true>();
     }
 
     // The same with two panels ahead.  From n on load() asks for nothing (a buffer of no
@@ -231,7 +269,21 @@ struct Product {
         landed<2 * LOADS>();
         read(x, b0, 0);
         order();
-        for (int i = 0;; i += 3) {
+        int first = 0;
+        if constexpr (FOLD) {
+            for (; first + CHAIN3 < n; first += CHAIN3) {
+                for (int i = first; i < first + CHAIN3; i += 3) {
+                    steps(x, y, b0);
+                    turn<LOADS>(x, y, b1, [&] { load(i + 3, b0, b0 + FIRST_BYTES); });
+                    steps(x, y, b1);
+                    turn<LOADS>(x, y, b2, [&] { load(i + 4, b1, b1 + FIRST_BYTES); });
+                    steps(x, y, b2);
+                    turn<LOADS>(x, y, b0, [&] { load(i + 5, b2, b2 + FIRST_BYTES); });
+                }
+                fold<false>();
+            }
+        }
+        for (int i = first;; i += 3) {
             steps(x, y, b0);
             turn<LOADS>(x, y, b1, [&] { load(i + 3, b0, b0 + FIRST_BYTES); });
             if (i + 1 >= n) break;
@@ -242,7 +294,7 @@ struct Product {
             turn<LOADS>(x, y, b0, [&] { load(i + 5, b2, b2 + FIRST_BYTES); });
             if (i + 3 >= n) break;
         }
-        settle<T>();
+        fold<true>();
         landed<0>();  // what was asked for past the end has no place in what follows
     }
 
